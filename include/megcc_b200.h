@@ -275,6 +275,46 @@ MB200_API int mb200_matmul_s8_qs8(
         int m, int n, int k, const int8_t* a, const int8_t* b_packed, int8_t* c, float acc_scale,
         float dst_scale, void* stream);
 
+/* ======================================================================================
+ * int8 products whose activations are quantised at run time: one scale per row (token), one
+ * per output channel. The reference's int8 operators know scales of whole tensors only, fixed when
+ * the model is compiled; these are for layers whose activations have no such scale. Activations
+ * and results are fp32, fp16 or bf16 (MB200_DTYPE_*), whole numbers int8, scales and bias fp32. Rows may lie
+ * apart (ld..: elements from one row to the next); a row's own elements are neighbours. m == 0 is allowed
+ * and does nothing. Every tensor may start at any element.
+ *
+ * A row x becomes whole numbers q with one scale: amax = max(max |x|, 2^-119),
+ *     scale = RN(amax * RN(1 / 127)),  inv = RN(RN(1 / amax) * 127),  q = x * inv to the nearest whole number
+ * (the product is not rounded before; ties to even), so -127 <= q <= 127 and x is near q * scale. A row
+ * with a NaN or an infinity gets scale NaN and zeros, and everything computed from it is NaN; other rows are
+ * not touched by it. ====================================================================== */
+enum { MB200_DTYPE_F32 = 0, MB200_DTYPE_F16 = 1, MB200_DTYPE_BF16 = 2 };
+
+/* x [m][k] -> q [m][k] and scales [m] */
+MB200_API int mb200_quantize_rows_s8(
+        const void* x, int dtype, int m, int k, long long ldx, int8_t* q, long long ldq, float* scales,
+        void* stream);
+
+/* c[i][j] = sum_l a[i][l] * b_packed[j][l] * a_scales[i] * b_scales[j] [+ bias[j]], the sum exact in int32
+ * (k <= 131071, more is refused with TinyNN_ERROR_OUT_OF_RANGE), the rest in fp32 and rounded to `dtype`
+ * once. b_packed: [n][k], the layout mb200_matmul_pack_b makes and most weights have. bias may be NULL.
+ * workspace: mb200_matmul_s8_scaled_workspace_bytes of the same operands, 256-byte aligned device memory;
+ * 0 bytes (and NULL) where rows of a and b_packed are whole 16-byte units or there are few of a. */
+MB200_API size_t mb200_matmul_s8_scaled_workspace_bytes(
+        int m, int n, int k, const int8_t* a, long long lda, const int8_t* b_packed);
+MB200_API int mb200_matmul_s8_scaled(
+        int m, int n, int k, const int8_t* a, long long lda, const int8_t* b_packed, const float* a_scales,
+        const float* b_scales, const float* bias, void* c, int dtype, long long ldc, void* workspace,
+        size_t workspace_bytes, void* stream);
+
+/* A linear layer: mb200_quantize_rows_s8 of x, then mb200_matmul_s8_scaled, in one call and with the same
+ * results. x [m][k] and y [m][n] are of type `dtype`. */
+MB200_API size_t mb200_linear_s8_workspace_bytes(int m, int n, int k, const int8_t* b_packed);
+MB200_API int mb200_linear_s8(
+        int m, int n, int k, const void* x, int dtype, long long ldx, const int8_t* b_packed,
+        const float* b_scales, const float* bias, void* y, long long ldy, void* workspace,
+        size_t workspace_bytes, void* stream);
+
 /* ---- Pooling qint8 (kernel_pooling_<MODE>_NCHW_p.._s.._w.._qsi8qsi8,
  * compiler/lib/KernelGen/BareMetal/Pooling.cpp:166-273), NHWC in/out ---- */
 MB200_API int mb200_pooling_qs8_nhwc(

@@ -76,6 +76,13 @@ SIGNATURES = {
     "mb200_matmul_s8_s32": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, _P, _P, _P]),
     "mb200_matmul_s8_qs8": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, _P, _P, C.c_float, C.c_float,
                                       _P]),
+    "mb200_quantize_rows_s8": (C.c_int, [_P] + [C.c_int] * 3 + [C.c_longlong, _P, C.c_longlong, _P, _P]),
+    "mb200_matmul_s8_scaled_workspace_bytes": (C.c_size_t, [C.c_int] * 3 + [_P, C.c_longlong, _P]),
+    "mb200_matmul_s8_scaled": (C.c_int, [C.c_int] * 3 + [_P, C.c_longlong] + [_P] * 5 + [
+        C.c_int, C.c_longlong, _P, C.c_size_t, _P]),
+    "mb200_linear_s8_workspace_bytes": (C.c_size_t, [C.c_int] * 3 + [_P]),
+    "mb200_linear_s8": (C.c_int, [C.c_int] * 3 + [_P, C.c_int, C.c_longlong] + [_P] * 4 + [
+        C.c_longlong, _P, C.c_size_t, _P]),
     "mb200_pooling_qs8_nhwc": (C.c_int, [_P, _P] + [C.c_int] * 11 + [_P]),
     "mb200_qelemwise_qs8": (C.c_int, [_P, _P, _P, C.c_int, C.c_size_t, C.c_float, C.c_float,
                                       C.c_float, _P]),
@@ -131,7 +138,9 @@ FAST = ("mb200_conv_bias_qs8_nhwc", "mb200_conv_bias_qs8_nhwc_fused", "mb200_con
         "mb200_matmul_s8_qs8", "mb200_qelemwise_qs8", "mb200_conv_bias_f32_nhwc",
         "mb200_conv_bias_qs8_nchw_workspace", "mb200_conv_nchw_in_place",
         "mb200_conv_bias_qs8_nchw_in_place", "mb200_matmul_f32_scratch_bytes_for",
-        "mb200_matmul_f32_product", "mb200_elemwise_f32")
+        "mb200_matmul_f32_product", "mb200_elemwise_f32", "mb200_quantize_rows_s8",
+        "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
+        "mb200_linear_s8_workspace_bytes", "mb200_linear_s8")
 _fast = None
 
 

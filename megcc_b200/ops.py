@@ -139,6 +139,85 @@ def matmul_s8_qs8(a, b_packed, acc_scale, dst_scale):
     return c
 
 
+# ---- int8 products with scales per row (token) and per output channel ----
+DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _rows(t, kinds, name):
+    """(rows, columns, elements between rows) of a matrix of the current device, whose rows'
+    elements are neighbours"""
+    if t.dtype not in kinds or t.dim() != 2 or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA matrix of {', '.join(str(k) for k in kinds)}, not "
+                         f"{tuple(t.shape)} of {t.dtype} on {t.device}")
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} is on {t.device}, not on the current device")
+    (m, k), (ld, one) = t.shape, t.stride()
+    if one != 1 and k > 1:
+        raise ValueError(f"{name}: elements of a row must be neighbours (strides {t.stride()})")
+    return m, k, ld
+
+
+def _vector(t, n, like, name):
+    """Address of a contiguous fp32 vector of n elements on the device of `like`"""
+    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous() or \
+            t.get_device() != like.get_device():
+        raise ValueError(f"{name}: {n} contiguous fp32 values on {like.device}, not "
+                         f"{tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _packed_b(b, k, like):
+    if b.dtype is not _S8 or b.dim() != 2 or b.shape[1] != k or not b.is_contiguous() or \
+            b.get_device() != like.get_device():
+        raise ValueError(f"b_packed: contiguous int8 [n, {k}] on {like.device}, not "
+                         f"{tuple(b.shape)} of {b.dtype} on {b.device}")
+    return b.shape[0]
+
+
+def quantize_rows_s8(x):
+    """Rows of an fp32 / fp16 / bf16 matrix as int8 with one fp32 scale each: (q, scales)."""
+    m, k, ld = _rows(x, DTYPE, "x")
+    q, scales = x.new_empty((m, k), dtype=_S8), x.new_empty((m,), dtype=torch.float32)
+    check(fast().mb200_quantize_rows_s8(x.data_ptr(), DTYPE[x.dtype], m, k, ld, q.data_ptr(), k,
+                                        scales.data_ptr(), _stream()))
+    return q, scales
+
+
+def matmul_s8_scaled(a, b_packed, a_scales, b_scales, bias=None, dtype=torch.float32):
+    """a [m, k] int8 times b_packed [n, k] int8 (matmul_pack_b), with a scale per row of a and per
+    row of b_packed, plus bias [n]: [m, n] of `dtype`."""
+    m, k, ld = _rows(a, (_S8,), "a")
+    n = _packed_b(b_packed, k, a)
+    if dtype not in DTYPE:
+        raise ValueError(f"results are fp32, fp16 or bf16, not {dtype}")
+    f = fast()
+    pa, pb = a.data_ptr(), b_packed.data_ptr()
+    sa, sb = _vector(a_scales, m, a, "a_scales"), _vector(b_scales, n, a, "b_scales")
+    bias = None if bias is None else _vector(bias, n, a, "bias")
+    c = a.new_empty((m, n), dtype=dtype)
+    nbytes = f.mb200_matmul_s8_scaled_workspace_bytes(m, n, k, pa, ld, pb)
+    keep, ws = _scratch(nbytes, a.device)
+    check(f.mb200_matmul_s8_scaled(m, n, k, pa, ld, pb, sa, sb, bias, c.data_ptr(), DTYPE[dtype], n,
+                                   ws, nbytes, _stream()))
+    return c
+
+
+def linear_s8(x, b_packed, b_scales, bias=None):
+    """x [m, k] fp32 / fp16 / bf16, quantised row by row, times b_packed [n, k] int8 with a scale per
+    row, plus bias [n]: [m, n] of x's type. The same as quantize_rows_s8 and matmul_s8_scaled."""
+    m, k, ld = _rows(x, DTYPE, "x")
+    n = _packed_b(b_packed, k, x)
+    f = fast()
+    pb, sb = b_packed.data_ptr(), _vector(b_scales, n, x, "b_scales")
+    bias = None if bias is None else _vector(bias, n, x, "bias")
+    y = x.new_empty((m, n))
+    nbytes = f.mb200_linear_s8_workspace_bytes(m, n, k, pb)
+    keep, ws = _scratch(nbytes, x.device)
+    check(f.mb200_linear_s8(m, n, k, x.data_ptr(), DTYPE[x.dtype], ld, pb, sb, bias, y.data_ptr(), n,
+                            ws, nbytes, _stream()))
+    return y
+
+
 def pooling_qs8_nhwc(src, mode, window, stride, pad):
     n, ih, iw, c = src.shape
     oh, ow = (ih + 2 * pad - window) // stride + 1, (iw + 2 * pad - window) // stride + 1
