@@ -315,6 +315,34 @@ MB200_API int mb200_linear_s8(
         const float* b_scales, const float* bias, void* y, long long ldy, void* workspace,
         size_t workspace_bytes, void* stream);
 
+/* A mixture-of-experts layer for a few tokens, in two kernels. For each of `tokens` rows x[t] (d elements) and its
+ * logits[t] ([tokens][experts] fp32, contiguous; the router's product is the caller's, mb200_matmul_f32 for
+ * instance):
+ *   p = softmax over all experts; the top_k largest logits are chosen (ties: the lowest index), their p divided
+ *       by the sum of the chosen ones' if renormalize != 0
+ *   z = the product of x's whole numbers with w1[expert] [2f][d], scaled by x's scale and w1_scales[expert][2f]; its
+ *       first f values are the gate's, the others the layer's: h = gate / (1 + exp(-gate)) * up
+ *   h in groups of 32 neighbours (the last may be shorter) as whole numbers with a scale each, by the same rule
+ *       as rows
+ *   y[t] = sum over the chosen of p * w2_scales[expert][d] * (w2[expert] [d][f] times h)
+ * Sums of whole numbers are exact, all others in fp32, in an order that is always the same. An expert whose p is 0 (a
+ * logit of -infinity masks it) adds nothing; with all logits at -infinity y[t] is 0 (a padded token); a NaN or
+ * +infinity among a token's logits, or a row x[t] without a scale, makes that y[t] NaN.
+ * 1 <= tokens <= 64, top_k <= 16 and <= experts <= 512, f <= 131071, d <= 20480 (10240 with more than 8 tokens):
+ * beyond them TinyNN_ERROR_OUT_OF_RANGE; tokens == 0 does nothing. ldx, ldy: elements from row to row.
+ * workspace: mb200_moe_s8_workspace_bytes(p) bytes of device memory, 256-byte aligned, whose content does not
+ * matter; two calls that may run at the same time need one each. */
+typedef struct mb200_moe_param {
+    int tokens, d, f, experts, top_k;
+    int renormalize;
+    int dtype; /* of x and y: MB200_DTYPE_* */
+} mb200_moe_param;
+MB200_API size_t mb200_moe_s8_workspace_bytes(const mb200_moe_param* p);
+MB200_API int mb200_moe_s8(
+        const mb200_moe_param* p, const void* x, long long ldx, const float* logits, const int8_t* w1,
+        const float* w1_scales, const int8_t* w2, const float* w2_scales, void* y, long long ldy, void* workspace,
+        size_t workspace_bytes, void* stream);
+
 /* ---- Pooling qint8 (kernel_pooling_<MODE>_NCHW_p.._s.._w.._qsi8qsi8,
  * compiler/lib/KernelGen/BareMetal/Pooling.cpp:166-273), NHWC in/out ---- */
 MB200_API int mb200_pooling_qs8_nhwc(

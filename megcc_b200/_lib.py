@@ -29,6 +29,11 @@ class ConvFuse(C.Structure):
                 ("out_scale", C.c_float)]
 
 
+class MoeParam(C.Structure):
+    """Mirror of ``mb200_moe_param``."""
+    _fields_ = [(k, C.c_int) for k in ("tokens", "d", "f", "experts", "top_k", "renormalize", "dtype")]
+
+
 _lib = None
 
 # name -> (restype, argtypes); every symbol declared in include/megcc_b200.h
@@ -82,6 +87,9 @@ SIGNATURES = {
         C.c_int, C.c_longlong, _P, C.c_size_t, _P]),
     "mb200_linear_s8_workspace_bytes": (C.c_size_t, [C.c_int] * 3 + [_P]),
     "mb200_linear_s8": (C.c_int, [C.c_int] * 3 + [_P, C.c_int, C.c_longlong] + [_P] * 4 + [
+        C.c_longlong, _P, C.c_size_t, _P]),
+    "mb200_moe_s8_workspace_bytes": (C.c_size_t, [C.POINTER(MoeParam)]),
+    "mb200_moe_s8": (C.c_int, [C.POINTER(MoeParam), _P, C.c_longlong] + [_P] * 6 + [
         C.c_longlong, _P, C.c_size_t, _P]),
     "mb200_pooling_qs8_nhwc": (C.c_int, [_P, _P] + [C.c_int] * 11 + [_P]),
     "mb200_qelemwise_qs8": (C.c_int, [_P, _P, _P, C.c_int, C.c_size_t, C.c_float, C.c_float,
@@ -140,7 +148,8 @@ FAST = ("mb200_conv_bias_qs8_nhwc", "mb200_conv_bias_qs8_nhwc_fused", "mb200_con
         "mb200_conv_bias_qs8_nchw_in_place", "mb200_matmul_f32_scratch_bytes_for",
         "mb200_matmul_f32_product", "mb200_elemwise_f32", "mb200_quantize_rows_s8",
         "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
-        "mb200_linear_s8_workspace_bytes", "mb200_linear_s8")
+        "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
+        "mb200_moe_s8")
 _fast = None
 
 

@@ -1,5 +1,6 @@
 // extern "C" entry points of the int8 operators with scales found at run time (include/megcc_b200.h).
 #include "../../include/megcc_b200.h"
+#include "moe_s8.h"
 #include "scaled_s8.cuh"
 
 using namespace mb200;
@@ -41,6 +42,29 @@ int check_product_sides(
     if (misaligned(b_scales, 4) || misaligned(bias, 4) || misaligned(c, dtype_bytes(dtype)))
         return set_error(ST_INVALID_LAYOUT, "%s: scales, bias and result must be aligned as their types are", what);
     return ST_SUCCESS;
+}
+
+int check_moe(const mb200_moe_param* p) {
+    if (!p)
+        return set_error(ST_NULL_PTR, "moe_s8: parameter block is NULL");
+    int rc = check_dtype(p->dtype, "moe_s8");
+    if (rc)
+        return rc;
+    if (p->tokens < 0 || p->d <= 0 || p->f <= 0 || p->experts <= 0 || p->top_k <= 0 || p->top_k > p->experts)
+        return set_error(ST_INVALID_LAYOUT, "moe_s8: %d tokens, d %d, f %d, %d of %d experts", p->tokens, p->d, p->f,
+                         p->top_k, p->experts);
+    if (p->tokens > kMoeMaxTokens || p->top_k > kMoeMaxTop || p->experts > kMoeMaxExperts || p->f > kMaxK ||
+        p->d > (p->tokens <= 8 ? kMoeMaxDepthFew : kMoeMaxDepth))
+        return set_error(ST_OUT_OF_RANGE, "moe_s8: %d tokens (64), d %d (20480, 10240 with more than 8 tokens), "
+                         "f %d (131071), %d of %d experts (16 of 512)", p->tokens, p->d, p->f, p->top_k, p->experts);
+    return ST_SUCCESS;
+}
+size_t moe_hidden_bytes(const mb200_moe_param* p) {  // whole numbers of the hidden layer
+    return align_up((size_t)p->tokens * p->top_k * align_up((size_t)p->f, 32), 256);
+}
+size_t moe_bytes(const mb200_moe_param* p) {
+    return moe_hidden_bytes(p) +
+           align_up((size_t)p->tokens * p->top_k * (align_up((size_t)p->f, 32) / 32) * sizeof(float), 256);
 }
 
 }  // namespace
@@ -133,6 +157,38 @@ int mb200_linear_s8(
     p.c = y, p.c_dtype = dtype, p.ldc = ldy;
     p.b_early = may_read_early(b_packed, (size_t)n * k, st);
     return launch_product_stream(p, st);
+}
+
+size_t mb200_moe_s8_workspace_bytes(const mb200_moe_param* p) {
+    return check_moe(p) ? 0 : moe_bytes(p);
+}
+
+int mb200_moe_s8(
+        const mb200_moe_param* p, const void* x, long long ldx, const float* logits, const int8_t* w1,
+        const float* w1_scales, const int8_t* w2, const float* w2_scales, void* y, long long ldy, void* workspace,
+        size_t workspace_bytes, void* stream) {
+    const int rc = check_moe(p);
+    if (rc || p->tokens == 0)
+        return rc;
+    if (!x || !logits || !w1 || !w1_scales || !w2 || !w2_scales || !y || !workspace)
+        return set_error(ST_NULL_PTR, "moe_s8: operand pointer is NULL");
+    if (p->tokens > 1 && (ldx < p->d || ldy < p->d))
+        return set_error(ST_INVALID_LAYOUT, "moe_s8: rows overlap");
+    if (misaligned(x, dtype_bytes(p->dtype)) || misaligned(y, dtype_bytes(p->dtype)) || misaligned(logits, 4) ||
+        misaligned(w1_scales, 4) || misaligned(w2_scales, 4))
+        return set_error(ST_INVALID_LAYOUT, "moe_s8: tensors must be aligned as their types are");
+    if (misaligned(workspace, 256) || workspace_bytes < moe_bytes(p))
+        return set_error(ST_INVALID_LAYOUT, "moe_s8: the workspace must be 256-byte aligned and hold %zu bytes",
+                         moe_bytes(p));
+    MoeArgs a{};
+    a.t = p->tokens, a.d = p->d, a.f = p->f, a.e = p->experts, a.top = p->top_k;
+    a.renormalize = p->renormalize, a.dtype = p->dtype;
+    a.x = x, a.ldx = ldx, a.logits = logits;
+    a.w1 = w1, a.s1 = w1_scales, a.w2 = w2, a.s2 = w2_scales;
+    a.y = y, a.ldy = ldy;
+    a.hq = (int8_t*)workspace, a.sh = (float*)((uint8_t*)workspace + moe_hidden_bytes(p));
+    a.workspace_bytes = moe_bytes(p);
+    return launch_moe(a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -7,7 +7,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import ConvF32Param, ConvFuse, ConvParam, check, fast, lib
+from ._lib import ConvF32Param, ConvFuse, ConvParam, MoeParam, check, fast, lib
 
 ACT = {"IDENTITY": 0, "RELU": 1, "H_SWISH": 2}
 POOL = {"MAX": 0, "AVERAGE": 1, "AVERAGE_COUNT_EXCLUDE_PADDING": 2}
@@ -215,6 +215,38 @@ def linear_s8(x, b_packed, b_scales, bias=None):
     keep, ws = _scratch(nbytes, x.device)
     check(f.mb200_linear_s8(m, n, k, x.data_ptr(), DTYPE[x.dtype], ld, pb, sb, bias, y.data_ptr(), n,
                             ws, nbytes, _stream()))
+    return y
+
+
+def _expert_weights(w, experts, like, name):
+    if w.dtype is not _S8 or w.dim() != 3 or w.shape[0] != experts or not w.is_contiguous() or \
+            w.get_device() != like.get_device():
+        raise ValueError(f"{name}: contiguous int8 [{experts}, rows, columns] on {like.device}, not "
+                         f"{tuple(w.shape)} of {w.dtype} on {w.device}")
+    return w.shape[1], w.shape[2]
+
+
+def moe_s8(x, logits, w1, w1_scales, w2, w2_scales, top_k, renormalize=True):
+    """Mixture-of-experts layer for up to 64 tokens: x [t, d] fp32 / fp16 / bf16, router logits [t, experts]
+    fp32, int8 weights w1 [experts, 2f, d] (gate rows, then up rows) and w2 [experts, d, f] with fp32 scales
+    per row; [t, d] of x's type (see mb200_moe_s8)."""
+    t, d, ld = _rows(x, DTYPE, "x")
+    if logits.dim() != 2 or logits.shape[0] != t:
+        raise ValueError(f"logits: [{t}, experts], not {tuple(logits.shape)}")
+    e = logits.shape[1]
+    pl = _vector(logits, t * e, x, "logits")
+    f2, d1 = _expert_weights(w1, e, x, "w1")
+    d2, f = _expert_weights(w2, e, x, "w2")
+    if f2 != 2 * f or d1 != d or d2 != d:
+        raise ValueError(f"w1 {tuple(w1.shape)} and w2 {tuple(w2.shape)} over rows of {d}")
+    s1, s2 = _vector(w1_scales, e * f2, x, "w1_scales"), _vector(w2_scales, e * d, x, "w2_scales")
+    p = MoeParam(t, d, f, e, top_k, int(renormalize), DTYPE[x.dtype])
+    at, fn = C.addressof(p), fast()
+    y = x.new_empty((t, d))
+    nbytes = fn.mb200_moe_s8_workspace_bytes(at)
+    keep, ws = _scratch(nbytes, x.device)
+    check(fn.mb200_moe_s8(at, x.data_ptr(), ld, pl, w1.data_ptr(), s1, w2.data_ptr(), s2, y.data_ptr(), d,
+                          ws, nbytes, _stream()))
     return y
 
 

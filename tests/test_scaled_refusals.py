@@ -57,3 +57,34 @@ def test_python_calls_want_matrices_on_the_gpu():
                  lambda: ops.matmul_s8_scaled(b, b, s, s), lambda: ops.linear_s8(x.double(), b, s)):
         with pytest.raises(ValueError):
             call()
+
+
+def moe(tokens=2, d=64, f=32, experts=4, top_k=2, renormalize=1, dtype=2, x=P, ldx=64, logits=P, w1=P, s1=P, w2=P,
+        s2=P, y=P, ldy=64, ws=P, nbytes=1 << 30):
+    import ctypes
+    p = _lib.MoeParam(tokens, d, f, experts, top_k, renormalize, dtype)
+    return _lib.lib().mb200_moe_s8(ctypes.byref(p), x, ldx, logits, w1, s1, w2, s2, y, ldy, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(x=None), NULL_PTR), (dict(logits=None), NULL_PTR), (dict(w1=None), NULL_PTR), (dict(s1=None), NULL_PTR),
+    (dict(w2=None), NULL_PTR), (dict(s2=None), NULL_PTR), (dict(y=None), NULL_PTR), (dict(ws=None), NULL_PTR),
+    (dict(dtype=3), DTYPE), (dict(tokens=-1), LAYOUT), (dict(d=0), LAYOUT), (dict(f=0), LAYOUT),
+    (dict(experts=0), LAYOUT), (dict(top_k=0), LAYOUT), (dict(top_k=5), LAYOUT), (dict(tokens=65), OUT_OF_RANGE),
+    (dict(experts=513), OUT_OF_RANGE), (dict(experts=40, top_k=17), OUT_OF_RANGE),
+    (dict(d=20481, ldx=30000, ldy=30000), OUT_OF_RANGE), (dict(tokens=9, d=10241, ldx=30000, ldy=30000), OUT_OF_RANGE),
+    (dict(f=131072), OUT_OF_RANGE), (dict(ldx=63), LAYOUT), (dict(ldy=63), LAYOUT), (dict(x=P + 1), LAYOUT),
+    (dict(y=P + 1), LAYOUT), (dict(logits=P + 2), LAYOUT), (dict(s1=P + 2), LAYOUT), (dict(s2=P + 1), LAYOUT),
+    (dict(ws=P + 128), LAYOUT), (dict(nbytes=100), LAYOUT), (dict(tokens=0, x=None, ws=None), 0)])
+def test_moe(change, status):
+    assert moe(**change) == status
+
+
+def test_moe_workspace_and_null_parameters():
+    import ctypes
+    size = _lib.lib().mb200_moe_s8_workspace_bytes
+    assert size(None) == 0 and _lib.lib().mb200_moe_s8(None, *[P, 64] + [P] * 6 + [64, P, 0, None]) == NULL_PTR
+    p = _lib.MoeParam(2, 64, 33, 4, 2, 1, 2)
+    assert size(ctypes.byref(p)) == 256 + 256  # 4 slots of 64 whole numbers, of 2 scales
+    p.tokens = 65
+    assert size(ctypes.byref(p)) == 0
