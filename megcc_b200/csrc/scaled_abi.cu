@@ -44,6 +44,45 @@ int check_product_sides(
     return ST_SUCCESS;
 }
 
+int check_workspace(const char* what, const void* workspace, size_t have, size_t need) {
+    if (need == 0)
+        return ST_SUCCESS;
+    if (!workspace)
+        return set_error(ST_NULL_PTR, "%s: needs a workspace of %zu bytes", what, need);
+    if (misaligned(workspace, 256) || have < need)
+        return set_error(ST_INVALID_LAYOUT, "%s: the workspace must be 256-byte aligned and hold %zu bytes", what,
+                         need);
+    return ST_SUCCESS;
+}
+
+// Few rows of activations: the kernel that takes the weights straight to registers, whatever the operands'
+// alignment; and so few that it makes whole numbers of them itself, every CTA again.
+bool streams(int m) {
+    return m <= 16;
+}
+bool streams_activations(int m) {
+    return m <= 8;
+}
+// What the TMA takes: 16-byte aligned, rows whole 16-byte units apart
+bool rows_fit(const void* p, int rows, long long ld) {
+    return !misaligned(p, 16) && (rows == 1 || ld % 16 == 0);
+}
+long long padded(int k) {
+    return ((long long)k + 15) / 16 * 16;
+}
+size_t padded_bytes(int rows, int k) {
+    return align_up((size_t)rows * (size_t)padded(k), 256);
+}
+// b as the TMA takes it, in the workspace where it is not yet
+int pad_b(ProductArgs* p, int8_t** ws, cudaStream_t st) {
+    if (rows_fit(p->b, p->n, p->ldb))
+        return ST_SUCCESS;
+    const int rc = launch_pad_rows(p->b, p->ldb, p->n, p->k, *ws, padded(p->k), st);
+    p->b = *ws, p->ldb = padded(p->k);
+    *ws += padded_bytes(p->n, p->k);
+    return rc;
+}
+
 int check_moe(const mb200_moe_param* p) {
     if (!p)
         return set_error(ST_NULL_PTR, "moe_s8: parameter block is NULL");
@@ -92,8 +131,9 @@ int mb200_quantize_rows_s8(
 
 size_t mb200_matmul_s8_scaled_workspace_bytes(
         int m, int n, int k, const int8_t* a, long long lda, const int8_t* b_packed) {
-    (void)m, (void)n, (void)k, (void)a, (void)lda, (void)b_packed;
-    return 0;
+    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || streams(m))
+        return 0;
+    return (rows_fit(a, m, lda) ? 0 : padded_bytes(m, k)) + (rows_fit(b_packed, n, k) ? 0 : padded_bytes(n, k));
 }
 
 int mb200_matmul_s8_scaled(
@@ -114,20 +154,37 @@ int mb200_matmul_s8_scaled(
         return set_error(ST_INVALID_LAYOUT, "matmul_s8_scaled: rows of the left operand overlap");
     if (misaligned(a_scales, 4))
         return set_error(ST_INVALID_LAYOUT, "matmul_s8_scaled: scales must be 4-byte aligned");
-    (void)workspace, (void)workspace_bytes;
+    rc = check_workspace("matmul_s8_scaled", workspace, workspace_bytes,
+                         mb200_matmul_s8_scaled_workspace_bytes(m, n, k, a, lda, b_packed));
+    if (rc)
+        return rc;
     cudaStream_t st = (cudaStream_t)stream;
     ProductArgs p{};
     p.m = m, p.n = n, p.k = k;
     p.a = a, p.x_dtype = -1, p.lda = lda;
-    p.b = b_packed, p.sa = a_scales, p.sb = b_scales, p.bias = bias;
+    p.b = b_packed, p.ldb = k, p.sa = a_scales, p.sb = b_scales, p.bias = bias;
     p.c = c, p.c_dtype = dtype, p.ldc = ldc;
-    p.b_early = may_read_early(b_packed, (size_t)n * k, st);
-    return launch_product_stream(p, st);
+    if (streams(m)) {
+        p.b_early = may_read_early(b_packed, (size_t)n * k, st);
+        return launch_product_stream(p, st);
+    }
+    int8_t* ws = (int8_t*)workspace;
+    rc = pad_b(&p, &ws, st);
+    if (!rc && !rows_fit(a, m, lda)) {
+        rc = launch_pad_rows(a, lda, m, k, ws, padded(k), st);
+        p.a = ws, p.lda = padded(k);
+    }
+    if (rc)
+        return rc;
+    p.b_early = may_read_early(p.b, (size_t)n * (size_t)p.ldb, st);
+    return launch_product_umma(p, st);
 }
 
 size_t mb200_linear_s8_workspace_bytes(int m, int n, int k, const int8_t* b_packed) {
-    (void)m, (void)n, (void)k, (void)b_packed;
-    return 0;
+    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || streams_activations(m))
+        return 0;
+    return padded_bytes(m, k) + align_up((size_t)m * 4, 256) +
+           (streams(m) || rows_fit(b_packed, n, k) ? 0 : padded_bytes(n, k));
 }
 
 int mb200_linear_s8(
@@ -148,15 +205,33 @@ int mb200_linear_s8(
         return set_error(ST_INVALID_LAYOUT, "linear_s8: rows of the activations overlap");
     if (misaligned(x, dtype_bytes(dtype)))
         return set_error(ST_INVALID_LAYOUT, "linear_s8: activations must be aligned as their type is");
-    (void)workspace, (void)workspace_bytes;
+    rc = check_workspace("linear_s8", workspace, workspace_bytes,
+                         mb200_linear_s8_workspace_bytes(m, n, k, b_packed));
+    if (rc)
+        return rc;
     cudaStream_t st = (cudaStream_t)stream;
     ProductArgs p{};
     p.m = m, p.n = n, p.k = k;
     p.a = x, p.x_dtype = dtype, p.lda = ldx;
-    p.b = b_packed, p.sb = b_scales, p.bias = bias;
+    p.b = b_packed, p.ldb = k, p.sb = b_scales, p.bias = bias;
     p.c = y, p.c_dtype = dtype, p.ldc = ldy;
-    p.b_early = may_read_early(b_packed, (size_t)n * k, st);
-    return launch_product_stream(p, st);
+    if (streams_activations(m)) {
+        p.b_early = may_read_early(b_packed, (size_t)n * k, st);
+        return launch_product_stream(p, st);
+    }
+    int8_t* ws = (int8_t*)workspace;
+    if (!streams(m)) {
+        rc = pad_b(&p, &ws, st);
+        if (rc)
+            return rc;
+    }
+    float* scales = (float*)(ws + padded_bytes(m, k));
+    rc = launch_quantize_rows(x, dtype, m, k, ldx, ws, padded(k), scales, st);
+    if (rc)
+        return rc;
+    p.a = ws, p.x_dtype = -1, p.lda = padded(k), p.sa = scales;
+    p.b_early = may_read_early(p.b, (size_t)n * (size_t)p.ldb, st);
+    return streams(m) ? launch_product_stream(p, st) : launch_product_umma(p, st);
 }
 
 size_t mb200_moe_s8_workspace_bytes(const mb200_moe_param* p) {

@@ -247,6 +247,7 @@ struct ProductArgs {
     int x_dtype;    // -1: int8
     long long lda;  // elements
     const int8_t* b;
+    long long ldb;
     const float *sa, *sb, *bias;
     void* c;
     int c_dtype;
@@ -258,7 +259,13 @@ struct ProductArgs {
 int launch_quantize_rows(
         const void* x, int dtype, int m, int k, long long ldx, int8_t* q, long long ldq, float* scales,
         cudaStream_t st);
+// for any operands, made for few rows of a; activations as they are (x_dtype >= 0) for 16 rows at most
 int launch_product_stream(const ProductArgs& a, cudaStream_t st);
+// the tensor-core kernels: int8 operands, 16-byte aligned, rows whole 16-byte units apart
+int launch_product_umma(const ProductArgs& a, cudaStream_t st);
+// rows of any alignment to rows `pitch` bytes apart (a multiple of 16, at least k), zeros behind each
+int launch_pad_rows(
+        const int8_t* src, long long ld, int rows, int k, int8_t* dst, long long pitch, cudaStream_t st);
 
 }  // namespace scaled
 }  // namespace mb200

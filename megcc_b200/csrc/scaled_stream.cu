@@ -86,7 +86,11 @@ int quantize_rows(
     constexpr int N = Vec<T>::N;
     const int vector_loads = ((uintptr_t)x & 15) == 0 && (m == 1 || ldx % N == 0);
     const int word_stores = ((uintptr_t)q & (N - 1)) == 0 && (m == 1 || ldq % N == 0);
-    const Writes writes{q, (size_t)(m - 1) * (size_t)ldq + (size_t)k};
+    // (numbers and scales, and what lies between them)
+    const uintptr_t q0 = (uintptr_t)q, q1 = q0 + (size_t)(m - 1) * (size_t)ldq + (size_t)k;
+    const uintptr_t s0 = (uintptr_t)scales, s1 = s0 + (size_t)m * 4;
+    const uintptr_t w0 = q0 < s0 ? q0 : s0, w1 = q1 > s1 ? q1 : s1;
+    const Writes writes{(const void*)w0, w1 - w0};
     cudaError_t e;
     if (k <= 32 * kHeld * N && m > 1)
         e = launch_pdl(writes, quantize_rows_kernel<T, 32>, dim3((unsigned)((m - 1) / 8 + 1)),
@@ -124,8 +128,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT <= 2 ? 2 : 1) product_stream_k
     const int m0 = blockIdx.y * kCols;
     const int k = p.k, chunks = (k + 63) >> 6;
     const int row_lo = n0 + g, row_hi = n0 + g + 8;
-    const int8_t* b_lo = p.b + (size_t)min(row_lo, p.n - 1) * k;
-    const int8_t* b_hi = p.b + (size_t)min(row_hi, p.n - 1) * k;
+    const int8_t* b_lo = p.b + (size_t)min(row_lo, p.n - 1) * p.ldb;
+    const int8_t* b_hi = p.b + (size_t)min(row_hi, p.n - 1) * p.ldb;
 
     uint4 w[U][2];
     auto load_weights = [&](int c0) {
@@ -254,6 +258,16 @@ __global__ void __launch_bounds__(32 * kWarps, NT <= 2 ? 2 : 1) product_stream_k
     }
 }
 
+__global__ void __launch_bounds__(256) pad_rows_kernel(
+        const int8_t* __restrict__ src, long long ld, int k, int8_t* __restrict__ dst, int units, long long total) {
+    pdl_start();
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const long long row = i / units;
+        const int at = (int)(i - row * units) * 16;
+        ((uint4*)dst)[i] = ld_any16(src + row * ld + at, k - at);
+    }
+}
+
 template <class XT, int NT>
 cudaError_t launch_stream(const ProductArgs& a, bool aligned, int x_vectors, cudaStream_t st) {
     const dim3 grid((unsigned)((a.n - 1) / kRows + 1), (unsigned)((a.m - 1) / (8 * NT) + 1));
@@ -284,8 +298,20 @@ int launch_quantize_rows(
     return quantize_rows((const __nv_bfloat16*)x, m, k, ldx, q, ldq, scales, st);
 }
 
+int launch_pad_rows(
+        const int8_t* src, long long ld, int rows, int k, int8_t* dst, long long pitch, cudaStream_t st) {
+    const int units = (int)(pitch / 16);
+    const long long total = (long long)rows * units, ctas = (total + 255) / 256;
+    const cudaError_t e = launch_pdl(
+            Writes{dst, (size_t)total * 16}, pad_rows_kernel, dim3((unsigned)(ctas < 4736 ? ctas : 4736)), dim3(256), 0,
+            st, src, ld, k, dst, units, total);
+    if (e != cudaSuccess)
+        return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
+    return check_launch("matmul_s8_scaled");
+}
+
 int launch_product_stream(const ProductArgs& a, cudaStream_t st) {
-    const bool b_aligned = ((uintptr_t)a.b & 15) == 0 && a.k % 16 == 0;
+    const bool b_aligned = ((uintptr_t)a.b & 15) == 0 && (a.n == 1 || a.ldb % 16 == 0) && a.k % 16 == 0;
     cudaError_t e;
     if (a.x_dtype < 0) {
         const bool aligned = b_aligned && ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % 16 == 0);

@@ -1,0 +1,779 @@
+// int8 products with a scale per row and per output channel on the tensor cores (tcgen05.mma kind::i8).
+//
+// Both operands are K-major, 128 bytes of K per pipeline stage, brought by tiled TMA loads with the
+// 128-byte swizzle; sums stay exact in int32 in tensor memory. The epilogue multiplies by the two scales in
+// fp32, adds the bias, rounds once and turns the tile round in shared memory so that a warp stores whole
+// 128-byte lines.
+//
+// Two kernels:
+//   pair   256 x 256 tiles on pairs of SMs (cta_group::2), persistent, two accumulator buffers. What bounds wide
+//          products is the SM's shared memory: per 128 bytes of K a 128 x 128 tile of one SM writes and reads 64 KB
+//          for 256 clocks of MMAs, 512 clocks at 128 B/clk; the pair's 256 x 256 the same bytes per SM
+//          for 512 clocks of MMAs.
+//   split  128 x 128 tiles, K cut over the 1, 2, 4 or 8 CTAs of a cluster where there are few tiles: there
+//          the weights' way from HBM bounds, and every SM has to take part in it. The partial sums meet in
+//          shared memory (whole numbers: in any order the same).
+#include "scaled_s8.cuh"
+#include "umma_pair.cuh"
+
+namespace mb200 {
+namespace scaled {
+
+using namespace umma;
+
+namespace {
+
+constexpr int kBM = 128;  // rows per CTA
+constexpr int kBK = 128;  // K bytes per stage
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kTileBytes = kBM * kBK;  // of either operand
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kMaxStages = 6;
+
+struct UmmaArgs {
+    int m, n, k_steps;
+    int m_tiles, n_tiles;
+    const float *sa, *sb, *bias;
+    void* c;
+    long long ldc;
+    int vector_stores;  // rows of c are whole 16-byte units
+    int b_early;
+    int a_rows;   // split: rows of A's box
+    int stages;   // split
+    int csplit;   // split: CTAs per tile
+    int* status;
+};
+
+template <class T>
+struct Out;
+template <>
+struct Out<float> {
+    static __device__ __forceinline__ uint4 unit(const float* v) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    static __device__ __forceinline__ float one(float v) {
+        return v;
+    }
+};
+template <>
+struct Out<__half> {
+    static __device__ __forceinline__ uint32_t two(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint4 unit(const float* v) {
+        return make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
+    }
+    static __device__ __forceinline__ __half one(float v) {
+        return __float2half_rn(v);
+    }
+};
+template <>
+struct Out<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t two(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint4 unit(const float* v) {
+        return make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
+    }
+    static __device__ __forceinline__ __nv_bfloat16 one(float v) {
+        return __float2bfloat16_rn(v);
+    }
+};
+
+// The scales and biases of a tile's columns, in shared memory (16-byte aligned)
+struct Columns {
+    const float *scale, *bias;  // bias: zeros where there is none
+};
+
+// 32 rows (a warp's lanes) times 128 bytes of results: from tensor memory through 4 KB of shared memory
+// to whole lines. `col`: the first column within `cols`; `taken()` is called once the sums are in registers.
+template <class T, class Taken>
+__device__ __forceinline__ void store_block(
+        uint32_t taddr, float sa, const Columns& cols, int col, bool has_bias, uint8_t* stage, int row0, int col0,
+        const UmmaArgs& p, Taken taken) {
+    constexpr int kUnit = 16 / (int)sizeof(T);  // results per 16 bytes
+    constexpr int kCols = 8 * kUnit;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < kCols / 32; ++h) {
+        uint32_t acc[32];
+        __syncwarp();
+        tmem_ld32(taddr + (uint32_t)(32 * h), acc);
+        if (h + 1 == kCols / 32)
+            taken();
+#pragma unroll
+        for (int u = 0; u < 32 / kUnit; ++u) {
+            float v[kUnit];
+#pragma unroll
+            for (int j = 0; j < kUnit; j += 4) {
+                const int at = col + 32 * h + u * kUnit + j;
+                const float4 s = *(const float4*)(cols.scale + at);
+                v[j] = scale_acc((int)acc[u * kUnit + j], sa, s.x);
+                v[j + 1] = scale_acc((int)acc[u * kUnit + j + 1], sa, s.y);
+                v[j + 2] = scale_acc((int)acc[u * kUnit + j + 2], sa, s.z);
+                v[j + 3] = scale_acc((int)acc[u * kUnit + j + 3], sa, s.w);
+                if (has_bias) {
+                    const float4 b = *(const float4*)(cols.bias + at);
+                    v[j] = __fadd_rn(v[j], b.x);
+                    v[j + 1] = __fadd_rn(v[j + 1], b.y);
+                    v[j + 2] = __fadd_rn(v[j + 2], b.z);
+                    v[j + 3] = __fadd_rn(v[j + 3], b.w);
+                }
+            }
+            // (16-byte units of a row in an order that depends on the row: no two lanes of eight share a bank)
+            const int unit = h * (32 / kUnit) + u;
+            *(uint4*)(stage + lane * 128 + ((unit ^ (lane & 7)) << 4)) = Out<T>::unit(v);
+        }
+    }
+    __syncwarp();
+    T* c = (T*)p.c;
+    if (p.vector_stores && col0 + kCols <= p.n) {
+        const int unit = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            const uint4 v = *(const uint4*)(stage + r * 128 + ((unit ^ (r & 7)) << 4));
+            if (row0 + r < p.m)
+                *(uint4*)(c + (long long)(row0 + r) * p.ldc + col0 + unit * kUnit) = v;
+        }
+    } else {
+        const int rows = min(32, p.m - row0);
+        for (int r = 0; r < rows; ++r)
+#pragma unroll
+            for (int i = 0; i < kCols; i += 32) {
+                const int j = i + lane;
+                if (col0 + j < p.n)
+                    c[(long long)(row0 + r) * p.ldc + col0 + j] =
+                            *(const T*)(stage + r * 128 + (((j / kUnit) ^ (r & 7)) << 4) + (j % kUnit) * sizeof(T));
+            }
+    }
+    __syncwarp();
+}
+
+// the epilogue warps' barrier
+__device__ __forceinline__ void epilogue_sync() {
+    asm volatile("bar.sync 1, %0;" ::"r"(32 * kEpilogueWarps) : "memory");
+}
+
+// Tiles in groups of eight rows of tiles, downwards first: what the SMs work on at one time shares its
+// operands in the L2.
+struct Tile {
+    int m, n;
+};
+__device__ __forceinline__ Tile tile_at(int i, int m_tiles, int n_tiles) {
+    constexpr int kGroup = 8;
+    const int group = i / (kGroup * n_tiles), first = group * kGroup;
+    const int rows = min(kGroup, m_tiles - first), j = i - group * kGroup * n_tiles;
+    return {first + j % rows, j / rows};
+}
+
+// ---- pairs of SMs ----
+constexpr int kPairBN = 256;
+constexpr int kPairStages = 5;
+constexpr int kPairStageOff = kPairStages * kStageBytes;           // the epilogue warps' 4 KB each
+constexpr int kPairColOff = kPairStageOff + kEpilogueWarps * 4096;  // [2][256] scales, [2][256] biases
+constexpr int kPairBarOff = kPairColOff + 4 * kPairBN * 4;
+constexpr int kPairDynamic = kPairBarOff + (2 * kPairStages + 5) * 8 + 16 + 1024;
+static_assert(kPairDynamic <= 232448, "shared memory of one SM");
+
+template <class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_pair_kernel(
+        const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const UmmaArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    // (the dynamic window starts at the same offset in both CTAs, so the aligned pointers agree)
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* col_scale = (float*)(smem + kPairColOff);
+    float* col_bias = col_scale + 2 * kPairBN;
+    uint64_t* full_bar = (uint64_t*)(smem + kPairBarOff);  // used in the leader only
+    uint64_t* empty_bar = full_bar + kPairStages;          // one set per CTA
+    uint64_t* acc_full = empty_bar + kPairStages;          // [2], one set per CTA
+    uint64_t* acc_empty = acc_full + 2;                    // [2], used in the leader only
+    uint64_t* drain_bar = acc_empty + 2;
+    uint32_t* tmem_slot = (uint32_t*)(drain_bar + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+    const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int total_tiles = p.m_tiles * p.n_tiles;
+    const int first_tile = (int)cluster_id_x(), tile_step = (int)num_clusters_x();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(&full_bar[s], 1);   // the leader's producer; both CTAs' bytes
+            mbar_init(&empty_bar[s], 1);  // one commit
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 2 * kEpilogueWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    } else if (threadIdx.x == 64) {
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+    }
+    if (warp == 1) {
+        asm volatile(
+                "tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                "r"(2 * kPairBN)
+                : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers exist before anything arrives on them
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t peer_abort = map_to_cta(smem_u32((const void*)abort_flag), rank ^ 1u);
+
+    auto give_up = [&](int code) {
+        if (!*abort_flag) {
+            *abort_flag = 1;
+            atomicExch(p.status, code);
+        }
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1) : "memory");
+    };
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs): own 128 rows of A and half of B's 256 ----------------
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            auto b_row = [&](const Tile& t) { return t.n * kPairBN + (int)rank * kBM; };
+            auto announce = [&](int stage) {
+                if (leader)
+                    mbar_expect_tx(&full_bar[stage], 2u * kStageBytes);
+            };
+            // weights of the first stages ahead of the end of the kernel in front
+            int ahead = 0;
+            if (p.b_early && first_tile < total_tiles) {
+                const Tile t = tile_at(first_tile, p.m_tiles, p.n_tiles);
+                for (; ahead < min(kPairStages, p.k_steps); ++ahead) {
+                    announce(ahead);
+                    tma_pair_load_2d(smem + ahead * kStageBytes + kTileBytes, &map_b,
+                                     map_to_cta(smem_u32(&full_bar[ahead]), 0), ahead * kBK, b_row(t));
+                }
+            }
+            pdl_start();
+            for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
+                const Tile t = tile_at(tile, p.m_tiles, p.n_tiles);
+                const int m0 = t.m * (2 * kBM) + (int)rank * kBM, n0 = b_row(t);
+                for (int it = 0; it < p.k_steps; ++it) {
+                    ok = mbar_wait_cluster(&empty_bar[s], phase ^ 1u, abort_flag);
+                    if (!ok) {
+                        give_up(ERR_PRODUCER_WAIT);
+                        break;
+                    }
+                    uint8_t* at = smem + s * kStageBytes;
+                    const uint32_t full_leader = map_to_cta(smem_u32(&full_bar[s]), 0);
+                    const bool b_there = tile == first_tile && it < ahead;
+                    if (!b_there)
+                        announce(s);
+                    tma_pair_load_2d(at, &map_a, full_leader, it * kBK, m0);
+                    if (!b_there)
+                        tma_pair_load_2d(at + kTileBytes, &map_b, full_leader, it * kBK, n0);
+                    if (++s == kPairStages) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (leader only) ----------------
+        if (leader && lane == 0) {
+            constexpr uint32_t idesc = umma_idesc_s8(2 * kBM, kPairBN);
+            int local = 0, s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            const uint64_t a0 = umma_smem_desc(smem_u32(smem), 16, 1024, 2);
+            const uint64_t b0 = umma_smem_desc(smem_u32(smem + kTileBytes), 16, 1024, 2);
+            for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step, ++local) {
+                const int buf = local & 1;
+                const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
+                // both CTAs' epilogues must have drained this accumulator buffer
+                ok = mbar_wait_cluster(&acc_empty[buf], acc_phase ^ 1u, abort_flag);
+                if (!ok) {
+                    give_up(ERR_MMA_ACC_WAIT);
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t tmem_d = tmem_base + (uint32_t)(buf * kPairBN);
+                for (int it = 0; it < p.k_steps; ++it) {
+                    ok = mbar_wait_cluster(&full_bar[s], phase, abort_flag);
+                    if (!ok) {
+                        give_up(ERR_MMA_WAIT);
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t adesc = a0 + (uint64_t)(s * (kStageBytes / 16));
+                    const uint64_t bdesc = b0 + (uint64_t)(s * (kStageBytes / 16));
+#pragma unroll
+                    for (int k = 0; k < kBK / 32; ++k)
+                        umma_pair_s8(tmem_d, adesc + k * 2, bdesc + k * 2, idesc, (it | k) != 0 ? 1u : 0u);
+                    // the stage is free in both CTAs once these MMAs retire
+                    const uint32_t e_local = smem_u32(&empty_bar[s]);
+                    umma_pair_commit(e_local);
+                    umma_pair_commit(map_to_cta(e_local, 1));
+                    if (++s == kPairStages) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (ok) {
+                    const uint32_t f_local = smem_u32(&acc_full[buf]);
+                    umma_pair_commit(f_local);
+                    umma_pair_commit(map_to_cta(f_local, 1));
+                }
+            }
+        }
+    } else {
+        // ---------------- epilogue (both CTAs): warps 2..9, tensor memory lanes 32 * (warp % 4) ----------------
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int et = (int)threadIdx.x - 64;
+        uint8_t* stage = smem + kPairStageOff + (warp - 2) * 4096;
+        int local = 0;
+        bool ok = true;
+        pdl_start();
+        for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step, ++local) {
+            const int buf = local & 1;
+            const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
+            const Tile t = tile_at(tile, p.m_tiles, p.n_tiles);
+            const int row0 = t.m * (2 * kBM) + (int)rank * kBM + q * 32, n0 = t.n * kPairBN;
+            float* scale = col_scale + buf * kPairBN;
+            float* bias = col_bias + buf * kPairBN;
+            scale[et] = n0 + et < p.n ? p.sb[n0 + et] : 0.f;
+            if (p.bias)
+                bias[et] = n0 + et < p.n ? p.bias[n0 + et] : 0.f;
+            const float sa = row0 + lane < p.m ? p.sa[row0 + lane] : 0.f;
+            epilogue_sync();
+            ok = mbar_wait_cluster(&acc_full[buf], acc_phase, abort_flag);
+            if (!ok)
+                give_up(ERR_EPILOGUE_WAIT);
+            ok = __all_sync(0xffffffffu, ok);
+            // (a warp that gave up still meets the others at the barrier in front of the next tile)
+            if (!ok) {
+                ok = true;
+                continue;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kPairBN);
+            constexpr int kCols = 128 / (int)sizeof(T);
+#pragma unroll 1
+            for (int c = half * 128; c < half * 128 + 128; c += kCols) {
+                const bool last = c + kCols == half * 128 + 128;
+                store_block<T>(taddr + (uint32_t)c, sa, Columns{scale, bias}, c, p.bias != nullptr, stage, row0,
+                               n0 + c, p, [&] {
+                                   if (last) {
+                                       // this warp's sums are in registers: one arrival on the leader's barrier
+                                       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                       __syncwarp();
+                                       if (lane == 0)
+                                           mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+                                   }
+                               });
+            }
+        }
+    }
+
+    // ---------------- teardown ----------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: let loads in flight land and MMAs retire (both bounded) before
+        // the shared memory and tensor memory are given back
+        if (warp == 1 && lane == 0 && leader) {
+            umma_pair_commit(smem_u32(drain_bar));
+            const long long t0 = clock64();
+            while (!mbar_try_wait_cluster(drain_bar, 0)) {
+                if (clock64() - t0 > kWaitCycles) {
+                    atomicExch(p.status, ERR_DRAIN_WAIT);
+                    break;
+                }
+            }
+        }
+        for (int i = 0; i < 200; ++i)
+            __nanosleep(1000);
+        __syncthreads();
+    }
+    // neither CTA may leave while the other can still reach its barriers, shared memory or accumulators
+    cluster_sync();
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * kPairBN)
+                     : "memory");
+    }
+}
+
+// ---- one tile per CTA, or per cluster ----
+constexpr int kSplitBN = 128;
+constexpr int kSplitBars = (2 * kMaxStages + 2) * 8 + 16;
+constexpr int kSplitCols = 2 * kSplitBN * 4;
+inline int split_dynamic(int stages) {
+    return stages * kStageBytes + kSplitCols + kSplitBars + 1024;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
+        const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const UmmaArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    // (the same offset in all CTAs of a cluster)
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* col_scale = (float*)(smem + p.stages * kStageBytes);
+    float* col_bias = col_scale + kSplitBN;
+    uint64_t* full_bar = (uint64_t*)(col_bias + kSplitBN);
+    uint64_t* empty_bar = full_bar + kMaxStages;
+    uint64_t* acc_full = empty_bar + kMaxStages;
+    uint64_t* drain_bar = acc_full + 1;
+    uint32_t* tmem_slot = (uint32_t*)(drain_bar + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    volatile int* never = (volatile int*)(tmem_slot + 2);
+
+    const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+    const int rank = p.csplit > 1 ? (int)cluster_rank() : 0;
+    const Tile t = tile_at((int)blockIdx.x / p.csplit, p.m_tiles, p.n_tiles);
+    const int m0 = t.m * kBM, n0 = t.n * kSplitBN;
+    const int k0 = (int)((long long)p.k_steps * rank / p.csplit);
+    const int k1 = (int)((long long)p.k_steps * (rank + 1) / p.csplit);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(drain_bar, 1);
+        *abort_flag = *never = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    } else if (threadIdx.x == 64) {
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+    }
+    if (warp == 1) {
+        asm volatile(
+                "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                "r"(kSplitBN)
+                : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+
+    auto give_up = [&](int code) {
+        if (!*abort_flag) {
+            *abort_flag = 1;
+            atomicExch(p.status, code);
+        }
+    };
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        if (lane == 0) {
+            const uint32_t bytes = (uint32_t)(p.a_rows * kBK + kTileBytes);
+            int ahead = k0;
+            if (p.b_early)
+                for (; ahead < min(k0 + p.stages, k1); ++ahead) {
+                    uint8_t* at = smem + (ahead - k0) * kStageBytes;
+                    mbar_expect_tx(&full_bar[ahead - k0], bytes);
+                    tma_load_2d(at + kTileBytes, &map_b, &full_bar[ahead - k0], ahead * kBK, n0);
+                }
+            pdl_start();
+            int s = 0;
+            uint32_t phase = 0;
+            for (int it = k0; it < k1; ++it) {
+                const bool ok = mbar_wait(&empty_bar[s], phase ^ 1u, abort_flag);
+                if (!ok) {
+                    give_up(ERR_PRODUCER_WAIT);
+                    break;
+                }
+                uint8_t* at = smem + s * kStageBytes;
+                if (it >= ahead) {
+                    mbar_expect_tx(&full_bar[s], bytes);
+                    tma_load_2d(at + kTileBytes, &map_b, &full_bar[s], it * kBK, n0);
+                }
+                tma_load_2d(at, &map_a, &full_bar[s], it * kBK, m0);
+                if (++s == p.stages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (the whole warp waits, one lane issues) ----------------
+        const uint32_t leader = elect_one() ? 1u : 0u;
+        constexpr uint32_t idesc = umma_idesc_s8(kBM, kSplitBN);
+        const uint64_t a0 = umma_smem_desc(smem_u32(smem), 16, 1024, 2);
+        const uint64_t b0 = umma_smem_desc(smem_u32(smem + kTileBytes), 16, 1024, 2);
+        const uint32_t a_hi = (uint32_t)(a0 >> 32), b_hi = (uint32_t)(b0 >> 32);
+        uint32_t a_lo = (uint32_t)a0, b_lo = (uint32_t)b0, phase = 0, acc = 0;
+        const uint32_t full_a = smem_u32(full_bar), empty_a = smem_u32(empty_bar);
+        int s = 0;
+        bool ok = true;
+        for (int it = k0; it < k1; ++it) {
+            ok = mbar_wait_u32(full_a + 8 * s, phase, abort_flag);
+            if (!ok) {
+                give_up(ERR_MMA_WAIT);
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < kBK / 32; ++k) {
+                umma_s8(leader, tmem_base, a_lo + k * 2, a_hi, b_lo + k * 2, b_hi, idesc, acc);
+                acc = 1;
+            }
+            umma_commit_if(leader, empty_a + 8 * s);
+            a_lo += kStageBytes / 16;
+            b_lo += kStageBytes / 16;
+            if (++s == p.stages) {
+                s = 0;
+                phase ^= 1u;
+                a_lo = (uint32_t)a0;
+                b_lo = (uint32_t)b0;
+            }
+        }
+        if (ok)
+            umma_commit_if(leader, smem_u32(acc_full));
+        __syncwarp();
+    } else {
+        // ---------------- epilogue ----------------
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int et = (int)threadIdx.x - 64;
+        const int row0 = m0 + q * 32;
+        pdl_start();
+        if (et < kSplitBN) {
+            col_scale[et] = n0 + et < p.n ? p.sb[n0 + et] : 0.f;
+            if (p.bias)
+                col_bias[et] = n0 + et < p.n ? p.bias[n0 + et] : 0.f;
+        }
+        const float sa = row0 + lane < p.m ? p.sa[row0 + lane] : 0.f;
+        epilogue_sync();
+        bool ok = mbar_wait(acc_full, 0, abort_flag);
+        if (!ok)
+            give_up(ERR_EPILOGUE_WAIT);
+        ok = __all_sync(0xffffffffu, ok);
+        // Behind the last MMA all loads have landed and been read: the stages are free.
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+            if (p.csplit == 1) {
+                constexpr int kCols = 128 / (int)sizeof(T);
+                uint8_t* stage = smem + (warp - 2) * 4096;
+#pragma unroll 1
+                for (int c = half * 64; c < half * 64 + 64; c += kCols)
+                    if (row0 < p.m)
+                        store_block<T>(taddr + (uint32_t)c, sa, Columns{col_scale, col_bias}, c, p.bias != nullptr,
+                                       stage, row0, n0 + c, p, [] {});
+            } else if (row0 < p.m) {
+                // the partial sums, [128 rows][32 units of four columns], units in an order by row
+                const int row = q * 32 + lane;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t acc[32];
+                    __syncwarp();
+                    tmem_ld32(taddr + (uint32_t)(half * 64 + 32 * h), acc);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int unit = (half * 2 + h) * 8 + (u ^ (lane & 7));
+                        *(uint4*)(smem + row * 512 + unit * 16) =
+                                make_uint4(acc[4 * u], acc[4 * u + 1], acc[4 * u + 2], acc[4 * u + 3]);
+                    }
+                }
+            }
+        }
+    }
+
+    if (p.csplit > 1) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2) {
+            // this CTA finishes 128 / csplit rows: a row per warp, four columns per lane
+            const int rows = kBM / p.csplit;
+            const uint32_t base = smem_u32(smem);
+            const int col = n0 + 4 * lane;
+            const float4 s = *(const float4*)(col_scale + 4 * lane);
+            const float4 b = p.bias ? *(const float4*)(col_bias + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int r = warp - 2; r < rows; r += kEpilogueWarps) {
+                const int row = rank * rows + r, m = m0 + row;
+                if (m >= p.m)
+                    break;
+                const int unit = (lane & ~7) + ((lane ^ row) & 7);
+                uint4 x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = i < p.csplit ? ld_cluster_v4(base + (uint32_t)(row * 512 + unit * 16), i)
+                                        : make_uint4(0, 0, 0, 0);
+                uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    v[0] += x[i].x;
+                    v[1] += x[i].y;
+                    v[2] += x[i].z;
+                    v[3] += x[i].w;
+                }
+                const float sa = p.sa[m];
+                float f[4] = {scale_acc((int)v[0], sa, s.x), scale_acc((int)v[1], sa, s.y),
+                              scale_acc((int)v[2], sa, s.z), scale_acc((int)v[3], sa, s.w)};
+                if (p.bias) {
+                    f[0] = __fadd_rn(f[0], b.x);
+                    f[1] = __fadd_rn(f[1], b.y);
+                    f[2] = __fadd_rn(f[2], b.z);
+                    f[3] = __fadd_rn(f[3], b.w);
+                }
+                T* c = (T*)p.c + (long long)m * p.ldc + col;
+                T o[4] = {Out<T>::one(f[0]), Out<T>::one(f[1]), Out<T>::one(f[2]), Out<T>::one(f[3])};
+                if (p.vector_stores && col + 4 <= p.n) {
+                    if (sizeof(T) == 4)
+                        *(uint4*)c = *(const uint4*)o;
+                    else
+                        *(uint2*)c = *(const uint2*)o;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < p.n)
+                            c[j] = o[j];
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();  // the others may still read this CTA's sums
+    }
+
+    // ---------------- teardown ----------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*abort_flag) {
+        if (warp == 1 && lane == 0) {
+            umma_commit(drain_bar);
+            const bool ok = mbar_wait(drain_bar, 0, never);
+            if (!ok)
+                atomicExch(p.status, ERR_DRAIN_WAIT);
+        }
+        for (int i = 0; i < 200; ++i)
+            __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kSplitBN)
+                     : "memory");
+    }
+}
+
+int encode(CUtensorMap* map, const void* p, int k, int rows, long long pitch, int box_rows) {
+    const DriverApi& api = driver_api();
+    if (!api.ok)
+        return set_error(ST_RUNTIME, "cuTensorMapEncode* entry points not found in the driver");
+    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = api.tiled(
+            map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? ST_SUCCESS : set_error(ST_RUNTIME, "cuTensorMapEncodeTiled failed: %d", (int)r);
+}
+
+// Which kernel, by the clocks of its busiest SM. A 128-byte step of K takes a 128 x 128 tile's SM 512 clocks and
+// a pair's two 560 (shared memory); in front of the first step and behind the last one stand the loads'
+// round trip and the epilogue, with a cluster's exchange where K is split.
+struct Choice {
+    bool pair;
+    int csplit;
+};
+Choice choose(const UmmaArgs& p, int sms) {
+    const long long steps = p.k_steps;
+    const long long pair_tiles = (long long)((p.m - 1) / (2 * kBM) + 1) * ((p.n - 1) / kPairBN + 1);
+    long long best = (pair_tiles + sms / 2 - 1) / (sms / 2) * steps * 560 + 6000;
+    Choice c = {true, 1};
+    const long long tiles = (long long)((p.m - 1) / kBM + 1) * ((p.n - 1) / kSplitBN + 1);
+    for (int split = 1; split <= 8; split *= 2) {
+        if (split > steps || (split > 1 && tiles * split > sms))
+            break;
+        const long long waves = (tiles * split + sms - 1) / sms;
+        const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 2500 : 1000);
+        if (t < best) {
+            best = t;
+            c = {false, split};
+        }
+    }
+    return c;
+}
+
+template <class T>
+int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t st) {
+    const int sms = sm_count();
+    const Choice choice = choose(p, sms);
+    CUtensorMap map_a, map_b;
+    cudaError_t e;
+    if (choice.pair) {
+        static KernelReady ready;
+        static ClusterCapacity capacity;
+        if (!ready.smem(product_pair_kernel<T>, kPairDynamic))
+            return check_launch("matmul_s8_scaled smem attribute");
+        p.m_tiles = (p.m - 1) / (2 * kBM) + 1;
+        p.n_tiles = (p.n - 1) / kPairBN + 1;
+        int rc = encode(&map_a, a.a, a.k, a.m, a.lda, kBM);
+        if (!rc)
+            rc = encode(&map_b, a.b, a.k, a.n, a.ldb, kBM);
+        if (rc)
+            return rc;
+        const long long total = (long long)p.m_tiles * p.n_tiles;
+        const int fit = capacity.clusters(product_pair_kernel<T>, 2, kThreads, kPairDynamic);
+        const int clusters = (int)(total < fit ? total : fit);
+        e = launch_pdl(writes, product_pair_kernel<T>, dim3((unsigned)(2 * clusters)), dim3(kThreads), kPairDynamic,
+                       st, map_a, map_b, p);
+    } else {
+        static KernelReady ready;
+        p.m_tiles = (p.m - 1) / kBM + 1;
+        p.n_tiles = (p.n - 1) / kSplitBN + 1;
+        p.csplit = choice.csplit;
+        p.a_rows = p.m >= kBM ? kBM : (p.m + 7) / 8 * 8;
+        const long long ctas = (long long)p.m_tiles * p.n_tiles * p.csplit;
+        // with more CTAs than SMs two share one: one's epilogue beside the other's loads
+        p.stages = ctas > sms ? 3 : kMaxStages;
+        if (!ready.smem(product_split_kernel<T>, split_dynamic(kMaxStages)))
+            return check_launch("matmul_s8_scaled smem attribute");
+        int rc = encode(&map_a, a.a, a.k, a.m, a.lda, p.a_rows);
+        if (!rc)
+            rc = encode(&map_b, a.b, a.k, a.n, a.ldb, kSplitBN);
+        if (rc)
+            return rc;
+        e = launch_pdl_cluster(writes, product_split_kernel<T>, dim3((unsigned)ctas), dim3(kThreads),
+                               (size_t)split_dynamic(p.stages), p.csplit, st, map_a, map_b, p);
+    }
+    if (e != cudaSuccess)
+        return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
+    return check_launch("matmul_s8_scaled");
+}
+
+}  // namespace
+
+int launch_product_umma(const ProductArgs& a, cudaStream_t st) {
+    UmmaArgs p{};
+    p.m = a.m, p.n = a.n;
+    p.k_steps = (a.k + kBK - 1) / kBK;
+    p.sa = a.sa, p.sb = a.sb, p.bias = a.bias;
+    p.c = a.c, p.ldc = a.ldc;
+    const size_t size = dtype_bytes(a.c_dtype);
+    p.vector_stores = ((uintptr_t)a.c & 15) == 0 && (a.m == 1 || (size_t)a.ldc * size % 16 == 0);
+    p.b_early = a.b_early;
+    p.status = device_status_word(st);
+    if (!p.status)
+        return ST_MALLOC;
+    const Writes writes{a.c, ((size_t)(a.m - 1) * (size_t)a.ldc + (size_t)a.n) * size};
+    return a.c_dtype == DT_F32   ? launch<float>(a, p, writes, st)
+           : a.c_dtype == DT_F16 ? launch<__half>(a, p, writes, st)
+                                 : launch<__nv_bfloat16>(a, p, writes, st);
+}
+
+}  // namespace scaled
+}  // namespace mb200
