@@ -328,7 +328,7 @@ MB200_API int mb200_linear_s8(
  * Sums of whole numbers are exact, all others in fp32, in an order that is always the same. An expert whose p is 0 (a
  * logit of -infinity masks it) adds nothing; with all logits at -infinity y[t] is 0 (a padded token); a NaN or
  * +infinity among a token's logits, or a row x[t] without a scale, makes that y[t] NaN.
- * 1 <= tokens <= 64, top_k <= 16 and <= experts <= 512, f <= 131071, d <= 20480 (10240 with more than 8 tokens):
+ * 1 <= tokens <= 64, top_k <= 16 and <= experts <= 512, f <= 131071, d <= 16384 (8192 with more than 8 tokens):
  * beyond them TinyNN_ERROR_OUT_OF_RANGE; tokens == 0 does nothing. ldx, ldy: elements from row to row.
  * workspace: mb200_moe_s8_workspace_bytes(p) bytes of device memory, 256-byte aligned, whose content does not
  * matter; two calls that may run at the same time need one each. */

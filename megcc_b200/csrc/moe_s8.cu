@@ -11,11 +11,11 @@
 // lets the CTA that made 32 hidden units finish them: nothing has to wait for the maximum over all of f.
 //
 // HBM: the chosen experts' weights, 3 * d * f bytes each, are read once and everything else is small, so
-// both kernels are mma.sync loops that take weights straight from global memory into registers, 16 (8)
-// neighbouring bytes per thread, with loads running ahead over the ends of rows, experts and tiles.
+// both kernels stream them through rings of asynchronous copies into mma.sync (stream_s8.cuh), over the ends of
+// rows, experts and tiles.
 // Every CTA of either kernel works the routing out for itself: it is a few thousand logits.
 #include "moe_s8.h"
-#include "scaled_s8.cuh"
+#include "stream_s8.cuh"
 #include "umma_ptx.cuh"
 
 namespace mb200 {
@@ -24,20 +24,49 @@ namespace scaled {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kMaxSlots = kMoeMaxTokens * kMoeMaxTop;
 constexpr int kUnits = 32;            // hidden units per tile of the first kernel, and per group of h
 constexpr int kPitch = 2 * kUnits + 4;  // ints per token in its exchange: 2 * 68 = 8 banks apart
 constexpr int kRows = 16;             // rows of w2 per CTA of the second kernel
 
+// Where the tokens go, in shared memory: as large as the call's tokens and experts ask for.
 struct Route {
-    float p[kMaxSlots];        // by slot = token * top + rank
-    short expert[kMaxSlots];   // -1: no share in the result
-    short order[kMaxSlots];    // slots by expert
-    short count[kMoeMaxExperts], start[kMoeMaxExperts];
+    float* p;          // by slot = token * top + rank
+    short* expert;     // -1: no share in the result
+    short* order;      // slots by expert
+    int *count, *at;   // by expert: its slots, and where the next one goes
     // the passes: an expert and up to `cols` of its slots
-    short pass_expert[kMoeMaxPasses], pass_start[kMoeMaxPasses], pass_cols[kMoeMaxPasses];
-    int passes;
+    short *pass_expert, *pass_start, *pass_cols;
+    int* passes;
 };
+__host__ __device__ constexpr int up16(int v) {
+    return (v + 15) / 16 * 16;
+}
+// every expert with tokens, and one more for each `cols` slots
+__host__ __device__ constexpr int most_passes(int slots, int experts, int cols) {
+    return (slots < experts ? slots : experts) + slots / cols;
+}
+__host__ __device__ constexpr int route_bytes(int slots, int experts, int cols) {
+    return up16(4 * slots) + 2 * up16(2 * slots) + 2 * up16(4 * experts) + 3 * up16(2 * most_passes(slots, experts, cols)) + 16;
+}
+__device__ __forceinline__ Route place_route(uint8_t* at, int slots, int experts, int cols) {
+    Route r;
+    r.p = (float*)at;
+    at += up16(4 * slots);
+    r.expert = (short*)at;
+    at += up16(2 * slots);
+    r.order = (short*)at;
+    at += up16(2 * slots);
+    r.count = (int*)at;
+    at += up16(4 * experts);
+    r.at = (int*)at;
+    at += up16(4 * experts);
+    const int n = up16(2 * most_passes(slots, experts, cols));
+    r.pass_expert = (short*)at;
+    r.pass_start = (short*)(at + n);
+    r.pass_cols = (short*)(at + 2 * n);
+    r.passes = (int*)(at + 3 * n);
+    return r;
+}
 
 // A float's bits in the order of the values: NaN lowest, then -infinity; 0 is nobody's
 __device__ __forceinline__ uint32_t rank_key(float v) {
@@ -46,12 +75,10 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
 }
 
 // A warp per token in turn; then the slots by expert, cut into passes of at most `cols`.
-__device__ void route_tokens(const MoeArgs& a, int cols, Route& r) {
+__device__ void route_tokens(const MoeArgs& a, int cols, const Route& r) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int e = threadIdx.x; e < a.e; e += kThreads)
         r.count[e] = 0;
-    if (threadIdx.x == 0)
-        r.passes = 0;
     constexpr int R = kMoeMaxExperts / 32;
     for (int t = warp; t < a.t; t += kWarps) {
         const float* row = a.logits + (size_t)t * a.e;
@@ -122,14 +149,10 @@ __device__ void route_tokens(const MoeArgs& a, int cols, Route& r) {
         }
     }
     __syncthreads();
-    // slots per expert: whole numbers, their order does not matter; one thread counts an expert's
     const int slots = a.t * a.top;
-    for (int e = threadIdx.x; e < a.e; e += kThreads) {
-        int n = 0;
-        for (int s = 0; s < slots; ++s)
-            n += r.expert[s] == e;
-        r.count[e] = (short)n;
-    }
+    for (int s = threadIdx.x; s < slots; s += kThreads)
+        if (r.expert[s] >= 0)
+            atomicAdd(&r.count[r.expert[s]], 1);
     __syncthreads();
     if (warp == 0) {
         int start = 0, passes = 0;
@@ -146,136 +169,129 @@ __device__ void route_tokens(const MoeArgs& a, int cols, Route& r) {
                 }
             }
             if (e < a.e)
-                r.start[e] = (short)(start + s - n);
+                r.at[e] = start + s - n;
             for (int i = 0; i < np; ++i) {
-                const int at = passes + q - np + i;
-                r.pass_expert[at] = (short)e;
-                r.pass_start[at] = (short)(start + s - n + i * cols);
-                r.pass_cols[at] = (short)min(cols, n - i * cols);
+                const int to = passes + q - np + i;
+                r.pass_expert[to] = (short)e;
+                r.pass_start[to] = (short)(start + s - n + i * cols);
+                r.pass_cols[to] = (short)min(cols, n - i * cols);
             }
             start += __shfl_sync(0xffffffffu, s, 31);
             passes += __shfl_sync(0xffffffffu, q, 31);
         }
         if (lane == 0)
-            r.passes = passes;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.e; e += kThreads) {
-        int at = r.start[e];
-        if (r.count[e])
-            for (int s = 0; s < slots; ++s)
-                if (r.expert[s] == e)
-                    r.order[at++] = (short)s;
-    }
-    __syncthreads();
-}
-
-// `cols` rows of x as whole numbers in shared memory, a warp per row
-template <class T>
-__device__ void quantize_tokens(
-        const MoeArgs& a, const short* order, int top, int cols, int8_t* xs, int pitch, float* scale,
-        int x_vectors) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int c = warp; c < cols; c += kWarps) {
-        const int t = order ? order[c] / top : c;
-        const T* row = (const T*)a.x + (long long)t * a.ldx;
-        uint32_t bits = 0;
-        for (int i = lane * 16; i < a.d; i += 512) {
-            float v[16];
-            load_piece(row, i, a.d, x_vectors, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                bits = max(bits, magnitude(v[j]));
-        }
-        const RowScale r = row_scale(__reduce_max_sync(0xffffffffu, bits));
-        if (lane == 0)
-            scale[c] = r.scale;
-        for (int i = lane * 16; i < a.d; i += 512) {
-            float v[16];
-            load_piece(row, i, a.d, x_vectors, v);
-            *(uint4*)(xs + c * pitch + i) = pack_piece(v, r);
+            *r.passes = passes;
+        __syncwarp();
+        // An expert's slots in ascending order: every CTA must cut them into the same passes.
+        for (int s0 = 0; s0 < slots; s0 += 32) {
+            const int s = s0 + lane, e = s < slots ? r.expert[s] : -1;
+            const uint32_t alike = __match_any_sync(0xffffffffu, e);
+            const int to = e >= 0 ? r.at[e] : 0, before = __popc(alike & ((1u << lane) - 1u));
+            __syncwarp();
+            if (e >= 0) {
+                r.order[to + before] = (short)s;
+                if (before == 0)
+                    r.at[e] = to + __popc(alike);
+            }
+            __syncwarp();
         }
     }
+    __syncthreads();
 }
 
 // ---- gate, up, activation, and h as whole numbers ----
-// Tiles of 32 hidden units (64 rows of w1), a tile per pass of its expert; a CTA takes neighbouring ones. Its
-// warps take the 64-byte chunks of d in turn. COLS tokens at once; with no more tokens than that all of them
-// stay in shared memory for the whole kernel.
+// Tiles of 32 hidden units (64 rows of w1), once per pass of their expert; a CTA takes neighbouring ones. Four
+// of its eight warps have 16 rows each (gate, gate, up, up) and every other step of d, the other four the same rows
+// and the remaining steps; each warp's ring runs on over the ends of tiles. COLS tokens at once; with no more
+// tokens than that all of them stay in shared memory for the whole kernel.
+template <int COLS, bool ALIGNED>
+struct Up {
+    static constexpr int kDepth = COLS == 8 || ALIGNED ? 4 : 3;
+    static constexpr int kHalves = 2;  // warps that share a tile's steps
+    typedef Rows<16, ALIGNED> W;
+    static constexpr int kRing = kWarps * kDepth * W::kBytes;
+    static constexpr int kExchange = kHalves * COLS * kPitch;  // ints; two of them, used in turn
+    static int smem(const MoeArgs& a) {
+        return kRing + 2 * kExchange * 4 + (a.t < COLS ? a.t : COLS) * xs_pitch(a.d) +
+               route_bytes(a.t * a.top, a.e, COLS);
+    }
+};
+
 template <class T, int COLS, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, int pitch, int x_vectors) {
-    constexpr int NT = COLS / 8;
-    extern __shared__ __align__(16) uint8_t dynamic[];
-    int* red = (int*)dynamic;                                    // [kWarps][COLS][kPitch]
-    int8_t* xs = (int8_t*)(dynamic + kWarps * COLS * kPitch * 4);  // [COLS][pitch]
-    __shared__ Route route;
+__global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, int x_vectors) {
+    typedef Up<COLS, ALIGNED> U;
+    constexpr int NT = COLS / 8, kDepth = U::kDepth;
+    extern __shared__ __align__(128) uint8_t dynamic[];
+    int* exchange = (int*)(dynamic + U::kRing);
+    int8_t* xs = (int8_t*)(exchange + 2 * U::kExchange);
+    const int pitch = xs_pitch(a.d);
+    const Route route = place_route((uint8_t*)xs + min(a.t, COLS) * pitch, a.t * a.top, a.e, COLS);
     __shared__ float x_scale[COLS];
+    __shared__ uint32_t part[16 * kWarps];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
-    pdl_start();
-    route_tokens(a, COLS, route);
     const bool resident = a.t <= COLS;
+    pdl_start();
+    if (resident)  // (the tokens arrive while the routing is worked out)
+        for (int t = 0; t < a.t; ++t)
+            ask_ahead<kThreads>((const T*)a.x + (long long)t * a.ldx, a.d * sizeof(T));
+    route_tokens(a, COLS, route);
     const int blocks = (a.f + kUnits - 1) / kUnits;
-    const long long tiles = (long long)route.passes * blocks;
+    const long long tiles = (long long)*route.passes * blocks;
     const int first = (int)(tiles * blockIdx.x / gridDim.x), last = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
     if (first == last)
         return;
-    const int chunks = (a.d + 63) >> 6;
-    const int mine = warp < chunks ? (chunks - warp + kWarps - 1) / kWarps : 0;  // chunks of this warp
+    const int steps = (a.d + kStep - 1) / kStep;
+    const int half = warp >> 2;                        // steps half, half + 2, ...
+    const int mine = (steps - half + 1) / U::kHalves;  // (none where there is one step only)
+    const uint32_t ring = shared_address(dynamic) + (uint32_t)(warp * kDepth * U::W::kBytes);
 
-    // loads run one chunk ahead of the MMAs, over the ends of tiles
-    uint4 w[2][8];
-    int l_tile = first, l_chunk = 0;
-    const int8_t* l_row[8];
-    auto open_tile = [&](int tile) {
-        const int e = route.pass_expert[tile / blocks], u0 = tile % blocks * kUnits;
-        const int8_t* w1 = a.w1 + (size_t)e * (2 * (size_t)a.f) * a.d;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int u = min(u0 + 8 * i + g, a.f - 1);
-            l_row[i] = w1 + (size_t)u * a.d;
-            l_row[4 + i] = w1 + ((size_t)a.f + u) * a.d;
-        }
+    // row r of this warp's 16 in a tile: block of 32 units `b` of a pass
+    const int block = warp & 3;
+    auto tile_row = [&](int pass, int b, int r) {
+        const int u = min(b * kUnits + (block & 1) * 16 + r, a.f - 1);
+        return a.w1 + ((size_t)route.pass_expert[pass] * 2 * a.f + (block >> 1) * (size_t)a.f + u) * (size_t)a.d;
     };
-    auto load_next = [&](uint4 (&v)[8]) {
-        if (l_tile >= last)
-            return;
-        const int kk = (warp + l_chunk * kWarps) * 64 + tig * 16;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (ALIGNED)
-                v[i] = kk < a.d ? ld_stream16(l_row[i] + kk) : make_uint4(0, 0, 0, 0);
-            else
-                v[i] = ld_any16(l_row[i] + kk, a.d - kk);
+    typename U::W w;
+    int l_tile = first, l_pass = first / blocks, l_block = first - l_pass * blocks, l_step = 0, stage_in = 0;
+    auto copy_next = [&] {
+        if (mine && l_tile < last) {
+            if (l_step == 0)
+                w.open([&](int r) { return tile_row(l_pass, l_block, r); }, a.d, half);
+            w.copy(ring + (uint32_t)(stage_in * U::W::kBytes), U::kHalves);
+            if (++l_step == mine) {
+                l_step = 0;
+                ++l_tile;
+                if (++l_block == blocks) {
+                    l_block = 0;
+                    ++l_pass;
+                }
+            }
         }
-        if (++l_chunk == mine) {
-            l_chunk = 0;
-            if (++l_tile < last)
-                open_tile(l_tile);
-        }
+        if (++stage_in == kDepth)
+            stage_in = 0;
+        copy_commit();
     };
-    if (mine) {
-        open_tile(first);
-        load_next(w[0]);
-    }
+    for (int i = 0; i < kDepth - 1; ++i)
+        copy_next();
+    auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
     if (resident)
-        quantize_tokens<T>(a, nullptr, 1, a.t, xs, pitch, x_scale, x_vectors);
+        quantize_cta<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
     __syncthreads();
 
-    int pass = -1, cols = 0, e = 0;
+    int pass = first / blocks, b = first - pass * blocks, cols = 0, e = 0, stage_out = 0;
     const short* order = nullptr;
-    int buf = 0;
     for (int tile = first; tile < last; ++tile) {
-        const int u0 = tile % blocks * kUnits;
-        if (tile / blocks != pass) {
-            pass = tile / blocks;
+        const int u0 = b * kUnits;
+        if (b == 0 || tile == first) {
             e = route.pass_expert[pass];
             cols = route.pass_cols[pass];
             order = route.order + route.pass_start[pass];
             if (!resident) {
                 __syncthreads();  // (the last pass's tokens have been read)
-                quantize_tokens<T>(a, order, a.top, cols, xs, pitch, x_scale, x_vectors);
+                quantize_cta<T, kWarps>([&](int c) { return token_row(order[c] / a.top); }, cols, a.d, xs, pitch,
+                                        x_scale, part, x_vectors);
                 __syncthreads();
             }
         }
@@ -289,47 +305,40 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
             const int c = min(8 * nt + g, cols - 1);
             frag[nt] = xs + (resident ? order[c] / a.top : c) * pitch + tig * 16;
         }
-        int acc[4][NT][4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                acc[b][nt][0] = acc[b][nt][1] = acc[b][nt][2] = acc[b][nt][3] = 0;
-        auto multiply = [&](const uint4 (&v)[8], int c) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const uint4 x = *(const uint4*)(frag[nt] + (warp + c * kWarps) * 64);
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    mma_64(acc[b][nt], v[2 * b], v[2 * b + 1], x);
-            }
-        };
-        for (int c = 0; c < mine; ++c) {
-            if (buf == 0) {
-                load_next(w[1]);
-                multiply(w[0], c);
-            } else {
-                load_next(w[0]);
-                multiply(w[1], c);
-            }
-            buf ^= 1;
-        }
+        const int s_lo = (int)((uintptr_t)tile_row(pass, b, g) & 15), s_hi = (int)((uintptr_t)tile_row(pass, b, g + 8) & 15);
+        int acc[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
+            acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
+        for (int i = 0; i < mine; ++i) {
+            copy_wait<kDepth - 2>();
+            __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
+            copy_next();
+            const uint32_t stage = ring + (uint32_t)(stage_out * U::W::kBytes);
+            if (++stage_out == kDepth)
+                stage_out = 0;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                // units 16 * (b % 2) + g and + 8; gate in front, up behind
-                int* at = red + (warp * COLS + 8 * nt + 2 * tig) * kPitch + (b >> 1) * kUnits + 16 * (b & 1) + g;
-                at[0] = acc[b][nt][0];
-                at[kPitch] = acc[b][nt][1];
-                at[8] = acc[b][nt][2];
-                at[kPitch + 8] = acc[b][nt][3];
+            for (int j = 0; j < kStep / 64; ++j) {
+                const uint4 lo = U::W::piece16(stage, g, 4 * j + tig, s_lo), hi = U::W::piece16(stage, g + 8, 4 * j + tig, s_hi);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_64(acc[nt], lo, hi, *(const uint4*)(frag[nt] + (half + i * U::kHalves) * kStep + 64 * j));
             }
-        __syncthreads();
+        }
+        int* red = exchange + (tile & 1) * U::kExchange;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            int* at = red + (half * COLS + 8 * nt + 2 * tig) * kPitch + block * 16 + g;
+            at[0] = acc[nt][0];
+            at[kPitch] = acc[nt][1];
+            at[8] = acc[nt][2];
+            at[kPitch + 8] = acc[nt][3];
+        }
+        __syncthreads();  // (the other exchange's readers are past their reading when this one is passed again)
         for (int c = warp; c < cols; c += kWarps) {
             int gate = 0, up = 0;
 #pragma unroll
-            for (int i = 0; i < kWarps; ++i) {
+            for (int i = 0; i < U::kHalves; ++i) {
                 gate += red[(i * COLS + c) * kPitch + lane];
                 up += red[(i * COLS + c) * kPitch + kUnits + lane];
             }
@@ -340,130 +349,174 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
             const RowScale r = row_scale(__reduce_max_sync(0xffffffffu, magnitude(h)));
             a.hq[(size_t)slot * (blocks * kUnits) + u] = (int8_t)(to_whole(h, r.inv) & r.keep);
             if (lane == 0)
-                a.sh[(size_t)slot * blocks + u0 / kUnits] = r.scale;
+                a.sh[(size_t)slot * blocks + b] = r.scale;
         }
-        __syncthreads();
+        if (++b == blocks) {
+            b = 0;
+            ++pass;
+        }
     }
 }
 
 // ---- down, and the experts' sum ----
-// A CTA makes 16 rows of every token: its warps take the groups of f in turn, expert after expert in the
-// order of their indices, and add into sums of their own, which meet at the end in the order of the warps:
-// no atomics, the same bits every time.
-template <class T, bool ALIGNED>
+// A CTA makes 16 rows of every token. All its steps, pass after pass in the order of the experts' indices, are one
+// sequence, of which each warp takes an eighth; it adds into sums of its own, which meet at the end in
+// the order of the warps: no float atomics, the same bits every time. (Neighbouring steps for each warp: with every
+// eighth step each warp would open every pass.)
+template <int NT, bool ALIGNED>
+struct Down {
+    static constexpr int kDepth = 4;
+    typedef Rows<kRows, ALIGNED> W;
+    typedef Rows<8 * NT, true> H;
+    static constexpr int kGroups = kStep / kUnits;
+    static constexpr int kScales = kGroups * 8 * NT * 4;
+    static constexpr int kStage = W::kBytes + H::kBytes + kScales;
+    static constexpr int kRing = kWarps * kDepth * kStage;
+    static int smem(const MoeArgs& a) {
+        return kRing + kWarps * a.t * kRows * 4 + route_bytes(a.t * a.top, a.e, 8 * NT);
+    }
+};
+
+template <int NT, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) {
-    constexpr int U = 8;  // groups in flight per warp
-    extern __shared__ __align__(16) float sums[];  // [kWarps][a.t][kRows]
-    __shared__ Route route;
+    typedef Down<NT, ALIGNED> D;
+    constexpr int kDepth = D::kDepth, kCols = 8 * NT;
+    extern __shared__ __align__(128) uint8_t dynamic[];
+    float* sums = (float*)(dynamic + D::kRing);  // [kWarps][a.t][kRows]
+    const Route route = place_route((uint8_t*)(sums + kWarps * a.t * kRows), a.t * a.top, a.e, kCols);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
     const int d0 = blockIdx.x * kRows;
     // Ahead of the first kernel's end: the routing and the first weights. What is read here was written before
     // the first kernel began, which let this one start behind its own wait for that.
-    route_tokens(a, 8, route);
+    route_tokens(a, kCols, route);
     const int groups = (a.f + kUnits - 1) / kUnits, width = groups * kUnits;
-    const int mine = warp < groups ? (groups - warp + kWarps - 1) / kWarps : 0;
-    const int steps = mine * route.passes;
+    const int steps = (a.f + kStep - 1) / kStep;  // of a pass
+    const int total = steps * *route.passes;
+    const int first = (int)((long long)total * warp / kWarps), mine = (int)((long long)total * (warp + 1) / kWarps) - first;
     float* own = sums + warp * a.t * kRows;
     for (int i = lane; i < a.t * kRows; i += 32)
         own[i] = 0.f;
-    __syncwarp();
+    const uint32_t ring = shared_address(dynamic) + (uint32_t)(warp * kDepth * D::kStage);
 
-    const int row_lo = min(d0 + g, a.d - 1), row_hi = min(d0 + g + 8, a.d - 1);
-    uint2 w[U][2], hq[U];
-    float sh[U][2];
-    // where the loads are: weights, and what the first kernel writes
-    int wp = 0, wu = 0, hp = 0, hu = 0;
-    const int8_t *w_lo = nullptr, *w_hi = nullptr;
-    const int8_t* h_row = nullptr;
-    const float *sh0 = nullptr, *sh1 = nullptr;
-    auto load_weights = [&](uint2 (&v)[2]) {
-        if (wu == 0) {
-            const int8_t* w2 = a.w2 + (size_t)route.pass_expert[wp] * a.d * a.f;
-            w_lo = w2 + (size_t)row_lo * a.f;
-            w_hi = w2 + (size_t)row_hi * a.f;
-        }
-        const int kk = (warp + wu * kWarps) * kUnits + tig * 8;
-        if (ALIGNED) {
-            v[0] = kk < a.f ? ld_stream8(w_lo + kk) : make_uint2(0, 0);
-            v[1] = kk < a.f ? ld_stream8(w_hi + kk) : make_uint2(0, 0);
-        } else {
-            v[0] = ld_any8(w_lo + kk, a.f - kk);
-            v[1] = ld_any8(w_hi + kk, a.f - kk);
-        }
-        if (++wu == mine) {
-            wu = 0;
-            ++wp;
-        }
+    // A place in the sequence of this warp's steps
+    struct At {
+        int pass, step;
     };
-    auto load_hidden = [&](uint2& q, float (&s)[2]) {
-        if (hu == 0) {
-            const short* order = route.order + route.pass_start[hp];
-            const int end = route.pass_cols[hp] - 1;
-            h_row = a.hq + (size_t)order[min(g, end)] * width;
-            sh0 = a.sh + (size_t)order[min(2 * tig, end)] * groups;
-            sh1 = a.sh + (size_t)order[min(2 * tig + 1, end)] * groups;
-        }
-        const int group = warp + hu * kWarps;
-        q = *(const uint2*)(h_row + group * kUnits + tig * 8);
-        s[0] = sh0[group];
-        s[1] = sh1[group];
-        if (++hu == mine) {
-            hu = 0;
-            ++hp;
-        }
+    auto advance = [&](At& at) {  // is it a pass's first step?
+        if (++at.step < steps)
+            return false;
+        at.step = 0;
+        ++at.pass;
+        return true;
     };
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-        if (i < steps)
-            load_weights(w[i]);
-    pdl_start();
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-        if (i < steps)
-            load_hidden(hq[i], sh[i]);
-
-    int pass = 0, u = 0;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    float s_lo = 0.f, s_hi = 0.f;
-    for (int step = 0; step < steps; step += U) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (step + i < steps) {
-                if (u == 0) {
-                    const float* s2 = a.s2 + (size_t)route.pass_expert[pass] * a.d;
-                    s_lo = s2[row_lo];
-                    s_hi = s2[row_hi];
-                }
-                int c[4] = {0, 0, 0, 0};
-                mma_16x8x32(c, w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, hq[i].x, hq[i].y);
-                acc[0] = __fmaf_rn(__int2float_rn(c[0]), sh[i][0], acc[0]);
-                acc[1] = __fmaf_rn(__int2float_rn(c[1]), sh[i][1], acc[1]);
-                acc[2] = __fmaf_rn(__int2float_rn(c[2]), sh[i][0], acc[2]);
-                acc[3] = __fmaf_rn(__int2float_rn(c[3]), sh[i][1], acc[3]);
-                if (step + i + U < steps) {
-                    load_weights(w[i]);
-                    load_hidden(hq[i], sh[i]);
-                }
-                if (++u == mine) {
-                    // this warp's share of the expert, to the sums of its tokens
-                    const short* order = route.order + route.pass_start[pass];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        if (2 * tig + j < route.pass_cols[pass]) {
-                            const int slot = order[2 * tig + j];
-                            const float p = route.p[slot];
-                            float* at = own + slot / a.top * kRows + g;
-                            at[0] = __fmaf_rn(__fmul_rn(acc[j], s_lo), p, at[0]);
-                            at[8] = __fmaf_rn(__fmul_rn(acc[2 + j], s_hi), p, at[8]);
-                        }
-                    __syncwarp();  // the next expert's lanes find them
-                    acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-                    u = 0;
-                    ++pass;
-                }
+    const At start = {first / steps, first % steps};
+    auto w2_row = [&](int pass, int r) {
+        return a.w2 + ((size_t)route.pass_expert[pass] * a.d + min(d0 + r, a.d - 1)) * (size_t)a.f;
+    };
+    typename D::W w;
+    typename D::H h;
+    const float* sh_from = nullptr;
+    At wl = start, hl = start;
+    int w_copied = 0, h_copied = 0;
+    bool w_new = true, h_new = true;
+    auto copy_weights = [&] {
+        if (w_copied < mine) {
+            if (w_new)
+                w.open([&](int r) { return w2_row(wl.pass, r); }, a.f, wl.step);
+            w.copy(ring + (uint32_t)(w_copied % kDepth * D::kStage), 1);
+            w_new = advance(wl);
+        }
+        ++w_copied;
+    };
+    auto copy_hidden = [&] {
+        if (h_copied < mine) {
+            if (h_new) {
+                const short* order = route.order + route.pass_start[hl.pass];
+                const int cols = route.pass_cols[hl.pass];
+                h.open([&](int r) { return r < cols ? a.hq + (size_t)order[r] * width : nullptr; }, width, hl.step);
+                // a lane copies the scales of a token's groups lane / kCols, and so on
+                sh_from = a.sh + (size_t)order[min(lane % kCols, cols - 1)] * groups;
             }
+            const uint32_t stage = ring + (uint32_t)(h_copied % kDepth * D::kStage + D::W::kBytes);
+            h.copy(stage, 1);
+#pragma unroll
+            for (int j = lane / kCols; j < D::kGroups; j += 32 / kCols) {
+                const int group = hl.step * D::kGroups + j;
+                copy_async4(stage + D::H::kBytes + 4 * (j * kCols + lane % kCols),
+                            group < groups ? sh_from + group : sh_from, group < groups);
+            }
+            h_new = advance(hl);
+        }
+        ++h_copied;
+        copy_commit();
+    };
+    for (int i = 0; i < kDepth - 1; ++i)
+        copy_weights();
+    pdl_start();
+    for (int i = 0; i < kDepth - 1; ++i)
+        copy_hidden();
+
+    At at = start;
+    float acc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+        acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+    float s_lo = 0.f, s_hi = 0.f;
+    int sh_lo = 0, sh_hi = 0;
+    bool fresh = true;
+    for (int i = 0; i < mine; ++i) {
+        copy_wait<kDepth - 2>();
+        __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
+        copy_weights();
+        copy_hidden();
+        if (fresh) {
+            const float* s2 = a.s2 + (size_t)route.pass_expert[at.pass] * a.d;
+            s_lo = s2[min(d0 + g, a.d - 1)];
+            s_hi = s2[min(d0 + g + 8, a.d - 1)];
+            sh_lo = (int)((uintptr_t)w2_row(at.pass, g) & 15);
+            sh_hi = (int)((uintptr_t)w2_row(at.pass, g + 8) & 15);
+        }
+        const uint32_t stage = ring + (uint32_t)(i % kDepth * D::kStage), hidden = stage + D::W::kBytes;
+#pragma unroll
+        for (int j = 0; j < D::kGroups; ++j) {
+            const uint2 lo = D::W::piece8(stage, g, 4 * j + tig, sh_lo), hi = D::W::piece8(stage, g + 8, 4 * j + tig, sh_hi);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint2 q = D::H::piece8(hidden, 8 * nt + g, 4 * j + tig, 0);
+                int c[4] = {0, 0, 0, 0};
+                mma_16x8x32(c, lo.x, hi.x, lo.y, hi.y, q.x, q.y);
+                const uint2 s = lds8(hidden + D::H::kBytes + (j * kCols + 8 * nt + 2 * tig) * 4);
+                const float s0 = __uint_as_float(s.x), s1 = __uint_as_float(s.y);
+                acc[nt][0] = __fmaf_rn(__int2float_rn(c[0]), s0, acc[nt][0]);
+                acc[nt][1] = __fmaf_rn(__int2float_rn(c[1]), s1, acc[nt][1]);
+                acc[nt][2] = __fmaf_rn(__int2float_rn(c[2]), s0, acc[nt][2]);
+                acc[nt][3] = __fmaf_rn(__int2float_rn(c[3]), s1, acc[nt][3]);
+            }
+        }
+        const int pass = at.pass;
+        fresh = advance(at);
+        if (fresh || i + 1 == mine) {
+            // this warp's share of the pass, to the sums of its tokens
+            const short* order = route.order + route.pass_start[pass];
+            const int cols = route.pass_cols[pass];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int c = 8 * nt + 2 * tig + j;
+                    if (c < cols) {
+                        const int slot = order[c];
+                        const float p = route.p[slot];
+                        float* to = own + slot / a.top * kRows + g;
+                        to[0] = __fmaf_rn(__fmul_rn(acc[nt][j], s_lo), p, to[0]);
+                        to[8] = __fmaf_rn(__fmul_rn(acc[nt][2 + j], s_hi), p, to[8]);
+                    }
+                }
+                acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+            }
+            __syncwarp();  // the next pass's lanes find them
         }
     }
     __syncthreads();
@@ -483,32 +536,45 @@ cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
     static umma::ResidentCtas resident;
     auto kernel = moe_up_kernel<T, COLS, ALIGNED>;
-    const int pitch = (a.d + 127) / 128 * 128 + 64;  // rows half of all banks apart
-    const int smem = kWarps * COLS * kPitch * 4 + COLS * pitch;
+    const int smem = Up<COLS, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx % Vec<T>::N == 0);
-    const long long slots = (long long)a.t * a.top;
-    const long long tiles = slots * ((a.f + kUnits - 1) / kUnits);  // at most
-    const long long fit = (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem + (int)sizeof(Route), 0);
+    const long long tiles = (long long)a.t * a.top * ((a.f + kUnits - 1) / kUnits);  // at most
+    const long long fit = (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0);
     const Writes writes{a.hq, a.workspace_bytes};
     return launch_pdl(writes, kernel, dim3((unsigned)(tiles < fit ? tiles : fit)), dim3(kThreads), (size_t)smem, st,
-                      a, pitch, x_vectors);
+                      a, x_vectors);
+}
+template <class T>
+cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
+    const bool aligned = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
+    if (a.t <= 8)
+        return aligned ? launch_up<T, 8, true>(a, st) : launch_up<T, 8, false>(a, st);
+    return aligned ? launch_up<T, 16, true>(a, st) : launch_up<T, 16, false>(a, st);
+}
+
+template <int NT, bool ALIGNED>
+cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
+    static umma::KernelReady ready;
+    auto kernel = moe_down_kernel<NT, ALIGNED>;
+    const int smem = Down<NT, ALIGNED>::smem(a);
+    if (!ready.smem(kernel, smem))
+        return cudaErrorInvalidValue;
+    const Writes writes{a.y, ((size_t)(a.t - 1) * (size_t)a.ldy + (size_t)a.d) * dtype_bytes(a.dtype)};
+    return launch_pdl(writes, kernel, dim3((unsigned)((a.d - 1) / kRows + 1)), dim3(kThreads), (size_t)smem, st, a);
+}
+cudaError_t launch_down(const MoeArgs& a, cudaStream_t st) {
+    const bool aligned = ((uintptr_t)a.w2 & 15) == 0 && a.f % 16 == 0;
+    if (a.t <= 8)
+        return aligned ? launch_down_as<1, true>(a, st) : launch_down_as<1, false>(a, st);
+    return aligned ? launch_down_as<2, true>(a, st) : launch_down_as<2, false>(a, st);
 }
 
 template <class T>
 cudaError_t launch_both(const MoeArgs& a, cudaStream_t st) {
-    const bool up16 = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
-    const bool down8 = ((uintptr_t)a.w2 & 7) == 0 && a.f % 8 == 0;
-    cudaError_t e = a.t <= 8 ? (up16 ? launch_up<T, 8, true>(a, st) : launch_up<T, 8, false>(a, st))
-                             : (up16 ? launch_up<T, 16, true>(a, st) : launch_up<T, 16, false>(a, st));
-    if (e != cudaSuccess)
-        return e;
-    const int smem = kWarps * a.t * kRows * 4;
-    const dim3 grid((unsigned)((a.d - 1) / kRows + 1));
-    const Writes writes{a.y, ((size_t)(a.t - 1) * (size_t)a.ldy + (size_t)a.d) * dtype_bytes(a.dtype)};
-    return down8 ? launch_pdl(writes, moe_down_kernel<T, true>, grid, dim3(kThreads), (size_t)smem, st, a)
-                 : launch_pdl(writes, moe_down_kernel<T, false>, grid, dim3(kThreads), (size_t)smem, st, a);
+    const cudaError_t e = launch_up<T>(a, st);
+    return e != cudaSuccess ? e : launch_down(a, st);
 }
 
 }  // namespace

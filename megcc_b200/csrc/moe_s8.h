@@ -8,10 +8,8 @@ namespace mb200 {
 namespace scaled {
 
 constexpr int kMoeMaxTokens = 64, kMoeMaxTop = 16, kMoeMaxExperts = 512;
-// every expert with tokens, and one pass more for each eight slots
-constexpr int kMoeMaxPasses = kMoeMaxExperts + kMoeMaxTokens * kMoeMaxTop / 8;
 // the tokens' whole numbers lie in shared memory: eight rows (sixteen with more than eight tokens)
-constexpr int kMoeMaxDepthFew = 20480, kMoeMaxDepth = 10240;
+constexpr int kMoeMaxDepthFew = 16384, kMoeMaxDepth = 8192;
 
 struct MoeArgs {
     int t, d, f, e, top, renormalize, dtype;

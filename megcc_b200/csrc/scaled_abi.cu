@@ -60,8 +60,8 @@ int check_workspace(const char* what, const void* workspace, size_t have, size_t
 bool streams(int m) {
     return m <= 16;
 }
-bool streams_activations(int m) {
-    return m <= 8;
+bool streams_activations(int m, int k) {
+    return m <= 8 && (long long)m * k <= 32768;
 }
 // What the TMA takes: 16-byte aligned, rows whole 16-byte units apart
 bool rows_fit(const void* p, int rows, long long ld) {
@@ -94,7 +94,7 @@ int check_moe(const mb200_moe_param* p) {
                          p->top_k, p->experts);
     if (p->tokens > kMoeMaxTokens || p->top_k > kMoeMaxTop || p->experts > kMoeMaxExperts || p->f > kMaxK ||
         p->d > (p->tokens <= 8 ? kMoeMaxDepthFew : kMoeMaxDepth))
-        return set_error(ST_OUT_OF_RANGE, "moe_s8: %d tokens (64), d %d (20480, 10240 with more than 8 tokens), "
+        return set_error(ST_OUT_OF_RANGE, "moe_s8: %d tokens (64), d %d (16384, 8192 with more than 8 tokens), "
                          "f %d (131071), %d of %d experts (16 of 512)", p->tokens, p->d, p->f, p->top_k, p->experts);
     return ST_SUCCESS;
 }
@@ -181,7 +181,7 @@ int mb200_matmul_s8_scaled(
 }
 
 size_t mb200_linear_s8_workspace_bytes(int m, int n, int k, const int8_t* b_packed) {
-    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || streams_activations(m))
+    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || streams_activations(m, k))
         return 0;
     return padded_bytes(m, k) + align_up((size_t)m * 4, 256) +
            (streams(m) || rows_fit(b_packed, n, k) ? 0 : padded_bytes(n, k));
@@ -215,7 +215,7 @@ int mb200_linear_s8(
     p.a = x, p.x_dtype = dtype, p.lda = ldx;
     p.b = b_packed, p.ldb = k, p.sb = b_scales, p.bias = bias;
     p.c = y, p.c_dtype = dtype, p.ldc = ldy;
-    if (streams_activations(m)) {
+    if (streams_activations(m, k)) {
         p.b_early = may_read_early(b_packed, (size_t)n * k, st);
         return launch_product_stream(p, st);
     }

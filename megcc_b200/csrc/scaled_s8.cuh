@@ -259,7 +259,7 @@ struct ProductArgs {
 int launch_quantize_rows(
         const void* x, int dtype, int m, int k, long long ldx, int8_t* q, long long ldq, float* scales,
         cudaStream_t st);
-// for any operands, made for few rows of a; activations as they are (x_dtype >= 0) for 16 rows at most
+// for any operands, made for few rows of a; activations as they are (x_dtype >= 0) as long as shared memory holds them
 int launch_product_stream(const ProductArgs& a, cudaStream_t st);
 // the tensor-core kernels: int8 operands, 16-byte aligned, rows whole 16-byte units apart
 int launch_product_umma(const ProductArgs& a, cudaStream_t st);

@@ -1,5 +1,6 @@
 // int8 products for few tokens, and the conversion of activations to int8 rows.
-#include "scaled_s8.cuh"
+#include "stream_s8.cuh"
+#include "umma_ptx.cuh"
 
 namespace mb200 {
 namespace scaled {
@@ -105,134 +106,122 @@ int quantize_rows(
 
 // ---- product for few tokens ----
 // HBM: n * k bytes of weights are read once, whatever m. A CTA makes 16 rows of weights times 8 * NT
-// tokens; its eight warps take the 64-byte chunks of K in turn and read them straight from global memory into
-// the registers of mma.sync (16 neighbouring bytes per thread; which K byte meets which word of the MMA
-// does not matter as long as the tokens' are laid out alike), so nothing waits for shared memory or
-// a barrier before the sums meet at the end.
+// tokens; its eight warps take the 128-byte steps of K in turn (stream_s8.cuh) and their sums meet at the end.
+// int8 tokens come through the ring beside the weights; activations that are still floats are made whole
+// numbers first, by every CTA again, while its first weights are on their way.
 constexpr int kWarps = 8;
 constexpr int kRows = 16;     // weight rows per CTA
 constexpr int kColPitch = 20; // ints per token in the exchange: 2 * 20 = 8 banks apart
 
 template <class XT, int NT, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps, NT <= 2 ? 2 : 1) product_stream_kernel(const ProductArgs p, int x_vectors) {
-    constexpr bool kFloat = sizeof(XT) > 1;
-    constexpr int U = NT == 1 ? 8 : NT == 2 ? 4 : 2;  // chunks in flight per warp
-    constexpr int kCols = 8 * NT;
-    __shared__ int red[kWarps][kCols][kColPitch];
-    __shared__ uint32_t part[kFloat ? kWarps : 1][kCols];
+struct Stream {
+    static constexpr bool kFloat = sizeof(XT) > 1;
+    static constexpr int kCols = 8 * NT;
+    static constexpr int kDepth = 4;
+    typedef Rows<kRows, ALIGNED> W;
+    typedef Rows<kCols, ALIGNED> A;
+    static constexpr int kStage = W::kBytes + (kFloat ? 0 : A::kBytes);
+    static constexpr int kRing = kWarps * kDepth * kStage;
+};
+
+template <class XT, int NT, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const ProductArgs p, int x_vectors) {
+    typedef Stream<XT, NT, ALIGNED> S;
+    constexpr bool kFloat = S::kFloat;
+    constexpr int kDepth = S::kDepth, kCols = S::kCols;
+    extern __shared__ __align__(128) uint8_t dynamic[];  // the rings, then (floats) xs
     __shared__ float col_scale[kCols];
+    __shared__ uint32_t part[kFloat ? 16 * kWarps : 1];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
     const int n0 = blockIdx.x * kRows;
     const int m0 = blockIdx.y * kCols;
-    const int k = p.k, chunks = (k + 63) >> 6;
-    const int row_lo = n0 + g, row_hi = n0 + g + 8;
-    const int8_t* b_lo = p.b + (size_t)min(row_lo, p.n - 1) * p.ldb;
-    const int8_t* b_hi = p.b + (size_t)min(row_hi, p.n - 1) * p.ldb;
+    const int k = p.k, steps = (k + kStep - 1) / kStep;
+    const int mine = warp < steps ? (steps - warp + kWarps - 1) / kWarps : 0;
+    const uint32_t ring = shared_address(dynamic) + (uint32_t)(warp * kDepth * S::kStage);
+    int8_t* xs = (int8_t*)dynamic + S::kRing;
+    const int pitch = xs_pitch(k);
 
-    uint4 w[U][2];
-    auto load_weights = [&](int c0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kk = (c0 + u * kWarps) * 64 + tig * 16;
-            if (ALIGNED) {
-                w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-                if (kk < k) {
-                    w[u][0] = ld_stream16(b_lo + kk);
-                    w[u][1] = ld_stream16(b_hi + kk);
-                }
-            } else {
-                w[u][0] = ld_any16(b_lo + kk, k - kk);
-                w[u][1] = ld_any16(b_hi + kk, k - kk);
-            }
-        }
+    auto b_row = [&](int r) { return p.b + (size_t)min(n0 + r, p.n - 1) * p.ldb; };
+    auto a_row = [&](int r) { return (const int8_t*)p.a + (long long)min(m0 + r, p.m - 1) * p.lda; };
+    typename S::W w;
+    typename S::A a;
+    w.open(b_row, k, warp);
+    if (!kFloat)
+        // (no copies for tokens that are not there: every CTA asks for the same few lines)
+        a.open([&](int r) { return m0 + r < p.m ? a_row(r) : nullptr; }, k, warp);
+    auto copy_weights = [&](int i) {
+        if (i < mine)
+            w.copy(ring + (uint32_t)(i % kDepth * S::kStage), kWarps);
+    };
+    auto copy_tokens = [&](int i) {
+        if (!kFloat && i < mine)
+            a.copy(ring + (uint32_t)(i % kDepth * S::kStage + S::W::kBytes), kWarps);
     };
     if (p.b_early)
-        load_weights(warp);
+        for (int i = 0; i < kDepth - 1; ++i)
+            copy_weights(i);
     pdl_start();
-    if (!p.b_early)
-        load_weights(warp);
-
-    // a thread's columns of B: tokens m0 + 8 * nt + g
-    const XT* a[NT];
-    bool have[NT];
-    RowScale rs[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int t = m0 + 8 * nt + g;
-        have[nt] = t < p.m;
-        a[nt] = (const XT*)p.a + (long long)min(t, p.m - 1) * p.lda;
+    for (int i = 0; i < kDepth - 1; ++i) {
+        if (!p.b_early)
+            copy_weights(i);
+        copy_tokens(i);
+        copy_commit();
     }
+    // scales of what this thread stores in the end
+    const int row = threadIdx.x & 15, n = n0 + row;
+    const float sb = n < p.n ? p.sb[n] : 0.f, bias = p.bias && n < p.n ? p.bias[n] : 0.f;
     if constexpr (kFloat) {
-        // the rows' scales: every warp has the maximum of its chunks
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            uint32_t bits = 0;
-            if (have[nt]) {
-                for (int c = warp; c < chunks; c += kWarps) {
-                    float v[16];
-                    load_piece(a[nt], c * 64 + tig * 16, k, x_vectors, v);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        bits = max(bits, magnitude(v[i]));
-                }
-            }
-            bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
-            bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-            if (tig == 0)
-                part[warp][8 * nt + g] = bits;
-        }
+        quantize_cta<XT, kWarps>([&](int r) { return (const XT*)p.a + (long long)(m0 + r) * p.lda; },
+                                 min(kCols, p.m - m0), k, xs, pitch, col_scale, part, x_vectors);
         __syncthreads();
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            uint32_t bits = 0;
-#pragma unroll
-            for (int i = 0; i < kWarps; ++i)
-                bits = max(bits, part[i][8 * nt + g]);
-            rs[nt] = row_scale(bits);
-            if (warp == 0 && tig == 0)
-                col_scale[8 * nt + g] = rs[nt].scale;
-        }
     } else {
         if (threadIdx.x < kCols)
             col_scale[threadIdx.x] = m0 + (int)threadIdx.x < p.m ? p.sa[m0 + threadIdx.x] : 0.f;
     }
-
+    // rows and columns of this thread's fragments
+    const int s_lo = (int)((uintptr_t)b_row(g) & 15), s_hi = (int)((uintptr_t)b_row(g + 8) & 15);
+    int s_a[NT];
+    const int8_t* x_at[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        s_a[nt] = kFloat ? 0 : (int)((uintptr_t)a_row(8 * nt + g) & 15);
+        x_at[nt] = xs + min(8 * nt + g, p.m - 1 - m0) * pitch + tig * 16;
+    }
     int acc[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
         acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
-    for (int c0 = warp; c0 < chunks; c0 += U * kWarps) {
-        if (c0 != warp)
-            load_weights(c0);
+    for (int i = 0; i < mine; ++i) {
+        copy_wait<kDepth - 2>();
+        __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
+        copy_weights(i + kDepth - 1);
+        copy_tokens(i + kDepth - 1);
+        copy_commit();
+        const uint32_t stage = ring + (uint32_t)(i % kDepth * S::kStage);
+        const int step = warp + i * kWarps;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            uint4 t[U];
+        for (int j = 0; j < kStep / 64; ++j) {
+            const int piece = 4 * j + tig;
+            const uint4 lo = S::W::piece16(stage, g, piece, s_lo), hi = S::W::piece16(stage, g + 8, piece, s_hi);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int kk = (c0 + u * kWarps) * 64 + tig * 16;
-                t[u] = make_uint4(0, 0, 0, 0);
+            for (int nt = 0; nt < NT; ++nt) {
+                uint4 t;
                 if constexpr (kFloat) {
-                    if (have[nt] && kk < k) {
-                        float v[16];
-                        load_piece(a[nt], kk, k, x_vectors, v);
-                        t[u] = pack_piece(v, rs[nt]);
-                    }
-                } else if (have[nt]) {
-                    if (ALIGNED) {
-                        if (kk < k)
-                            t[u] = *(const uint4*)((const int8_t*)a[nt] + kk);
-                    } else {
-                        t[u] = ld_any16((const int8_t*)a[nt] + kk, k - kk);
-                    }
+                    t = *(const uint4*)(x_at[nt] + step * kStep + 64 * j);
+                } else {
+                    t = S::A::piece16(stage + S::W::kBytes, 8 * nt + g, piece, s_a[nt]);
+                    if (!ALIGNED && step == steps - 1)  // (aligned rows end with a unit, zeros lie behind it)
+                        t = first_bytes(t, k - step * kStep - piece * 16);
                 }
+                mma_64(acc[nt], lo, hi, t);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                mma_64(acc[nt], w[u][0], w[u][1], t[u]);
         }
     }
+    copy_wait<0>();
+    __syncthreads();
+    int(*red)[kCols][kColPitch] = (int(*)[kCols][kColPitch])dynamic;  // (the rings are done with)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         int(*r)[kColPitch] = red[warp] + 8 * nt + 2 * tig;
@@ -242,10 +231,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT <= 2 ? 2 : 1) product_stream_k
         r[1][g + 8] = acc[nt][3];
     }
     __syncthreads();
-    const int row = threadIdx.x & 15, n = n0 + row;
     if (n >= p.n)
         return;
-    const float sb = p.sb[n], bias = p.bias ? p.bias[n] : 0.f;
     for (int col = threadIdx.x >> 4; col < kCols && m0 + col < p.m; col += 2 * kWarps) {
         int sum = 0;
 #pragma unroll
@@ -268,22 +255,29 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(
     }
 }
 
+template <class XT, int NT, bool ALIGNED>
+cudaError_t launch_stream_as(const ProductArgs& a, int x_vectors, cudaStream_t st) {
+    typedef Stream<XT, NT, ALIGNED> S;
+    static umma::KernelReady ready;
+    static_assert(S::kRing >= kWarps * S::kCols * kColPitch * 4, "the exchange lies where the rings were");
+    auto kernel = product_stream_kernel<XT, NT, ALIGNED>;
+    const int smem = S::kRing + (S::kFloat ? (a.m < S::kCols ? a.m : S::kCols) * xs_pitch(a.k) : 0);
+    if (!ready.smem(kernel, smem))
+        return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)((a.n - 1) / kRows + 1), (unsigned)((a.m - 1) / S::kCols + 1));
+    const Writes writes{a.c, ((size_t)(a.m - 1) * (size_t)a.ldc + (size_t)a.n) * dtype_bytes(a.c_dtype)};
+    return launch_pdl(writes, kernel, grid, dim3(32 * kWarps), (size_t)smem, st, a, x_vectors);
+}
 template <class XT, int NT>
 cudaError_t launch_stream(const ProductArgs& a, bool aligned, int x_vectors, cudaStream_t st) {
-    const dim3 grid((unsigned)((a.n - 1) / kRows + 1), (unsigned)((a.m - 1) / (8 * NT) + 1));
-    const size_t size = dtype_bytes(a.c_dtype);
-    const Writes writes{a.c, ((size_t)(a.m - 1) * (size_t)a.ldc + (size_t)a.n) * size};
-    return aligned ? launch_pdl(writes, product_stream_kernel<XT, NT, true>, grid, dim3(32 * kWarps), 0, st, a,
-                                x_vectors)
-                   : launch_pdl(writes, product_stream_kernel<XT, NT, false>, grid, dim3(32 * kWarps), 0, st, a,
-                                x_vectors);
+    return aligned ? launch_stream_as<XT, NT, true>(a, x_vectors, st)
+                   : launch_stream_as<XT, NT, false>(a, x_vectors, st);
 }
 
 template <class XT>
 cudaError_t launch_stream_float(const ProductArgs& a, bool aligned, cudaStream_t st) {
     const int x_vectors = ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % Vec<XT>::N == 0);
-    return a.m <= 8 ? launch_stream<XT, 1>(a, aligned, x_vectors, st)
-                    : launch_stream<XT, 2>(a, aligned, x_vectors, st);
+    return launch_stream<XT, 1>(a, aligned, x_vectors, st);
 }
 
 }  // namespace
@@ -315,10 +309,7 @@ int launch_product_stream(const ProductArgs& a, cudaStream_t st) {
     cudaError_t e;
     if (a.x_dtype < 0) {
         const bool aligned = b_aligned && ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % 16 == 0);
-        e = a.m <= 8    ? launch_stream<int8_t, 1>(a, aligned, 0, st)
-            : a.m <= 16 ? launch_stream<int8_t, 2>(a, aligned, 0, st)
-            : a.m <= 32 ? launch_stream<int8_t, 4>(a, aligned, 0, st)
-                        : launch_stream<int8_t, 8>(a, aligned, 0, st);
+        e = a.m <= 8 ? launch_stream<int8_t, 1>(a, aligned, 0, st) : launch_stream<int8_t, 2>(a, aligned, 0, st);
     } else if (a.x_dtype == DT_F32) {
         e = launch_stream_float<float>(a, b_aligned, st);
     } else if (a.x_dtype == DT_F16) {

@@ -1,0 +1,206 @@
+// Weights streamed through a warp's own ring of shared memory into mma.sync: what the kernels for few
+// tokens have in common. HBM is what bounds them, so the ring's only job is to keep enough bytes on their way
+// (an SM's share of 6.5 TB/s times a microsecond is 45 KB). Asynchronous copies do that without registers, and
+// in order: a ring in registers made the compiler wait for the youngest load with the oldest (0.86 us a
+// step of the second expert kernel, the whole latency of a load). A warp fills and reads its ring
+// alone, so no barrier of the CTA stands in the stream.
+//
+// A step is 128 bytes of K of each of 16 rows: whole lines, and few enough instructions per byte (with 64 bytes
+// the expert kernels took 100 to 230 of them per KB and were bound by their issue: 33 us for 100 MB). Rows may
+// start at any byte: ALIGNED rows are eight 16-byte units, others the nine units that hold their 128 bytes,
+// shifted into place when they are read.
+#pragma once
+#include "scaled_s8.cuh"
+
+namespace mb200 {
+namespace scaled {
+
+constexpr int kStep = 128;
+
+__device__ __forceinline__ void copy_async16(uint32_t smem, const void* p, bool there) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem), "l"(p), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t smem, const void* p, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem), "l"(p), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+
+// ROWS rows of a step in shared memory
+template <int ROWS, bool ALIGNED>
+struct Rows {
+    static constexpr int kUnits = ALIGNED ? 8 : 9;
+    static constexpr int kPitch = 16 * kUnits;
+    static constexpr int kBytes = ROWS * kPitch;
+    static constexpr int kCopies = (ROWS * kUnits + 31) / 32;  // of a lane, per step
+
+    // Where a unit lies in its row: a read of 16 (8) bytes by the lanes of two (four) rows meets every bank once
+    static __device__ __forceinline__ int unit_at(int row, int unit) {
+        return ALIGNED ? unit ^ (((row & 1) << 2) | (row & 2)) : unit;
+    }
+
+    // what a lane copies next: its units' places in global memory, and how far their rows go from there
+    const int8_t* from[kCopies];
+    int left[ALIGNED ? 1 : kCopies];
+    uint32_t there;      // a bit per copy: its row is one to read
+    const int8_t* any;   // an address for copies of nothing
+    int to[kCopies];     // in the stage
+
+    // (once per kernel: the places in the stage)
+    __device__ __forceinline__ Rows() {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int q = lane + 32 * i, r = q / kUnits, u = q % kUnits;
+            to[i] = r * kPitch + unit_at(r, u) * 16;
+        }
+    }
+    // row(r): address of row r, or null for a row of zeros (row 0 is none); k: its bytes; step: the first
+    template <class RowAt>
+    __device__ __forceinline__ void open(RowAt row, int k, int step) {
+        const int lane = threadIdx.x & 31;
+        any = row(0);
+        any -= (uintptr_t)any & 15;
+        there = 0;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int q = lane + 32 * i, r = q / kUnits, u = q % kUnits;
+            const int8_t* p = ROWS * kUnits % 32 == 0 || r < ROWS ? row(r) : nullptr;
+            if (p)
+                there |= 1u << i;
+            // (a unit is read if it holds at least one byte of the row)
+            const int s = ALIGNED ? 0 : (int)((uintptr_t)p & 15);
+            from[i] = (p ? p - s : any) + step * kStep + 16 * u;
+            if (!ALIGNED || i == 0)
+                left[i] = k + s - 16 * u - step * kStep;
+        }
+    }
+    // the next step; `by`: how many steps further the one behind it is
+    __device__ __forceinline__ void copy(uint32_t stage, int by) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            if (ROWS * kUnits % 32 == 0 || lane + 32 * i < ROWS * kUnits) {
+                const bool some = (ALIGNED ? left[0] : left[i]) > 0 && (there >> i & 1);
+                copy_async16(stage + to[i], some ? from[i] : any, some);
+            }
+            from[i] += by * kStep;
+            if (!ALIGNED || i + 1 == kCopies)
+                left[ALIGNED ? 0 : i] -= by * kStep;
+        }
+    }
+    // 16 bytes of row r from byte 16 * part on; s: the row's address modulo 16
+    static __device__ __forceinline__ uint4 piece16(uint32_t stage, int r, int part, int s) {
+        if (ALIGNED)
+            return lds16(stage + r * kPitch + unit_at(r, part) * 16);
+        const uint32_t at = stage + r * kPitch + part * 16 + (s & ~3);
+        uint32_t w[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            w[i] = lds4(at + 4 * i);
+        const int bits = (s & 3) * 8;
+        return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                          __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
+    // 8 bytes from byte 8 * part on
+    static __device__ __forceinline__ uint2 piece8(uint32_t stage, int r, int part, int s) {
+        if (ALIGNED)
+            return lds8(stage + r * kPitch + unit_at(r, part >> 1) * 16 + (part & 1) * 8);
+        const uint32_t at = stage + r * kPitch + part * 8 + (s & ~3);
+        const uint32_t a = lds4(at), b = lds4(at + 4), c = lds4(at + 8);
+        const int bits = (s & 3) * 8;
+        return make_uint2(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits));
+    }
+};
+
+// the first `n` bytes (n <= 0: none) of 16
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
+    auto cut = [](uint32_t w, int left) { return left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u); };
+    return make_uint4(cut(v.x, n), cut(v.y, n - 4), cut(v.z, n - 8), cut(v.w, n - 12));
+}
+
+// `rows` (up to 16) rows of activations as whole numbers in shared memory, zeros behind them up to whole steps, by all
+// threads of a CTA; row(r): the row's address. part: [16][WARPS] words of shared memory. A barrier of the
+// CTA has to follow before they are read.
+template <class T, int WARPS, class RowAt>
+__device__ __forceinline__ void quantize_cta(
+        RowAt row, int rows, int k, int8_t* xs, int pitch, float* scale, uint32_t* part, bool vectors) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kAhead = 2;  // rows whose loads are on their way together
+    for (int r0 = 0; r0 < rows; r0 += kAhead) {
+        uint32_t bits[kAhead] = {0};
+        for (int i = tid * 16; i < k; i += WARPS * 512) {
+            float v[kAhead][16];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (r0 + j < rows)
+                    load_piece((const T*)row(r0 + j), i, k, vectors, v[j]);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (r0 + j < rows)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        bits[j] = max(bits[j], magnitude(v[j][e]));
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (r0 + j < rows) {
+                const uint32_t b = __reduce_max_sync(0xffffffffu, bits[j]);
+                if (lane == 0)
+                    part[(r0 + j) * WARPS + warp] = b;
+            }
+    }
+    __syncthreads();
+    const int end = (k + kStep - 1) / kStep * kStep;
+    for (int r = 0; r < rows; ++r) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+            bits = max(bits, part[r * WARPS + w]);
+        const RowScale s = row_scale(bits);
+        if (tid == 0)
+            scale[r] = s.scale;
+        for (int i = tid * 16; i < end; i += WARPS * 512) {
+            float v[16];
+            load_piece((const T*)row(r), i, k, vectors, v);
+            *(uint4*)(xs + r * pitch + i) = pack_piece(v, s);
+        }
+    }
+}
+// Asks for what the CTA's threads will read soon: `bytes` from p on, into the L1.
+template <int THREADS>
+__device__ __forceinline__ void ask_ahead(const void* p, size_t bytes) {
+    const uintptr_t first = (uintptr_t)p & ~(uintptr_t)127, end = (uintptr_t)p + bytes;
+    for (uintptr_t at = first + threadIdx.x * 128u; at < end; at += THREADS * 128u)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+}
+// bytes between rows of xs: whole steps, and two rows on other banks
+__host__ __device__ constexpr int xs_pitch(int k) {
+    return (k + 127) / 128 * 128 + 64;
+}
+
+}  // namespace scaled
+}  // namespace mb200

@@ -80,8 +80,8 @@ def test_moe(t, d, f, e, top, renorm, dtype):
 
 def test_moe_of_wide_layers():
     check(layer(1, 4096, 1536, 16, 1), 8, True)
-    check(layer(2, 20480, 64, 3, 2), 2, True)
-    check(layer(10, 10240, 40, 3, 3), 1, False)
+    check(layer(2, 16384, 64, 3, 2), 2, True)
+    check(layer(10, 8192, 40, 3, 3), 1, False)
     check(layer(4, 48, 5000, 3, 4), 2, True)
     check(layer(3, 64, 32, 512, 5), 16, True)
 

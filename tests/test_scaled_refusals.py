@@ -72,7 +72,7 @@ def moe(tokens=2, d=64, f=32, experts=4, top_k=2, renormalize=1, dtype=2, x=P, l
     (dict(dtype=3), DTYPE), (dict(tokens=-1), LAYOUT), (dict(d=0), LAYOUT), (dict(f=0), LAYOUT),
     (dict(experts=0), LAYOUT), (dict(top_k=0), LAYOUT), (dict(top_k=5), LAYOUT), (dict(tokens=65), OUT_OF_RANGE),
     (dict(experts=513), OUT_OF_RANGE), (dict(experts=40, top_k=17), OUT_OF_RANGE),
-    (dict(d=20481, ldx=30000, ldy=30000), OUT_OF_RANGE), (dict(tokens=9, d=10241, ldx=30000, ldy=30000), OUT_OF_RANGE),
+    (dict(d=16385, ldx=30000, ldy=30000), OUT_OF_RANGE), (dict(tokens=9, d=8193, ldx=30000, ldy=30000), OUT_OF_RANGE),
     (dict(f=131072), OUT_OF_RANGE), (dict(ldx=63), LAYOUT), (dict(ldy=63), LAYOUT), (dict(x=P + 1), LAYOUT),
     (dict(y=P + 1), LAYOUT), (dict(logits=P + 2), LAYOUT), (dict(s1=P + 2), LAYOUT), (dict(s2=P + 1), LAYOUT),
     (dict(ws=P + 128), LAYOUT), (dict(nbytes=100), LAYOUT), (dict(tokens=0, x=None, ws=None), 0)])
