@@ -146,10 +146,7 @@ FAST = ("mb200_conv_bias_qs8_nhwc", "mb200_conv_bias_qs8_nhwc_fused", "mb200_con
         "mb200_matmul_s8_qs8", "mb200_qelemwise_qs8", "mb200_conv_bias_f32_nhwc",
         "mb200_conv_bias_qs8_nchw_workspace", "mb200_conv_nchw_in_place",
         "mb200_conv_bias_qs8_nchw_in_place", "mb200_matmul_f32_scratch_bytes_for",
-        "mb200_matmul_f32_product", "mb200_elemwise_f32", "mb200_quantize_rows_s8",
-        "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
-        "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
-        "mb200_moe_s8")
+        "mb200_matmul_f32_product", "mb200_elemwise_f32")
 _fast = None
 
 
@@ -171,6 +168,26 @@ def fast():
             setattr(f, name, _fastcall.bind(C.cast(fn, C.c_void_p).value, kinds))
         _fast = f
     return _fast
+
+
+_tensor_calls = None
+
+
+def tensor_calls():
+    """The calls of megcc_b200/fastcall/torchcall.cpp, over the functions of the library."""
+    global _tensor_calls
+    if _tensor_calls is None:
+        try:
+            from . import _torchcall
+        except ImportError as e:
+            raise RuntimeError("megcc_b200/_torchcall.so is missing or made for another torch: build it with "
+                               "`python -m megcc_b200.build` (there is no fallback)") from e
+        _torchcall.bind(check, *(C.cast(getattr(lib(), name), C.c_void_p).value for name in (
+            "mb200_quantize_rows_s8", "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
+            "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
+            "mb200_moe_s8")))
+        _tensor_calls = _torchcall
+    return _tensor_calls
 
 
 class MegccError(RuntimeError):

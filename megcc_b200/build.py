@@ -25,6 +25,7 @@ NVCC_FLAGS = [
 COMPILER_DIR = os.path.join(HERE, "compiler")
 COMPILER_LIB = os.path.join(HERE, "libmegcc_b200_compiler.so")
 FASTCALL = os.path.join(HERE, "_fastcall.so")
+TORCHCALL = os.path.join(HERE, "_torchcall.so")
 
 
 def _sources():
@@ -72,6 +73,31 @@ def build_fastcall(verbose=False, force=False):
     return FASTCALL
 
 
+def build_torchcall(verbose=False, force=False):
+    """The extension module of operator calls on tensors (C++ against torch's headers)."""
+    src = os.path.join(HERE, "fastcall", "torchcall.cpp")
+    deps = [src, os.path.join(os.path.dirname(HERE), "include", "megcc_b200.h")]
+    if not force and not _stale(TORCHCALL, deps):
+        return TORCHCALL
+    import torch  # (its headers and libraries; the rest of the build does without)
+    at = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else os.environ.get("CXX", "g++")
+    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(at, "include"),
+           "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"],
+           "-o", TORCHCALL, src, "-L" + os.path.join(at, "lib"), "-Wl,-rpath," + os.path.join(at, "lib"),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if verbose or r.returncode:
+        sys.stderr.write(r.stdout)
+    if r.returncode:
+        raise RuntimeError("building the tensor call extension failed")
+    return TORCHCALL
+
+
 def _stale(target, deps):
     if not os.path.exists(target):
         return True
@@ -82,6 +108,7 @@ def _stale(target, deps):
 def build(verbose=False, force=False):
     build_compiler(verbose, force)
     build_fastcall(verbose, force)
+    build_torchcall(verbose, force)
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     srcs = _sources()
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]

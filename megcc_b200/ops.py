@@ -7,7 +7,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import ConvF32Param, ConvFuse, ConvParam, MoeParam, check, fast, lib
+from ._lib import ConvF32Param, ConvFuse, ConvParam, check, fast, lib, tensor_calls
 
 ACT = {"IDENTITY": 0, "RELU": 1, "H_SWISH": 2}
 POOL = {"MAX": 0, "AVERAGE": 1, "AVERAGE_COUNT_EXCLUDE_PADDING": 2}
@@ -140,114 +140,29 @@ def matmul_s8_qs8(a, b_packed, acc_scale, dst_scale):
 
 
 # ---- int8 products with scales per row (token) and per output channel ----
-DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
-def _rows(t, kinds, name):
-    """(rows, columns, elements between rows) of a matrix of the current device, whose rows'
-    elements are neighbours"""
-    if t.dtype not in kinds or t.dim() != 2 or not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA matrix of {', '.join(str(k) for k in kinds)}, not "
-                         f"{tuple(t.shape)} of {t.dtype} on {t.device}")
-    if t.get_device() != torch._C._cuda_getDevice():
-        raise ValueError(f"{name} is on {t.device}, not on the current device")
-    (m, k), (ld, one) = t.shape, t.stride()
-    if one != 1 and k > 1:
-        raise ValueError(f"{name}: elements of a row must be neighbours (strides {t.stride()})")
-    return m, k, ld
-
-
-def _vector(t, n, like, name):
-    """Address of a contiguous fp32 vector of n elements on the device of `like`"""
-    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous() or \
-            t.get_device() != like.get_device():
-        raise ValueError(f"{name}: {n} contiguous fp32 values on {like.device}, not "
-                         f"{tuple(t.shape)} of {t.dtype} on {t.device}")
-    return t.data_ptr()
-
-
-def _packed_b(b, k, like):
-    if b.dtype is not _S8 or b.dim() != 2 or b.shape[1] != k or not b.is_contiguous() or \
-            b.get_device() != like.get_device():
-        raise ValueError(f"b_packed: contiguous int8 [n, {k}] on {like.device}, not "
-                         f"{tuple(b.shape)} of {b.dtype} on {b.device}")
-    return b.shape[0]
-
-
 def quantize_rows_s8(x):
-    """Rows of an fp32 / fp16 / bf16 matrix as int8 with one fp32 scale each: (q, scales)."""
-    m, k, ld = _rows(x, DTYPE, "x")
-    q, scales = x.new_empty((m, k), dtype=_S8), x.new_empty((m,), dtype=torch.float32)
-    check(fast().mb200_quantize_rows_s8(x.data_ptr(), DTYPE[x.dtype], m, k, ld, q.data_ptr(), k,
-                                        scales.data_ptr(), _stream()))
-    return q, scales
+    """Rows of an fp32 / fp16 / bf16 matrix as int8 with one fp32 scale each: (q, scales). (A row's
+    elements must be neighbours, here and below; rows may lie apart. Arguments that do not fit raise ValueError.)"""
+    return tensor_calls().quantize_rows_s8(x)
 
 
 def matmul_s8_scaled(a, b_packed, a_scales, b_scales, bias=None, dtype=torch.float32):
-    """a [m, k] int8 times b_packed [n, k] int8 (matmul_pack_b), with a scale per row of a and per
-    row of b_packed, plus bias [n]: [m, n] of `dtype`."""
-    m, k, ld = _rows(a, (_S8,), "a")
-    n = _packed_b(b_packed, k, a)
-    if dtype not in DTYPE:
-        raise ValueError(f"results are fp32, fp16 or bf16, not {dtype}")
-    f = fast()
-    pa, pb = a.data_ptr(), b_packed.data_ptr()
-    sa, sb = _vector(a_scales, m, a, "a_scales"), _vector(b_scales, n, a, "b_scales")
-    bias = None if bias is None else _vector(bias, n, a, "bias")
-    c = a.new_empty((m, n), dtype=dtype)
-    nbytes = f.mb200_matmul_s8_scaled_workspace_bytes(m, n, k, pa, ld, pb)
-    keep, ws = _scratch(nbytes, a.device)
-    check(f.mb200_matmul_s8_scaled(m, n, k, pa, ld, pb, sa, sb, bias, c.data_ptr(), DTYPE[dtype], n,
-                                   ws, nbytes, _stream()))
-    return c
+    """a [m, k] int8 times b_packed [n, k] int8 (matmul_pack_b), with an fp32 scale per row of a and per
+    row of b_packed, plus bias [n] fp32: [m, n] of `dtype` (fp32, fp16 or bf16)."""
+    return tensor_calls().matmul_s8_scaled(a, b_packed, a_scales, b_scales, bias, dtype)
 
 
 def linear_s8(x, b_packed, b_scales, bias=None):
     """x [m, k] fp32 / fp16 / bf16, quantised row by row, times b_packed [n, k] int8 with a scale per
     row, plus bias [n]: [m, n] of x's type. The same as quantize_rows_s8 and matmul_s8_scaled."""
-    m, k, ld = _rows(x, DTYPE, "x")
-    n = _packed_b(b_packed, k, x)
-    f = fast()
-    pb, sb = b_packed.data_ptr(), _vector(b_scales, n, x, "b_scales")
-    bias = None if bias is None else _vector(bias, n, x, "bias")
-    y = x.new_empty((m, n))
-    nbytes = f.mb200_linear_s8_workspace_bytes(m, n, k, pb)
-    keep, ws = _scratch(nbytes, x.device)
-    check(f.mb200_linear_s8(m, n, k, x.data_ptr(), DTYPE[x.dtype], ld, pb, sb, bias, y.data_ptr(), n,
-                            ws, nbytes, _stream()))
-    return y
-
-
-def _expert_weights(w, experts, like, name):
-    if w.dtype is not _S8 or w.dim() != 3 or w.shape[0] != experts or not w.is_contiguous() or \
-            w.get_device() != like.get_device():
-        raise ValueError(f"{name}: contiguous int8 [{experts}, rows, columns] on {like.device}, not "
-                         f"{tuple(w.shape)} of {w.dtype} on {w.device}")
-    return w.shape[1], w.shape[2]
+    return tensor_calls().linear_s8(x, b_packed, b_scales, bias)
 
 
 def moe_s8(x, logits, w1, w1_scales, w2, w2_scales, top_k, renormalize=True):
     """Mixture-of-experts layer for up to 64 tokens: x [t, d] fp32 / fp16 / bf16, router logits [t, experts]
     fp32, int8 weights w1 [experts, 2f, d] (gate rows, then up rows) and w2 [experts, d, f] with fp32 scales
     per row; [t, d] of x's type (see mb200_moe_s8)."""
-    t, d, ld = _rows(x, DTYPE, "x")
-    if logits.dim() != 2 or logits.shape[0] != t:
-        raise ValueError(f"logits: [{t}, experts], not {tuple(logits.shape)}")
-    e = logits.shape[1]
-    pl = _vector(logits, t * e, x, "logits")
-    f2, d1 = _expert_weights(w1, e, x, "w1")
-    d2, f = _expert_weights(w2, e, x, "w2")
-    if f2 != 2 * f or d1 != d or d2 != d:
-        raise ValueError(f"w1 {tuple(w1.shape)} and w2 {tuple(w2.shape)} over rows of {d}")
-    s1, s2 = _vector(w1_scales, e * f2, x, "w1_scales"), _vector(w2_scales, e * d, x, "w2_scales")
-    p = MoeParam(t, d, f, e, top_k, int(renormalize), DTYPE[x.dtype])
-    at, fn = C.addressof(p), fast()
-    y = x.new_empty((t, d))
-    nbytes = fn.mb200_moe_s8_workspace_bytes(at)
-    keep, ws = _scratch(nbytes, x.device)
-    check(fn.mb200_moe_s8(at, x.data_ptr(), ld, pl, w1.data_ptr(), s1, w2.data_ptr(), s2, y.data_ptr(), d,
-                          ws, nbytes, _stream()))
-    return y
+    return tensor_calls().moe_s8(x, logits, w1, w1_scales, w2, w2_scales, top_k, renormalize)
 
 
 def pooling_qs8_nhwc(src, mode, window, stride, pad):

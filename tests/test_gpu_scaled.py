@@ -160,7 +160,7 @@ def call_linear(x, b, sb, y, ldy):
     nbytes = lib().mb200_linear_s8_workspace_bytes(m, n, k, b.data_ptr())
     ws = torch.empty(nbytes + 256, dtype=torch.uint8, device="cuda")
     base = ws.data_ptr() + -ws.data_ptr() % 256
-    check(lib().mb200_linear_s8(m, n, k, x.data_ptr(), ops.DTYPE[x.dtype], x.stride(0), b.data_ptr(),
+    check(lib().mb200_linear_s8(m, n, k, x.data_ptr(), TYPES.index(x.dtype), x.stride(0), b.data_ptr(),
                                 sb.data_ptr(), None, y.data_ptr(), ldy, base, nbytes, ops._stream()))
 
 
