@@ -30,41 +30,31 @@ constexpr int kRows = 16;             // rows of w2 per CTA of the second kernel
 
 // Where the tokens go, in shared memory: as large as the call's tokens and experts ask for.
 struct Route {
-    float* p;          // by slot = token * top + rank
-    short* expert;     // -1: no share in the result
-    short* order;      // slots by expert
-    int *count, *at;   // by expert: its slots, and where the next one goes
+    float* p;      // by slot = token * top + rank
+    short* order;  // slots by expert
     // the passes: an expert and up to `cols` of its slots
     short *pass_expert, *pass_start, *pass_cols;
     int* passes;
+    // while it is worked out (in memory that is used for something else afterwards)
+    int* expert;       // by slot; -1: no share in the result
+    int *count, *at;   // by expert: its slots, and where the next one goes
 };
-__host__ __device__ constexpr int up16(int v) {
-    return (v + 15) / 16 * 16;
-}
-// every expert with tokens, and one more for each `cols` slots
-__host__ __device__ constexpr int most_passes(int slots, int experts, int cols) {
-    return (slots < experts ? slots : experts) + slots / cols;
-}
-__host__ __device__ constexpr int route_bytes(int slots, int experts, int cols) {
-    return up16(4 * slots) + 2 * up16(2 * slots) + 2 * up16(4 * experts) + 3 * up16(2 * most_passes(slots, experts, cols)) + 16;
-}
-__device__ __forceinline__ Route place_route(uint8_t* at, int slots, int experts, int cols) {
+constexpr int kMostBuild = up16(4 * kMoeMaxTokens * kMoeMaxTop) + 2 * up16(4 * kMoeMaxExperts);
+__device__ __forceinline__ Route place_route(uint8_t* at, uint8_t* build, int slots, int experts, int cols) {
     Route r;
     r.p = (float*)at;
     at += up16(4 * slots);
-    r.expert = (short*)at;
-    at += up16(2 * slots);
     r.order = (short*)at;
     at += up16(2 * slots);
-    r.count = (int*)at;
-    at += up16(4 * experts);
-    r.at = (int*)at;
-    at += up16(4 * experts);
     const int n = up16(2 * most_passes(slots, experts, cols));
     r.pass_expert = (short*)at;
     r.pass_start = (short*)(at + n);
     r.pass_cols = (short*)(at + 2 * n);
     r.passes = (int*)(at + 3 * n);
+    r.expert = (int*)build;
+    build += up16(4 * slots);
+    r.count = (int*)build;
+    r.at = (int*)(build + up16(4 * experts));
     return r;
 }
 
@@ -74,79 +64,147 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
     return v != v ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// A warp per token in turn; then the slots by expert, cut into passes of at most `cols`.
-__device__ void route_tokens(const MoeArgs& a, int cols, const Route& r) {
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+// One token's experts, by a warp: lane j < top gets the j-th choice's index and p. 32 * R experts at most.
+template <int R>
+__device__ __forceinline__ void choose_experts(const MoeArgs& a, const float* row, int* expert, float* share) {
+    const int lane = threadIdx.x & 31;
+    const float inf = __uint_as_float(0x7f800000u);
+    uint32_t key[R];
+    uint32_t odd = 0;  // a NaN or +infinity among the logits
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int e = i * 32 + lane;
+        const float v = e < a.e ? row[e] : -inf;
+        key[i] = e < a.e ? rank_key(v) : 0u;
+        odd |= !(v < inf);
+    }
+    odd = __any_sync(0xffffffffu, odd);
+    float top_value = 0.f, sum = 0.f, chosen = 0.f, mine = 0.f;
+    int mine_e = -1;
+    for (int j = 0; j < a.top; ++j) {
+        uint32_t best = 0;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (key[i] > best) {
+                best = key[i];
+                at = i;
+            }
+        const uint32_t high = __reduce_max_sync(0xffffffffu, best);
+        const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)(at * 32 + lane) : ~0u);
+        const float v = key_value(high);
+        if (j == 0) {
+            // (the first choice is the largest logit) all exponentials, from the keys still in place
+            top_value = v;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (key[i] != 0)
+                    sum += expf(key_value(key[i]) - top_value);
+#pragma unroll
+            for (int s = 16; s; s >>= 1)
+                sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        }
+        if (lane == j) {
+            mine = v;
+            mine_e = e;
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i * 32 + lane == e)
+                key[i] = 0;
+    }
+    mine = lane < a.top ? expf(mine - top_value) : 0.f;
+    for (int j = 0; j < a.top; ++j)
+        chosen += __shfl_sync(0xffffffffu, mine, j);
+    float p = __fdiv_rn(mine, a.renormalize ? chosen : sum);
+    if (top_value == -inf)
+        p = 0.f;  // every expert is masked: no share in any
+    if (odd)
+        p = __uint_as_float(0x7fffffffu);
+    *share = p;
+    *expert = lane >= a.top || p == 0.f ? -1 : mine_e;
+}
+
+// A value at the same place in another CTA of the cluster
+__device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_address(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// A warp per token in turn (500 instructions in a chain, 2 us each: the CTAs of a cluster share the tokens
+// out); then the slots by expert, cut into passes of at most `cols`. Barriers of the CTA stand before and behind,
+// and with a cluster umma::cluster_wait() has to follow before r.expert's memory is used for something else.
+__device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int rank, int cluster) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto choose = [&](int t, int* e, float* p) {
+        const float* row = a.logits + (size_t)t * a.e;
+        if (a.e <= 32)
+            choose_experts<1>(a, row, e, p);
+        else if (a.e <= 64)
+            choose_experts<2>(a, row, e, p);
+        else if (a.e <= 128)
+            choose_experts<4>(a, row, e, p);
+        else if (a.e <= 256)
+            choose_experts<8>(a, row, e, p);
+        else
+            choose_experts<kMoeMaxExperts / 32>(a, row, e, p);
+    };
+    if (a.t == 1) {
+        // one token: a pass for each of its experts, in the order of their indices
+        if (warp == 0) {
+            int e;
+            float p;
+            choose(0, &e, &p);
+            int before = 0;
+            for (int j = 0; j < a.top; ++j) {
+                const int other = __shfl_sync(0xffffffffu, e, j);
+                before += other >= 0 && other < e;
+            }
+            if (lane < a.top)
+                r.p[lane] = p;
+            if (e >= 0) {
+                r.order[before] = (short)lane;
+                r.pass_expert[before] = (short)e;
+                r.pass_start[before] = (short)before;
+                r.pass_cols[before] = 1;
+            }
+            const uint32_t some = __ballot_sync(0xffffffffu, e >= 0);
+            if (lane == 0)
+                *r.passes = __popc(some);
+        }
+        __syncthreads();
+        return;
+    }
     for (int e = threadIdx.x; e < a.e; e += kThreads)
         r.count[e] = 0;
-    constexpr int R = kMoeMaxExperts / 32;
-    for (int t = warp; t < a.t; t += kWarps) {
-        const float* row = a.logits + (size_t)t * a.e;
-        uint32_t key[R];
-        float top_value = 0.f, sum = 0.f;
-        uint32_t odd = 0;  // a NaN or +infinity among the logits
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            key[i] = 0;
-            if (i * 32 < a.e) {
-                const int e = i * 32 + lane;
-                if (e < a.e) {
-                    const float v = row[e];
-                    key[i] = rank_key(v);
-                    odd |= !(v < __uint_as_float(0x7f800000u));
-                }
-            }
-        }
-        odd = __any_sync(0xffffffffu, odd);
-        float chosen = 0.f;  // the sum of the chosen ones' exponentials
-        float mine = 0.f;    // lane j: the j-th choice's
-        int mine_e = -1;
-        for (int j = 0; j < a.top; ++j) {
-            uint32_t best = 0;
-            int at = 0;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (i * 32 < a.e && key[i] > best) {
-                    best = key[i];
-                    at = i;
-                }
-            const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-            const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)(at * 32 + lane) : ~0u);
-            const uint32_t bits = (high & 0x80000000u) ? high & 0x7fffffffu : ~high;
-            const float v = __uint_as_float(bits);
-            if (j == 0) {
-                // (the first choice is the largest logit) all exponentials, from the keys still in place
-                top_value = v;
-#pragma unroll
-                for (int i = 0; i < R; ++i)
-                    if (i * 32 < a.e && i * 32 + lane < a.e) {
-                        const uint32_t b = (key[i] & 0x80000000u) ? key[i] & 0x7fffffffu : ~key[i];
-                        sum += expf(__uint_as_float(b) - top_value);
-                    }
-#pragma unroll
-                for (int s = 16; s; s >>= 1)
-                    sum += __shfl_xor_sync(0xffffffffu, sum, s);
-            }
-            const float w = expf(v - top_value);
-            chosen += w;
-            if (lane == j) {
-                mine = w;
-                mine_e = e;
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (i * 32 + lane == e)
-                    key[i] = 0;
-        }
+    for (int t = rank * kWarps + warp; t < a.t; t += cluster * kWarps) {
+        int e;
+        float p;
+        choose(t, &e, &p);
         if (lane < a.top) {
-            float p = __fdiv_rn(mine, a.renormalize ? chosen : sum);
-            if (top_value == -__uint_as_float(0x7f800000u))
-                p = 0.f;  // every expert is masked: no share in any
-            if (odd)
-                p = __uint_as_float(0x7fffffffu);
             r.p[t * a.top + lane] = p;
-            r.expert[t * a.top + lane] = p == 0.f ? -1 : mine_e;
+            r.expert[t * a.top + lane] = e;
         }
+    }
+    if (cluster > 1) {
+        __syncwarp();
+        umma::cluster_arrive();
+        umma::cluster_wait();
+        for (int s = threadIdx.x; s < a.t * a.top; s += kThreads) {
+            const int owner = s / a.top / kWarps % cluster;
+            if (owner != rank) {
+                r.p[s] = __uint_as_float(peer_word(r.p + s, owner));
+                r.expert[s] = (int)peer_word(r.expert + s, owner);
+            }
+        }
+        __syncwarp();
+        umma::cluster_arrive();
     }
     __syncthreads();
     const int slots = a.t * a.top;
@@ -218,14 +276,15 @@ struct Up {
 };
 
 template <class T, int COLS, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, int x_vectors) {
+__global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, int x_vectors, int cluster) {
     typedef Up<COLS, ALIGNED> U;
     constexpr int NT = COLS / 8, kDepth = U::kDepth;
     extern __shared__ __align__(128) uint8_t dynamic[];
     int* exchange = (int*)(dynamic + U::kRing);
     int8_t* xs = (int8_t*)(exchange + 2 * U::kExchange);
     const int pitch = xs_pitch(a.d);
-    const Route route = place_route((uint8_t*)xs + min(a.t, COLS) * pitch, a.t * a.top, a.e, COLS);
+    const Route route = place_route((uint8_t*)xs + min(a.t, COLS) * pitch, dynamic, a.t * a.top, a.e, COLS);
+    static_assert(U::kRing >= kMostBuild, "the routing is worked out where the rings will be");
     __shared__ float x_scale[COLS];
     __shared__ uint32_t part[16 * kWarps];
 
@@ -233,10 +292,19 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
     const int g = lane >> 2, tig = lane & 3;
     const bool resident = a.t <= COLS;
     pdl_start();
-    if (resident)  // (the tokens arrive while the routing is worked out)
-        for (int t = 0; t < a.t; ++t)
-            ask_ahead<kThreads>((const T*)a.x + (long long)t * a.ldx, a.d * sizeof(T));
-    route_tokens(a, COLS, route);
+    auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
+    if (resident)
+        largest_of_rows<T, kWarps>(token_row, a.t, a.d, part, x_vectors);
+    route_tokens(a, COLS, route, cluster > 1 ? (int)umma::cluster_rank() : 0, cluster);
+    if (a.t > 8 && blockIdx.x == 0) {
+        const int units = route_bytes(a.t * a.top, a.e, COLS) / 16;
+        for (int i = threadIdx.x; i < units; i += kThreads)
+            a.route[i] = ((const uint4*)route.p)[i];
+    }
+    if (cluster > 1) {
+        __syncwarp();
+        umma::cluster_wait();  // nobody reads this CTA's choices any more
+    }
     const int blocks = (a.f + kUnits - 1) / kUnits;
     const long long tiles = (long long)*route.passes * blocks;
     const int first = (int)(tiles * blockIdx.x / gridDim.x), last = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
@@ -254,12 +322,13 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
         return a.w1 + ((size_t)route.pass_expert[pass] * 2 * a.f + (block >> 1) * (size_t)a.f + u) * (size_t)a.d;
     };
     typename U::W w;
-    int l_tile = first, l_pass = first / blocks, l_block = first - l_pass * blocks, l_step = 0, stage_in = 0;
+    int l_tile = first, l_pass = first / blocks, l_block = first - l_pass * blocks, l_step = 0;
+    uint32_t stage_in = ring, stage_out = ring;
     auto copy_next = [&] {
         if (mine && l_tile < last) {
             if (l_step == 0)
                 w.open([&](int r) { return tile_row(l_pass, l_block, r); }, a.d, half);
-            w.copy(ring + (uint32_t)(stage_in * U::W::kBytes), U::kHalves);
+            w.template copy<true>(stage_in, U::kHalves, a.d - (half + l_step * U::kHalves) * kStep >= U::W::kWhole);
             if (++l_step == mine) {
                 l_step = 0;
                 ++l_tile;
@@ -269,18 +338,16 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
                 }
             }
         }
-        if (++stage_in == kDepth)
-            stage_in = 0;
+        next_stage<kDepth, U::W::kBytes>(stage_in, ring);
         copy_commit();
     };
     for (int i = 0; i < kDepth - 1; ++i)
         copy_next();
-    auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
     if (resident)
-        quantize_cta<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
+        rows_to_whole<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
     __syncthreads();
 
-    int pass = first / blocks, b = first - pass * blocks, cols = 0, e = 0, stage_out = 0;
+    int pass = first / blocks, b = first - pass * blocks, cols = 0, e = 0;
     const short* order = nullptr;
     for (int tile = first; tile < last; ++tile) {
         const int u0 = b * kUnits;
@@ -289,9 +356,10 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
             cols = route.pass_cols[pass];
             order = route.order + route.pass_start[pass];
             if (!resident) {
-                __syncthreads();  // (the last pass's tokens have been read)
-                quantize_cta<T, kWarps>([&](int c) { return token_row(order[c] / a.top); }, cols, a.d, xs, pitch,
-                                        x_scale, part, x_vectors);
+                auto slot_row = [&](int c) { return token_row(order[c] / a.top); };
+                largest_of_rows<T, kWarps>(slot_row, cols, a.d, part, x_vectors);
+                __syncthreads();  // (the last pass's tokens have been read, too)
+                rows_to_whole<T, kWarps>(slot_row, cols, a.d, xs, pitch, x_scale, part, x_vectors);
                 __syncthreads();
             }
         }
@@ -314,9 +382,8 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
             copy_wait<kDepth - 2>();
             __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
             copy_next();
-            const uint32_t stage = ring + (uint32_t)(stage_out * U::W::kBytes);
-            if (++stage_out == kDepth)
-                stage_out = 0;
+            const uint32_t stage = stage_out;
+            next_stage<kDepth, U::W::kBytes>(stage_out, ring);
 #pragma unroll
             for (int j = 0; j < kStep / 64; ++j) {
                 const uint4 lo = U::W::piece16(stage, g, 4 * j + tig, s_lo), hi = U::W::piece16(stage, g + 8, 4 * j + tig, s_hi);
@@ -359,13 +426,13 @@ __global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, in
 }
 
 // ---- down, and the experts' sum ----
-// A CTA makes 16 rows of every token. All its steps, pass after pass in the order of the experts' indices, are one
-// sequence, of which each warp takes an eighth; it adds into sums of its own, which meet at the end in
+// A CTA, or a cluster of CTAs, makes 16 rows of every token. All its steps, pass after pass in the order of the experts' indices, are one
+// sequence, of which each warp takes an equal run; it adds into sums of its own, which meet at the end in
 // the order of the warps: no float atomics, the same bits every time. (Neighbouring steps for each warp: with every
-// eighth step each warp would open every pass.)
-template <int NT, bool ALIGNED>
+// eighth step each warp would open every pass.) Clusters: where d has fewer tiles than the GPU has SMs.
+template <int NT, int DEPTH, bool ALIGNED>
 struct Down {
-    static constexpr int kDepth = 4;
+    static constexpr int kDepth = DEPTH;
     typedef Rows<kRows, ALIGNED> W;
     typedef Rows<8 * NT, true> H;
     static constexpr int kGroups = kStep / kUnits;
@@ -377,24 +444,36 @@ struct Down {
     }
 };
 
-template <int NT, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) {
-    typedef Down<NT, ALIGNED> D;
+template <int NT, int DEPTH, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a, int cluster) {
+    typedef Down<NT, DEPTH, ALIGNED> D;
     constexpr int kDepth = D::kDepth, kCols = 8 * NT;
     extern __shared__ __align__(128) uint8_t dynamic[];
     float* sums = (float*)(dynamic + D::kRing);  // [kWarps][a.t][kRows]
-    const Route route = place_route((uint8_t*)(sums + kWarps * a.t * kRows), a.t * a.top, a.e, kCols);
+    const Route route = place_route((uint8_t*)(sums + kWarps * a.t * kRows), dynamic, a.t * a.top, a.e, kCols);
+    static_assert(D::kRing >= kMostBuild, "the routing is worked out where the rings will be");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
-    const int d0 = blockIdx.x * kRows;
-    // Ahead of the first kernel's end: the routing and the first weights. What is read here was written before
-    // the first kernel began, which let this one start behind its own wait for that.
-    route_tokens(a, kCols, route);
+    const int rank = cluster > 1 ? (int)umma::cluster_rank() : 0;
+    const int d0 = (int)blockIdx.x / cluster * kRows;
+    // Ahead of the first kernel's end: the routing of a few tokens, and with it the first weights. What is read here
+    // was written before the first kernel began, which let this one start behind its own wait for that. The routing
+    // of more takes longer than to fetch the first kernel's.
+    if (a.t <= 8) {
+        route_tokens(a, kCols, route, 0, 1);
+    } else {
+        pdl_start();
+        const int units = route_bytes(a.t * a.top, a.e, kCols) / 16;
+        for (int i = threadIdx.x; i < units; i += kThreads)
+            ((uint4*)route.p)[i] = a.route[i];
+        __syncthreads();
+    }
     const int groups = (a.f + kUnits - 1) / kUnits, width = groups * kUnits;
     const int steps = (a.f + kStep - 1) / kStep;  // of a pass
     const int total = steps * *route.passes;
-    const int first = (int)((long long)total * warp / kWarps), mine = (int)((long long)total * (warp + 1) / kWarps) - first;
+    const int runs = cluster * kWarps, run = rank * kWarps + warp;
+    const int first = (int)((long long)total * run / runs), mine = (int)((long long)total * (run + 1) / runs) - first;
     float* own = sums + warp * a.t * kRows;
     for (int i = lane; i < a.t * kRows; i += 32)
         own[i] = 0.f;
@@ -421,31 +500,37 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) 
     At wl = start, hl = start;
     int w_copied = 0, h_copied = 0;
     bool w_new = true, h_new = true;
-    auto copy_weights = [&] {
+    auto copy_weights = [&](uint32_t stage) {
         if (w_copied < mine) {
             if (w_new)
                 w.open([&](int r) { return w2_row(wl.pass, r); }, a.f, wl.step);
-            w.copy(ring + (uint32_t)(w_copied % kDepth * D::kStage), 1);
+            w.template copy<true>(stage, 1, a.f - wl.step * kStep >= D::W::kWhole);
             w_new = advance(wl);
         }
         ++w_copied;
     };
-    auto copy_hidden = [&] {
+    auto copy_hidden = [&](uint32_t stage) {
         if (h_copied < mine) {
             if (h_new) {
                 const short* order = route.order + route.pass_start[hl.pass];
                 const int cols = route.pass_cols[hl.pass];
                 h.open([&](int r) { return r < cols ? a.hq + (size_t)order[r] * width : nullptr; }, width, hl.step);
                 // a lane copies the scales of a token's groups lane / kCols, and so on
-                sh_from = a.sh + (size_t)order[min(lane % kCols, cols - 1)] * groups;
+                sh_from = a.sh + (size_t)order[min(lane % kCols, cols - 1)] * groups + lane / kCols;
             }
-            const uint32_t stage = ring + (uint32_t)(h_copied % kDepth * D::kStage + D::W::kBytes);
-            h.copy(stage, 1);
+            // (of tokens that are not there: nothing)
+            const bool whole = width - hl.step * kStep >= kStep;
+            const uint32_t hidden = stage + D::W::kBytes, scales = hidden + D::H::kBytes + 4 * lane;
+            h.template copy<false>(hidden, 1, whole);
+            const float* from = sh_from + hl.step * D::kGroups;
 #pragma unroll
-            for (int j = lane / kCols; j < D::kGroups; j += 32 / kCols) {
-                const int group = hl.step * D::kGroups + j;
-                copy_async4(stage + D::H::kBytes + 4 * (j * kCols + lane % kCols),
-                            group < groups ? sh_from + group : sh_from, group < groups);
+            for (int j = 0; j < D::kGroups; j += 32 / kCols) {
+                if (whole) {
+                    copy_async4(scales + 4 * kCols * j, from + j);
+                } else {
+                    const bool some = hl.step * D::kGroups + j + lane / kCols < groups;
+                    copy_async4(scales + 4 * kCols * j, some ? from + j : a.sh, some);
+                }
             }
             h_new = advance(hl);
         }
@@ -453,10 +538,12 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) 
         copy_commit();
     };
     for (int i = 0; i < kDepth - 1; ++i)
-        copy_weights();
-    pdl_start();
+        copy_weights(ring + (uint32_t)(i * D::kStage));
+    if (a.t <= 8)
+        pdl_start();
     for (int i = 0; i < kDepth - 1; ++i)
-        copy_hidden();
+        copy_hidden(ring + (uint32_t)(i * D::kStage));
+    uint32_t stage = ring, free_stage = ring + (uint32_t)((kDepth - 1) * D::kStage);
 
     At at = start;
     float acc[NT][4];
@@ -469,8 +556,9 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) 
     for (int i = 0; i < mine; ++i) {
         copy_wait<kDepth - 2>();
         __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
-        copy_weights();
-        copy_hidden();
+        copy_weights(free_stage);
+        copy_hidden(free_stage);
+        next_stage<kDepth, D::kStage>(free_stage, ring);
         if (fresh) {
             const float* s2 = a.s2 + (size_t)route.pass_expert[at.pass] * a.d;
             s_lo = s2[min(d0 + g, a.d - 1)];
@@ -478,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) 
             sh_lo = (int)((uintptr_t)w2_row(at.pass, g) & 15);
             sh_hi = (int)((uintptr_t)w2_row(at.pass, g + 8) & 15);
         }
-        const uint32_t stage = ring + (uint32_t)(i % kDepth * D::kStage), hidden = stage + D::W::kBytes;
+        const uint32_t hidden = stage + D::W::kBytes;
 #pragma unroll
         for (int j = 0; j < D::kGroups; ++j) {
             const uint2 lo = D::W::piece8(stage, g, 4 * j + tig, sh_lo), hi = D::W::piece8(stage, g + 8, 4 * j + tig, sh_hi);
@@ -495,6 +583,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) 
                 acc[nt][3] = __fmaf_rn(__int2float_rn(c[3]), s1, acc[nt][3]);
             }
         }
+        next_stage<kDepth, D::kStage>(stage, ring);
         const int pass = at.pass;
         fresh = advance(at);
         if (fresh || i + 1 == mine) {
@@ -520,55 +609,105 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a) 
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < a.t * kRows; i += kThreads) {
+    auto store = [&](int i, float v) {
         const int t = i / kRows, d = d0 + i % kRows;
+        if (d < a.d)
+            store_as(a.y, a.dtype, (size_t)t * (size_t)a.ldy + d, v);
+    };
+    for (int i = threadIdx.x; i < a.t * kRows; i += kThreads) {
         float v = 0.f;
 #pragma unroll
         for (int s = 0; s < kWarps; ++s)
             v += sums[s * a.t * kRows + i];
-        if (d < a.d)
-            store_as(a.y, a.dtype, (size_t)t * (size_t)a.ldy + d, v);
+        if (cluster == 1)
+            store(i, v);
+        else
+            sums[i] = v;  // (what this thread alone has read)
     }
+    if (cluster > 1) {
+        // each CTA finishes its share of the tokens' rows
+        __syncwarp();
+        umma::cluster_arrive();
+        umma::cluster_wait();
+        const uint32_t base = shared_address(sums);
+        for (int i = (rank * kThreads + (int)threadIdx.x) * 4; i < a.t * kRows; i += cluster * kThreads * 4) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < cluster; ++c) {
+                const uint4 w = umma::ld_cluster_v4(base + 4u * (uint32_t)i, c);
+                v[0] += __uint_as_float(w.x);
+                v[1] += __uint_as_float(w.y);
+                v[2] += __uint_as_float(w.z);
+                v[3] += __uint_as_float(w.w);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                store(i + j, v[j]);
+        }
+        __syncwarp();
+        umma::cluster_arrive();
+        umma::cluster_wait();  // the others may still read this CTA's sums
+    }
+}
+
+// Passes of eight tokens or of sixteen: eight unless an expert has more than that on average (weights that are read
+// twice come from the L2 the second time, and passes of sixteen leave room for one CTA per SM only)
+bool few_columns(const MoeArgs& a) {
+    return a.t <= 8 || a.t * a.top <= 4 * a.e;
 }
 
 template <class T, int COLS, bool ALIGNED>
 cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
     static umma::ResidentCtas resident;
+    static umma::ClusterCapacity capacity;
     auto kernel = moe_up_kernel<T, COLS, ALIGNED>;
     const int smem = Up<COLS, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx % Vec<T>::N == 0);
     const long long tiles = (long long)a.t * a.top * ((a.f + kUnits - 1) / kUnits);  // at most
-    const long long fit = (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0);
     const Writes writes{a.hq, a.workspace_bytes};
-    return launch_pdl(writes, kernel, dim3((unsigned)(tiles < fit ? tiles : fit)), dim3(kThreads), (size_t)smem, st,
-                      a, x_vectors);
+    // clusters of four for the routing of many tokens (whole clusters live inside a GPC: eight would leave SMs idle)
+    const int cluster = a.t <= 8 ? 1 : 4;
+    const long long fit = cluster == 1 ? (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0)
+                                       : 4LL * capacity.clusters(kernel, 4, kThreads, smem);
+    const long long ctas = tiles < fit ? (tiles + cluster - 1) / cluster * cluster : fit;
+    return launch_pdl_cluster(writes, kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, cluster, st, a,
+                              x_vectors, cluster);
 }
 template <class T>
 cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
     const bool aligned = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
-    if (a.t <= 8)
+    if (few_columns(a))
         return aligned ? launch_up<T, 8, true>(a, st) : launch_up<T, 8, false>(a, st);
     return aligned ? launch_up<T, 16, true>(a, st) : launch_up<T, 16, false>(a, st);
 }
 
-template <int NT, bool ALIGNED>
+template <int NT, int DEPTH, bool ALIGNED>
 cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
-    auto kernel = moe_down_kernel<NT, ALIGNED>;
-    const int smem = Down<NT, ALIGNED>::smem(a);
+    auto kernel = moe_down_kernel<NT, DEPTH, ALIGNED>;
+    const int smem = Down<NT, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     const Writes writes{a.y, ((size_t)(a.t - 1) * (size_t)a.ldy + (size_t)a.d) * dtype_bytes(a.dtype)};
-    return launch_pdl(writes, kernel, dim3((unsigned)((a.d - 1) / kRows + 1)), dim3(kThreads), (size_t)smem, st, a);
+    // a CTA for every SM where each warp still has two steps (experts with tokens: at most as many as slots)
+    const int tiles = (a.d - 1) / kRows + 1, slots = a.t * a.top;
+    const long long steps = (long long)(slots < a.e ? slots : a.e) * ((a.f + kStep - 1) / kStep);
+    int cluster = 1;
+    while (cluster < 8 && tiles * cluster < umma::sm_count() && steps >= 2LL * 2 * cluster * kWarps)
+        cluster *= 2;
+    return launch_pdl_cluster(writes, kernel, dim3((unsigned)(tiles * cluster)), dim3(kThreads), (size_t)smem, cluster,
+                              st, a, cluster);
 }
 cudaError_t launch_down(const MoeArgs& a, cudaStream_t st) {
     const bool aligned = ((uintptr_t)a.w2 & 15) == 0 && a.f % 16 == 0;
+    // (as deep a ring as leaves room for two CTAs per SM beside their tokens' sums)
     if (a.t <= 8)
-        return aligned ? launch_down_as<1, true>(a, st) : launch_down_as<1, false>(a, st);
-    return aligned ? launch_down_as<2, true>(a, st) : launch_down_as<2, false>(a, st);
+        return aligned ? launch_down_as<1, 4, true>(a, st) : launch_down_as<1, 4, false>(a, st);
+    if (few_columns(a))
+        return aligned ? launch_down_as<1, 3, true>(a, st) : launch_down_as<1, 3, false>(a, st);
+    return aligned ? launch_down_as<2, 3, true>(a, st) : launch_down_as<2, 3, false>(a, st);
 }
 
 template <class T>

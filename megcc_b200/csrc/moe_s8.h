@@ -4,6 +4,12 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#if defined(__CUDACC__)
+#define MB200_HD __host__ __device__
+#else
+#define MB200_HD
+#endif
+
 namespace mb200 {
 namespace scaled {
 
@@ -11,6 +17,17 @@ constexpr int kMoeMaxTokens = 64, kMoeMaxTop = 16, kMoeMaxExperts = 512;
 // the tokens' whole numbers lie in shared memory: eight rows (sixteen with more than eight tokens)
 constexpr int kMoeMaxDepthFew = 16384, kMoeMaxDepth = 8192;
 
+// The routing, as the kernels keep it: bytes for `slots` token-expert pairs in passes of `cols` tokens at most
+MB200_HD constexpr int up16(int v) {
+    return (v + 15) / 16 * 16;
+}
+// every expert with tokens, and one more for each `cols` slots
+MB200_HD constexpr int most_passes(int slots, int experts, int cols) {
+    return (slots < experts ? slots : experts) + slots / cols;
+}
+MB200_HD constexpr int route_bytes(int slots, int experts, int cols) {
+    return up16(4 * slots) + up16(2 * slots) + 3 * up16(2 * most_passes(slots, experts, cols)) + 16;
+}
 struct MoeArgs {
     int t, d, f, e, top, renormalize, dtype;
     const void* x;
@@ -23,6 +40,7 @@ struct MoeArgs {
     // the hidden layer: [slots][f rounded up to 32] whole numbers, [slots][f / 32 rounded up] scales
     int8_t* hq;
     float* sh;
+    uint4* route;  // the first kernel's routing, for the second (more than eight tokens)
     size_t workspace_bytes;
 };
 

@@ -101,9 +101,12 @@ int check_moe(const mb200_moe_param* p) {
 size_t moe_hidden_bytes(const mb200_moe_param* p) {  // whole numbers of the hidden layer
     return align_up((size_t)p->tokens * p->top_k * align_up((size_t)p->f, 32), 256);
 }
+size_t moe_scale_bytes(const mb200_moe_param* p) {  // and their groups' scales
+    return align_up((size_t)p->tokens * p->top_k * (align_up((size_t)p->f, 32) / 32) * sizeof(float), 256);
+}
 size_t moe_bytes(const mb200_moe_param* p) {
-    return moe_hidden_bytes(p) +
-           align_up((size_t)p->tokens * p->top_k * (align_up((size_t)p->f, 32) / 32) * sizeof(float), 256);
+    return moe_hidden_bytes(p) + moe_scale_bytes(p) +
+           align_up((size_t)route_bytes(p->tokens * p->top_k, p->experts, 8), 256);
 }
 
 }  // namespace
@@ -262,6 +265,7 @@ int mb200_moe_s8(
     a.w1 = w1, a.s1 = w1_scales, a.w2 = w2, a.s2 = w2_scales;
     a.y = y, a.ldy = ldy;
     a.hq = (int8_t*)workspace, a.sh = (float*)((uint8_t*)workspace + moe_hidden_bytes(p));
+    a.route = (uint4*)((uint8_t*)a.sh + moe_scale_bytes(p));
     a.workspace_bytes = moe_bytes(p);
     return launch_moe(a, (cudaStream_t)stream);
 }

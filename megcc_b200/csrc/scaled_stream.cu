@@ -151,30 +151,34 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     if (!kFloat)
         // (no copies for tokens that are not there: every CTA asks for the same few lines)
         a.open([&](int r) { return m0 + r < p.m ? a_row(r) : nullptr; }, k, warp);
-    auto copy_weights = [&](int i) {
+    auto copy_weights = [&](uint32_t stage, int i) {
         if (i < mine)
-            w.copy(ring + (uint32_t)(i % kDepth * S::kStage), kWarps);
+            w.template copy<true>(stage, kWarps, k - (warp + i * kWarps) * kStep >= S::W::kWhole);
     };
-    auto copy_tokens = [&](int i) {
+    auto copy_tokens = [&](uint32_t stage, int i) {
         if (!kFloat && i < mine)
-            a.copy(ring + (uint32_t)(i % kDepth * S::kStage + S::W::kBytes), kWarps);
+            a.template copy<false>(stage + S::W::kBytes, kWarps, k - (warp + i * kWarps) * kStep >= S::A::kWhole);
     };
     if (p.b_early)
         for (int i = 0; i < kDepth - 1; ++i)
-            copy_weights(i);
+            copy_weights(ring + (uint32_t)(i * S::kStage), i);
     pdl_start();
     for (int i = 0; i < kDepth - 1; ++i) {
+        const uint32_t stage = ring + (uint32_t)(i * S::kStage);
         if (!p.b_early)
-            copy_weights(i);
-        copy_tokens(i);
+            copy_weights(stage, i);
+        copy_tokens(stage, i);
         copy_commit();
     }
     // scales of what this thread stores in the end
     const int row = threadIdx.x & 15, n = n0 + row;
     const float sb = n < p.n ? p.sb[n] : 0.f, bias = p.bias && n < p.n ? p.bias[n] : 0.f;
     if constexpr (kFloat) {
-        quantize_cta<XT, kWarps>([&](int r) { return (const XT*)p.a + (long long)(m0 + r) * p.lda; },
-                                 min(kCols, p.m - m0), k, xs, pitch, col_scale, part, x_vectors);
+        auto x_row = [&](int r) { return (const XT*)p.a + (long long)(m0 + r) * p.lda; };
+        const int rows = min(kCols, p.m - m0);
+        largest_of_rows<XT, kWarps>(x_row, rows, k, part, x_vectors);
+        __syncthreads();
+        rows_to_whole<XT, kWarps>(x_row, rows, k, xs, pitch, col_scale, part, x_vectors);
         __syncthreads();
     } else {
         if (threadIdx.x < kCols)
@@ -193,13 +197,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
         acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
+    uint32_t stage = ring, free_stage = ring + (uint32_t)((kDepth - 1) * S::kStage);
     for (int i = 0; i < mine; ++i) {
         copy_wait<kDepth - 2>();
         __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
-        copy_weights(i + kDepth - 1);
-        copy_tokens(i + kDepth - 1);
+        copy_weights(free_stage, i + kDepth - 1);
+        copy_tokens(free_stage, i + kDepth - 1);
         copy_commit();
-        const uint32_t stage = ring + (uint32_t)(i % kDepth * S::kStage);
+        next_stage<kDepth, S::kStage>(free_stage, ring);
         const int step = warp + i * kWarps;
 #pragma unroll
         for (int j = 0; j < kStep / 64; ++j) {
@@ -218,6 +223,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
                 mma_64(acc[nt], lo, hi, t);
             }
         }
+        next_stage<kDepth, S::kStage>(stage, ring);
     }
     copy_wait<0>();
     __syncthreads();

@@ -20,6 +20,12 @@ constexpr int kStep = 128;
 __device__ __forceinline__ void copy_async16(uint32_t smem, const void* p, bool there) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem), "l"(p), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy_async16(uint32_t smem, const void* p) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem), "l"(p) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t smem, const void* p) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem), "l"(p) : "memory");
+}
 __device__ __forceinline__ void copy_async4(uint32_t smem, const void* p, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem), "l"(p), "r"(there ? 4 : 0) : "memory");
 }
@@ -78,7 +84,7 @@ struct Rows {
             to[i] = r * kPitch + unit_at(r, u) * 16;
         }
     }
-    // row(r): address of row r, or null for a row of zeros (row 0 is none); k: its bytes; step: the first
+    // row(r): address of row r, or null for one that is not there (row 0 is); k: its bytes; step: the first
     template <class RowAt>
     __device__ __forceinline__ void open(RowAt row, int k, int step) {
         const int lane = threadIdx.x & 31;
@@ -98,18 +104,31 @@ struct Rows {
                 left[i] = k + s - 16 * u - step * kStep;
         }
     }
-    // the next step; `by`: how many steps further the one behind it is
-    __device__ __forceinline__ void copy(uint32_t stage, int by) {
+    // The next step; `by`: how many steps further the one behind it is. whole: rows go on for kWhole bytes at
+    // least, the same for all lanes (every step but a row's last: those that it has zeros behind). Rows that are not
+    // there are left out: what stands in their place is multiplied, and its column of the result not looked at.
+    static constexpr int kWhole = 16 * kUnits;
+    template <bool ALL_THERE>
+    __device__ __forceinline__ void copy(uint32_t stage, int by, bool whole) {
         const int lane = threadIdx.x & 31;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i)
+                if ((ROWS * kUnits % 32 == 0 || lane + 32 * i < ROWS * kUnits) && (ALL_THERE || (there >> i & 1)))
+                    copy_async16(stage + to[i], from[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i)
+                if ((ROWS * kUnits % 32 == 0 || lane + 32 * i < ROWS * kUnits) && (ALL_THERE || (there >> i & 1))) {
+                    const bool some = left[ALIGNED ? 0 : i] > 0;
+                    copy_async16(stage + to[i], some ? from[i] : any, some);
+                }
+        }
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            if (ROWS * kUnits % 32 == 0 || lane + 32 * i < ROWS * kUnits) {
-                const bool some = (ALIGNED ? left[0] : left[i]) > 0 && (there >> i & 1);
-                copy_async16(stage + to[i], some ? from[i] : any, some);
-            }
             from[i] += by * kStep;
-            if (!ALIGNED || i + 1 == kCopies)
-                left[ALIGNED ? 0 : i] -= by * kStep;
+            if (!ALIGNED || i == 0)
+                left[i] -= by * kStep;
         }
     }
     // 16 bytes of row r from byte 16 * part on; s: the row's address modulo 16
@@ -136,66 +155,84 @@ struct Rows {
     }
 };
 
+// A place in a ring of DEPTH stages
+template <int DEPTH, int BYTES>
+__device__ __forceinline__ void next_stage(uint32_t& stage, uint32_t ring) {
+    stage += BYTES;
+    if (stage == ring + (uint32_t)(DEPTH * BYTES))
+        stage = ring;
+}
+
 // the first `n` bytes (n <= 0: none) of 16
 __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
     auto cut = [](uint32_t w, int left) { return left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u); };
     return make_uint4(cut(v.x, n), cut(v.y, n - 4), cut(v.z, n - 8), cut(v.w, n - 12));
 }
 
-// `rows` (up to 16) rows of activations as whole numbers in shared memory, zeros behind them up to whole steps, by all
-// threads of a CTA; row(r): the row's address. part: [16][WARPS] words of shared memory. A barrier of the
-// CTA has to follow before they are read.
+// Rows of activations (up to 16) as whole numbers in shared memory, by all threads of a CTA, in two halves with a
+// barrier of the CTA between them and another behind. WARPS / rows warps (one at least) share a row, so that a few
+// rows' loads are on their way together. row(r): a row's address; part: [16][WARPS] words of shared memory.
+template <int WARPS>
+__device__ __forceinline__ int warps_per_row(int rows) {
+    return rows >= WARPS ? 1 : rows * 2 >= WARPS ? 2 : rows * 4 >= WARPS ? 4 : WARPS;
+}
 template <class T, int WARPS, class RowAt>
-__device__ __forceinline__ void quantize_cta(
-        RowAt row, int rows, int k, int8_t* xs, int pitch, float* scale, uint32_t* part, bool vectors) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kAhead = 2;  // rows whose loads are on their way together
-    for (int r0 = 0; r0 < rows; r0 += kAhead) {
-        uint32_t bits[kAhead] = {0};
-        for (int i = tid * 16; i < k; i += WARPS * 512) {
-            float v[kAhead][16];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (r0 + j < rows)
-                    load_piece((const T*)row(r0 + j), i, k, vectors, v[j]);
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (r0 + j < rows)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        bits[j] = max(bits[j], magnitude(v[j][e]));
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-            if (r0 + j < rows) {
-                const uint32_t b = __reduce_max_sync(0xffffffffu, bits[j]);
-                if (lane == 0)
-                    part[(r0 + j) * WARPS + warp] = b;
-            }
-    }
-    __syncthreads();
-    const int end = (k + kStep - 1) / kStep * kStep;
-    for (int r = 0; r < rows; ++r) {
+__device__ __forceinline__ void largest_of_rows(RowAt row, int rows, int k, uint32_t* part, bool vectors) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int share = warps_per_row<WARPS>(rows), stride = share * 512;
+    for (int r = warp / share; r < rows; r += WARPS / share) {
+        const T* x = (const T*)row(r);
         uint32_t bits = 0;
+        int i = (warp % share * 32 + lane) * 16;
+        if (vectors) {
+            constexpr int N = 16 / Vec<T>::N;  // loads of a piece
+            uint32_t vm = 0;
+            for (; i + stride + 16 <= k; i += 2 * stride) {
+                uint4 w[2 * N];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w)
+                for (int j = 0; j < N; ++j) {
+                    w[j] = ((const uint4*)(x + i))[j];
+                    w[N + j] = ((const uint4*)(x + i + stride))[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 2 * N; ++j)
+                    vm = vec_max<T>(vm, w[j]);
+            }
+            bits = max_bits<T>(vm);
+        }
+        for (; i < k; i += stride) {
+            float v[16];
+            load_piece(x, i, k, vectors, v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                bits = max(bits, magnitude(v[e]));
+        }
+        bits = __reduce_max_sync(0xffffffffu, bits);
+        if (lane == 0)
+            part[r * WARPS + warp % share] = bits;
+    }
+}
+// (zeros behind each row up to whole steps)
+template <class T, int WARPS, class RowAt>
+__device__ __forceinline__ void rows_to_whole(
+        RowAt row, int rows, int k, int8_t* xs, int pitch, float* scale, const uint32_t* part, bool vectors) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int share = warps_per_row<WARPS>(rows), end = (k + kStep - 1) / kStep * kStep;
+    for (int r = warp / share; r < rows; r += WARPS / share) {
+        const T* x = (const T*)row(r);
+        uint32_t bits = 0;
+        for (int w = 0; w < share; ++w)
             bits = max(bits, part[r * WARPS + w]);
         const RowScale s = row_scale(bits);
-        if (tid == 0)
+        if (warp % share == 0 && lane == 0)
             scale[r] = s.scale;
-        for (int i = tid * 16; i < end; i += WARPS * 512) {
+#pragma unroll 2
+        for (int i = (warp % share * 32 + lane) * 16; i < end; i += share * 512) {
             float v[16];
-            load_piece((const T*)row(r), i, k, vectors, v);
+            load_piece(x, i, k, vectors, v);
             *(uint4*)(xs + r * pitch + i) = pack_piece(v, s);
         }
     }
-}
-// Asks for what the CTA's threads will read soon: `bytes` from p on, into the L1.
-template <int THREADS>
-__device__ __forceinline__ void ask_ahead(const void* p, size_t bytes) {
-    const uintptr_t first = (uintptr_t)p & ~(uintptr_t)127, end = (uintptr_t)p + bytes;
-    for (uintptr_t at = first + threadIdx.x * 128u; at < end; at += THREADS * 128u)
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
 }
 // bytes between rows of xs: whole steps, and two rows on other banks
 __host__ __device__ constexpr int xs_pitch(int k) {

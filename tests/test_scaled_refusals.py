@@ -85,6 +85,6 @@ def test_moe_workspace_and_null_parameters():
     size = _lib.lib().mb200_moe_s8_workspace_bytes
     assert size(None) == 0 and _lib.lib().mb200_moe_s8(None, *[P, 64] + [P] * 6 + [64, P, 0, None]) == NULL_PTR
     p = _lib.MoeParam(2, 64, 33, 4, 2, 1, 2)
-    assert size(ctypes.byref(p)) == 256 + 256  # 4 slots of 64 whole numbers, of 2 scales
+    assert size(ctypes.byref(p)) == 256 + 256 + 256  # 4 slots of 64 whole numbers, of 2 scales, the routing
     p.tokens = 65
     assert size(ctypes.byref(p)) == 0
