@@ -69,8 +69,13 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 }
 
 // One token's experts, by a warp: lane j < top gets the j-th choice's index and p. 32 * R experts at most.
+// (Not in line: five of them in a kernel cost each launch several fetches of instructions.)
+struct Choice {
+    int expert;
+    float p;
+};
 template <int R>
-__device__ __forceinline__ void choose_experts(const MoeArgs& a, const float* row, int* expert, float* share) {
+__device__ __noinline__ Choice choose_experts(const float* row, int experts, int top, int renormalize) {
     const int lane = threadIdx.x & 31;
     const float inf = __uint_as_float(0x7f800000u);
     uint32_t key[R];
@@ -78,14 +83,14 @@ __device__ __forceinline__ void choose_experts(const MoeArgs& a, const float* ro
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int e = i * 32 + lane;
-        const float v = e < a.e ? row[e] : -inf;
-        key[i] = e < a.e ? rank_key(v) : 0u;
+        const float v = e < experts ? row[e] : -inf;
+        key[i] = e < experts ? rank_key(v) : 0u;
         odd |= !(v < inf);
     }
     odd = __any_sync(0xffffffffu, odd);
     float top_value = 0.f, sum = 0.f, chosen = 0.f, mine = 0.f;
     int mine_e = -1;
-    for (int j = 0; j < a.top; ++j) {
+    for (int j = 0; j < top; ++j) {
         uint32_t best = 0;
         int at = 0;
 #pragma unroll
@@ -117,16 +122,15 @@ __device__ __forceinline__ void choose_experts(const MoeArgs& a, const float* ro
             if (i * 32 + lane == e)
                 key[i] = 0;
     }
-    mine = lane < a.top ? expf(mine - top_value) : 0.f;
-    for (int j = 0; j < a.top; ++j)
+    mine = lane < top ? expf(mine - top_value) : 0.f;
+    for (int j = 0; j < top; ++j)
         chosen += __shfl_sync(0xffffffffu, mine, j);
-    float p = __fdiv_rn(mine, a.renormalize ? chosen : sum);
+    float p = __fdiv_rn(mine, renormalize ? chosen : sum);
     if (top_value == -inf)
         p = 0.f;  // every expert is masked: no share in any
     if (odd)
         p = __uint_as_float(0x7fffffffu);
-    *share = p;
-    *expert = lane >= a.top || p == 0.f ? -1 : mine_e;
+    return {lane >= top || p == 0.f ? -1 : mine_e, p};
 }
 
 // A value at the same place in another CTA of the cluster
@@ -142,55 +146,48 @@ __device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
 // and with a cluster umma::cluster_wait() has to follow before r.expert's memory is used for something else.
 __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int rank, int cluster) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto choose = [&](int t, int* e, float* p) {
+    if (a.t > 1)
+        for (int e = threadIdx.x; e < a.e; e += kThreads)
+            r.count[e] = 0;
+    for (int t = rank * kWarps + warp; t < a.t; t += cluster * kWarps) {
         const float* row = a.logits + (size_t)t * a.e;
+        Choice c;
         if (a.e <= 32)
-            choose_experts<1>(a, row, e, p);
+            c = choose_experts<1>(row, a.e, a.top, a.renormalize);
         else if (a.e <= 64)
-            choose_experts<2>(a, row, e, p);
+            c = choose_experts<2>(row, a.e, a.top, a.renormalize);
         else if (a.e <= 128)
-            choose_experts<4>(a, row, e, p);
+            c = choose_experts<4>(row, a.e, a.top, a.renormalize);
         else if (a.e <= 256)
-            choose_experts<8>(a, row, e, p);
+            c = choose_experts<8>(row, a.e, a.top, a.renormalize);
         else
-            choose_experts<kMoeMaxExperts / 32>(a, row, e, p);
-    };
-    if (a.t == 1) {
-        // one token: a pass for each of its experts, in the order of their indices
-        if (warp == 0) {
-            int e;
-            float p;
-            choose(0, &e, &p);
+            c = choose_experts<kMoeMaxExperts / 32>(row, a.e, a.top, a.renormalize);
+        if (lane < a.top)
+            r.p[t * a.top + lane] = c.p;
+        if (a.t > 1) {
+            if (lane < a.top)
+                r.expert[t * a.top + lane] = c.expert;
+        } else {
+            // one token: a pass for each of its experts, in the order of their indices
             int before = 0;
             for (int j = 0; j < a.top; ++j) {
-                const int other = __shfl_sync(0xffffffffu, e, j);
-                before += other >= 0 && other < e;
+                const int other = __shfl_sync(0xffffffffu, c.expert, j);
+                before += other >= 0 && other < c.expert;
             }
-            if (lane < a.top)
-                r.p[lane] = p;
-            if (e >= 0) {
+            if (c.expert >= 0) {
                 r.order[before] = (short)lane;
-                r.pass_expert[before] = (short)e;
+                r.pass_expert[before] = (short)c.expert;
                 r.pass_start[before] = (short)before;
                 r.pass_cols[before] = 1;
             }
-            const uint32_t some = __ballot_sync(0xffffffffu, e >= 0);
+            const uint32_t some = __ballot_sync(0xffffffffu, c.expert >= 0);
             if (lane == 0)
                 *r.passes = __popc(some);
         }
+    }
+    if (a.t == 1) {
         __syncthreads();
         return;
-    }
-    for (int e = threadIdx.x; e < a.e; e += kThreads)
-        r.count[e] = 0;
-    for (int t = rank * kWarps + warp; t < a.t; t += cluster * kWarps) {
-        int e;
-        float p;
-        choose(t, &e, &p);
-        if (lane < a.top) {
-            r.p[t * a.top + lane] = p;
-            r.expert[t * a.top + lane] = e;
-        }
     }
     if (cluster > 1) {
         __syncwarp();
