@@ -259,9 +259,9 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
 // of its eight warps have 16 rows each (gate, gate, up, up) and every other step of d, the other four the same rows
 // and the remaining steps; each warp's ring runs on over the ends of tiles. COLS tokens at once; with no more
 // tokens than that all of them stay in shared memory for the whole kernel.
-template <int COLS, bool ALIGNED>
+template <int COLS, int DEPTH, bool ALIGNED>
 struct Up {
-    static constexpr int kDepth = COLS == 8 || ALIGNED ? 4 : 3;
+    static constexpr int kDepth = DEPTH;
     static constexpr int kHalves = 2;  // warps that share a tile's steps
     typedef Rows<16, ALIGNED> W;
     static constexpr int kRing = kWarps * kDepth * W::kBytes;
@@ -272,9 +272,9 @@ struct Up {
     }
 };
 
-template <class T, int COLS, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 2) moe_up_kernel(const MoeArgs a, int x_vectors, int cluster) {
-    typedef Up<COLS, ALIGNED> U;
+template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a, int x_vectors, int cluster) {
+    typedef Up<COLS, DEPTH, ALIGNED> U;
     constexpr int NT = COLS / 8, kDepth = U::kDepth;
     extern __shared__ __align__(128) uint8_t dynamic[];
     int* exchange = (int*)(dynamic + U::kRing);
@@ -441,8 +441,8 @@ struct Down {
     }
 };
 
-template <int NT, int DEPTH, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const MoeArgs a, int cluster) {
+template <int NT, int DEPTH, int CTAS, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs a, int cluster) {
     typedef Down<NT, DEPTH, ALIGNED> D;
     constexpr int kDepth = D::kDepth, kCols = 8 * NT;
     extern __shared__ __align__(128) uint8_t dynamic[];
@@ -652,13 +652,13 @@ bool few_columns(const MoeArgs& a) {
     return a.t <= 8 || a.t * a.top <= 4 * a.e;
 }
 
-template <class T, int COLS, bool ALIGNED>
-cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
+template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
+cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
     static umma::ResidentCtas resident;
     static umma::ClusterCapacity capacity;
-    auto kernel = moe_up_kernel<T, COLS, ALIGNED>;
-    const int smem = Up<COLS, ALIGNED>::smem(a);
+    auto kernel = moe_up_kernel<T, COLS, DEPTH, CTAS, ALIGNED>;
+    const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx % Vec<T>::N == 0);
@@ -675,15 +675,17 @@ cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
 template <class T>
 cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
     const bool aligned = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
+    if (a.t <= 8)
+        return aligned ? launch_up_as<T, 8, 3, 3, true>(a, st) : launch_up_as<T, 8, 3, 3, false>(a, st);
     if (few_columns(a))
-        return aligned ? launch_up<T, 8, true>(a, st) : launch_up<T, 8, false>(a, st);
-    return aligned ? launch_up<T, 16, true>(a, st) : launch_up<T, 16, false>(a, st);
+        return aligned ? launch_up_as<T, 8, 4, 2, true>(a, st) : launch_up_as<T, 8, 4, 2, false>(a, st);
+    return aligned ? launch_up_as<T, 16, 4, 2, true>(a, st) : launch_up_as<T, 16, 3, 2, false>(a, st);
 }
 
-template <int NT, int DEPTH, bool ALIGNED>
+template <int NT, int DEPTH, int CTAS, bool ALIGNED>
 cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
-    auto kernel = moe_down_kernel<NT, DEPTH, ALIGNED>;
+    auto kernel = moe_down_kernel<NT, DEPTH, CTAS, ALIGNED>;
     const int smem = Down<NT, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
@@ -701,10 +703,10 @@ cudaError_t launch_down(const MoeArgs& a, cudaStream_t st) {
     const bool aligned = ((uintptr_t)a.w2 & 15) == 0 && a.f % 16 == 0;
     // (as deep a ring as leaves room for two CTAs per SM beside their tokens' sums)
     if (a.t <= 8)
-        return aligned ? launch_down_as<1, 4, true>(a, st) : launch_down_as<1, 4, false>(a, st);
+        return aligned ? launch_down_as<1, 3, 3, true>(a, st) : launch_down_as<1, 3, 3, false>(a, st);
     if (few_columns(a))
-        return aligned ? launch_down_as<1, 3, true>(a, st) : launch_down_as<1, 3, false>(a, st);
-    return aligned ? launch_down_as<2, 3, true>(a, st) : launch_down_as<2, 3, false>(a, st);
+        return aligned ? launch_down_as<1, 3, 2, true>(a, st) : launch_down_as<1, 3, 2, false>(a, st);
+    return aligned ? launch_down_as<2, 3, 2, true>(a, st) : launch_down_as<2, 3, 2, false>(a, st);
 }
 
 template <class T>
