@@ -31,7 +31,7 @@ constexpr int kRows = 16;             // rows of w2 per CTA of the second kernel
 // Where the tokens go, in shared memory: as large as the call's tokens and experts ask for.
 struct Route {
     float* p;      // by slot = token * top + rank
-    short* order;  // slots by expert
+    int* order;    // slots by expert, each with its token in the upper half
     // the passes: an expert and up to `cols` of its slots
     short *pass_expert, *pass_start, *pass_cols;
     int* passes;
@@ -44,8 +44,8 @@ __device__ __forceinline__ Route place_route(uint8_t* at, uint8_t* build, int sl
     Route r;
     r.p = (float*)at;
     at += up16(4 * slots);
-    r.order = (short*)at;
-    at += up16(2 * slots);
+    r.order = (int*)at;
+    at += up16(4 * slots);
     const int n = up16(2 * most_passes(slots, experts, cols));
     r.pass_expert = (short*)at;
     r.pass_start = (short*)(at + n);
@@ -68,14 +68,15 @@ __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-// One token's experts, by a warp: lane j < top gets the j-th choice's index and p. 32 * R experts at most.
-// (Not in line: five of them in a kernel cost each launch several fetches of instructions.)
+// One token's experts, by a warp: lane j < top gets the j-th choice's index and p. Each choice is the largest of what
+// comes behind the one before it (smaller, or equal with a higher index), so nothing is crossed out and the
+// logits may be read again and again: the first 128 from registers.
 struct Choice {
     int expert;
     float p;
 };
-template <int R>
 __device__ __noinline__ Choice choose_experts(const float* row, int experts, int top, int renormalize) {
+    constexpr int R = 4;
     const int lane = threadIdx.x & 31;
     const float inf = __uint_as_float(0x7f800000u);
     uint32_t key[R];
@@ -87,48 +88,60 @@ __device__ __noinline__ Choice choose_experts(const float* row, int experts, int
         key[i] = e < experts ? rank_key(v) : 0u;
         odd |= !(v < inf);
     }
-    odd = __any_sync(0xffffffffu, odd);
-    float top_value = 0.f, sum = 0.f, chosen = 0.f, mine = 0.f;
+    uint32_t last = ~0u;
+    int last_e = -1;
+    float top_value = 0.f, mine = 0.f;
     int mine_e = -1;
+#pragma unroll 1
     for (int j = 0; j < top; ++j) {
         uint32_t best = 0;
         int at = 0;
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (key[i] > best) {
+        for (int i = 0; i < R; ++i) {
+            const int e = i * 32 + lane;
+            if (key[i] > best && (key[i] < last || (key[i] == last && e > last_e))) {
                 best = key[i];
-                at = i;
+                at = e;
             }
-        const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-        const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)(at * 32 + lane) : ~0u);
-        const float v = key_value(high);
-        if (j == 0) {
-            // (the first choice is the largest logit) all exponentials, from the keys still in place
-            top_value = v;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (key[i] != 0)
-                    sum += expf(key_value(key[i]) - top_value);
-#pragma unroll
-            for (int s = 16; s; s >>= 1)
-                sum += __shfl_xor_sync(0xffffffffu, sum, s);
         }
+#pragma unroll 1
+        for (int e = R * 32 + lane; e < experts; e += 32) {
+            const uint32_t k = rank_key(row[e]);
+            if (k > best && (k < last || (k == last && e > last_e))) {
+                best = k;
+                at = e;
+            }
+        }
+        last = __reduce_max_sync(0xffffffffu, best);
+        last_e = (int)__reduce_min_sync(0xffffffffu, best == last ? (uint32_t)at : ~0u);
+        if (j == 0)
+            top_value = key_value(last);
         if (lane == j) {
-            mine = v;
-            mine_e = e;
+            mine = key_value(last);
+            mine_e = last_e;
         }
+    }
+    float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (i * 32 + lane == e)
-                key[i] = 0;
+    for (int i = 0; i < R; ++i)
+        if (key[i] != 0)
+            sum += expf(key_value(key[i]) - top_value);
+#pragma unroll 1
+    for (int e = R * 32 + lane; e < experts; e += 32) {
+        odd |= !(row[e] < inf);
+        sum += expf(row[e] - top_value);
     }
     mine = lane < top ? expf(mine - top_value) : 0.f;
-    for (int j = 0; j < top; ++j)
-        chosen += __shfl_sync(0xffffffffu, mine, j);
+    float chosen = mine;
+#pragma unroll
+    for (int s = 16; s; s >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        chosen += __shfl_xor_sync(0xffffffffu, chosen, s);
+    }
     float p = __fdiv_rn(mine, renormalize ? chosen : sum);
     if (top_value == -inf)
         p = 0.f;  // every expert is masked: no share in any
-    if (odd)
+    if (__any_sync(0xffffffffu, odd))
         p = __uint_as_float(0x7fffffffu);
     return {lane >= top || p == 0.f ? -1 : mine_e, p};
 }
@@ -149,19 +162,10 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
     if (a.t > 1)
         for (int e = threadIdx.x; e < a.e; e += kThreads)
             r.count[e] = 0;
+#pragma unroll 1
     for (int t = rank * kWarps + warp; t < a.t; t += cluster * kWarps) {
         const float* row = a.logits + (size_t)t * a.e;
-        Choice c;
-        if (a.e <= 32)
-            c = choose_experts<1>(row, a.e, a.top, a.renormalize);
-        else if (a.e <= 64)
-            c = choose_experts<2>(row, a.e, a.top, a.renormalize);
-        else if (a.e <= 128)
-            c = choose_experts<4>(row, a.e, a.top, a.renormalize);
-        else if (a.e <= 256)
-            c = choose_experts<8>(row, a.e, a.top, a.renormalize);
-        else
-            c = choose_experts<kMoeMaxExperts / 32>(row, a.e, a.top, a.renormalize);
+        const Choice c = choose_experts(row, a.e, a.top, a.renormalize);
         if (lane < a.top)
             r.p[t * a.top + lane] = c.p;
         if (a.t > 1) {
@@ -170,12 +174,13 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
         } else {
             // one token: a pass for each of its experts, in the order of their indices
             int before = 0;
+#pragma unroll 1
             for (int j = 0; j < a.top; ++j) {
                 const int other = __shfl_sync(0xffffffffu, c.expert, j);
                 before += other >= 0 && other < c.expert;
             }
             if (c.expert >= 0) {
-                r.order[before] = (short)lane;
+                r.order[before] = lane;
                 r.pass_expert[before] = (short)c.expert;
                 r.pass_start[before] = (short)before;
                 r.pass_cols[before] = 1;
@@ -193,6 +198,7 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
         __syncwarp();
         umma::cluster_arrive();
         umma::cluster_wait();
+#pragma unroll 1
         for (int s = threadIdx.x; s < a.t * a.top; s += kThreads) {
             const int owner = s / a.top / kWarps % cluster;
             if (owner != rank) {
@@ -205,12 +211,14 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
     }
     __syncthreads();
     const int slots = a.t * a.top;
+#pragma unroll 1
     for (int s = threadIdx.x; s < slots; s += kThreads)
         if (r.expert[s] >= 0)
             atomicAdd(&r.count[r.expert[s]], 1);
     __syncthreads();
     if (warp == 0) {
         int start = 0, passes = 0;
+#pragma unroll 1
         for (int e0 = 0; e0 < a.e; e0 += 32) {
             const int e = e0 + lane;
             const int n = e < a.e ? r.count[e] : 0, np = (n + cols - 1) / cols;
@@ -225,6 +233,7 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
             }
             if (e < a.e)
                 r.at[e] = start + s - n;
+#pragma unroll 1
             for (int i = 0; i < np; ++i) {
                 const int to = passes + q - np + i;
                 r.pass_expert[to] = (short)e;
@@ -238,13 +247,14 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
             *r.passes = passes;
         __syncwarp();
         // An expert's slots in ascending order: every CTA must cut them into the same passes.
+#pragma unroll 1
         for (int s0 = 0; s0 < slots; s0 += 32) {
             const int s = s0 + lane, e = s < slots ? r.expert[s] : -1;
             const uint32_t alike = __match_any_sync(0xffffffffu, e);
             const int to = e >= 0 ? r.at[e] : 0, before = __popc(alike & ((1u << lane) - 1u));
             __syncwarp();
             if (e >= 0) {
-                r.order[to + before] = (short)s;
+                r.order[to + before] = s / a.top << 16 | s;
                 if (before == 0)
                     r.at[e] = to + __popc(alike);
             }
@@ -290,8 +300,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
     const bool resident = a.t <= COLS;
     pdl_start();
     auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
+    // (the logits, and with few tokens those, are on their way while the routing is worked out)
+    ask_ahead<kThreads>(a.logits, a.t * a.e * 4);
     if (resident)
-        largest_of_rows<T, kWarps>(token_row, a.t, a.d, part, x_vectors);
+#pragma unroll 1
+        for (int t = 0; t < a.t; ++t)
+            ask_ahead<kThreads>(token_row(t), a.d * (int)sizeof(T));
     route_tokens(a, COLS, route, cluster > 1 ? (int)umma::cluster_rank() : 0, cluster);
     if (a.t > 8 && blockIdx.x == 0) {
         const int units = route_bytes(a.t * a.top, a.e, COLS) / 16;
@@ -303,7 +317,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
         umma::cluster_wait();  // nobody reads this CTA's choices any more
     }
     const int blocks = (a.f + kUnits - 1) / kUnits;
-    const long long tiles = (long long)*route.passes * blocks;
+    // (1024 slots of 4096 blocks at most, in 1024 CTAs: products that 32 bits hold)
+    const unsigned tiles = (unsigned)(*route.passes * blocks);
     const int first = (int)(tiles * blockIdx.x / gridDim.x), last = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
     if (first == last)
         return;
@@ -338,25 +353,23 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
         next_stage<kDepth, U::W::kBytes>(stage_in, ring);
         copy_commit();
     };
+#pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i)
         copy_next();
-    if (resident)
-        rows_to_whole<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
-    __syncthreads();
 
     int pass = first / blocks, b = first - pass * blocks, cols = 0, e = 0;
-    const short* order = nullptr;
+    const int* order = nullptr;
+#pragma unroll 1
     for (int tile = first; tile < last; ++tile) {
         const int u0 = b * kUnits;
         if (b == 0 || tile == first) {
             e = route.pass_expert[pass];
             cols = route.pass_cols[pass];
             order = route.order + route.pass_start[pass];
-            if (!resident) {
-                auto slot_row = [&](int c) { return token_row(order[c] / a.top); };
-                largest_of_rows<T, kWarps>(slot_row, cols, a.d, part, x_vectors);
-                __syncthreads();  // (the last pass's tokens have been read, too)
-                rows_to_whole<T, kWarps>(slot_row, cols, a.d, xs, pitch, x_scale, part, x_vectors);
+            if (!resident || tile == first) {
+                // (behind the barrier in it all warps are done with the last pass's tokens)
+                rows_to_whole<T, kWarps>([&](int c) { return token_row(resident ? c : order[c] >> 16); },
+                                         resident ? a.t : cols, a.d, xs, pitch, x_scale, part, x_vectors);
                 __syncthreads();
             }
         }
@@ -368,13 +381,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int c = min(8 * nt + g, cols - 1);
-            frag[nt] = xs + (resident ? order[c] / a.top : c) * pitch + tig * 16;
+            frag[nt] = xs + (resident ? order[c] >> 16 : c) * pitch + tig * 16;
         }
         const int s_lo = (int)((uintptr_t)tile_row(pass, b, g) & 15), s_hi = (int)((uintptr_t)tile_row(pass, b, g + 8) & 15);
         int acc[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
+#pragma unroll 1
         for (int i = 0; i < mine; ++i) {
             copy_wait<kDepth - 2>();
             __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
@@ -399,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
             at[kPitch + 8] = acc[nt][3];
         }
         __syncthreads();  // (the other exchange's readers are past their reading when this one is passed again)
+#pragma unroll 1
         for (int c = warp; c < cols; c += kWarps) {
             int gate = 0, up = 0;
 #pragma unroll
@@ -406,8 +421,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
                 gate += red[(i * COLS + c) * kPitch + lane];
                 up += red[(i * COLS + c) * kPitch + kUnits + lane];
             }
-            const int slot = order[c];
-            const float sx = x_scale[resident ? slot / a.top : c];
+            const int slot = order[c] & 0xffff;
+            const float sx = x_scale[resident ? order[c] >> 16 : c];
             const float zg = scale_acc(gate, sx, s_gate), zu = scale_acc(up, sx, s_up);
             const float h = u < a.f ? __fmul_rn(__fdiv_rn(zg, __fadd_rn(1.f, expf(-zg))), zu) : 0.f;
             const RowScale r = row_scale(__reduce_max_sync(0xffffffffu, magnitude(h)));
@@ -469,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
     const int groups = (a.f + kUnits - 1) / kUnits, width = groups * kUnits;
     const int steps = (a.f + kStep - 1) / kStep;  // of a pass
     const int total = steps * *route.passes;
-    const int runs = cluster * kWarps, run = rank * kWarps + warp;
-    const int first = (int)((long long)total * run / runs), mine = (int)((long long)total * (run + 1) / runs) - first;
+    const unsigned runs = (unsigned)(cluster * kWarps), run = (unsigned)(rank * kWarps + warp);
+    const int first = (int)((unsigned)total * run / runs), mine = (int)((unsigned)total * (run + 1) / runs) - first;
     float* own = sums + warp * a.t * kRows;
     for (int i = lane; i < a.t * kRows; i += 32)
         own[i] = 0.f;
@@ -509,11 +524,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
     auto copy_hidden = [&](uint32_t stage) {
         if (h_copied < mine) {
             if (h_new) {
-                const short* order = route.order + route.pass_start[hl.pass];
+                const int* order = route.order + route.pass_start[hl.pass];
                 const int cols = route.pass_cols[hl.pass];
-                h.open([&](int r) { return r < cols ? a.hq + (size_t)order[r] * width : nullptr; }, width, hl.step);
+                h.open([&](int r) { return r < cols ? a.hq + (size_t)(order[r] & 0xffff) * width : nullptr; }, width,
+                       hl.step);
                 // a lane copies the scales of a token's groups lane / kCols, and so on
-                sh_from = a.sh + (size_t)order[min(lane % kCols, cols - 1)] * groups + lane / kCols;
+                sh_from = a.sh + (size_t)(order[min(lane % kCols, cols - 1)] & 0xffff) * groups + lane / kCols;
             }
             // (of tokens that are not there: nothing)
             const bool whole = width - hl.step * kStep >= kStep;
@@ -534,10 +550,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
         ++h_copied;
         copy_commit();
     };
+#pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i)
         copy_weights(ring + (uint32_t)(i * D::kStage));
     if (a.t <= 8)
         pdl_start();
+#pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i)
         copy_hidden(ring + (uint32_t)(i * D::kStage));
     uint32_t stage = ring, free_stage = ring + (uint32_t)((kDepth - 1) * D::kStage);
@@ -550,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
     float s_lo = 0.f, s_hi = 0.f;
     int sh_lo = 0, sh_hi = 0;
     bool fresh = true;
+#pragma unroll 1
     for (int i = 0; i < mine; ++i) {
         copy_wait<kDepth - 2>();
         __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read
@@ -585,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
         fresh = advance(at);
         if (fresh || i + 1 == mine) {
             // this warp's share of the pass, to the sums of its tokens
-            const short* order = route.order + route.pass_start[pass];
+            const int* order = route.order + route.pass_start[pass];
             const int cols = route.pass_cols[pass];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -593,9 +612,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
                 for (int j = 0; j < 2; ++j) {
                     const int c = 8 * nt + 2 * tig + j;
                     if (c < cols) {
-                        const int slot = order[c];
-                        const float p = route.p[slot];
-                        float* to = own + slot / a.top * kRows + g;
+                        const float p = route.p[order[c] & 0xffff];
+                        float* to = own + (order[c] >> 16) * kRows + g;
                         to[0] = __fmaf_rn(__fmul_rn(acc[nt][j], s_lo), p, to[0]);
                         to[8] = __fmaf_rn(__fmul_rn(acc[nt][2 + j], s_hi), p, to[8]);
                     }
@@ -611,6 +629,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
         if (d < a.d)
             store_as(a.y, a.dtype, (size_t)t * (size_t)a.ldy + d, v);
     };
+#pragma unroll 1
     for (int i = threadIdx.x; i < a.t * kRows; i += kThreads) {
         float v = 0.f;
 #pragma unroll
@@ -627,6 +646,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
         umma::cluster_arrive();
         umma::cluster_wait();
         const uint32_t base = shared_address(sums);
+#pragma unroll 1
         for (int i = (rank * kThreads + (int)threadIdx.x) * 4; i < a.t * kRows; i += cluster * kThreads * 4) {
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             for (int c = 0; c < cluster; ++c) {

@@ -26,7 +26,7 @@ MB200_HD constexpr int most_passes(int slots, int experts, int cols) {
     return (slots < experts ? slots : experts) + slots / cols;
 }
 MB200_HD constexpr int route_bytes(int slots, int experts, int cols) {
-    return up16(4 * slots) + up16(2 * slots) + 3 * up16(2 * most_passes(slots, experts, cols)) + 16;
+    return 2 * up16(4 * slots) + 3 * up16(2 * most_passes(slots, experts, cols)) + 16;
 }
 struct MoeArgs {
     int t, d, f, e, top, renormalize, dtype;

@@ -210,25 +210,6 @@ __device__ __forceinline__ void mma_64(int (&c)[4], const uint4& lo, const uint4
     mma_16x8x32(c, lo.z, hi.z, lo.w, hi.w, t.z, t.w);
 }
 
-// 16 elements of a row of activations as floats, from element `kk` on; zeros behind its end
-template <class T>
-__device__ __forceinline__ void load_piece(const T* row, int kk, int k, bool aligned, float (&v)[16]) {
-    if (aligned && kk + 16 <= k) {
-        constexpr int N = Vec<T>::N;
-        const uint4* p = (const uint4*)(row + kk);
-        uint4 w[16 / N];
-#pragma unroll
-        for (int i = 0; i < 16 / N; ++i)
-            w[i] = p[i];
-#pragma unroll
-        for (int i = 0; i < 16 / N; ++i)
-            Vec<T>::unpack(w[i], v + N * i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            v[i] = kk + i < k ? to_float(row[kk + i]) : 0.f;
-    }
-}
 __device__ __forceinline__ uint4 pack_piece(const float (&v)[16], const RowScale& r) {
     uint4 q;
     q.x = pack_whole(v[0], v[1], v[2], v[3], r.inv) & r.keep;

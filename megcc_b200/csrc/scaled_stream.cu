@@ -160,9 +160,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
             a.template copy<false>(stage + S::W::kBytes, kWarps, k - (warp + i * kWarps) * kStep >= S::A::kWhole);
     };
     if (p.b_early)
+#pragma unroll 1
         for (int i = 0; i < kDepth - 1; ++i)
             copy_weights(ring + (uint32_t)(i * S::kStage), i);
     pdl_start();
+#pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i) {
         const uint32_t stage = ring + (uint32_t)(i * S::kStage);
         if (!p.b_early)
@@ -174,11 +176,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     const int row = threadIdx.x & 15, n = n0 + row;
     const float sb = n < p.n ? p.sb[n] : 0.f, bias = p.bias && n < p.n ? p.bias[n] : 0.f;
     if constexpr (kFloat) {
-        auto x_row = [&](int r) { return (const XT*)p.a + (long long)(m0 + r) * p.lda; };
-        const int rows = min(kCols, p.m - m0);
-        largest_of_rows<XT, kWarps>(x_row, rows, k, part, x_vectors);
-        __syncthreads();
-        rows_to_whole<XT, kWarps>(x_row, rows, k, xs, pitch, col_scale, part, x_vectors);
+        rows_to_whole<XT, kWarps>([&](int r) { return (const XT*)p.a + (long long)(m0 + r) * p.lda; },
+                                  min(kCols, p.m - m0), k, xs, pitch, col_scale, part, x_vectors);
         __syncthreads();
     } else {
         if (threadIdx.x < kCols)
@@ -198,6 +197,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     for (int nt = 0; nt < NT; ++nt)
         acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0;
     uint32_t stage = ring, free_stage = ring + (uint32_t)((kDepth - 1) * S::kStage);
+#pragma unroll 1
     for (int i = 0; i < mine; ++i) {
         copy_wait<kDepth - 2>();
         __syncwarp();  // all lanes' copies of this step are there, and the last step's stage has been read

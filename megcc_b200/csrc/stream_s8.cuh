@@ -169,70 +169,75 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
     return make_uint4(cut(v.x, n), cut(v.y, n - 4), cut(v.z, n - 8), cut(v.w, n - 12));
 }
 
-// Rows of activations (up to 16) as whole numbers in shared memory, by all threads of a CTA, in two halves with a
-// barrier of the CTA between them and another behind. WARPS / rows warps (one at least) share a row, so that a few
-// rows' loads are on their way together. row(r): a row's address; part: [16][WARPS] words of shared memory.
-template <int WARPS>
-__device__ __forceinline__ int warps_per_row(int rows) {
-    return rows >= WARPS ? 1 : rows * 2 >= WARPS ? 2 : rows * 4 >= WARPS ? 4 : WARPS;
-}
+// Rows of activations (up to 16) as whole numbers in shared memory, by all threads of a CTA; zeros behind each row up
+// to whole steps. WARPS / rows warps (one at least) share a row, so that a few rows' loads are on their way
+// together. row(r): a row's address; part: [16][WARPS] words of shared memory. A barrier of the CTA has to
+// follow before the rows are read. (Loops stay rolled here and in the kernels where their bodies are long: a launch
+// fetches its instructions anew, and 115 KB of them cost the expert kernels 5 us each.)
 template <class T, int WARPS, class RowAt>
-__device__ __forceinline__ void largest_of_rows(RowAt row, int rows, int k, uint32_t* part, bool vectors) {
+__device__ __forceinline__ void rows_to_whole(
+        RowAt row, int rows, int k, int8_t* xs, int pitch, float* scale, uint32_t* part, bool vectors) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int share = warps_per_row<WARPS>(rows), stride = share * 512;
+    const int share = rows >= WARPS ? 1 : rows * 2 >= WARPS ? 2 : rows * 4 >= WARPS ? 4 : WARPS;
+    const int stride = share * 512, first = (warp % share * 32 + lane) * 16;
+    const int in_vectors = vectors ? k & ~15 : 0;  // elements taken 16 at a time; the others one by one
+    constexpr int N = 16 / Vec<T>::N;              // loads of 16 elements
+#pragma unroll 1
     for (int r = warp / share; r < rows; r += WARPS / share) {
         const T* x = (const T*)row(r);
-        uint32_t bits = 0;
-        int i = (warp % share * 32 + lane) * 16;
-        if (vectors) {
-            constexpr int N = 16 / Vec<T>::N;  // loads of a piece
-            uint32_t vm = 0;
-            for (; i + stride + 16 <= k; i += 2 * stride) {
-                uint4 w[2 * N];
+        uint32_t vm = 0;
+#pragma unroll 2
+        for (int i = first; i < in_vectors; i += stride) {
+            uint4 w[N];
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    w[j] = ((const uint4*)(x + i))[j];
-                    w[N + j] = ((const uint4*)(x + i + stride))[j];
-                }
+            for (int j = 0; j < N; ++j)
+                w[j] = ((const uint4*)(x + i))[j];
 #pragma unroll
-                for (int j = 0; j < 2 * N; ++j)
-                    vm = vec_max<T>(vm, w[j]);
-            }
-            bits = max_bits<T>(vm);
+            for (int j = 0; j < N; ++j)
+                vm = vec_max<T>(vm, w[j]);
         }
-        for (; i < k; i += stride) {
-            float v[16];
-            load_piece(x, i, k, vectors, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                bits = max(bits, magnitude(v[e]));
-        }
+        uint32_t bits = max_bits<T>(vm);
+#pragma unroll 1
+        for (int i = in_vectors + first / 16; i < k; i += stride / 16)
+            bits = max(bits, magnitude(to_float(x[i])));
         bits = __reduce_max_sync(0xffffffffu, bits);
         if (lane == 0)
             part[r * WARPS + warp % share] = bits;
     }
-}
-// (zeros behind each row up to whole steps)
-template <class T, int WARPS, class RowAt>
-__device__ __forceinline__ void rows_to_whole(
-        RowAt row, int rows, int k, int8_t* xs, int pitch, float* scale, const uint32_t* part, bool vectors) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int share = warps_per_row<WARPS>(rows), end = (k + kStep - 1) / kStep * kStep;
+    __syncthreads();
+    const int end = (k + kStep - 1) / kStep * kStep;
+#pragma unroll 1
     for (int r = warp / share; r < rows; r += WARPS / share) {
         const T* x = (const T*)row(r);
         uint32_t bits = 0;
+#pragma unroll 1
         for (int w = 0; w < share; ++w)
             bits = max(bits, part[r * WARPS + w]);
         const RowScale s = row_scale(bits);
         if (warp % share == 0 && lane == 0)
             scale[r] = s.scale;
-#pragma unroll 2
-        for (int i = (warp % share * 32 + lane) * 16; i < end; i += share * 512) {
+        int8_t* to = xs + r * pitch;
+#pragma unroll 1
+        for (int i = first; i < in_vectors; i += stride) {
             float v[16];
-            load_piece(x, i, k, vectors, v);
-            *(uint4*)(xs + r * pitch + i) = pack_piece(v, s);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                Vec<T>::unpack(((const uint4*)(x + i))[j], v + Vec<T>::N * j);
+            *(uint4*)(to + i) = pack_piece(v, s);
         }
+#pragma unroll 1
+        for (int i = in_vectors + first / 16; i < end; i += stride / 16)
+            to[i] = i < k ? (int8_t)(to_whole(to_float(x[i]), s.inv) & s.keep) : 0;
     }
+}
+// Asks for what the CTA's threads will read soon: `bytes` from p on, into the L1.
+template <int THREADS>
+__device__ __forceinline__ void ask_ahead(const void* p, int bytes) {
+    const uintptr_t first = (uintptr_t)p & ~(uintptr_t)127;
+    const int end = (int)((uintptr_t)p - first) + bytes;
+#pragma unroll 1
+    for (int at = threadIdx.x * 128; at < end; at += THREADS * 128)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(first + at));
 }
 // bytes between rows of xs: whole steps, and two rows on other banks
 __host__ __device__ constexpr int xs_pitch(int k) {
