@@ -68,9 +68,9 @@ __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-// One token's experts, by a warp: lane j < top gets the j-th choice's index and p. Each choice is the largest of what
-// comes behind the one before it (smaller, or equal with a higher index), so nothing is crossed out and the
-// logits may be read again and again: the first 128 from registers.
+// One token's experts, by a warp: lane j < top gets the j-th choice's index and p. The first 128 logits are kept in
+// registers; of those behind them each choice is the largest that comes behind the one before it (smaller, or
+// equal with a higher index).
 struct Choice {
     int expert;
     float p;
@@ -80,7 +80,7 @@ __device__ __noinline__ Choice choose_experts(const float* row, int experts, int
     const int lane = threadIdx.x & 31;
     const float inf = __uint_as_float(0x7f800000u);
     uint32_t key[R];
-    uint32_t odd = 0;  // a NaN or +infinity among the logits
+    bool odd = false;  // a NaN or +infinity among the logits
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int e = i * 32 + lane;
@@ -88,22 +88,20 @@ __device__ __noinline__ Choice choose_experts(const float* row, int experts, int
         key[i] = e < experts ? rank_key(v) : 0u;
         odd |= !(v < inf);
     }
+    float sum = 0.f;  // of all exponentials, where it is asked for
     uint32_t last = ~0u;
-    int last_e = -1;
+    int last_e = -1, mine_e = -1;
     float top_value = 0.f, mine = 0.f;
-    int mine_e = -1;
 #pragma unroll 1
     for (int j = 0; j < top; ++j) {
         uint32_t best = 0;
         int at = 0;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int e = i * 32 + lane;
-            if (key[i] > best && (key[i] < last || (key[i] == last && e > last_e))) {
+        for (int i = 0; i < R; ++i)
+            if (key[i] > best) {
                 best = key[i];
-                at = e;
+                at = i * 32 + lane;
             }
-        }
 #pragma unroll 1
         for (int e = R * 32 + lane; e < experts; e += 32) {
             const uint32_t k = rank_key(row[e]);
@@ -114,31 +112,35 @@ __device__ __noinline__ Choice choose_experts(const float* row, int experts, int
         }
         last = __reduce_max_sync(0xffffffffu, best);
         last_e = (int)__reduce_min_sync(0xffffffffu, best == last ? (uint32_t)at : ~0u);
-        if (j == 0)
+        if (j == 0) {
             top_value = key_value(last);
+            if (!renormalize) {
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+                    sum += key[i] != 0 ? expf(key_value(key[i]) - top_value) : 0.f;
+            }
+        }
         if (lane == j) {
             mine = key_value(last);
             mine_e = last_e;
         }
-    }
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-        if (key[i] != 0)
-            sum += expf(key_value(key[i]) - top_value);
+        for (int i = 0; i < R; ++i)
+            if (i * 32 + lane == last_e)
+                key[i] = 0;
+    }
+    mine = lane < top ? expf(mine - top_value) : 0.f;
 #pragma unroll 1
     for (int e = R * 32 + lane; e < experts; e += 32) {
         odd |= !(row[e] < inf);
-        sum += expf(row[e] - top_value);
+        sum += renormalize ? 0.f : expf(row[e] - top_value);
     }
-    mine = lane < top ? expf(mine - top_value) : 0.f;
-    float chosen = mine;
+    if (renormalize)
+        sum = mine;
 #pragma unroll
-    for (int s = 16; s; s >>= 1) {
+    for (int s = 16; s; s >>= 1)
         sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        chosen += __shfl_xor_sync(0xffffffffu, chosen, s);
-    }
-    float p = __fdiv_rn(mine, renormalize ? chosen : sum);
+    float p = __fdiv_rn(mine, sum);
     if (top_value == -inf)
         p = 0.f;  // every expert is masked: no share in any
     if (__any_sync(0xffffffffu, odd))
@@ -156,8 +158,11 @@ __device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
 
 // A warp per token in turn (500 instructions in a chain, 2 us each: the CTAs of a cluster share the tokens
 // out); then the slots by expert, cut into passes of at most `cols`. Barriers of the CTA stand before and behind,
-// and with a cluster umma::cluster_wait() has to follow before r.expert's memory is used for something else.
-__device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int rank, int cluster) {
+// and with a cluster umma::cluster_wait() has to follow before r.expert's memory is used for something else. With four
+// tokens at most the upper half of the warps has none and calls meanwhile().
+template <class Meanwhile>
+__device__ __forceinline__ void route_tokens(
+        const MoeArgs& a, int cols, const Route& r, int rank, int cluster, Meanwhile meanwhile) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (a.t > 1)
         for (int e = threadIdx.x; e < a.e; e += kThreads)
@@ -172,24 +177,20 @@ __device__ void route_tokens(const MoeArgs& a, int cols, const Route& r, int ran
             if (lane < a.top)
                 r.expert[t * a.top + lane] = c.expert;
         } else {
-            // one token: a pass for each of its experts, in the order of their indices
-            int before = 0;
-#pragma unroll 1
-            for (int j = 0; j < a.top; ++j) {
-                const int other = __shfl_sync(0xffffffffu, c.expert, j);
-                before += other >= 0 && other < c.expert;
-            }
+            // one token: a pass for each of its experts, from the largest p down (any p that is 0 comes last)
             if (c.expert >= 0) {
-                r.order[before] = lane;
-                r.pass_expert[before] = (short)c.expert;
-                r.pass_start[before] = (short)before;
-                r.pass_cols[before] = 1;
+                r.order[lane] = lane;
+                r.pass_expert[lane] = (short)c.expert;
+                r.pass_start[lane] = (short)lane;
+                r.pass_cols[lane] = 1;
             }
             const uint32_t some = __ballot_sync(0xffffffffu, c.expert >= 0);
             if (lane == 0)
                 *r.passes = __popc(some);
         }
     }
+    if (a.t <= 4 && warp >= 4)
+        meanwhile();
     if (a.t == 1) {
         __syncthreads();
         return;
@@ -302,11 +303,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
     auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
     // (the logits, and with few tokens those, are on their way while the routing is worked out)
     ask_ahead<kThreads>(a.logits, a.t * a.e * 4);
-    if (resident)
+    if (resident && a.t > 4)
 #pragma unroll 1
         for (int t = 0; t < a.t; ++t)
             ask_ahead<kThreads>(token_row(t), a.d * (int)sizeof(T));
-    route_tokens(a, COLS, route, cluster > 1 ? (int)umma::cluster_rank() : 0, cluster);
+    route_tokens(a, COLS, route, cluster > 1 ? (int)umma::cluster_rank() : 0, cluster, [&] {
+        if (resident)
+            rows_to_whole<T, 4, 4>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
+    });
     if (a.t > 8 && blockIdx.x == 0) {
         const int units = route_bytes(a.t * a.top, a.e, COLS) / 16;
         for (int i = threadIdx.x; i < units; i += kThreads)
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
             e = route.pass_expert[pass];
             cols = route.pass_cols[pass];
             order = route.order + route.pass_start[pass];
-            if (!resident || tile == first) {
+            if (!resident || (tile == first && a.t > 4)) {
                 // (behind the barrier in it all warps are done with the last pass's tokens)
                 rows_to_whole<T, kWarps>([&](int c) { return token_row(resident ? c : order[c] >> 16); },
                                          resident ? a.t : cols, a.d, xs, pitch, x_scale, part, x_vectors);
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
     // was written before the first kernel began, which let this one start behind its own wait for that. The routing
     // of more takes longer than to fetch the first kernel's.
     if (a.t <= 8) {
-        route_tokens(a, kCols, route, 0, 1);
+        route_tokens(a, kCols, route, 0, 1, [] {});
     } else {
         pdl_start();
         const int units = route_bytes(a.t * a.top, a.e, kCols) / 16;

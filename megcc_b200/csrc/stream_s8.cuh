@@ -169,15 +169,16 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
     return make_uint4(cut(v.x, n), cut(v.y, n - 4), cut(v.z, n - 8), cut(v.w, n - 12));
 }
 
-// Rows of activations (up to 16) as whole numbers in shared memory, by all threads of a CTA; zeros behind each row up
+// Rows of activations (up to 16) as whole numbers in shared memory, by the threads of a CTA; zeros behind each row up
 // to whole steps. WARPS / rows warps (one at least) share a row, so that a few rows' loads are on their way
-// together. row(r): a row's address; part: [16][WARPS] words of shared memory. A barrier of the CTA has to
-// follow before the rows are read. (Loops stay rolled here and in the kernels where their bodies are long: a launch
+// together. row(r): a row's address; part: [16][WARPS] words of shared memory. With FIRST > 0
+// the warps from FIRST on do it (WARPS of them; barrier 1 is theirs). A barrier of the CTA has to follow before the
+// rows are read. (Loops stay rolled here and in the kernels where their bodies are long: a launch
 // fetches its instructions anew, and 115 KB of them cost the expert kernels 5 us each.)
-template <class T, int WARPS, class RowAt>
+template <class T, int WARPS, int FIRST = 0, class RowAt>
 __device__ __forceinline__ void rows_to_whole(
         RowAt row, int rows, int k, int8_t* xs, int pitch, float* scale, uint32_t* part, bool vectors) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = (int)(threadIdx.x >> 5) - FIRST, lane = threadIdx.x & 31;
     const int share = rows >= WARPS ? 1 : rows * 2 >= WARPS ? 2 : rows * 4 >= WARPS ? 4 : WARPS;
     const int stride = share * 512, first = (warp % share * 32 + lane) * 16;
     const int in_vectors = vectors ? k & ~15 : 0;  // elements taken 16 at a time; the others one by one
@@ -204,7 +205,10 @@ __device__ __forceinline__ void rows_to_whole(
         if (lane == 0)
             part[r * WARPS + warp % share] = bits;
     }
-    __syncthreads();
+    if (FIRST == 0)
+        __syncthreads();
+    else
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
     const int end = (k + kStep - 1) / kStep * kStep;
 #pragma unroll 1
     for (int r = warp / share; r < rows; r += WARPS / share) {
