@@ -73,14 +73,15 @@ long long padded(int k) {
 size_t padded_bytes(int rows, int k) {
     return align_up((size_t)rows * (size_t)padded(k), 256);
 }
-// b as the TMA takes it, in the workspace where it is not yet
-int pad_b(ProductArgs* p, int8_t** ws, cudaStream_t st) {
-    if (rows_fit(p->b, p->n, p->ldb))
-        return ST_SUCCESS;
-    const int rc = launch_pad_rows(p->b, p->ldb, p->n, p->k, *ws, padded(p->k), st);
-    p->b = *ws, p->ldb = padded(p->k);
-    *ws += padded_bytes(p->n, p->k);
-    return rc;
+// A matrix as the TMA takes it, in the workspace where it is not yet: what is to be done for that
+PadRows pad_job(const int8_t** src, long long* ld, int rows, int k, int8_t** ws) {
+    PadRows j{};
+    if (!rows_fit(*src, rows, *ld)) {
+        j = {*src, *ld, rows, k, *ws, padded(k)};
+        *src = *ws, *ld = padded(k);
+        *ws += padded_bytes(rows, k);
+    }
+    return j;
 }
 
 int check_moe(const mb200_moe_param* p) {
@@ -172,11 +173,9 @@ int mb200_matmul_s8_scaled(
         return launch_product_stream(p, st);
     }
     int8_t* ws = (int8_t*)workspace;
-    rc = pad_b(&p, &ws, st);
-    if (!rc && !rows_fit(a, m, lda)) {
-        rc = launch_pad_rows(a, lda, m, k, ws, padded(k), st);
-        p.a = ws, p.lda = padded(k);
-    }
+    const PadRows pad_b = pad_job(&p.b, &p.ldb, n, k, &ws), pad_a = pad_job(&a, &p.lda, m, k, &ws);
+    p.a = a;
+    rc = launch_pad_rows(pad_b, pad_a, st);
     if (rc)
         return rc;
     p.b_early = may_read_early(p.b, (size_t)n * (size_t)p.ldb, st);
@@ -224,7 +223,7 @@ int mb200_linear_s8(
     }
     int8_t* ws = (int8_t*)workspace;
     if (!streams(m)) {
-        rc = pad_b(&p, &ws, st);
+        rc = launch_pad_rows(pad_job(&p.b, &p.ldb, n, k, &ws), PadRows{}, st);
         if (rc)
             return rc;
     }

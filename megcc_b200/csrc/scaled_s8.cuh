@@ -244,9 +244,16 @@ int launch_quantize_rows(
 int launch_product_stream(const ProductArgs& a, cudaStream_t st);
 // the tensor-core kernels: int8 operands, 16-byte aligned, rows whole 16-byte units apart
 int launch_product_umma(const ProductArgs& a, cudaStream_t st);
-// rows of any alignment to rows `pitch` bytes apart (a multiple of 16, at least k), zeros behind each
-int launch_pad_rows(
-        const int8_t* src, long long ld, int rows, int k, int8_t* dst, long long pitch, cudaStream_t st);
+// Rows of any alignment to rows `pitch` bytes apart (a multiple of 16, at least k), zeros behind each; two matrices in
+// one launch (rows == 0: none)
+struct PadRows {
+    const int8_t* src;
+    long long ld;
+    int rows, k;
+    int8_t* dst;
+    long long pitch;
+};
+int launch_pad_rows(const PadRows& a, const PadRows& b, cudaStream_t st);
 
 }  // namespace scaled
 }  // namespace mb200

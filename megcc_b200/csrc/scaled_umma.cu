@@ -23,13 +23,11 @@ using namespace umma;
 
 namespace {
 
+constexpr int ERR_SHARED_WINDOW = 0x106;
+
 constexpr int kBM = 128;  // rows per CTA
 constexpr int kBK = 128;  // K bytes per stage
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kTileBytes = kBM * kBK;  // of either operand
-constexpr int kStageBytes = 2 * kTileBytes;
-constexpr int kMaxStages = 6;
+constexpr int kTileBytes = kBM * kBK;  // of 128 rows
 
 struct UmmaArgs {
     int m, n, k_steps;
@@ -39,9 +37,11 @@ struct UmmaArgs {
     long long ldc;
     int vector_stores;  // rows of c are whole 16-byte units
     int b_early;
-    int a_rows;   // split: rows of A's box
-    int stages;   // split
-    int csplit;   // split: CTAs per tile
+    // split:
+    int a_rows;      // rows of A's box
+    int a_bytes;     // of a stage, B's part behind it
+    int stages;
+    int csplit;      // CTAs per tile
     int* status;
 };
 
@@ -51,6 +51,9 @@ template <>
 struct Out<float> {
     static __device__ __forceinline__ uint4 unit(const float* v) {
         return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    static __device__ __forceinline__ uint4 unit4(const float* v) {
+        return unit(v);
     }
     static __device__ __forceinline__ float one(float v) {
         return v;
@@ -65,6 +68,9 @@ struct Out<__half> {
     static __device__ __forceinline__ uint4 unit(const float* v) {
         return make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
     }
+    static __device__ __forceinline__ uint4 unit4(const float* v) {
+        return make_uint4(two(v[0], v[1]), two(v[2], v[3]), 0, 0);
+    }
     static __device__ __forceinline__ __half one(float v) {
         return __float2half_rn(v);
     }
@@ -78,84 +84,100 @@ struct Out<__nv_bfloat16> {
     static __device__ __forceinline__ uint4 unit(const float* v) {
         return make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
     }
+    static __device__ __forceinline__ uint4 unit4(const float* v) {
+        return make_uint4(two(v[0], v[1]), two(v[2], v[3]), 0, 0);
+    }
     static __device__ __forceinline__ __nv_bfloat16 one(float v) {
         return __float2bfloat16_rn(v);
     }
 };
 
-// The scales and biases of a tile's columns, in shared memory (16-byte aligned)
-struct Columns {
-    const float *scale, *bias;  // bias: zeros where there is none
-};
-
-// 32 rows (a warp's lanes) times 128 bytes of results: from tensor memory through 4 KB of shared memory
-// to whole lines. `col`: the first column within `cols`; `taken()` is called once the sums are in registers.
+// 32 rows (a warp's lanes) times 64 bytes of results: from tensor memory through 2 KB of shared memory to whole
+// sectors. scale, bias: of the columns, in shared memory (16-byte aligned); `taken()` is called once the sums are
+// in registers.
+template <class T>
+constexpr int kRoundCols = 64 / (int)sizeof(T);
+constexpr int kRoundBytes = 32 * 64;
 template <class T, class Taken>
-__device__ __forceinline__ void store_block(
-        uint32_t taddr, float sa, const Columns& cols, int col, bool has_bias, uint8_t* stage, int row0, int col0,
-        const UmmaArgs& p, Taken taken) {
+__device__ __forceinline__ void store_round(
+        uint32_t taddr, float sa, const float* scale, const float* bias, bool has_bias, uint8_t* stage, int row0,
+        int col0, const UmmaArgs& p, const CUtensorMap* map_c, Taken taken) {
     constexpr int kUnit = 16 / (int)sizeof(T);  // results per 16 bytes
-    constexpr int kCols = 8 * kUnit;
+    constexpr int kCols = kRoundCols<T>;
     const int lane = threadIdx.x & 31;
+    uint32_t acc[kCols];
+    if (map_c) {
+        // the last round's bytes have left the stage
+        if (lane == 0)
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    }
+    __syncwarp();
+    if constexpr (kCols == 32)
+        tmem_ld32(taddr, acc);
+    else
+        tmem_ld16(taddr, acc);
+    taken();
 #pragma unroll
-    for (int h = 0; h < kCols / 32; ++h) {
-        uint32_t acc[32];
-        __syncwarp();
-        tmem_ld32(taddr + (uint32_t)(32 * h), acc);
-        if (h + 1 == kCols / 32)
-            taken();
+    for (int u = 0; u < 4; ++u) {
+        float v[kUnit];
 #pragma unroll
-        for (int u = 0; u < 32 / kUnit; ++u) {
-            float v[kUnit];
-#pragma unroll
-            for (int j = 0; j < kUnit; j += 4) {
-                const int at = col + 32 * h + u * kUnit + j;
-                const float4 s = *(const float4*)(cols.scale + at);
-                v[j] = scale_acc((int)acc[u * kUnit + j], sa, s.x);
-                v[j + 1] = scale_acc((int)acc[u * kUnit + j + 1], sa, s.y);
-                v[j + 2] = scale_acc((int)acc[u * kUnit + j + 2], sa, s.z);
-                v[j + 3] = scale_acc((int)acc[u * kUnit + j + 3], sa, s.w);
-                if (has_bias) {
-                    const float4 b = *(const float4*)(cols.bias + at);
-                    v[j] = __fadd_rn(v[j], b.x);
-                    v[j + 1] = __fadd_rn(v[j + 1], b.y);
-                    v[j + 2] = __fadd_rn(v[j + 2], b.z);
-                    v[j + 3] = __fadd_rn(v[j + 3], b.w);
-                }
+        for (int j = 0; j < kUnit; j += 4) {
+            const int at = u * kUnit + j;
+            const float4 s = *(const float4*)(scale + at);
+            v[j] = scale_acc((int)acc[at], sa, s.x);
+            v[j + 1] = scale_acc((int)acc[at + 1], sa, s.y);
+            v[j + 2] = scale_acc((int)acc[at + 2], sa, s.z);
+            v[j + 3] = scale_acc((int)acc[at + 3], sa, s.w);
+            if (has_bias) {
+                const float4 b = *(const float4*)(bias + at);
+                v[j] = __fadd_rn(v[j], b.x);
+                v[j + 1] = __fadd_rn(v[j + 1], b.y);
+                v[j + 2] = __fadd_rn(v[j + 2], b.z);
+                v[j + 3] = __fadd_rn(v[j + 3], b.w);
             }
-            // (16-byte units of a row in an order that depends on the row: no two lanes of eight share a bank)
-            const int unit = h * (32 / kUnit) + u;
-            *(uint4*)(stage + lane * 128 + ((unit ^ (lane & 7)) << 4)) = Out<T>::unit(v);
         }
+        // (a row's 16-byte units in an order that depends on the row: no two lanes of eight share a bank; it is the
+        // TMA's 64-byte swizzle)
+        *(uint4*)(stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = Out<T>::unit(v);
+    }
+    if (map_c) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && row0 < p.m && col0 < p.n) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                                 (uint64_t)map_c),
+                         "r"(smem_u32(stage)), "r"(col0), "r"(row0)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        return;
     }
     __syncwarp();
     T* c = (T*)p.c;
     if (p.vector_stores && col0 + kCols <= p.n) {
-        const int unit = lane & 7;
+        const int unit = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3);
-            const uint4 v = *(const uint4*)(stage + r * 128 + ((unit ^ (r & 7)) << 4));
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2);
+            const uint4 v = *(const uint4*)(stage + r * 64 + ((unit ^ ((r >> 1) & 3)) << 4));
             if (row0 + r < p.m)
                 *(uint4*)(c + (long long)(row0 + r) * p.ldc + col0 + unit * kUnit) = v;
         }
     } else {
-        const int rows = min(32, p.m - row0);
-        for (int r = 0; r < rows; ++r)
-#pragma unroll
-            for (int i = 0; i < kCols; i += 32) {
-                const int j = i + lane;
-                if (col0 + j < p.n)
-                    c[(long long)(row0 + r) * p.ldc + col0 + j] =
-                            *(const T*)(stage + r * 128 + (((j / kUnit) ^ (r & 7)) << 4) + (j % kUnit) * sizeof(T));
-            }
+        const int j = lane % kCols;
+#pragma unroll 8
+        for (int r = lane / kCols; r < 32; r += 32 / kCols)
+            if (row0 + r < p.m && col0 + j < p.n)
+                c[(long long)(row0 + r) * p.ldc + col0 + j] =
+                        *(const T*)(stage + r * 64 + (((j / kUnit) ^ ((r >> 1) & 3)) << 4) + (j % kUnit) * sizeof(T));
     }
     __syncwarp();
 }
 
 // the epilogue warps' barrier
+template <int WARPS>
 __device__ __forceinline__ void epilogue_sync() {
-    asm volatile("bar.sync 1, %0;" ::"r"(32 * kEpilogueWarps) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
 }
 
 // Tiles in groups of eight rows of tiles, downwards first: what the SMs work on at one time shares its
@@ -172,21 +194,31 @@ __device__ __forceinline__ Tile tile_at(int i, int m_tiles, int n_tiles) {
 
 // ---- pairs of SMs ----
 constexpr int kPairBN = 256;
-constexpr int kPairStages = 5;
-constexpr int kPairStageOff = kPairStages * kStageBytes;           // the epilogue warps' 4 KB each
-constexpr int kPairColOff = kPairStageOff + kEpilogueWarps * 4096;  // [2][256] scales, [2][256] biases
-constexpr int kPairBarOff = kPairColOff + 4 * kPairBN * 4;
-constexpr int kPairDynamic = kPairBarOff + (2 * kPairStages + 5) * 8 + 16 + 1024;
+constexpr int kPairStages = 6;
+constexpr int kPairWarps = 16;  // epilogue; with eight a tile's epilogue took 4 us, the MMAs of 6 steps of K 2
+constexpr int kPairThreads = 64 + 32 * kPairWarps;
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kPairRoundOff = kPairStages * kStageBytes;                // the epilogue warps' 2 KB each
+constexpr int kPairColOff = kPairRoundOff + kPairWarps * kRoundBytes;  // [256] scales, [256] biases
+constexpr int kPairBarOff = kPairColOff + 2 * kPairBN * 4;
+constexpr int kPairDynamic = kPairBarOff + (2 * kPairStages + 5) * 8 + 16;
 static_assert(kPairDynamic <= 232448, "shared memory of one SM");
 
 template <class T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_pair_kernel(
-        const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const UmmaArgs p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) product_pair_kernel(
+        const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+        const __grid_constant__ CUtensorMap map_c, const UmmaArgs p) {
     extern __shared__ uint8_t smem_raw[];
-    // (the dynamic window starts at the same offset in both CTAs, so the aligned pointers agree)
-    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    // A kernel without static shared memory has its window on a 1024-byte boundary, as the swizzle wants it; there
+    // is no room to move it up, so one that is not there would leave before it touches anything.
+    uint8_t* smem = smem_raw;
+    if (smem_u32(smem) & 1023) {
+        if (threadIdx.x == 0)
+            atomicExch(p.status, ERR_SHARED_WINDOW);
+        return;
+    }
     float* col_scale = (float*)(smem + kPairColOff);
-    float* col_bias = col_scale + 2 * kPairBN;
+    float* col_bias = col_scale + kPairBN;
     uint64_t* full_bar = (uint64_t*)(smem + kPairBarOff);  // used in the leader only
     uint64_t* empty_bar = full_bar + kPairStages;          // one set per CTA
     uint64_t* acc_full = empty_bar + kPairStages;          // [2], one set per CTA
@@ -208,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 2 * kEpilogueWarps);
+            mbar_init(&acc_empty[b], 2 * kPairWarps);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -334,42 +366,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             }
         }
     } else {
-        // ---------------- epilogue (both CTAs): warps 2..9, tensor memory lanes 32 * (warp % 4) ----------------
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        // ---------------- epilogue (both CTAs): warps 2..17, tensor memory lanes 32 * (warp % 4) ----------------
+        const int q = warp & 3, quarter = (warp - 2) >> 2;
         const int et = (int)threadIdx.x - 64;
-        uint8_t* stage = smem + kPairStageOff + (warp - 2) * 4096;
+        uint8_t* stage = smem + kPairRoundOff + (warp - 2) * kRoundBytes;
         int local = 0;
         bool ok = true;
         pdl_start();
-        for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step, ++local) {
+        // half of the threads have a column's scale, half its bias; a tile's come while the one before is stored
+        const float* sides = et < kPairBN ? p.sb : p.bias;
+        const int column = et & (kPairBN - 1);
+        float side = 0.f, sa = 0.f;
+        auto fetch = [&](int tile) {
+            if (tile < total_tiles) {
+                const Tile t = tile_at(tile, p.m_tiles, p.n_tiles);
+                const int row = t.m * (2 * kBM) + (int)rank * kBM + q * 32 + lane, n = t.n * kPairBN + column;
+                sa = row < p.m ? p.sa[row] : 0.f;
+                side = sides && n < p.n ? sides[n] : 0.f;
+            }
+        };
+        fetch(first_tile);
+        for (int tile = first_tile; tile < total_tiles; tile += tile_step, ++local) {
             const int buf = local & 1;
             const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
             const Tile t = tile_at(tile, p.m_tiles, p.n_tiles);
             const int row0 = t.m * (2 * kBM) + (int)rank * kBM + q * 32, n0 = t.n * kPairBN;
-            float* scale = col_scale + buf * kPairBN;
-            float* bias = col_bias + buf * kPairBN;
-            scale[et] = n0 + et < p.n ? p.sb[n0 + et] : 0.f;
-            if (p.bias)
-                bias[et] = n0 + et < p.n ? p.bias[n0 + et] : 0.f;
-            const float sa = row0 + lane < p.m ? p.sa[row0 + lane] : 0.f;
-            epilogue_sync();
+            epilogue_sync<kPairWarps>();  // (the last tile's have been read)
+            (et < kPairBN ? col_scale : col_bias)[column] = side;
+            const float row_scale = sa;
+            epilogue_sync<kPairWarps>();
+            fetch(tile + tile_step);
             ok = mbar_wait_cluster(&acc_full[buf], acc_phase, abort_flag);
             if (!ok)
                 give_up(ERR_EPILOGUE_WAIT);
             ok = __all_sync(0xffffffffu, ok);
-            // (a warp that gave up still meets the others at the barrier in front of the next tile)
-            if (!ok) {
-                ok = true;
-                continue;
-            }
+            if (!ok)
+                continue;  // (still meets the others at the barrier in front of the next tile)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kPairBN);
-            constexpr int kCols = 128 / (int)sizeof(T);
 #pragma unroll 1
-            for (int c = half * 128; c < half * 128 + 128; c += kCols) {
-                const bool last = c + kCols == half * 128 + 128;
-                store_block<T>(taddr + (uint32_t)c, sa, Columns{scale, bias}, c, p.bias != nullptr, stage, row0,
-                               n0 + c, p, [&] {
+            for (int c = quarter * 64; c < quarter * 64 + 64; c += kRoundCols<T>) {
+                const bool last = c + kRoundCols<T> == quarter * 64 + 64;
+                store_round<T>(taddr + (uint32_t)c, row_scale, col_scale + c, col_bias + c, p.bias != nullptr, stage, row0,
+                               n0 + c, p, p.vector_stores ? &map_c : nullptr, [&] {
                                    if (last) {
                                        // this warp's sums are in registers: one arrival on the leader's barrier
                                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -380,6 +419,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
                                });
             }
         }
+        if (lane == 0)
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     // ---------------- teardown ----------------
@@ -412,21 +453,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
 
 // ---- one tile per CTA, or per cluster ----
 constexpr int kSplitBN = 128;
+constexpr int kMaxStages = 6;
+constexpr int kSplitWarps = 8;  // epilogue
+constexpr int kSplitThreads = 64 + 32 * kSplitWarps;
 constexpr int kSplitBars = (2 * kMaxStages + 2) * 8 + 16;
-constexpr int kSplitCols = 2 * kSplitBN * 4;
-inline int split_dynamic(int stages) {
-    return stages * kStageBytes + kSplitCols + kSplitBars + 1024;
+constexpr int kSplitSides = (2 * kSplitBN + kBM) * 4;  // scales and biases of columns, scales of rows
+inline int split_dynamic(int stages, int a_bytes) {
+    return stages * (a_bytes + kTileBytes) + kSplitSides + kSplitBars + 1024;
+}
+
+// The cluster's partial sums of this CTA's share of the rows: a row per warp, four columns per lane, 16 loads of
+// other CTAs' shared memory in two turns.
+template <class T, int SPLIT>
+__device__ __forceinline__ void finish_rows(
+        uint32_t partials, int rank, int m0, int n0, const float* col_scale, const float* col_bias,
+        const float* row_scale, const UmmaArgs& p) {
+    constexpr int kRows = 8 / SPLIT;  // of a turn
+    const int warp = (int)(threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
+    const int col = n0 + 4 * lane;
+    const float4 s = *(const float4*)(col_scale + 4 * lane);
+    const float4 b = p.bias ? *(const float4*)(col_bias + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+        uint4 x[kRows][SPLIT];
+        int row[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            row[i] = rank * (kBM / SPLIT) + (turn * kRows + i) * kSplitWarps + warp;
+            const uint32_t at = partials + (uint32_t)(row[i] * 512 + ((lane & ~7) + ((lane ^ row[i]) & 7)) * 16);
+#pragma unroll
+            for (int j = 0; j < SPLIT; ++j)
+                x[i][j] = m0 + row[i] < p.m ? ld_cluster_v4(at, j) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int m = m0 + row[i];
+            if (m >= p.m)
+                continue;
+            uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < SPLIT; ++j) {
+                v[0] += x[i][j].x;
+                v[1] += x[i][j].y;
+                v[2] += x[i][j].z;
+                v[3] += x[i][j].w;
+            }
+            const float sa = row_scale[row[i]];
+            float f[4] = {scale_acc((int)v[0], sa, s.x), scale_acc((int)v[1], sa, s.y), scale_acc((int)v[2], sa, s.z),
+                          scale_acc((int)v[3], sa, s.w)};
+            if (p.bias) {
+                f[0] = __fadd_rn(f[0], b.x);
+                f[1] = __fadd_rn(f[1], b.y);
+                f[2] = __fadd_rn(f[2], b.z);
+                f[3] = __fadd_rn(f[3], b.w);
+            }
+            T* c = (T*)p.c + (long long)m * p.ldc + col;
+            if (p.vector_stores && col + 4 <= p.n) {
+                const uint4 u = Out<T>::unit4(f);
+                if (sizeof(T) == 4)
+                    *(uint4*)c = u;
+                else
+                    *(uint2*)c = make_uint2(u.x, u.y);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < p.n)
+                        c[j] = Out<T>::one(f[j]);
+            }
+        }
+    }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
+__global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
         const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const UmmaArgs p) {
     extern __shared__ uint8_t smem_raw[];
     // (the same offset in all CTAs of a cluster)
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* col_scale = (float*)(smem + p.stages * kStageBytes);
+    const int stage_bytes = p.a_bytes + kTileBytes;
+    float* col_scale = (float*)(smem + p.stages * stage_bytes);
     float* col_bias = col_scale + kSplitBN;
-    uint64_t* full_bar = (uint64_t*)(col_bias + kSplitBN);
+    float* row_scale = col_bias + kSplitBN;
+    uint64_t* full_bar = (uint64_t*)(row_scale + kBM);
     uint64_t* empty_bar = full_bar + kMaxStages;
     uint64_t* acc_full = empty_bar + kMaxStages;
     uint64_t* drain_bar = acc_full + 1;
@@ -480,9 +588,9 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
             int ahead = k0;
             if (p.b_early)
                 for (; ahead < min(k0 + p.stages, k1); ++ahead) {
-                    uint8_t* at = smem + (ahead - k0) * kStageBytes;
+                    uint8_t* at = smem + (ahead - k0) * stage_bytes;
                     mbar_expect_tx(&full_bar[ahead - k0], bytes);
-                    tma_load_2d(at + kTileBytes, &map_b, &full_bar[ahead - k0], ahead * kBK, n0);
+                    tma_load_2d(at + p.a_bytes, &map_b, &full_bar[ahead - k0], ahead * kBK, n0);
                 }
             pdl_start();
             int s = 0;
@@ -493,10 +601,10 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
                     give_up(ERR_PRODUCER_WAIT);
                     break;
                 }
-                uint8_t* at = smem + s * kStageBytes;
+                uint8_t* at = smem + s * stage_bytes;
                 if (it >= ahead) {
                     mbar_expect_tx(&full_bar[s], bytes);
-                    tma_load_2d(at + kTileBytes, &map_b, &full_bar[s], it * kBK, n0);
+                    tma_load_2d(at + p.a_bytes, &map_b, &full_bar[s], it * kBK, n0);
                 }
                 tma_load_2d(at, &map_a, &full_bar[s], it * kBK, m0);
                 if (++s == p.stages) {
@@ -510,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
         const uint32_t leader = elect_one() ? 1u : 0u;
         constexpr uint32_t idesc = umma_idesc_s8(kBM, kSplitBN);
         const uint64_t a0 = umma_smem_desc(smem_u32(smem), 16, 1024, 2);
-        const uint64_t b0 = umma_smem_desc(smem_u32(smem + kTileBytes), 16, 1024, 2);
+        const uint64_t b0 = umma_smem_desc(smem_u32(smem + p.a_bytes), 16, 1024, 2);
         const uint32_t a_hi = (uint32_t)(a0 >> 32), b_hi = (uint32_t)(b0 >> 32);
         uint32_t a_lo = (uint32_t)a0, b_lo = (uint32_t)b0, phase = 0, acc = 0;
         const uint32_t full_a = smem_u32(full_bar), empty_a = smem_u32(empty_bar);
@@ -529,8 +637,8 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
                 acc = 1;
             }
             umma_commit_if(leader, empty_a + 8 * s);
-            a_lo += kStageBytes / 16;
-            b_lo += kStageBytes / 16;
+            a_lo += (uint32_t)stage_bytes / 16;
+            b_lo += (uint32_t)stage_bytes / 16;
             if (++s == p.stages) {
                 s = 0;
                 phase ^= 1u;
@@ -551,9 +659,11 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
             col_scale[et] = n0 + et < p.n ? p.sb[n0 + et] : 0.f;
             if (p.bias)
                 col_bias[et] = n0 + et < p.n ? p.bias[n0 + et] : 0.f;
+        } else {
+            row_scale[et - kBM] = m0 + et - kBM < p.m ? p.sa[m0 + et - kBM] : 0.f;
         }
-        const float sa = row0 + lane < p.m ? p.sa[row0 + lane] : 0.f;
-        epilogue_sync();
+        epilogue_sync<kSplitWarps>();
+        const float sa = row_scale[q * 32 + lane];
         bool ok = mbar_wait(acc_full, 0, abort_flag);
         if (!ok)
             give_up(ERR_EPILOGUE_WAIT);
@@ -563,13 +673,12 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
             if (p.csplit == 1) {
-                constexpr int kCols = 128 / (int)sizeof(T);
-                uint8_t* stage = smem + (warp - 2) * 4096;
+                uint8_t* stage = smem + (warp - 2) * kRoundBytes;
 #pragma unroll 1
-                for (int c = half * 64; c < half * 64 + 64; c += kCols)
-                    if (row0 < p.m)
-                        store_block<T>(taddr + (uint32_t)c, sa, Columns{col_scale, col_bias}, c, p.bias != nullptr,
-                                       stage, row0, n0 + c, p, [] {});
+                for (int c = half * 64; c < half * 64 + 64; c += kRoundCols<T>)
+                    if (row0 < p.m && n0 + c < p.n)
+                        store_round<T>(taddr + (uint32_t)c, sa, col_scale + c, col_bias + c, p.bias != nullptr,
+                                       stage, row0, n0 + c, p, nullptr, [] {});
             } else if (row0 < p.m) {
                 // the partial sums, [128 rows][32 units of four columns], units in an order by row
                 const int row = q * 32 + lane;
@@ -594,54 +703,13 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
         cluster_arrive();
         cluster_wait();
         if (warp >= 2) {
-            // this CTA finishes 128 / csplit rows: a row per warp, four columns per lane
-            const int rows = kBM / p.csplit;
-            const uint32_t base = smem_u32(smem);
-            const int col = n0 + 4 * lane;
-            const float4 s = *(const float4*)(col_scale + 4 * lane);
-            const float4 b = p.bias ? *(const float4*)(col_bias + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-            for (int r = warp - 2; r < rows; r += kEpilogueWarps) {
-                const int row = rank * rows + r, m = m0 + row;
-                if (m >= p.m)
-                    break;
-                const int unit = (lane & ~7) + ((lane ^ row) & 7);
-                uint4 x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[i] = i < p.csplit ? ld_cluster_v4(base + (uint32_t)(row * 512 + unit * 16), i)
-                                        : make_uint4(0, 0, 0, 0);
-                uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[0] += x[i].x;
-                    v[1] += x[i].y;
-                    v[2] += x[i].z;
-                    v[3] += x[i].w;
-                }
-                const float sa = p.sa[m];
-                float f[4] = {scale_acc((int)v[0], sa, s.x), scale_acc((int)v[1], sa, s.y),
-                              scale_acc((int)v[2], sa, s.z), scale_acc((int)v[3], sa, s.w)};
-                if (p.bias) {
-                    f[0] = __fadd_rn(f[0], b.x);
-                    f[1] = __fadd_rn(f[1], b.y);
-                    f[2] = __fadd_rn(f[2], b.z);
-                    f[3] = __fadd_rn(f[3], b.w);
-                }
-                T* c = (T*)p.c + (long long)m * p.ldc + col;
-                T o[4] = {Out<T>::one(f[0]), Out<T>::one(f[1]), Out<T>::one(f[2]), Out<T>::one(f[3])};
-                if (p.vector_stores && col + 4 <= p.n) {
-                    if (sizeof(T) == 4)
-                        *(uint4*)c = *(const uint4*)o;
-                    else
-                        *(uint2*)c = *(const uint2*)o;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < p.n)
-                            c[j] = o[j];
-                }
-            }
+            const uint32_t partials = smem_u32(smem);
+            if (p.csplit == 2)
+                finish_rows<T, 2>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
+            else if (p.csplit == 4)
+                finish_rows<T, 4>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
+            else
+                finish_rows<T, 8>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
         }
         __syncwarp();
         cluster_arrive();
@@ -668,38 +736,47 @@ __global__ void __launch_bounds__(kThreads, 2) product_split_kernel(
     }
 }
 
-int encode(CUtensorMap* map, const void* p, int k, int rows, long long pitch, int box_rows) {
+// a matrix of rows of `cols` elements, `pitch` bytes apart, in boxes of rows of 128 (operands) or 64 bytes (results)
+int encode_as(
+        CUtensorMap* map, CUtensorMapDataType type, const void* p, int cols, int rows, long long pitch, int box_cols,
+        int box_rows, CUtensorMapSwizzle swizzle) {
     const DriverApi& api = driver_api();
     if (!api.ok)
         return set_error(ST_RUNTIME, "cuTensorMapEncode* entry points not found in the driver");
-    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)pitch};
-    cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     const CUresult r = api.tiled(
-            map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            map, type, 2, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? ST_SUCCESS : set_error(ST_RUNTIME, "cuTensorMapEncodeTiled failed: %d", (int)r);
 }
 
+int encode(CUtensorMap* map, const void* p, int k, int rows, long long pitch, int box_rows) {
+    return encode_as(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p, k, rows, pitch, kBK, box_rows,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // Which kernel, by the clocks of its busiest SM. A 128-byte step of K takes a 128 x 128 tile's SM 512 clocks and
-// a pair's two 560 (shared memory); in front of the first step and behind the last one stand the loads'
-// round trip and the epilogue, with a cluster's exchange where K is split.
+// a pair's two 560 (shared memory); in front of the first step and behind the last one stand the loads' round
+// trip and the epilogue, with a cluster's exchange where K is split.
 struct Choice {
     bool pair;
     int csplit;
 };
-Choice choose(const UmmaArgs& p, int sms) {
+template <class Fit>
+Choice choose(const UmmaArgs& p, int sms, Fit clusters_that_fit) {
     const long long steps = p.k_steps;
     const long long pair_tiles = (long long)((p.m - 1) / (2 * kBM) + 1) * ((p.n - 1) / kPairBN + 1);
-    long long best = (pair_tiles + sms / 2 - 1) / (sms / 2) * steps * 560 + 6000;
+    long long best = (pair_tiles + sms / 2 - 1) / (sms / 2) * (steps * 560 < 3000 ? 3000 : steps * 560) + 6000;
     Choice c = {true, 1};
     const long long tiles = (long long)((p.m - 1) / kBM + 1) * ((p.n - 1) / kSplitBN + 1);
     for (int split = 1; split <= 8; split *= 2) {
-        if (split > steps || (split > 1 && tiles * split > sms))
+        if (split > steps || (split > 1 && tiles > clusters_that_fit(split)))
             break;
         const long long waves = (tiles * split + sms - 1) / sms;
-        const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 2500 : 1000);
+        const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 3000 : 1000);
         if (t < best) {
             best = t;
             c = {false, split};
@@ -711,7 +788,13 @@ Choice choose(const UmmaArgs& p, int sms) {
 template <class T>
 int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t st) {
     const int sms = sm_count();
-    const Choice choice = choose(p, sms);
+    static ClusterCapacity split_capacity;
+    static KernelReady split_ready;
+    if (!split_ready.smem(product_split_kernel<T>, split_dynamic(kMaxStages, kTileBytes)))
+        return check_launch("matmul_s8_scaled smem attribute");
+    const Choice choice = choose(p, sms, [&](int split) {
+        return split_capacity.clusters(product_split_kernel<T>, split, kSplitThreads, split_dynamic(3, kTileBytes));
+    });
     CUtensorMap map_a, map_b;
     cudaError_t e;
     if (choice.pair) {
@@ -724,31 +807,40 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
         int rc = encode(&map_a, a.a, a.k, a.m, a.lda, kBM);
         if (!rc)
             rc = encode(&map_b, a.b, a.k, a.n, a.ldb, kBM);
+        CUtensorMap map_c = map_b;  // (not used where rows of c are no whole 16-byte units)
+        if (!rc && p.vector_stores)
+            rc = encode_as(&map_c,
+                           a.c_dtype == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                           : a.c_dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                           a.c, a.n, a.m, a.ldc * (long long)sizeof(T), kRoundCols<T>, 32, CU_TENSOR_MAP_SWIZZLE_64B);
         if (rc)
             return rc;
         const long long total = (long long)p.m_tiles * p.n_tiles;
-        const int fit = capacity.clusters(product_pair_kernel<T>, 2, kThreads, kPairDynamic);
+        const int fit = capacity.clusters(product_pair_kernel<T>, 2, kPairThreads, kPairDynamic);
         const int clusters = (int)(total < fit ? total : fit);
-        e = launch_pdl(writes, product_pair_kernel<T>, dim3((unsigned)(2 * clusters)), dim3(kThreads), kPairDynamic,
-                       st, map_a, map_b, p);
+        e = launch_pdl(writes, product_pair_kernel<T>, dim3((unsigned)(2 * clusters)), dim3(kPairThreads), kPairDynamic,
+                       st, map_a, map_b, map_c, p);
     } else {
-        static KernelReady ready;
         p.m_tiles = (p.m - 1) / kBM + 1;
         p.n_tiles = (p.n - 1) / kSplitBN + 1;
         p.csplit = choice.csplit;
         p.a_rows = p.m >= kBM ? kBM : (p.m + 7) / 8 * 8;
         const long long ctas = (long long)p.m_tiles * p.n_tiles * p.csplit;
-        // with more CTAs than SMs two share one: one's epilogue beside the other's loads
-        p.stages = ctas > sms ? 3 : kMaxStages;
-        if (!ready.smem(product_split_kernel<T>, split_dynamic(kMaxStages)))
-            return check_launch("matmul_s8_scaled smem attribute");
+        p.a_bytes = (p.a_rows * kBK + 1023) / 1024 * 1024;
+        // With more CTAs than SMs two share one, one's epilogue beside the other's loads: half the shared memory for
+        // each. Otherwise all of it (61 x 14336 x 4096: 13.0 us, 15.0 with half, although the next product's
+        // first weights could then be fetched beside this one)
+        p.stages = ctas > sms ? ((112 << 10) - split_dynamic(0, 0)) / (p.a_bytes + kTileBytes) : kMaxStages;
+        if (p.stages > kMaxStages)
+            p.stages = kMaxStages;
         int rc = encode(&map_a, a.a, a.k, a.m, a.lda, p.a_rows);
         if (!rc)
             rc = encode(&map_b, a.b, a.k, a.n, a.ldb, kSplitBN);
         if (rc)
             return rc;
-        e = launch_pdl_cluster(writes, product_split_kernel<T>, dim3((unsigned)ctas), dim3(kThreads),
-                               (size_t)split_dynamic(p.stages), p.csplit, st, map_a, map_b, p);
+        e = launch_pdl_cluster(writes, product_split_kernel<T>, dim3((unsigned)ctas), dim3(kSplitThreads),
+                               (size_t)split_dynamic(p.stages, p.a_bytes), p.csplit, st, map_a, map_b, p);
     }
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
