@@ -67,8 +67,9 @@ bool streams_activations(int m, int k) {
 bool rows_fit(const void* p, int rows, long long ld) {
     return !misaligned(p, 16) && (rows == 1 || ld % 16 == 0);
 }
+// (whole lines: 128 bytes of K then come as one line of the L2, not as parts of two)
 long long padded(int k) {
-    return ((long long)k + 15) / 16 * 16;
+    return ((long long)k + 127) / 128 * 128;
 }
 size_t padded_bytes(int rows, int k) {
     return align_up((size_t)rows * (size_t)padded(k), 256);

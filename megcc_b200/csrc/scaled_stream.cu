@@ -11,44 +11,53 @@ namespace {
 // HBM: every element is read once and written once as a byte. LANES threads share a row: a warp where
 // a row fits its registers (no barrier), else a whole CTA. The first HELD * LANES vectors of the row stay
 // in registers between the maximum and the conversion, what lies behind them is read again.
-constexpr int kRowThreads = 256;
-
-template <class T, int LANES, int HELD>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(
+template <class T, int LANES, int HELD, int THREADS>
+__global__ void __launch_bounds__(THREADS) quantize_rows_kernel(
         const T* __restrict__ x, int m, int k, long long ldx, int8_t* __restrict__ q, long long ldq,
         float* __restrict__ scales, int vector_loads, int word_stores) {
     constexpr int N = Vec<T>::N;
-    __shared__ uint32_t part[kRowThreads / 32];
+    __shared__ uint32_t part[THREADS / 32];
     pdl_start();
     const int lane = threadIdx.x % LANES;
-    const long long row = (long long)blockIdx.x * (kRowThreads / LANES) + threadIdx.x / LANES;
+    const long long row = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
     if (LANES == 32 && row >= m)
         return;  // (a whole warp; no barrier follows in this form)
     const T* src = x + row * ldx;
     int8_t* dst = q + row * ldq;
-    const int nvec = vector_loads ? k / N : 0;  // the elements behind them one by one
+    const int nvec = (k + N - 1) / N;
+    // (rows that start anywhere, and a row's end, come through the 16-byte units that hold them, zeros behind)
+    auto load = [&](int v) {
+        return vector_loads && (v + 1) * N <= k ? ((const uint4*)src)[v]
+                                                : ld_any16((const int8_t*)(src + v * N), (k - v * N) * (int)sizeof(T));
+    };
     uint4 held[HELD];
     uint32_t vm = 0;
+    if (vector_loads && nvec * N == k) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int v = lane + i * LANES;
-        held[i] = v < nvec ? ((const uint4*)src)[v] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < HELD; ++i) {
+            const int v = lane + i * LANES;
+            held[i] = v < nvec ? ((const uint4*)src)[v] : make_uint4(0, 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int v = lane + i * LANES;
+            held[i] = v < nvec ? load(v) : make_uint4(0, 0, 0, 0);
+        }
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
         vm = vec_max<T>(vm, held[i]);
     for (int v = lane + HELD * LANES; v < nvec; v += LANES)
-        vm = vec_max<T>(vm, ((const uint4*)src)[v]);
+        vm = vec_max<T>(vm, load(v));
     uint32_t bits = max_bits<T>(vm);
-    for (int i = nvec * N + lane; i < k; i += LANES)
-        bits = max(bits, magnitude(to_float(src[i])));
     bits = __reduce_max_sync(0xffffffffu, bits);
     if (LANES > 32) {
         if ((threadIdx.x & 31) == 0)
             part[threadIdx.x >> 5] = bits;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kRowThreads / 32; ++w)
+        for (int w = 0; w < THREADS / 32; ++w)
             bits = max(bits, part[w]);
     }
     const RowScale r = row_scale(bits);
@@ -61,7 +70,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(
 #pragma unroll
         for (int i = 0; i < N / 4; ++i)
             o[i] = pack_whole(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], r.inv) & r.keep;
-        if (word_stores) {
+        if (word_stores && (v + 1) * N <= k) {
             if (N == 8)
                 *(uint2*)(dst + (size_t)v * N) = make_uint2(o[0], o[N / 4 - 1]);
             else
@@ -69,7 +78,8 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                dst[(size_t)v * N + i] = (int8_t)(o[i / 4] >> (8 * (i % 4)));
+                if (v * N + i < k)
+                    dst[(size_t)v * N + i] = (int8_t)(o[i / 4] >> (8 * (i % 4)));
         }
     };
 #pragma unroll
@@ -77,9 +87,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(
         if (lane + i * LANES < nvec)
             put(lane + i * LANES, held[i]);
     for (int v = lane + HELD * LANES; v < nvec; v += LANES)
-        put(v, ((const uint4*)src)[v]);
-    for (int i = nvec * N + lane; i < k; i += LANES)
-        dst[i] = (int8_t)(to_whole(to_float(src[i]), r.inv) & r.keep);
+        put(v, load(v));
 }
 
 template <class T>
@@ -93,15 +101,15 @@ int quantize_rows(
     const uintptr_t s0 = (uintptr_t)scales, s1 = s0 + (size_t)m * 4;
     const uintptr_t w0 = q0 < s0 ? q0 : s0, w1 = q1 > s1 ? q1 : s1;
     const Writes writes{(const void*)w0, w1 - w0};
-    auto launch = [&](auto kernel, int rows) {
-        return launch_pdl(writes, kernel, dim3((unsigned)((m - 1) / rows + 1)), dim3(kRowThreads), 0, st, x, m, k, ldx,
+    auto launch = [&](auto kernel, int rows, int threads) {
+        return launch_pdl(writes, kernel, dim3((unsigned)((m - 1) / rows + 1)), dim3((unsigned)threads), 0, st, x, m, k, ldx,
                           q, ldq, scales, vector_loads, word_stores);
     };
     // A warp per row where it holds the row and there are rows enough for every SM's warps: 4001 x 4096 fp16 in
     // 8.6 us, by whole CTAs in 12.3
-    const cudaError_t e = m > 1 && k <= 32 * 4 * N            ? launch(quantize_rows_kernel<T, 32, 4>, 8)
-                          : m >= 2048 && k <= 32 * 16 * N     ? launch(quantize_rows_kernel<T, 32, 16>, 8)
-                                                              : launch(quantize_rows_kernel<T, kRowThreads, 4>, 1);
+    const cudaError_t e = m > 1 && k <= 32 * 4 * N            ? launch(quantize_rows_kernel<T, 32, 4, 256>, 8, 256)
+                          : m >= 2048 && k <= 32 * 16 * N     ? launch(quantize_rows_kernel<T, 32, 16, 64>, 2, 64)
+                                                              : launch(quantize_rows_kernel<T, 256, 4, 256>, 1, 256);
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "quantize_rows: %s", cudaGetErrorString(e));
     return check_launch("quantize_rows");

@@ -181,8 +181,11 @@ __device__ __forceinline__ void rows_to_whole(
     const int warp = (int)(threadIdx.x >> 5) - FIRST, lane = threadIdx.x & 31;
     const int share = rows >= WARPS ? 1 : rows * 2 >= WARPS ? 2 : rows * 4 >= WARPS ? 4 : WARPS;
     const int stride = share * 512, first = (warp % share * 32 + lane) * 16;
-    const int in_vectors = vectors ? k & ~15 : 0;  // elements taken 16 at a time; the others one by one
-    constexpr int N = 16 / Vec<T>::N;              // loads of 16 elements
+    // Elements taken 16 at a time; the others (of rows that start anywhere: all) 16 bytes at a time, through the
+    // units that hold them
+    const int in_vectors = vectors ? k & ~15 : 0;
+    constexpr int V = Vec<T>::N, N = 16 / V;  // elements of a load, loads of 16 elements
+    const int any_first = in_vectors + first / 16 * V, any_stride = share * 32 * V;
 #pragma unroll 1
     for (int r = warp / share; r < rows; r += WARPS / share) {
         const T* x = (const T*)row(r);
@@ -199,8 +202,8 @@ __device__ __forceinline__ void rows_to_whole(
         }
         uint32_t bits = max_bits<T>(vm);
 #pragma unroll 1
-        for (int i = in_vectors + first / 16; i < k; i += stride / 16)
-            bits = max(bits, magnitude(to_float(x[i])));
+        for (int i = any_first; i < k; i += any_stride)
+            bits = max(bits, max_bits<T>(vec_max<T>(0, ld_any16((const int8_t*)(x + i), (k - i) * (int)sizeof(T)))));
         bits = __reduce_max_sync(0xffffffffu, bits);
         if (lane == 0)
             part[r * WARPS + warp % share] = bits;
@@ -226,12 +229,17 @@ __device__ __forceinline__ void rows_to_whole(
             float v[16];
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                Vec<T>::unpack(((const uint4*)(x + i))[j], v + Vec<T>::N * j);
+                Vec<T>::unpack(((const uint4*)(x + i))[j], v + V * j);
             *(uint4*)(to + i) = pack_piece(v, s);
         }
 #pragma unroll 1
-        for (int i = in_vectors + first / 16; i < end; i += stride / 16)
-            to[i] = i < k ? (int8_t)(to_whole(to_float(x[i]), s.inv) & s.keep) : 0;
+        for (int i = any_first; i < end; i += any_stride) {
+            float v[V];
+            Vec<T>::unpack(ld_any16((const int8_t*)(x + i), (k - i) * (int)sizeof(T)), v);
+#pragma unroll
+            for (int j = 0; j < V; j += 4)
+                *(uint32_t*)(to + i + j) = pack_whole(v[j], v[j + 1], v[j + 2], v[j + 3], s.inv) & s.keep;
+        }
     }
 }
 // Asks for what the CTA's threads will read soon: `bytes` from p on, into the L1.
