@@ -55,17 +55,26 @@ int check_workspace(const char* what, const void* workspace, size_t have, size_t
     return ST_SUCCESS;
 }
 
-// Few rows of activations: the kernel that takes the weights straight to registers, whatever the operands'
-// alignment; and so few that it makes whole numbers of them itself, every CTA again.
-bool streams(int m) {
-    return m <= 16;
-}
-bool streams_activations(int m, int k) {
-    return m <= 8 && (long long)m * k <= 32768;
-}
 // What the TMA takes: 16-byte aligned, rows whole 16-byte units apart
 bool rows_fit(const void* p, int rows, long long ld) {
     return !misaligned(p, 16) && (rows == 1 || ld % 16 == 0);
+}
+// Few rows of activations, or little of everything: the kernel that streams the weights past them, whatever the
+// operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles): 17 rows 1024 x 1024 1.9 / 5.2,
+// 4096 x 4096 4.4 / 7.0, 4096 x 14336 14.3 / 13.6; 16 rows 4096 x 14336 10.7 / 13.6, 14336 x 4096 13.8 / 12.7, 32768 x 2048
+// 17.8 / 13.3: tiles of whole K win where they are enough for the SMs, or where tokens weigh as much as weights.
+// `fits`: the tiles' operands need no copies (4100 x 4100, 32 rows: 13.7 / 15.4).
+bool streams(int m, int n, int k, bool fits) {
+    const long long weights = (long long)n * k, many = 1 << 25;
+    if (m <= 16)
+        return !fits || weights <= many || n < 74 * 128;
+    if (m <= 32)
+        return !fits || weights <= many;
+    return m <= (1 << 20) && (m + 31) / 32 * weights <= 1 << 22;  // a pass over the weights per 32 rows
+}
+// So few that it makes whole numbers of them itself, every CTA again
+bool streams_activations(int m, int k) {
+    return m <= 8 && (long long)m * k <= 32768;
 }
 // (whole lines: 128 bytes of K then come as one line of the L2, not as parts of two)
 long long padded(int k) {
@@ -136,7 +145,8 @@ int mb200_quantize_rows_s8(
 
 size_t mb200_matmul_s8_scaled_workspace_bytes(
         int m, int n, int k, const int8_t* a, long long lda, const int8_t* b_packed) {
-    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || streams(m))
+    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK ||
+        streams(m, n, k, rows_fit(a, m, lda) && rows_fit(b_packed, n, k)))
         return 0;
     return (rows_fit(a, m, lda) ? 0 : padded_bytes(m, k)) + (rows_fit(b_packed, n, k) ? 0 : padded_bytes(n, k));
 }
@@ -169,7 +179,7 @@ int mb200_matmul_s8_scaled(
     p.a = a, p.x_dtype = -1, p.lda = lda;
     p.b = b_packed, p.ldb = k, p.sa = a_scales, p.sb = b_scales, p.bias = bias;
     p.c = c, p.c_dtype = dtype, p.ldc = ldc;
-    if (streams(m)) {
+    if (streams(m, n, k, rows_fit(a, m, lda) && rows_fit(b_packed, n, k))) {
         p.b_early = may_read_early(b_packed, (size_t)n * k, st);
         return launch_product_stream(p, st);
     }
@@ -187,7 +197,7 @@ size_t mb200_linear_s8_workspace_bytes(int m, int n, int k, const int8_t* b_pack
     if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || streams_activations(m, k))
         return 0;
     return padded_bytes(m, k) + align_up((size_t)m * 4, 256) +
-           (streams(m) || rows_fit(b_packed, n, k) ? 0 : padded_bytes(n, k));
+           (rows_fit(b_packed, n, k) || streams(m, n, k, false) ? 0 : padded_bytes(n, k));
 }
 
 int mb200_linear_s8(
@@ -223,7 +233,8 @@ int mb200_linear_s8(
         return launch_product_stream(p, st);
     }
     int8_t* ws = (int8_t*)workspace;
-    if (!streams(m)) {
+    const bool few = streams(m, n, k, rows_fit(b_packed, n, k));
+    if (!few) {
         rc = launch_pad_rows(pad_job(&p.b, &p.ldb, n, k, &ws), PadRows{}, st);
         if (rc)
             return rc;
@@ -234,7 +245,7 @@ int mb200_linear_s8(
         return rc;
     p.a = ws, p.x_dtype = -1, p.lda = padded(k), p.sa = scales;
     p.b_early = may_read_early(p.b, (size_t)n * (size_t)p.ldb, st);
-    return streams(m) ? launch_product_stream(p, st) : launch_product_umma(p, st);
+    return few ? launch_product_stream(p, st) : launch_product_umma(p, st);
 }
 
 size_t mb200_moe_s8_workspace_bytes(const mb200_moe_param* p) {

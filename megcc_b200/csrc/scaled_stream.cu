@@ -109,7 +109,8 @@ int quantize_rows(
     // 8.6 us, by whole CTAs in 12.3
     const cudaError_t e = m > 1 && k <= 32 * 4 * N            ? launch(quantize_rows_kernel<T, 32, 4, 256>, 8, 256)
                           : m >= 2048 && k <= 32 * 16 * N     ? launch(quantize_rows_kernel<T, 32, 16, 64>, 2, 64)
-                                                              : launch(quantize_rows_kernel<T, 256, 4, 256>, 1, 256);
+                          : k <= 256 * 4 * N                  ? launch(quantize_rows_kernel<T, 256, 4, 256>, 1, 256)
+                                                              : launch(quantize_rows_kernel<T, 256, 8, 256>, 1, 256);
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "quantize_rows: %s", cudaGetErrorString(e));
     return check_launch("quantize_rows");
@@ -128,7 +129,7 @@ template <class XT, int NT, bool ALIGNED>
 struct Stream {
     static constexpr bool kFloat = sizeof(XT) > 1;
     static constexpr int kCols = 8 * NT;
-    static constexpr int kDepth = 4;
+    static constexpr int kDepth = NT == 1 ? 4 : NT == 2 ? 3 : 2;  // (room for two CTAs per SM)
     typedef Rows<kRows, ALIGNED> W;
     typedef Rows<kCols, ALIGNED> A;
     static constexpr int kStage = W::kBytes + (kFloat ? 0 : A::kBytes);
@@ -339,7 +340,9 @@ int launch_product_stream(const ProductArgs& a, cudaStream_t st) {
     cudaError_t e;
     if (a.x_dtype < 0) {
         const bool aligned = b_aligned && ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % 16 == 0);
-        e = a.m <= 8 ? launch_stream<int8_t, 1>(a, aligned, 0, st) : launch_stream<int8_t, 2>(a, aligned, 0, st);
+        e = a.m <= 8    ? launch_stream<int8_t, 1>(a, aligned, 0, st)
+            : a.m <= 16 ? launch_stream<int8_t, 2>(a, aligned, 0, st)
+                        : launch_stream<int8_t, 4>(a, aligned, 0, st);
     } else if (a.x_dtype == DT_F32) {
         e = launch_stream_float<float>(a, b_aligned, st);
     } else if (a.x_dtype == DT_F16) {

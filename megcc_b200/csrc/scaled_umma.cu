@@ -165,11 +165,22 @@ __device__ __forceinline__ void store_round(
         }
     } else {
         const int j = lane % kCols;
-#pragma unroll 8
-        for (int r = lane / kCols; r < 32; r += 32 / kCols)
-            if (row0 + r < p.m && col0 + j < p.n)
-                c[(long long)(row0 + r) * p.ldc + col0 + j] =
-                        *(const T*)(stage + r * 64 + (((j / kUnit) ^ ((r >> 1) & 3)) << 4) + (j % kUnit) * sizeof(T));
+        T* to = c + (long long)(row0 + lane / kCols) * p.ldc + col0 + j;
+#pragma unroll
+        for (int r0 = lane / kCols; r0 < 32; r0 += 8 * (32 / kCols)) {
+            T v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i * (32 / kCols);
+                v[i] = *(const T*)(stage + r * 64 + (((j / kUnit) ^ ((r >> 1) & 3)) << 4) + (j % kUnit) * sizeof(T));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (row0 + r0 + i * (32 / kCols) < p.m && col0 + j < p.n)
+                    *to = v[i];
+                to += (32 / kCols) * p.ldc;
+            }
+        }
     }
     __syncwarp();
 }
@@ -456,70 +467,62 @@ constexpr int kSplitBN = 128;
 constexpr int kMaxStages = 6;
 constexpr int kSplitWarps = 8;  // epilogue
 constexpr int kSplitThreads = 64 + 32 * kSplitWarps;
+constexpr int kSplitMost = 227 * 1024;
 constexpr int kSplitBars = (2 * kMaxStages + 2) * 8 + 16;
 constexpr int kSplitSides = (2 * kSplitBN + kBM) * 4;  // scales and biases of columns, scales of rows
-inline int split_dynamic(int stages, int a_bytes) {
-    return stages * (a_bytes + kTileBytes) + kSplitSides + kSplitBars + 1024;
+// [CTAs of the cluster][their share of the 128 rows][32 units of four columns] of the cluster's partial sums
+constexpr int kPartialBytes = kBM * kSplitBN * 4;
+inline int split_dynamic(int stages, int a_bytes, int csplit) {
+    return stages * (a_bytes + kTileBytes) + (csplit > 1 ? kPartialBytes : 0) + kSplitSides + kSplitBars + 1024;
 }
 
-// The cluster's partial sums of this CTA's share of the rows: a row per warp, four columns per lane, 16 loads of
-// other CTAs' shared memory in two turns.
+// The cluster's partial sums of this CTA's share of the rows, which all its CTAs have brought here: a row per
+// warp, four columns per lane. (Fetched from the others' shared memory instead they took 2.1 us, twice a load's way
+// there and back; now the sums go one way, behind the last MMA of each CTA.)
 template <class T, int SPLIT>
 __device__ __forceinline__ void finish_rows(
-        uint32_t partials, int rank, int m0, int n0, const float* col_scale, const float* col_bias,
+        const uint8_t* partials, int rank, int m0, int n0, const float* col_scale, const float* col_bias,
         const float* row_scale, const UmmaArgs& p) {
-    constexpr int kRows = 8 / SPLIT;  // of a turn
+    constexpr int kShare = kBM / SPLIT;
     const int warp = (int)(threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
     const int col = n0 + 4 * lane;
     const float4 s = *(const float4*)(col_scale + 4 * lane);
     const float4 b = p.bias ? *(const float4*)(col_bias + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int turn = 0; turn < 2; ++turn) {
-        uint4 x[kRows][SPLIT];
-        int row[kRows];
+#pragma unroll 2
+    for (int r = warp; r < kShare; r += kSplitWarps) {
+        const int m = m0 + rank * kShare + r;
+        if (m >= p.m)
+            break;
+        uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            row[i] = rank * (kBM / SPLIT) + (turn * kRows + i) * kSplitWarps + warp;
-            const uint32_t at = partials + (uint32_t)(row[i] * 512 + ((lane & ~7) + ((lane ^ row[i]) & 7)) * 16);
-#pragma unroll
-            for (int j = 0; j < SPLIT; ++j)
-                x[i][j] = m0 + row[i] < p.m ? ld_cluster_v4(at, j) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < SPLIT; ++j) {
+            const uint4 x = *(const uint4*)(partials + (j * kShare + r) * 512 + ((lane & ~7) + ((lane ^ r) & 7)) * 16);
+            v[0] += x.x;
+            v[1] += x.y;
+            v[2] += x.z;
+            v[3] += x.w;
         }
+        const float sa = row_scale[rank * kShare + r];
+        float f[4] = {scale_acc((int)v[0], sa, s.x), scale_acc((int)v[1], sa, s.y), scale_acc((int)v[2], sa, s.z),
+                      scale_acc((int)v[3], sa, s.w)};
+        if (p.bias) {
+            f[0] = __fadd_rn(f[0], b.x);
+            f[1] = __fadd_rn(f[1], b.y);
+            f[2] = __fadd_rn(f[2], b.z);
+            f[3] = __fadd_rn(f[3], b.w);
+        }
+        T* c = (T*)p.c + (long long)m * p.ldc + col;
+        if (p.vector_stores && col + 4 <= p.n) {
+            const uint4 u = Out<T>::unit4(f);
+            if (sizeof(T) == 4)
+                *(uint4*)c = u;
+            else
+                *(uint2*)c = make_uint2(u.x, u.y);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const int m = m0 + row[i];
-            if (m >= p.m)
-                continue;
-            uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < SPLIT; ++j) {
-                v[0] += x[i][j].x;
-                v[1] += x[i][j].y;
-                v[2] += x[i][j].z;
-                v[3] += x[i][j].w;
-            }
-            const float sa = row_scale[row[i]];
-            float f[4] = {scale_acc((int)v[0], sa, s.x), scale_acc((int)v[1], sa, s.y), scale_acc((int)v[2], sa, s.z),
-                          scale_acc((int)v[3], sa, s.w)};
-            if (p.bias) {
-                f[0] = __fadd_rn(f[0], b.x);
-                f[1] = __fadd_rn(f[1], b.y);
-                f[2] = __fadd_rn(f[2], b.z);
-                f[3] = __fadd_rn(f[3], b.w);
-            }
-            T* c = (T*)p.c + (long long)m * p.ldc + col;
-            if (p.vector_stores && col + 4 <= p.n) {
-                const uint4 u = Out<T>::unit4(f);
-                if (sizeof(T) == 4)
-                    *(uint4*)c = u;
-                else
-                    *(uint2*)c = make_uint2(u.x, u.y);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (col + j < p.n)
-                        c[j] = Out<T>::one(f[j]);
-            }
+            for (int j = 0; j < 4; ++j)
+                if (col + j < p.n)
+                    c[j] = Out<T>::one(f[j]);
         }
     }
 }
@@ -531,7 +534,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
     // (the same offset in all CTAs of a cluster)
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = p.a_bytes + kTileBytes;
-    float* col_scale = (float*)(smem + p.stages * stage_bytes);
+    uint8_t* partials = smem + p.stages * stage_bytes;
+    float* col_scale = (float*)(partials + (p.csplit > 1 ? kPartialBytes : 0));
     float* col_bias = col_scale + kSplitBN;
     float* row_scale = col_bias + kSplitBN;
     uint64_t* full_bar = (uint64_t*)(row_scale + kBM);
@@ -573,6 +577,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+    if (p.csplit > 1)
+        cluster_arrive();  // (waited for before anything is stored in another CTA: all of them must have begun)
 
     auto give_up = [&](int code) {
         if (!*abort_flag) {
@@ -581,6 +587,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
         }
     };
 
+    bool waited = false;  // for the cluster's first barrier
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
@@ -680,30 +687,34 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
                         store_round<T>(taddr + (uint32_t)c, sa, col_scale + c, col_bias + c, p.bias != nullptr,
                                        stage, row0, n0 + c, p, nullptr, [] {});
             } else if (row0 < p.m) {
-                // the partial sums, [128 rows][32 units of four columns], units in an order by row
-                const int row = q * 32 + lane;
+                // each row to the CTA that finishes it, units of four columns in an order by row
+                const int share = kBM / p.csplit, row = q * 32 + lane, owner = row / share;
+                const uint32_t at = map_to_cta(smem_u32(partials) + (uint32_t)((rank * share + row % share) * 512),
+                                               (uint32_t)owner);
+                __syncwarp();
+                cluster_wait();
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t acc[32];
                     __syncwarp();
                     tmem_ld32(taddr + (uint32_t)(half * 64 + 32 * h), acc);
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const int unit = (half * 2 + h) * 8 + (u ^ (lane & 7));
-                        *(uint4*)(smem + row * 512 + unit * 16) =
-                                make_uint4(acc[4 * u], acc[4 * u + 1], acc[4 * u + 2], acc[4 * u + 3]);
-                    }
+                    for (int u = 0; u < 8; ++u)
+                        st_cluster_v4(at + (uint32_t)(((half * 2 + h) * 8 + (u ^ (row & 7))) * 16),
+                                      make_uint4(acc[4 * u], acc[4 * u + 1], acc[4 * u + 2], acc[4 * u + 3]));
                 }
+                waited = true;
             }
         }
     }
 
     if (p.csplit > 1) {
         __syncwarp();
+        if (!waited)
+            cluster_wait();
         cluster_arrive();
-        cluster_wait();
+        cluster_wait();  // all partial sums have been stored
         if (warp >= 2) {
-            const uint32_t partials = smem_u32(smem);
             if (p.csplit == 2)
                 finish_rows<T, 2>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
             else if (p.csplit == 4)
@@ -711,9 +722,6 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
             else
                 finish_rows<T, 8>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
         }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();  // the others may still read this CTA's sums
     }
 
     // ---------------- teardown ----------------
@@ -776,7 +784,7 @@ Choice choose(const UmmaArgs& p, int sms, Fit clusters_that_fit) {
         if (split > steps || (split > 1 && tiles > clusters_that_fit(split)))
             break;
         const long long waves = (tiles * split + sms - 1) / sms;
-        const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 3000 : 1000);
+        const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 5500 : 1000);
         if (t < best) {
             best = t;
             c = {false, split};
@@ -790,10 +798,10 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
     const int sms = sm_count();
     static ClusterCapacity split_capacity;
     static KernelReady split_ready;
-    if (!split_ready.smem(product_split_kernel<T>, split_dynamic(kMaxStages, kTileBytes)))
+    if (!split_ready.smem(product_split_kernel<T>, kSplitMost))
         return check_launch("matmul_s8_scaled smem attribute");
     const Choice choice = choose(p, sms, [&](int split) {
-        return split_capacity.clusters(product_split_kernel<T>, split, kSplitThreads, split_dynamic(3, kTileBytes));
+        return split_capacity.clusters(product_split_kernel<T>, split, kSplitThreads, split_dynamic(3, kTileBytes, split));
     });
     CUtensorMap map_a, map_b;
     cudaError_t e;
@@ -831,7 +839,8 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
         // With more CTAs than SMs two share one, one's epilogue beside the other's loads: half the shared memory for
         // each. Otherwise all of it (61 x 14336 x 4096: 13.0 us, 15.0 with half, although the next product's
         // first weights could then be fetched beside this one)
-        p.stages = ctas > sms ? ((112 << 10) - split_dynamic(0, 0)) / (p.a_bytes + kTileBytes) : kMaxStages;
+        const int room = (p.csplit == 1 && ctas > sms ? 112 << 10 : kSplitMost) - split_dynamic(0, 0, p.csplit);
+        p.stages = room / (p.a_bytes + kTileBytes);
         if (p.stages > kMaxStages)
             p.stages = kMaxStages;
         int rc = encode(&map_a, a.a, a.k, a.m, a.lda, p.a_rows);
@@ -840,7 +849,7 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
         if (rc)
             return rc;
         e = launch_pdl_cluster(writes, product_split_kernel<T>, dim3((unsigned)ctas), dim3(kSplitThreads),
-                               (size_t)split_dynamic(p.stages, p.a_bytes), p.csplit, st, map_a, map_b, p);
+                               (size_t)split_dynamic(p.stages, p.a_bytes, p.csplit), p.csplit, st, map_a, map_b, p);
     }
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
