@@ -92,97 +92,158 @@ struct Out<__nv_bfloat16> {
     }
 };
 
-// 32 rows (a warp's lanes) times 64 bytes of results: from tensor memory through 2 KB of shared memory to whole
-// sectors. scale, bias: of the columns, in shared memory (16-byte aligned); `taken()` is called once the sums are
-// in registers.
-template <class T>
-constexpr int kRoundCols = 64 / (int)sizeof(T);
+// What a lane needs of the scales for 32 rows times 64 columns of sums. tcgen05.ld 16x256b hands it, of each 16 rows, the
+// rows lane / 4 and lane / 4 + 8, and of each eight columns 2 * (lane % 4) and the one behind: so four rows' and sixteen
+// columns' scales stay in registers, where a row per lane would read all 64 columns' from shared memory, which the
+// MMAs and the TMA keep busy (8192^3: 333 -> 325 us).
+struct Sides {
+    float row[4];
+    float2 scale[8], bias[8];
+    // rows: the lane's own row's scale; scale, bias: of the 64 columns, in shared memory
+    __device__ __forceinline__ void take(float rows, const float* col_scale, const float* col_bias, bool has_bias) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            row[i] = __shfl_sync(0xffffffffu, rows, 8 * i + (lane >> 2));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            scale[j] = *(const float2*)(col_scale + 8 * j + 2 * (lane & 3));
+            bias[j] = has_bias ? *(const float2*)(col_bias + 8 * j + 2 * (lane & 3)) : make_float2(0.f, 0.f);
+        }
+    }
+    __device__ __forceinline__ float2 apply(uint32_t a, uint32_t b, int i, int j, bool has_bias) const {
+        float2 v = make_float2(scale_acc((int)a, row[i], scale[j].x), scale_acc((int)b, row[i], scale[j].y));
+        if (has_bias)
+            v = make_float2(__fadd_rn(v.x, bias[j].x), __fadd_rn(v.y, bias[j].y));
+        return v;
+    }
+};
+// 16 lanes of tensor memory times 8 * N columns; 4 * N words per lane of the warp
+__device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+              "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+            : "r"(taddr)
+            : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait2(uint32_t (&a)[16], uint32_t (&b)[16]) {
+    tmem_ld_wait16(a);
+    tmem_ld_wait16(b);
+}
+__device__ __forceinline__ void stmatrix_x4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
+
+// 32 rows (of the warp's tensor memory lanes) times 64 columns of results, through 2 KB of shared memory to whole
+// sectors: 64 bytes of each row at a time. With map_c the TMA stores them; else the warp does.
+// `taken()` is called once the sums are in registers.
 constexpr int kRoundBytes = 32 * 64;
 template <class T, class Taken>
-__device__ __forceinline__ void store_round(
-        uint32_t taddr, float sa, const float* scale, const float* bias, bool has_bias, uint8_t* stage, int row0,
-        int col0, const UmmaArgs& p, const CUtensorMap* map_c, Taken taken) {
+__device__ __forceinline__ void store_columns(
+        uint32_t taddr, const Sides& sides, bool has_bias, uint8_t* stage, int row0, int col0, const UmmaArgs& p,
+        const CUtensorMap* map_c, Taken taken) {
     constexpr int kUnit = 16 / (int)sizeof(T);  // results per 16 bytes
-    constexpr int kCols = kRoundCols<T>;
+    constexpr int kCols = 4 * kUnit;            // of a round
     const int lane = threadIdx.x & 31;
-    uint32_t acc[kCols];
-    if (map_c) {
-        // the last round's bytes have left the stage
-        if (lane == 0)
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    }
-    __syncwarp();
-    if constexpr (kCols == 32)
-        tmem_ld32(taddr, acc);
-    else
-        tmem_ld16(taddr, acc);
-    taken();
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        float v[kUnit];
-#pragma unroll
-        for (int j = 0; j < kUnit; j += 4) {
-            const int at = u * kUnit + j;
-            const float4 s = *(const float4*)(scale + at);
-            v[j] = scale_acc((int)acc[at], sa, s.x);
-            v[j + 1] = scale_acc((int)acc[at + 1], sa, s.y);
-            v[j + 2] = scale_acc((int)acc[at + 2], sa, s.z);
-            v[j + 3] = scale_acc((int)acc[at + 3], sa, s.w);
-            if (has_bias) {
-                const float4 b = *(const float4*)(bias + at);
-                v[j] = __fadd_rn(v[j], b.x);
-                v[j + 1] = __fadd_rn(v[j + 1], b.y);
-                v[j + 2] = __fadd_rn(v[j + 2], b.z);
-                v[j + 3] = __fadd_rn(v[j + 3], b.w);
-            }
-        }
-        // (a row's 16-byte units in an order that depends on the row: no two lanes of eight share a bank; it is the
-        // TMA's 64-byte swizzle)
-        *(uint4*)(stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = Out<T>::unit(v);
-    }
-    if (map_c) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0 && row0 < p.m && col0 < p.n) {
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                                 (uint64_t)map_c),
-                         "r"(smem_u32(stage)), "r"(col0), "r"(row0)
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-        return;
-    }
-    __syncwarp();
+    const uint32_t at = smem_u32(stage);
     T* c = (T*)p.c;
-    if (p.vector_stores && col0 + kCols <= p.n) {
-        const int unit = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2);
-            const uint4 v = *(const uint4*)(stage + r * 64 + ((unit ^ ((r >> 1) & 3)) << 4));
-            if (row0 + r < p.m)
-                *(uint4*)(c + (long long)(row0 + r) * p.ldc + col0 + unit * kUnit) = v;
-        }
-    } else {
-        const int j = lane % kCols;
-        T* to = c + (long long)(row0 + lane / kCols) * p.ldc + col0 + j;
+    for (int h = 0; h < 2; ++h) {  // 32 columns
+        uint32_t acc[2][16];
+        __syncwarp();
+        tmem_ld_16x256b(taddr + (uint32_t)(32 * h), acc[0]);
+        tmem_ld_16x256b(taddr + (16u << 16) + (uint32_t)(32 * h), acc[1]);
+        tmem_ld_wait2(acc[0], acc[1]);
+        if (h == 1)
+            taken();
 #pragma unroll
-        for (int r0 = lane / kCols; r0 < 32; r0 += 8 * (32 / kCols)) {
-            T v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = r0 + i * (32 / kCols);
-                v[i] = *(const T*)(stage + r * 64 + (((j / kUnit) ^ ((r >> 1) & 3)) << 4) + (j % kUnit) * sizeof(T));
+        for (int round = 0; round < 32 / kCols; ++round) {
+            const int col = col0 + 32 * h + round * kCols;
+            if (map_c) {
+                // the last round's bytes have left the stage
+                if (lane == 0)
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
             }
+            // (a row's 16-byte units in an order that depends on the row, the TMA's 64-byte swizzle)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (row0 + r0 + i * (32 / kCols) < p.m && col0 + j < p.n)
-                    *to = v[i];
-                to += (32 / kCols) * p.ldc;
+            for (int q = 0; q < 2; ++q) {  // 16 rows
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = 2 * jj + (i >> 1);
+                            const float2 v = sides.apply(acc[q][4 * j + 2 * (i & 1)], acc[q][4 * j + 2 * (i & 1) + 1],
+                                                         2 * q + (i & 1), 4 * h + j, has_bias);
+                            w[i] = Out<T>::two(v.x, v.y);
+                        }
+                        const int r = 16 * q + (lane & 15), unit = 2 * jj + (lane >> 4);
+                        stmatrix_x4(at + (uint32_t)(r * 64 + ((unit ^ ((r >> 1) & 3)) << 4)), w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int jc = 2 * round + j;
+                            const float2 v = sides.apply(acc[q][4 * jc + 2 * i], acc[q][4 * jc + 2 * i + 1], 2 * q + i,
+                                                         4 * h + jc, has_bias);
+                            const int r = 16 * q + 8 * i + (lane >> 2), unit = 2 * j + ((lane & 3) >> 1);
+                            *(float2*)(stage + r * 64 + ((unit ^ ((r >> 1) & 3)) << 4) + 8 * (lane & 1)) = v;
+                        }
+                }
             }
+            if (map_c) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0 && row0 < p.m && col < p.n) {
+                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                                         (uint64_t)map_c),
+                                 "r"(at), "r"(col), "r"(row0)
+                                 : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+                continue;
+            }
+            __syncwarp();
+            if (p.vector_stores && col + kCols <= p.n) {
+                const int unit = lane & 3;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 8 * i + (lane >> 2);
+                    const uint4 v = *(const uint4*)(stage + r * 64 + ((unit ^ ((r >> 1) & 3)) << 4));
+                    if (row0 + r < p.m)
+                        *(uint4*)(c + (long long)(row0 + r) * p.ldc + col + unit * kUnit) = v;
+                }
+            } else {
+                const int j = lane % kCols;
+                T* to = c + (long long)(row0 + lane / kCols) * p.ldc + col + j;
+#pragma unroll 1
+                for (int r0 = lane / kCols; r0 < 32; r0 += 8 * (32 / kCols)) {
+                    T v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i * (32 / kCols);
+                        v[i] = *(const T*)(stage + r * 64 + (((j / kUnit) ^ ((r >> 1) & 3)) << 4) +
+                                           (j % kUnit) * sizeof(T));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (row0 + r0 + i * (32 / kCols) < p.m && col + j < p.n)
+                            *to = v[i];
+                        to += (32 / kCols) * p.ldc;
+                    }
+                }
+            }
+            __syncwarp();
         }
     }
-    __syncwarp();
 }
 
 // the epilogue warps' barrier
@@ -415,20 +476,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
                 continue;  // (still meets the others at the barrier in front of the next tile)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kPairBN);
-#pragma unroll 1
-            for (int c = quarter * 64; c < quarter * 64 + 64; c += kRoundCols<T>) {
-                const bool last = c + kRoundCols<T> == quarter * 64 + 64;
-                store_round<T>(taddr + (uint32_t)c, row_scale, col_scale + c, col_bias + c, p.bias != nullptr, stage, row0,
-                               n0 + c, p, p.vector_stores ? &map_c : nullptr, [&] {
-                                   if (last) {
-                                       // this warp's sums are in registers: one arrival on the leader's barrier
-                                       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                                       __syncwarp();
-                                       if (lane == 0)
-                                           mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
-                                   }
-                               });
-            }
+Sides sides;
+            sides.take(row_scale, col_scale + quarter * 64, col_bias + quarter * 64, p.bias != nullptr);
+            store_columns<T>(taddr + (uint32_t)(quarter * 64), sides, p.bias != nullptr, stage, row0, n0 + quarter * 64, p,
+                             p.vector_stores ? &map_c : nullptr, [&] {
+                                 // this warp's sums are in registers: one arrival on the leader's barrier
+                                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                 __syncwarp();
+                                 if (lane == 0)
+                                     mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+                             });
         }
         if (lane == 0)
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -681,11 +738,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
             if (p.csplit == 1) {
                 uint8_t* stage = smem + (warp - 2) * kRoundBytes;
-#pragma unroll 1
-                for (int c = half * 64; c < half * 64 + 64; c += kRoundCols<T>)
-                    if (row0 < p.m && n0 + c < p.n)
-                        store_round<T>(taddr + (uint32_t)c, sa, col_scale + c, col_bias + c, p.bias != nullptr,
-                                       stage, row0, n0 + c, p, nullptr, [] {});
+if (row0 < p.m && n0 + half * 64 < p.n) {
+                    Sides sides;
+                    sides.take(sa, col_scale + half * 64, col_bias + half * 64, p.bias != nullptr);
+                    store_columns<T>(taddr + (uint32_t)(half * 64), sides, p.bias != nullptr, stage, row0,
+                                     n0 + half * 64, p, nullptr, [] {});
+                }
             } else if (row0 < p.m) {
                 // each row to the CTA that finishes it, units of four columns in an order by row
                 const int share = kBM / p.csplit, row = q * 32 + lane, owner = row / share;
@@ -821,7 +879,8 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
                            a.c_dtype == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                            : a.c_dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                           a.c, a.n, a.m, a.ldc * (long long)sizeof(T), kRoundCols<T>, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+                           a.c, a.n, a.m, a.ldc * (long long)sizeof(T), 64 / (int)sizeof(T), 32,
+                           CU_TENSOR_MAP_SWIZZLE_64B);
         if (rc)
             return rc;
         const long long total = (long long)p.m_tiles * p.n_tiles;
