@@ -37,9 +37,10 @@ struct Route {
     int* passes;
     // while it is worked out (in memory that is used for something else afterwards)
     int* expert;       // by slot; -1: no share in the result
-    int *count, *at;   // by expert: its slots, and where the next one goes
+    uint32_t* tokens;  // by expert: a bit for each of its tokens
+    int* at;           // by expert: where its slots begin
 };
-constexpr int kMostBuild = up16(4 * kMoeMaxTokens * kMoeMaxTop) + 2 * up16(4 * kMoeMaxExperts);
+constexpr int kMostBuild = up16(4 * kMoeMaxTokens * kMoeMaxTop) + up16(8 * kMoeMaxExperts) + up16(4 * kMoeMaxExperts);
 __device__ __forceinline__ Route place_route(uint8_t* at, uint8_t* build, int slots, int experts, int cols) {
     Route r;
     r.p = (float*)at;
@@ -53,8 +54,8 @@ __device__ __forceinline__ Route place_route(uint8_t* at, uint8_t* build, int sl
     r.passes = (int*)(at + 3 * n);
     r.expert = (int*)build;
     build += up16(4 * slots);
-    r.count = (int*)build;
-    r.at = (int*)(build + up16(4 * experts));
+    r.tokens = (uint32_t*)build;
+    r.at = (int*)(build + up16(8 * experts));
     return r;
 }
 
@@ -68,84 +69,115 @@ __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-// One token's experts, by a warp: lane j < top gets the j-th choice's index and p. The first 128 logits are kept in
+// N tokens' experts, by a warp: lane j < top gets the j-th choice's index and p. The first 128 logits are kept in
 // registers; of those behind them each choice is the largest that comes behind the one before it (smaller, or
-// equal with a higher index).
+// equal with a higher index). A choice waits for two reductions over the warp (145 ns): two tokens wait together.
 struct Choice {
     int expert;
     float p;
 };
-__device__ __noinline__ Choice choose_experts(const float* row, int experts, int top, int renormalize) {
+template <int N>
+struct Choices {
+    Choice of[N];
+};
+template <int N>
+__device__ __noinline__ Choices<N> choose_experts(
+        const float* first, size_t to_next, int experts, int top, int renormalize) {
     constexpr int R = 4;
     const int lane = threadIdx.x & 31;
     const float inf = __uint_as_float(0x7f800000u);
-    uint32_t key[R];
-    bool odd = false;  // a NaN or +infinity among the logits
+    const float* row[N];
+    uint32_t key[N][R];
+    bool odd[N];    // a NaN or +infinity among the logits
+    float sum[N];   // of all exponentials, where it is asked for
+    float top_value[N], mine[N];
+    uint32_t last[N];
+    int last_e[N], mine_e[N];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int e = i * 32 + lane;
-        const float v = e < experts ? row[e] : -inf;
-        key[i] = e < experts ? rank_key(v) : 0u;
-        odd |= !(v < inf);
+    for (int n = 0; n < N; ++n) {
+        row[n] = first + n * to_next;
+        odd[n] = false;
+        sum[n] = top_value[n] = mine[n] = 0.f;
+        last[n] = ~0u;
+        last_e[n] = mine_e[n] = -1;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int e = i * 32 + lane;
+            const float v = e < experts ? row[n][e] : -inf;
+            key[n][i] = e < experts ? rank_key(v) : 0u;
+            odd[n] |= !(v < inf);
+        }
     }
-    float sum = 0.f;  // of all exponentials, where it is asked for
-    uint32_t last = ~0u;
-    int last_e = -1, mine_e = -1;
-    float top_value = 0.f, mine = 0.f;
 #pragma unroll 1
     for (int j = 0; j < top; ++j) {
-        uint32_t best = 0;
-        int at = 0;
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                at = i * 32 + lane;
+        for (int n = 0; n < N; ++n) {
+            uint32_t best = 0;
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (key[n][i] > best) {
+                    best = key[n][i];
+                    at = i * 32 + lane;
+                }
+#pragma unroll 1
+            for (int e = R * 32 + lane; e < experts; e += 32) {
+                const uint32_t k = rank_key(row[n][e]);
+                if (k > best && (k < last[n] || (k == last[n] && e > last_e[n]))) {
+                    best = k;
+                    at = e;
+                }
             }
+            last[n] = __reduce_max_sync(0xffffffffu, best);
+            last_e[n] = (int)__reduce_min_sync(0xffffffffu, best == last[n] ? (uint32_t)at : ~0u);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (j == 0) {
+                top_value[n] = key_value(last[n]);
+                if (!renormalize) {
+#pragma unroll
+                    for (int i = 0; i < R; ++i)
+                        sum[n] += key[n][i] != 0 ? expf(key_value(key[n][i]) - top_value[n]) : 0.f;
+                }
+            }
+            if (lane == j) {
+                mine[n] = key_value(last[n]);
+                mine_e[n] = last_e[n];
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i * 32 + lane == last_e[n])
+                    key[n][i] = 0;
+        }
+    }
+    Choices<N> c;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        mine[n] = lane < top ? expf(mine[n] - top_value[n]) : 0.f;
 #pragma unroll 1
         for (int e = R * 32 + lane; e < experts; e += 32) {
-            const uint32_t k = rank_key(row[e]);
-            if (k > best && (k < last || (k == last && e > last_e))) {
-                best = k;
-                at = e;
-            }
+            odd[n] |= !(row[n][e] < inf);
+            sum[n] += renormalize ? 0.f : expf(row[n][e] - top_value[n]);
         }
-        last = __reduce_max_sync(0xffffffffu, best);
-        last_e = (int)__reduce_min_sync(0xffffffffu, best == last ? (uint32_t)at : ~0u);
-        if (j == 0) {
-            top_value = key_value(last);
-            if (!renormalize) {
-#pragma unroll
-                for (int i = 0; i < R; ++i)
-                    sum += key[i] != 0 ? expf(key_value(key[i]) - top_value) : 0.f;
-            }
-        }
-        if (lane == j) {
-            mine = key_value(last);
-            mine_e = last_e;
-        }
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (i * 32 + lane == last_e)
-                key[i] = 0;
+        if (renormalize)
+            sum[n] = mine[n];
     }
-    mine = lane < top ? expf(mine - top_value) : 0.f;
-#pragma unroll 1
-    for (int e = R * 32 + lane; e < experts; e += 32) {
-        odd |= !(row[e] < inf);
-        sum += renormalize ? 0.f : expf(row[e] - top_value);
-    }
-    if (renormalize)
-        sum = mine;
 #pragma unroll
     for (int s = 16; s; s >>= 1)
-        sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    float p = __fdiv_rn(mine, sum);
-    if (top_value == -inf)
-        p = 0.f;  // every expert is masked: no share in any
-    if (__any_sync(0xffffffffu, odd))
-        p = __uint_as_float(0x7fffffffu);
-    return {lane >= top || p == 0.f ? -1 : mine_e, p};
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], s);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        float p = __fdiv_rn(mine[n], sum[n]);
+        if (top_value[n] == -inf)
+            p = 0.f;  // every expert is masked: no share in any
+        if (__any_sync(0xffffffffu, odd[n]))
+            p = __uint_as_float(0x7fffffffu);
+        c.of[n] = {lane >= top || p == 0.f ? -1 : mine_e[n], p};
+    }
+    return c;
 }
 
 // A value at the same place in another CTA of the cluster
@@ -156,7 +188,7 @@ __device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
     return v;
 }
 
-// A warp per token in turn (500 instructions in a chain, 2 us each: the CTAs of a cluster share the tokens
+// A warp for a token or two in turn (each a chain of 2 us or more: the CTAs of a cluster share the tokens
 // out); then the slots by expert, cut into passes of at most `cols`. Barriers of the CTA stand before and behind,
 // and with a cluster umma::cluster_wait() has to follow before r.expert's memory is used for something else. With four
 // tokens at most the upper half of the warps has none and calls meanwhile().
@@ -165,18 +197,28 @@ __device__ __forceinline__ void route_tokens(
         const MoeArgs& a, int cols, const Route& r, int rank, int cluster, Meanwhile meanwhile) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (a.t > 1)
-        for (int e = threadIdx.x; e < a.e; e += kThreads)
-            r.count[e] = 0;
-#pragma unroll 1
-    for (int t = rank * kWarps + warp; t < a.t; t += cluster * kWarps) {
-        const float* row = a.logits + (size_t)t * a.e;
-        const Choice c = choose_experts(row, a.e, a.top, a.renormalize);
-        if (lane < a.top)
+        for (int e = threadIdx.x; e < 2 * a.e; e += kThreads)
+            r.tokens[e] = 0;
+    // tokens rank * kWarps + warp, and every cluster * kWarps further, two at a time while there are two
+    const int stride = cluster * kWarps;
+    auto keep = [&](int t, const Choice& c) {
+        if (lane < a.top) {
             r.p[t * a.top + lane] = c.p;
-        if (a.t > 1) {
-            if (lane < a.top)
+            if (a.t > 1)
                 r.expert[t * a.top + lane] = c.expert;
-        } else {
+        }
+    };
+    int t = rank * kWarps + warp;
+#pragma unroll 1
+    for (; t + stride < a.t; t += 2 * stride) {
+        const Choices<2> c = choose_experts<2>(a.logits + (size_t)t * a.e, (size_t)stride * a.e, a.e, a.top, a.renormalize);
+        keep(t, c.of[0]);
+        keep(t + stride, c.of[1]);
+    }
+    if (t < a.t) {
+        const Choice c = choose_experts<1>(a.logits + (size_t)t * a.e, 0, a.e, a.top, a.renormalize).of[0];
+        keep(t, c);
+        if (a.t == 1) {
             // one token: a pass for each of its experts, from the largest p down (any p that is 0 comes last)
             if (c.expert >= 0) {
                 r.order[lane] = lane;
@@ -191,75 +233,69 @@ __device__ __forceinline__ void route_tokens(
     }
     if (a.t <= 4 && warp >= 4)
         meanwhile();
-    if (a.t == 1) {
-        __syncthreads();
+    __syncthreads();
+    if (a.t == 1)
         return;
+    if (cluster > 1) {
+        umma::cluster_arrive();
+        umma::cluster_wait();
+    }
+    // A bit per expert and token: what an expert's slots are follows from them alone, whatever order they come in, so
+    // every CTA cuts them into the same passes.
+    const int slots = a.t * a.top;
+#pragma unroll 1
+    for (int s = threadIdx.x; s < slots; s += kThreads) {
+        const int token = s / a.top, owner = token / kWarps % cluster;
+        if (owner != rank) {
+            r.p[s] = __uint_as_float(peer_word(r.p + s, owner));
+            r.expert[s] = (int)peer_word(r.expert + s, owner);
+        }
+        const int e = r.expert[s];
+        if (e >= 0)
+            atomicOr(r.tokens + 2 * e + (token >> 5), 1u << (token & 31));
     }
     if (cluster > 1) {
         __syncwarp();
         umma::cluster_arrive();
-        umma::cluster_wait();
-#pragma unroll 1
-        for (int s = threadIdx.x; s < a.t * a.top; s += kThreads) {
-            const int owner = s / a.top / kWarps % cluster;
-            if (owner != rank) {
-                r.p[s] = __uint_as_float(peer_word(r.p + s, owner));
-                r.expert[s] = (int)peer_word(r.expert + s, owner);
-            }
-        }
-        __syncwarp();
-        umma::cluster_arrive();
     }
     __syncthreads();
-    const int slots = a.t * a.top;
-#pragma unroll 1
-    for (int s = threadIdx.x; s < slots; s += kThreads)
-        if (r.expert[s] >= 0)
-            atomicAdd(&r.count[r.expert[s]], 1);
-    __syncthreads();
     if (warp == 0) {
-        int start = 0, passes = 0;
+        int before = 0;  // slots in the lower half, passes in the upper one
 #pragma unroll 1
         for (int e0 = 0; e0 < a.e; e0 += 32) {
             const int e = e0 + lane;
-            const int n = e < a.e ? r.count[e] : 0, np = (n + cols - 1) / cols;
-            int s = n, q = np;
+            const int n = e < a.e ? __popc(r.tokens[2 * e]) + __popc(r.tokens[2 * e + 1]) : 0, np = (n + cols - 1) / cols;
+            int sum = np << 16 | n;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int s1 = __shfl_up_sync(0xffffffffu, s, d), q1 = __shfl_up_sync(0xffffffffu, q, d);
-                if (lane >= d) {
-                    s += s1;
-                    q += q1;
-                }
+                const int other = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d)
+                    sum += other;
             }
+            const int from = before + sum - (np << 16 | n), start = from & 0xffff;
             if (e < a.e)
-                r.at[e] = start + s - n;
+                r.at[e] = start;
 #pragma unroll 1
             for (int i = 0; i < np; ++i) {
-                const int to = passes + q - np + i;
+                const int to = (from >> 16) + i;
                 r.pass_expert[to] = (short)e;
-                r.pass_start[to] = (short)(start + s - n + i * cols);
+                r.pass_start[to] = (short)(start + i * cols);
                 r.pass_cols[to] = (short)min(cols, n - i * cols);
             }
-            start += __shfl_sync(0xffffffffu, s, 31);
-            passes += __shfl_sync(0xffffffffu, q, 31);
+            before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (lane == 0)
-            *r.passes = passes;
-        __syncwarp();
-        // An expert's slots in ascending order: every CTA must cut them into the same passes.
+            *r.passes = before >> 16;
+    }
+    __syncthreads();
 #pragma unroll 1
-        for (int s0 = 0; s0 < slots; s0 += 32) {
-            const int s = s0 + lane, e = s < slots ? r.expert[s] : -1;
-            const uint32_t alike = __match_any_sync(0xffffffffu, e);
-            const int to = e >= 0 ? r.at[e] : 0, before = __popc(alike & ((1u << lane) - 1u));
-            __syncwarp();
-            if (e >= 0) {
-                r.order[to + before] = s / a.top << 16 | s;
-                if (before == 0)
-                    r.at[e] = to + __popc(alike);
-            }
-            __syncwarp();
+    for (int s = threadIdx.x; s < slots; s += kThreads) {
+        const int e = r.expert[s], token = s / a.top;
+        if (e >= 0) {
+            const uint32_t lower = (1u << (token & 31)) - 1u;
+            const int rank_of = token < 32 ? __popc(r.tokens[2 * e] & lower)
+                                           : __popc(r.tokens[2 * e]) + __popc(r.tokens[2 * e + 1] & lower);
+            r.order[r.at[e] + rank_of] = token << 16 | s;
         }
     }
     __syncthreads();
