@@ -476,7 +476,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
                 continue;  // (still meets the others at the barrier in front of the next tile)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kPairBN);
-Sides sides;
+            Sides sides;
             sides.take(row_scale, col_scale + quarter * 64, col_bias + quarter * 64, p.bias != nullptr);
             store_columns<T>(taddr + (uint32_t)(quarter * 64), sides, p.bias != nullptr, stage, row0, n0 + quarter * 64, p,
                              p.vector_stores ? &map_c : nullptr, [&] {
@@ -525,20 +525,21 @@ constexpr int kMaxStages = 6;
 constexpr int kSplitWarps = 8;  // epilogue
 constexpr int kSplitThreads = 64 + 32 * kSplitWarps;
 constexpr int kSplitMost = 227 * 1024;
-constexpr int kSplitBars = (2 * kMaxStages + 2) * 8 + 16;
+constexpr int kSplitBars = (2 * kMaxStages + 3) * 8 + 16;
 constexpr int kSplitSides = (2 * kSplitBN + kBM) * 4;  // scales and biases of columns, scales of rows
-// [CTAs of the cluster][their share of the 128 rows][32 units of four columns] of the cluster's partial sums
+// [CTAs of the cluster][their share of the 128 rows][32 units of four columns] of the others' partial sums
 constexpr int kPartialBytes = kBM * kSplitBN * 4;
 inline int split_dynamic(int stages, int a_bytes, int csplit) {
     return stages * (a_bytes + kTileBytes) + (csplit > 1 ? kPartialBytes : 0) + kSplitSides + kSplitBars + 1024;
 }
 
-// The cluster's partial sums of this CTA's share of the rows, which all its CTAs have brought here: a row per
-// warp, four columns per lane. (Fetched from the others' shared memory instead they took 2.1 us, twice a load's way
-// there and back; now the sums go one way, behind the last MMA of each CTA.)
+// The cluster's partial sums of this CTA's share of the rows: a row per warp, four columns per lane. The others'
+// have come by bulk copies between the CTAs' shared memories, 16 KB or so in one. (16-byte loads from there took 2.1 us,
+// 16-byte stores to there 2.5.)
 template <class T, int SPLIT>
 __device__ __forceinline__ void finish_rows(
-        const uint8_t* partials, int rank, int m0, int n0, const float* col_scale, const float* col_bias,
+        const uint8_t* own, const uint8_t* partials, int rank, int m0, int n0, const float* col_scale,
+        const float* col_bias,
         const float* row_scale, const UmmaArgs& p) {
     constexpr int kShare = kBM / SPLIT;
     const int warp = (int)(threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
@@ -553,7 +554,8 @@ __device__ __forceinline__ void finish_rows(
         uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < SPLIT; ++j) {
-            const uint4 x = *(const uint4*)(partials + (j * kShare + r) * 512 + ((lane & ~7) + ((lane ^ r) & 7)) * 16);
+            const uint8_t* row = j == rank ? own + (rank * kShare + r) * 512 : partials + (j * kShare + r) * 512;
+            const uint4 x = *(const uint4*)(row + ((lane & ~7) + ((lane ^ r) & 7)) * 16);
             v[0] += x.x;
             v[1] += x.y;
             v[2] += x.z;
@@ -598,7 +600,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
     uint64_t* full_bar = (uint64_t*)(row_scale + kBM);
     uint64_t* empty_bar = full_bar + kMaxStages;
     uint64_t* acc_full = empty_bar + kMaxStages;
-    uint64_t* drain_bar = acc_full + 1;
+    uint64_t* part_bar = acc_full + 1;  // the others' partial sums
+    uint64_t* drain_bar = part_bar + 1;
     uint32_t* tmem_slot = (uint32_t*)(drain_bar + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* never = (volatile int*)(tmem_slot + 2);
@@ -616,9 +619,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
             mbar_init(&empty_bar[s], 1);
         }
         mbar_init(acc_full, 1);
+        mbar_init(part_bar, 1);
         mbar_init(drain_bar, 1);
         *abort_flag = *never = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (p.csplit > 1)
+            mbar_expect_tx(part_bar, (uint32_t)((p.csplit - 1) * (kPartialBytes / p.csplit)));
     } else if (threadIdx.x == 64) {
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);
@@ -738,19 +744,15 @@ __global__ void __launch_bounds__(kSplitThreads, 2) product_split_kernel(
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
             if (p.csplit == 1) {
                 uint8_t* stage = smem + (warp - 2) * kRoundBytes;
-if (row0 < p.m && n0 + half * 64 < p.n) {
+                if (row0 < p.m && n0 + half * 64 < p.n) {
                     Sides sides;
                     sides.take(sa, col_scale + half * 64, col_bias + half * 64, p.bias != nullptr);
                     store_columns<T>(taddr + (uint32_t)(half * 64), sides, p.bias != nullptr, stage, row0,
                                      n0 + half * 64, p, nullptr, [] {});
                 }
             } else if (row0 < p.m) {
-                // each row to the CTA that finishes it, units of four columns in an order by row
-                const int share = kBM / p.csplit, row = q * 32 + lane, owner = row / share;
-                const uint32_t at = map_to_cta(smem_u32(partials) + (uint32_t)((rank * share + row % share) * 512),
-                                               (uint32_t)owner);
-                __syncwarp();
-                cluster_wait();
+                // the partial sums, [128 rows][32 units of four columns], units in an order by row
+                const int row = q * 32 + lane;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t acc[32];
@@ -758,28 +760,49 @@ if (row0 < p.m && n0 + half * 64 < p.n) {
                     tmem_ld32(taddr + (uint32_t)(half * 64 + 32 * h), acc);
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
-                        st_cluster_v4(at + (uint32_t)(((half * 2 + h) * 8 + (u ^ (row & 7))) * 16),
-                                      make_uint4(acc[4 * u], acc[4 * u + 1], acc[4 * u + 2], acc[4 * u + 3]));
+                        *(uint4*)(smem + row * 512 + ((half * 2 + h) * 8 + (u ^ (row & 7))) * 16) =
+                                make_uint4(acc[4 * u], acc[4 * u + 1], acc[4 * u + 2], acc[4 * u + 3]);
                 }
-                waited = true;
+            }
+        }
+        if (p.csplit > 1) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            cluster_wait();  // (all CTAs have begun)
+            waited = true;
+            epilogue_sync<kSplitWarps>();
+            const int share_bytes = kPartialBytes / p.csplit;
+            if (ok && warp == 2 && lane < p.csplit && lane != rank)
+                // each CTA its share of the rows
+                asm volatile(
+                        "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                map_to_cta(smem_u32(partials + rank * share_bytes), (uint32_t)lane)),
+                        "r"(smem_u32(smem + lane * share_bytes)), "r"(share_bytes),
+                        "r"(map_to_cta(smem_u32(part_bar), (uint32_t)lane))
+                        : "memory");
+            __syncwarp();
+            ok = mbar_wait_cluster(part_bar, 0, abort_flag);
+            if (!ok)
+                give_up(ERR_EPILOGUE_WAIT);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                if (p.csplit == 2)
+                    finish_rows<T, 2>(smem, partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
+                else if (p.csplit == 4)
+                    finish_rows<T, 4>(smem, partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
+                else
+                    finish_rows<T, 8>(smem, partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
             }
         }
     }
 
     if (p.csplit > 1) {
+        // nobody leaves before what it sends has arrived
         __syncwarp();
         if (!waited)
             cluster_wait();
         cluster_arrive();
-        cluster_wait();  // all partial sums have been stored
-        if (warp >= 2) {
-            if (p.csplit == 2)
-                finish_rows<T, 2>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
-            else if (p.csplit == 4)
-                finish_rows<T, 4>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
-            else
-                finish_rows<T, 8>(partials, rank, m0, n0, col_scale, col_bias, row_scale, p);
-        }
+        cluster_wait();
     }
 
     // ---------------- teardown ----------------
