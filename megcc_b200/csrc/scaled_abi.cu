@@ -70,7 +70,9 @@ bool streams(int m, int n, int k, bool fits) {
         return !fits || weights <= many || n < 74 * 128;
     if (m <= 32)
         return !fits || weights <= many;
-    return m <= (1 << 20) && (m + 31) / 32 * weights <= 1 << 22;  // a pass over the weights per 32 rows
+    // a pass over the weights per 32 rows, in no more CTAs than the SMs hold at once
+    const long long passes = ((long long)m + 31) / 32;
+    return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= 2 * 148;
 }
 // So few that it makes whole numbers of them itself, every CTA again
 bool streams_activations(int m, int k) {

@@ -117,15 +117,17 @@ int quantize_rows(
 }
 
 // ---- product for few tokens ----
-// HBM: n * k bytes of weights are read once, whatever m. A CTA makes 16 rows of weights times 8 * NT
+// HBM: n * k bytes of weights are read once, whatever m. SHARED: a CTA makes 16 rows of weights times 8 * NT
 // tokens; its eight warps take the 128-byte steps of K in turn (stream_s8.cuh) and their sums meet at the end.
+// Otherwise each warp makes 16 rows of its own: for short K, where a warp of eight had a step or none, and enough
+// rows for the SMs (2 x 12735 x 74: 6.1 us shared).
 // int8 tokens come through the ring beside the weights; activations that are still floats are made whole
 // numbers first, by every CTA again, while its first weights are on their way.
 constexpr int kWarps = 8;
 constexpr int kRows = 16;     // weight rows per CTA
 constexpr int kColPitch = 20; // ints per token in the exchange: 2 * 20 = 8 banks apart
 
-template <class XT, int NT, bool ALIGNED>
+template <class XT, int NT, bool ALIGNED, bool SHARED>
 struct Stream {
     static constexpr bool kFloat = sizeof(XT) > 1;
     static constexpr int kCols = 8 * NT;
@@ -134,11 +136,12 @@ struct Stream {
     typedef Rows<kCols, ALIGNED> A;
     static constexpr int kStage = W::kBytes + (kFloat ? 0 : A::kBytes);
     static constexpr int kRing = kWarps * kDepth * kStage;
+    static constexpr int kCtaRows = SHARED ? kRows : kRows * kWarps;
 };
 
-template <class XT, int NT, bool ALIGNED>
+template <class XT, int NT, bool ALIGNED, bool SHARED>
 __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const ProductArgs p, int x_vectors) {
-    typedef Stream<XT, NT, ALIGNED> S;
+    typedef Stream<XT, NT, ALIGNED, SHARED> S;
     constexpr bool kFloat = S::kFloat;
     constexpr int kDepth = S::kDepth, kCols = S::kCols;
     extern __shared__ __align__(128) uint8_t dynamic[];  // the rings, then (floats) xs
@@ -147,10 +150,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
-    const int n0 = blockIdx.x * kRows;
+    const int n0 = blockIdx.x * S::kCtaRows + (SHARED ? 0 : warp * kRows);
     const int m0 = blockIdx.y * kCols;
     const int k = p.k, steps = (k + kStep - 1) / kStep;
-    const int mine = warp < steps ? (steps - warp + kWarps - 1) / kWarps : 0;
+    // this warp's steps: its first one, how far apart they are, how many
+    const int first = SHARED ? warp : 0, by = SHARED ? kWarps : 1;
+    const int mine = first < steps ? (steps - first + by - 1) / by : 0;
     const uint32_t ring = shared_address(dynamic) + (uint32_t)(warp * kDepth * S::kStage);
     int8_t* xs = (int8_t*)dynamic + S::kRing;
     const int pitch = xs_pitch(k);
@@ -159,17 +164,17 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     auto a_row = [&](int r) { return (const int8_t*)p.a + (long long)min(m0 + r, p.m - 1) * p.lda; };
     typename S::W w;
     typename S::A a;
-    w.open(b_row, k, warp);
+    w.open(b_row, k, first);
     if (!kFloat)
         // (no copies for tokens that are not there: every CTA asks for the same few lines)
-        a.open([&](int r) { return m0 + r < p.m ? a_row(r) : nullptr; }, k, warp);
+        a.open([&](int r) { return m0 + r < p.m ? a_row(r) : nullptr; }, k, first);
     auto copy_weights = [&](uint32_t stage, int i) {
         if (i < mine)
-            w.template copy<true>(stage, kWarps, k - (warp + i * kWarps) * kStep >= S::W::kWhole);
+            w.template copy<true>(stage, by, k - (first + i * by) * kStep >= S::W::kWhole);
     };
     auto copy_tokens = [&](uint32_t stage, int i) {
         if (!kFloat && i < mine)
-            a.template copy<false>(stage + S::W::kBytes, kWarps, k - (warp + i * kWarps) * kStep >= S::A::kWhole);
+            a.template copy<false>(stage + S::W::kBytes, by, k - (first + i * by) * kStep >= S::A::kWhole);
     };
     if (p.b_early)
 #pragma unroll 1
@@ -217,7 +222,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
         copy_tokens(free_stage, i + kDepth - 1);
         copy_commit();
         next_stage<kDepth, S::kStage>(free_stage, ring);
-        const int step = warp + i * kWarps;
+        const int step = first + i * by;
 #pragma unroll
         for (int j = 0; j < kStep / 64; ++j) {
             const int piece = 4 * j + tig;
@@ -239,7 +244,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     }
     copy_wait<0>();
     __syncthreads();
-    int(*red)[kCols][kColPitch] = (int(*)[kCols][kColPitch])dynamic;  // (the rings are done with)
+    // (the rings are done with)
+    int(*red)[kCols][kColPitch] = (int(*)[kCols][kColPitch])dynamic;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         int(*r)[kColPitch] = red[warp] + 8 * nt + 2 * tig;
@@ -251,11 +257,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     __syncthreads();
     if (n >= p.n)
         return;
-    for (int col = threadIdx.x >> 4; col < kCols && m0 + col < p.m; col += 2 * kWarps) {
-        int sum = 0;
+    for (int col = (SHARED ? threadIdx.x : lane) >> 4; col < kCols && m0 + col < p.m; col += SHARED ? 2 * kWarps : 2) {
+        int sum = SHARED ? 0 : red[warp][col][row];
+        if (SHARED)
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i)
-            sum += red[i][col][row];
+            for (int i = 0; i < kWarps; ++i)
+                sum += red[i][col][row];
         float v = scale_acc(sum, col_scale[col], sb);
         if (p.bias)
             v = __fadd_rn(v, bias);
@@ -263,10 +270,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     }
 }
 
-// Rows of any alignment to rows of whole 16-byte units, a warp per row
+// Rows of any alignment to rows of whole 16-byte units, a warp per row, or a CTA where there are few
+template <int LANES>
 __global__ void __launch_bounds__(256) pad_rows_kernel(const PadRows a, const PadRows b) {
     pdl_start();
-    const long long job = blockIdx.x * 8LL + (threadIdx.x >> 5);
+    const long long job = blockIdx.x * (256LL / LANES) + threadIdx.x / LANES;
     const bool second = job >= a.rows;
     const PadRows& j = second ? b : a;
     const long long row = second ? job - a.rows : job;
@@ -275,27 +283,32 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const PadRows a, const Pa
     const int8_t* src = j.src + row * j.ld;
     uint4* dst = (uint4*)(j.dst + row * j.pitch);
 #pragma unroll 4
-    for (int u = threadIdx.x & 31; u < (int)(j.pitch / 16); u += 32)
+    for (int u = threadIdx.x % LANES; u < (int)(j.pitch / 16); u += LANES)
         dst[u] = ld_any16(src + 16 * u, j.k - 16 * u);
 }
 
-template <class XT, int NT, bool ALIGNED>
+template <class XT, int NT, bool ALIGNED, bool SHARED>
 cudaError_t launch_stream_as(const ProductArgs& a, int x_vectors, cudaStream_t st) {
-    typedef Stream<XT, NT, ALIGNED> S;
+    typedef Stream<XT, NT, ALIGNED, SHARED> S;
     static umma::KernelReady ready;
     static_assert(S::kRing >= kWarps * S::kCols * kColPitch * 4, "the exchange lies where the rings were");
-    auto kernel = product_stream_kernel<XT, NT, ALIGNED>;
+    auto kernel = product_stream_kernel<XT, NT, ALIGNED, SHARED>;
     const int smem = S::kRing + (S::kFloat ? (a.m < S::kCols ? a.m : S::kCols) * xs_pitch(a.k) : 0);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)((a.n - 1) / kRows + 1), (unsigned)((a.m - 1) / S::kCols + 1));
+    const dim3 grid((unsigned)((a.n - 1) / S::kCtaRows + 1), (unsigned)((a.m - 1) / S::kCols + 1));
     const Writes writes{a.c, ((size_t)(a.m - 1) * (size_t)a.ldc + (size_t)a.n) * dtype_bytes(a.c_dtype)};
     return launch_pdl(writes, kernel, grid, dim3(32 * kWarps), (size_t)smem, st, a, x_vectors);
 }
 template <class XT, int NT>
 cudaError_t launch_stream(const ProductArgs& a, bool aligned, int x_vectors, cudaStream_t st) {
-    return aligned ? launch_stream_as<XT, NT, true>(a, x_vectors, st)
-                   : launch_stream_as<XT, NT, false>(a, x_vectors, st);
+    // warps of their own where shared tiles would take several turns on the SMs for a step or two per warp
+    const long long ctas = ((long long)(a.n - 1) / kRows + 1) * ((a.m - 1) / (8 * NT) + 1);
+    if (a.k <= 8 * kStep && ctas > 2LL * umma::sm_count())
+        return aligned ? launch_stream_as<XT, NT, true, false>(a, x_vectors, st)
+                       : launch_stream_as<XT, NT, false, false>(a, x_vectors, st);
+    return aligned ? launch_stream_as<XT, NT, true, true>(a, x_vectors, st)
+                   : launch_stream_as<XT, NT, false, true>(a, x_vectors, st);
 }
 
 template <class XT>
@@ -328,8 +341,10 @@ int launch_pad_rows(const PadRows& a, const PadRows& b, cudaStream_t st) {
             lo = at < lo ? at : lo;
             hi = end > hi ? end : hi;
         }
-    const cudaError_t e = launch_pdl(Writes{(const void*)lo, hi - lo}, pad_rows_kernel,
-                                     dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, b);
+    const Writes writes{(const void*)lo, hi - lo};
+    const cudaError_t e =
+            rows < 16 * 148 ? launch_pdl(writes, pad_rows_kernel<256>, dim3((unsigned)rows), dim3(256), 0, st, a, b)
+                            : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, b);
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
     return check_launch("matmul_s8_scaled");

@@ -6,13 +6,16 @@
 // 128-byte lines.
 //
 // Two kernels:
-//   pair   256 x 256 tiles on pairs of SMs (cta_group::2), persistent, two accumulator buffers. What bounds wide
+//   pair   256 x 256 tiles (or x 192, x 128, where those come out even) on pairs of SMs (cta_group::2), persistent, two
+//          accumulator buffers. What bounds wide
 //          products is the SM's shared memory: per 128 bytes of K a 128 x 128 tile of one SM writes and reads 64 KB
 //          for 256 clocks of MMAs, 512 clocks at 128 B/clk; the pair's 256 x 256 the same bytes per SM
 //          for 512 clocks of MMAs.
 //   split  128 x 128 tiles, K cut over the 1, 2, 4 or 8 CTAs of a cluster where there are few tiles: there
 //          the weights' way from HBM bounds, and every SM has to take part in it. The partial sums meet in
 //          shared memory (whole numbers: in any order the same).
+#include <limits.h>
+
 #include "scaled_s8.cuh"
 #include "umma_pair.cuh"
 
@@ -37,6 +40,7 @@ struct UmmaArgs {
     long long ldc;
     int vector_stores;  // rows of c are whole 16-byte units
     int b_early;
+    int bn;          // pair: columns of a tile, 256, 192 or 128
     // split:
     int a_rows;      // rows of A's box
     int a_bytes;     // of a stage, B's part behind it
@@ -349,10 +353,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
             int s = 0;
             uint32_t phase = 0;
             bool ok = true;
-            auto b_row = [&](const Tile& t) { return t.n * kPairBN + (int)rank * kBM; };
+            auto b_row = [&](const Tile& t) { return t.n * p.bn + (int)rank * (p.bn / 2); };
             auto announce = [&](int stage) {
                 if (leader)
-                    mbar_expect_tx(&full_bar[stage], 2u * kStageBytes);
+                    mbar_expect_tx(&full_bar[stage], 2u * (uint32_t)(kTileBytes + p.bn / 2 * kBK));
             };
             // weights of the first stages ahead of the end of the kernel in front
             int ahead = 0;
@@ -392,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
     } else if (warp == 1) {
         // ---------------- MMA issuer (leader only) ----------------
         if (leader && lane == 0) {
-            constexpr uint32_t idesc = umma_idesc_s8(2 * kBM, kPairBN);
+            const uint32_t idesc = umma_idesc_s8(2 * kBM, p.bn);
             int local = 0, s = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -452,9 +456,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
         auto fetch = [&](int tile) {
             if (tile < total_tiles) {
                 const Tile t = tile_at(tile, p.m_tiles, p.n_tiles);
-                const int row = t.m * (2 * kBM) + (int)rank * kBM + q * 32 + lane, n = t.n * kPairBN + column;
+                const int row = t.m * (2 * kBM) + (int)rank * kBM + q * 32 + lane, n = t.n * p.bn + column;
                 sa = row < p.m ? p.sa[row] : 0.f;
-                side = sides && n < p.n ? sides[n] : 0.f;
+                side = sides && column < p.bn && n < p.n ? sides[n] : 0.f;
             }
         };
         fetch(first_tile);
@@ -462,7 +466,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
             const int buf = local & 1;
             const uint32_t acc_phase = (uint32_t)(local >> 1) & 1u;
             const Tile t = tile_at(tile, p.m_tiles, p.n_tiles);
-            const int row0 = t.m * (2 * kBM) + (int)rank * kBM + q * 32, n0 = t.n * kPairBN;
+            const int row0 = t.m * (2 * kBM) + (int)rank * kBM + q * 32, n0 = t.n * p.bn;
             epilogue_sync<kPairWarps>();  // (the last tile's have been read)
             (et < kPairBN ? col_scale : col_bias)[column] = side;
             const float row_scale = sa;
@@ -476,6 +480,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
                 continue;  // (still meets the others at the barrier in front of the next tile)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kPairBN);
+            if (quarter * 64 >= p.bn) {
+                // (no columns of a narrow tile for this warp)
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                if (lane == 0)
+                    mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+                continue;
+            }
             Sides sides;
             sides.take(row_scale, col_scale + quarter * 64, col_bias + quarter * 64, p.bias != nullptr);
             store_columns<T>(taddr + (uint32_t)(quarter * 64), sides, p.bias != nullptr, stage, row0, n0 + quarter * 64, p,
@@ -848,18 +859,26 @@ int encode(CUtensorMap* map, const void* p, int k, int rows, long long pitch, in
 }
 
 // Which kernel, by the clocks of its busiest SM. A 128-byte step of K takes a 128 x 128 tile's SM 512 clocks and
-// a pair's two 560 (shared memory); in front of the first step and behind the last one stand the loads' round
-// trip and the epilogue, with a cluster's exchange where K is split.
+// a pair's two 560 at 256 columns (shared memory: the bytes of A's and B's rows in and out); in front of the first
+// step and behind the last one stand the loads' round trip and the epilogue, with a cluster's exchange where K is split.
 struct Choice {
     bool pair;
-    int csplit;
+    int bn, csplit;
 };
 template <class Fit>
 Choice choose(const UmmaArgs& p, int sms, Fit clusters_that_fit) {
     const long long steps = p.k_steps;
-    const long long pair_tiles = (long long)((p.m - 1) / (2 * kBM) + 1) * ((p.n - 1) / kPairBN + 1);
-    long long best = (pair_tiles + sms / 2 - 1) / (sms / 2) * (steps * 560 < 3000 ? 3000 : steps * 560) + 6000;
-    Choice c = {true, 1};
+    long long best = LLONG_MAX;
+    Choice c = {true, kPairBN, 1};
+    for (int bn = kPairBN; bn >= 128; bn -= 64) {
+        const long long pair_tiles = (long long)((p.m - 1) / (2 * kBM) + 1) * ((p.n - 1) / bn + 1);
+        const long long tile = steps * (48 + 256 + bn), least = 12 * bn;  // (the epilogue's)
+        const long long t = (pair_tiles + sms / 2 - 1) / (sms / 2) * (tile < least ? least : tile) + 6000;
+        if (t < best) {
+            best = t;
+            c.bn = bn;
+        }
+    }
     const long long tiles = (long long)((p.m - 1) / kBM + 1) * ((p.n - 1) / kSplitBN + 1);
     for (int split = 1; split <= 8; split *= 2) {
         if (split > steps || (split > 1 && tiles > clusters_that_fit(split)))
@@ -868,7 +887,7 @@ Choice choose(const UmmaArgs& p, int sms, Fit clusters_that_fit) {
         const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 5500 : 1000);
         if (t < best) {
             best = t;
-            c = {false, split};
+            c = {false, kSplitBN, split};
         }
     }
     return c;
@@ -892,10 +911,11 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
         if (!ready.smem(product_pair_kernel<T>, kPairDynamic))
             return check_launch("matmul_s8_scaled smem attribute");
         p.m_tiles = (p.m - 1) / (2 * kBM) + 1;
-        p.n_tiles = (p.n - 1) / kPairBN + 1;
+        p.bn = choice.bn;
+        p.n_tiles = (p.n - 1) / p.bn + 1;
         int rc = encode(&map_a, a.a, a.k, a.m, a.lda, kBM);
         if (!rc)
-            rc = encode(&map_b, a.b, a.k, a.n, a.ldb, kBM);
+            rc = encode(&map_b, a.b, a.k, a.n, a.ldb, p.bn / 2);
         CUtensorMap map_c = map_b;  // (not used where rows of c are no whole 16-byte units)
         if (!rc && p.vector_stores)
             rc = encode_as(&map_c,

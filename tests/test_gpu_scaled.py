@@ -98,7 +98,10 @@ def test_quantize_rows_that_lie_apart(dtype, offset, pitch):
 SIZES = [(1, 1, 1), (1, 16, 64), (1, 17, 63), (7, 1000, 512), (8, 130, 65), (9, 33, 4096), (16, 48, 48),
          (17, 100, 1000), (24, 1000, 512), (33, 257, 129), (64, 64, 2047), (65, 70, 272), (127, 300, 640),
          (128, 128, 128), (129, 129, 144), (200, 1000, 4099), (256, 512, 96), (300, 260, 16), (511, 136, 1040),
-         (1000, 999, 333), (1, 5000, 11008), (2, 24, 131071), (1025, 2048, 256), (1, 100, 8000), (8, 64, 9000)]
+         (1000, 999, 333), (1, 5000, 11008), (2, 24, 131071), (1025, 2048, 256), (1, 100, 8000), (8, 64, 9000),
+         # short sums of many columns; tiles of 192 and of 128 columns; K split over two, four and eight CTAs
+         (2, 12735, 74), (7, 5000, 1024), (20, 9999, 130), (500, 9700, 1024), (256, 9472, 8192), (130, 4200, 1600),
+         (128, 2000, 4096), (100, 200, 6400)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
