@@ -281,7 +281,7 @@ MB200_API int mb200_matmul_s8_qs8(
  * the model is compiled; these are for layers whose activations have no such scale. Activations
  * and results are fp32, fp16 or bf16 (MB200_DTYPE_*), whole numbers int8, scales and bias fp32. Rows may lie
  * apart (ld..: elements from one row to the next); a row's own elements are neighbours. m == 0 is allowed
- * and does nothing. Every tensor may start at any element.
+ * and does nothing. Every tensor may start at any element. Results and workspace overlap no operand.
  *
  * A row x becomes whole numbers q with one scale: amax = max(max |x|, 2^-119),
  *     scale = RN(amax * RN(1 / 127)),  inv = RN(RN(1 / amax) * 127),  q = x * inv to the nearest whole number
@@ -296,8 +296,9 @@ MB200_API int mb200_quantize_rows_s8(
         void* stream);
 
 /* c[i][j] = sum_l a[i][l] * b_packed[j][l] * a_scales[i] * b_scales[j] [+ bias[j]], the sum exact in int32
- * (k <= 131071, more is refused with TinyNN_ERROR_OUT_OF_RANGE), the rest in fp32 and rounded to `dtype`
- * once. b_packed: [n][k], the layout mb200_matmul_pack_b makes and most weights have. bias may be NULL.
+ * (k <= 131071; more, and m or n beyond 2^31 - 512, is refused with TinyNN_ERROR_OUT_OF_RANGE), the rest in
+ * fp32, in this order, and rounded to `dtype` once. b_packed: [n][k], the layout mb200_matmul_pack_b makes and
+ * most weights have. bias may be NULL.
  * workspace: mb200_matmul_s8_scaled_workspace_bytes of the same operands, 256-byte aligned device memory;
  * 0 bytes (and NULL) where rows of a and b_packed are whole 16-byte units or there are few of a. */
 MB200_API size_t mb200_matmul_s8_scaled_workspace_bytes(
@@ -326,8 +327,8 @@ MB200_API int mb200_linear_s8(
  *       as rows
  *   y[t] = sum over the chosen of p * w2_scales[expert][d] * (w2[expert] [d][f] times h)
  * Sums of whole numbers are exact, all others in fp32, in an order that is always the same. An expert whose p is 0 (a
- * logit of -infinity masks it) adds nothing; with all logits at -infinity y[t] is 0 (a padded token); a NaN or
- * +infinity among a token's logits, or a row x[t] without a scale, makes that y[t] NaN.
+ * logit of -infinity masks it) adds nothing; with all logits at -infinity y[t] is 0 (a padded token, whatever its
+ * x[t]); a NaN or +infinity among a token's logits, or else a row x[t] without a scale, makes that y[t] NaN.
  * 1 <= tokens <= 64, top_k <= 16 and <= experts <= 512, f <= 131071, d <= 16384 (8192 with more than 8 tokens):
  * beyond them TinyNN_ERROR_OUT_OF_RANGE; tokens == 0 does nothing. ldx, ldy: elements from row to row.
  * workspace: mb200_moe_s8_workspace_bytes(p) bytes of device memory, 256-byte aligned, whose content does not

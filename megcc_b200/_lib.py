@@ -182,7 +182,8 @@ def tensor_calls():
         except ImportError as e:
             raise RuntimeError("megcc_b200/_torchcall.so is missing or made for another torch: build it with "
                                "`python -m megcc_b200.build` (there is no fallback)") from e
-        _torchcall.bind(check, *(C.cast(getattr(lib(), name), C.c_void_p).value for name in (
+        import torch
+        _torchcall.bind(check, torch.OutOfMemoryError, *(C.cast(getattr(lib(), name), C.c_void_p).value for name in (
             "mb200_quantize_rows_s8", "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
             "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
             "mb200_moe_s8")))

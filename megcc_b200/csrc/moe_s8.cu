@@ -478,10 +478,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
 }
 
 // ---- down, and the experts' sum ----
-// A CTA, or a cluster of CTAs, makes 16 rows of every token. All its steps, pass after pass in the order of the experts' indices, are one
-// sequence, of which each warp takes an equal run; it adds into sums of its own, which meet at the end in
-// the order of the warps: no float atomics, the same bits every time. (Neighbouring steps for each warp: with every
-// eighth step each warp would open every pass.) Clusters: where d has fewer tiles than the GPU has SMs.
+// A CTA, or a cluster of CTAs, makes 16 rows of every token. All its steps, pass after pass in the order of the
+// experts' indices, are one sequence, of which each warp takes an equal run; it adds into sums of its own, which meet
+// at the end in the order of the warps: no float atomics, the same bits every time. (Neighbouring steps for each warp:
+// with every eighth step each warp would open every pass.) Clusters: where d has fewer tiles than the GPU has SMs.
 template <int NT, int DEPTH, bool ALIGNED>
 struct Down {
     static constexpr int kDepth = DEPTH;
@@ -712,11 +712,29 @@ bool few_columns(const MoeArgs& a) {
     return a.t <= 8 || a.t * a.top <= 4 * a.e;
 }
 
+// How many clusters of four the GPU holds at once, asked again where the shared memory is another one
+struct ClustersOfFour {
+    std::atomic<long long> known[64] = {};  // shared memory << 16 | clusters
+    template <class Kernel>
+    int fit(Kernel kernel, int smem) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+            dev = 0;
+        const long long k = known[dev].load(std::memory_order_relaxed);
+        if (k && k >> 16 == smem)
+            return (int)(k & 0xffff);
+        umma::ClusterCapacity capacity;
+        const int n = capacity.clusters(kernel, 4, kThreads, smem);
+        known[dev].store((long long)smem << 16 | n, std::memory_order_relaxed);
+        return n;
+    }
+};
+
 template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
 cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
     static umma::ResidentCtas resident;
-    static umma::ClusterCapacity capacity;
+    static ClustersOfFour clusters;
     auto kernel = moe_up_kernel<T, COLS, DEPTH, CTAS, ALIGNED>;
     const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
@@ -727,8 +745,9 @@ cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     // clusters of four for the routing of many tokens (whole clusters live inside a GPC: eight would leave SMs idle)
     const int cluster = a.t <= 8 ? 1 : 4;
     const long long fit = cluster == 1 ? (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0)
-                                       : 4LL * capacity.clusters(kernel, 4, kThreads, smem);
-    const long long ctas = tiles < fit ? (tiles + cluster - 1) / cluster * cluster : fit;
+                                       : 4LL * clusters.fit(kernel, smem);
+    const long long some = fit > 0 ? fit : cluster;
+    const long long ctas = tiles < some ? (tiles + cluster - 1) / cluster * cluster : some;
     return launch_pdl_cluster(writes, kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, cluster, st, a,
                               x_vectors, cluster);
 }

@@ -20,6 +20,8 @@ int check_extents(const char* what, int m, int n, int k) {
     if (k > kMaxK)
         return set_error(ST_OUT_OF_RANGE, "%s: k = %d, sums of more than %d products may leave an int32", what, k,
                          kMaxK);
+    if (m > kMaxExtent || n > kMaxExtent)
+        return set_error(ST_OUT_OF_RANGE, "%s: extents %d x %d (at most %d)", what, m, n, kMaxExtent);
     return ST_SUCCESS;
 }
 
@@ -61,8 +63,9 @@ bool rows_fit(const void* p, int rows, long long ld) {
 }
 // Few rows of activations, or little of everything: the kernel that streams the weights past them, whatever the
 // operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles): 17 rows 1024 x 1024 1.9 / 5.2,
-// 4096 x 4096 4.4 / 7.0, 4096 x 14336 14.3 / 13.6; 16 rows 4096 x 14336 10.7 / 13.6, 14336 x 4096 13.8 / 12.7, 32768 x 2048
-// 17.8 / 13.3: tiles of whole K win where they are enough for the SMs, or where tokens weigh as much as weights.
+// 4096 x 4096 4.4 / 7.0, 4096 x 14336 14.3 / 13.6; 16 rows 4096 x 14336 10.7 / 13.6, 14336 x 4096 13.8 / 12.7,
+// 32768 x 2048 17.8 / 13.3: tiles of whole K win where they are enough for the SMs, or where tokens weigh as much as
+// weights.
 // `fits`: the tiles' operands need no copies (4100 x 4100, 32 rows: 13.7 / 15.4).
 bool streams(int m, int n, int k, bool fits) {
     const long long weights = (long long)n * k, many = 1 << 25;

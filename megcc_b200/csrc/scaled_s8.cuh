@@ -24,6 +24,8 @@ inline size_t dtype_bytes(int t) {
 }
 // 2^31 / 128^2: deeper sums may leave an int32
 constexpr int kMaxK = 131071;
+// of rows and columns: the last tile's indices still fit an int
+constexpr int kMaxExtent = 0x7fffffff - 511;
 
 #if defined(__CUDACC__)
 
@@ -138,20 +140,6 @@ __device__ __forceinline__ float scale_acc(int acc, float sa, float sb) {
     return __fmul_rn(__fmul_rn(__int2float_rn(acc), sa), sb);
 }
 
-// Weights are read once: past the L1, which the activations use.
-__device__ __forceinline__ uint4 ld_stream16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-
 // `valid` (1 .. 16, or nothing at 0 and below) bytes from any address, zeros behind them. Whole
 // 16-byte units are read: each holds at least one of the bytes that are asked for, so none reaches
 // into memory that the tensor's own last byte does not share a unit with.
@@ -186,10 +174,6 @@ __device__ __forceinline__ uint4 ld_any16(const int8_t* p, int valid) {
     }
     o[0] = out[0], o[1] = out[1], o[2] = out[2], o[3] = out[3];
     return r;
-}
-__device__ __forceinline__ uint2 ld_any8(const int8_t* p, int valid) {
-    const uint4 v = ld_any16(p, min(valid, 8));
-    return make_uint2(v.x, v.y);
 }
 
 // 16 x 8 sums over 32 bytes of K: A is 16 rows (of weights), B 8 columns (tokens). A thread's words

@@ -2,8 +2,8 @@
 //
 // Both operands are K-major, 128 bytes of K per pipeline stage, brought by tiled TMA loads with the
 // 128-byte swizzle; sums stay exact in int32 in tensor memory. The epilogue multiplies by the two scales in
-// fp32, adds the bias, rounds once and turns the tile round in shared memory so that a warp stores whole
-// 128-byte lines.
+// fp32, adds the bias, rounds once and turns the tile round in shared memory, 64 bytes of 32 rows at a time, from where
+// the TMA stores it (or, where rows of the result are no whole 16-byte units, the warp).
 //
 // Two kernels:
 //   pair   256 x 256 tiles (or x 192, x 128, where those come out even) on pairs of SMs (cta_group::2), persistent, two
@@ -53,11 +53,8 @@ template <class T>
 struct Out;
 template <>
 struct Out<float> {
-    static __device__ __forceinline__ uint4 unit(const float* v) {
-        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    }
     static __device__ __forceinline__ uint4 unit4(const float* v) {
-        return unit(v);
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
     static __device__ __forceinline__ float one(float v) {
         return v;
@@ -68,9 +65,6 @@ struct Out<__half> {
     static __device__ __forceinline__ uint32_t two(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    static __device__ __forceinline__ uint4 unit(const float* v) {
-        return make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
     }
     static __device__ __forceinline__ uint4 unit4(const float* v) {
         return make_uint4(two(v[0], v[1]), two(v[2], v[3]), 0, 0);
@@ -85,9 +79,6 @@ struct Out<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    static __device__ __forceinline__ uint4 unit(const float* v) {
-        return make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
-    }
     static __device__ __forceinline__ uint4 unit4(const float* v) {
         return make_uint4(two(v[0], v[1]), two(v[2], v[3]), 0, 0);
     }
@@ -99,7 +90,7 @@ struct Out<__nv_bfloat16> {
 // What a lane needs of the scales for 32 rows times 64 columns of sums. tcgen05.ld 16x256b hands it, of each 16 rows, the
 // rows lane / 4 and lane / 4 + 8, and of each eight columns 2 * (lane % 4) and the one behind: so four rows' and sixteen
 // columns' scales stay in registers, where a row per lane would read all 64 columns' from shared memory, which the
-// MMAs and the TMA keep busy (8192^3: 333 -> 325 us).
+// MMAs and the TMA keep busy (fp32 results of 6970 x 4576 x 1264: 49.7 us, 51.5 so).
 struct Sides {
     float row[4];
     float2 scale[8], bias[8];
@@ -844,7 +835,8 @@ int encode_as(
     if (!api.ok)
         return set_error(ST_RUNTIME, "cuTensorMapEncode* entry points not found in the driver");
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    // (a single row may name any pitch, the map wants whole 16-byte units all the same)
+    cuuint64_t strides[1] = {rows == 1 ? (cuuint64_t)cols * 4 / 16 * 16 + 16 : (cuuint64_t)pitch};
     cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     const CUresult r = api.tiled(

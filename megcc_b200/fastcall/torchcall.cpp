@@ -31,6 +31,7 @@ struct Abi {
     decltype(&mb200_moe_s8) moe;
 } abi;
 PyObject* on_status = nullptr;
+PyObject* out_of_memory = nullptr;  // torch.OutOfMemoryError
 
 // A refused argument: ValueError with this text
 struct Refused : std::exception {
@@ -137,6 +138,8 @@ PyObject* guarded(F f) {
         return f();
     } catch (const Refused& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const c10::OutOfMemoryError& e) {
+        PyErr_SetString(out_of_memory, e.what_without_backtrace());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     }
@@ -255,8 +258,8 @@ PyObject* moe_s8(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* bind(PyObject*, PyObject* args) {
     unsigned long long at[7];
-    PyObject* fail;
-    if (!PyArg_ParseTuple(args, "OKKKKKKK", &fail, at, at + 1, at + 2, at + 3, at + 4, at + 5, at + 6))
+    PyObject *fail, *memory;
+    if (!PyArg_ParseTuple(args, "OOKKKKKKK", &fail, &memory, at, at + 1, at + 2, at + 3, at + 4, at + 5, at + 6))
         return nullptr;
     abi.quantize_rows = (decltype(abi.quantize_rows))(uintptr_t)at[0];
     abi.matmul_workspace = (decltype(abi.matmul_workspace))(uintptr_t)at[1];
@@ -267,11 +270,13 @@ PyObject* bind(PyObject*, PyObject* args) {
     abi.moe = (decltype(abi.moe))(uintptr_t)at[6];
     Py_INCREF(fail);
     Py_XSETREF(on_status, fail);
+    Py_INCREF(memory);
+    Py_XSETREF(out_of_memory, memory);
     Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
-        {"bind", bind, METH_VARARGS, "bind(raises for a status, addresses of the library's functions)"},
+        {"bind", bind, METH_VARARGS, "bind(raises for a status, torch.OutOfMemoryError, addresses of the library's functions)"},
         {"quantize_rows_s8", (PyCFunction)(void*)quantize_rows_s8, METH_FASTCALL, "(x) -> (q, scales)"},
         {"matmul_s8_scaled", (PyCFunction)(void*)matmul_s8_scaled, METH_FASTCALL,
          "(a, b_packed, a_scales, b_scales, bias, dtype) -> c"},

@@ -118,6 +118,63 @@ def test_moe_ties_and_masks():
     assert bool((y[3] == 0).all())
 
 
+# The same behind the logits that a warp keeps in registers (128 of them)
+@pytest.mark.parametrize("t", [1, 4, 12])
+def test_moe_ties_and_masks_of_many_experts(t):
+    x, logits, w1, s1, w2, s2 = layer(t, 48, 32, 300, 14)
+    row = logits[t - 1]
+    for renorm in (True, False):
+        row[:] = 0                       # ties on both sides
+        check((x, logits, w1, s1, w2, s2), 16, renorm)
+        row[:] = -1
+        row[130::7] = 2.5                # 25 ties, all behind
+        row[200] = 3
+        check((x, logits, w1, s1, w2, s2), 16, renorm)
+        row[:] = float("-inf")
+        row[290:] = torch.randn(10, generator=gen(15), device="cuda")
+        check((x, logits, w1, s1, w2, s2), 16, renorm)
+        row[:] = float("-inf")
+        assert bool((ops.moe_s8(x, logits, w1, s1, w2, s2, 16, renorm)[t - 1] == 0).all())
+        for bad in ("nan", "inf"):
+            row[:] = 0
+            row[299] = float(bad)
+            y = ops.moe_s8(x, logits, w1, s1, w2, s2, 16, renorm)
+            assert bool(y[t - 1].isnan().all()) and not bool(y[:t - 1].isnan().any())
+
+
+# Two captured calls, replayed at once on two streams beside eager ones: each has a workspace of its own
+def test_moe_graphs_at_once():
+    args = [layer(t, 192, 96, 24, t) for t in (6, 40)]
+    wants = [ops.moe_s8(*a, 4) for a in args]
+    torch.cuda.synchronize()
+    graphs = []
+    for a in args:
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = [ops.moe_s8(*a, 4) for _ in range(5)]
+        graphs.append((stream, graph, got))
+    for _ in range(10):
+        for stream, graph, got in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [ops.moe_s8(*a, 4) for a in args]
+        torch.cuda.synchronize()
+        for want, now, (_, _, got) in zip(wants, eager, graphs):
+            assert torch.equal(now, want) and all(torch.equal(g, want) for g in got)
+
+
+def test_moe_without_dependent_launches():
+    from megcc_b200._lib import check as ok, lib
+    args = [layer(t, 100, 40, 9, t) for t in (1, 7, 30)]
+    wants = [ops.moe_s8(*a, 3) for a in args]
+    ok(lib().mb200_set_option(b"pdl", 0))
+    try:
+        for a, want in zip(args, wants):
+            assert torch.equal(ops.moe_s8(*a, 3), want)
+    finally:
+        ok(lib().mb200_set_option(b"pdl", 1))
+
+
 @pytest.mark.parametrize("t", [4, 20])
 def test_moe_of_special_values(t):
     x, logits, w1, s1, w2, s2 = layer(t, 96, 64, 8, 5, torch.float32)

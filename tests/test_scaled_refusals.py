@@ -34,7 +34,8 @@ def test_quantize_rows(change, status):
     (dict(c=None), NULL_PTR), (dict(dtype=7), DTYPE), (dict(m=-3), LAYOUT), (dict(n=0), LAYOUT),
     (dict(k=-1), LAYOUT), (dict(k=131072, lda=131072), OUT_OF_RANGE), (dict(lda=60), LAYOUT),
     (dict(ldc=7), LAYOUT), (dict(sa=P + 2), LAYOUT), (dict(sb=P + 2), LAYOUT), (dict(bias=P + 1), LAYOUT),
-    (dict(c=P + 2), LAYOUT), (dict(c=P + 1, dtype=2), LAYOUT), (dict(m=0, a=None, b=None, c=None), 0)])
+    (dict(c=P + 2), LAYOUT), (dict(c=P + 1, dtype=2), LAYOUT), (dict(m=0, a=None, b=None, c=None), 0),
+    (dict(m=2 ** 31 - 511), OUT_OF_RANGE), (dict(n=2 ** 31 - 1, ldc=2 ** 31), OUT_OF_RANGE)])
 def test_product(change, status):
     assert product(**change) == status
     if status:
@@ -46,7 +47,8 @@ def test_product(change, status):
     (dict(dtype=3), DTYPE), (dict(m=-3), LAYOUT), (dict(n=0), LAYOUT), (dict(k=0), LAYOUT),
     (dict(k=200000, ldx=200000), OUT_OF_RANGE), (dict(ldx=60), LAYOUT), (dict(ldy=7), LAYOUT),
     (dict(x=P + 2), LAYOUT), (dict(sb=P + 2), LAYOUT), (dict(bias=P + 1), LAYOUT),
-    (dict(y=P + 1, dtype=1), LAYOUT), (dict(m=0, x=None), 0)])
+    (dict(y=P + 1, dtype=1), LAYOUT), (dict(m=0, x=None), 0), (dict(m=2 ** 31 - 1), OUT_OF_RANGE),
+    (dict(n=2 ** 31 - 511, ldy=2 ** 31), OUT_OF_RANGE)])
 def test_linear(change, status):
     assert linear(**change) == status
 
