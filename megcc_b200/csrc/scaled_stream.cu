@@ -11,49 +11,62 @@ namespace {
 // HBM: every element is read once and written once as a byte. LANES threads share a row: a warp where
 // a row fits its registers (no barrier), else a whole CTA. The first HELD * LANES vectors of the row stay
 // in registers between the maximum and the conversion, what lies behind them is read again.
+// Vectors are the 16-byte units that the row lies in, zeros around it: with aligned == 0 rows start anywhere in their
+// first one, and their numbers go anywhere in a word (4001 x 4095 fp16: 21.9 us, 39.3 with its numbers stored one by
+// one).
 template <class T, int LANES, int HELD, int THREADS>
-__global__ void __launch_bounds__(THREADS) quantize_rows_kernel(
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 0) quantize_rows_kernel(
         const T* __restrict__ x, int m, int k, long long ldx, int8_t* __restrict__ q, long long ldq,
-        float* __restrict__ scales, int vector_loads, int word_stores) {
+        float* __restrict__ scales, int aligned) {
     constexpr int N = Vec<T>::N;
     __shared__ uint32_t part[THREADS / 32];
     pdl_start();
-    const int lane = threadIdx.x % LANES;
+    const int lane = threadIdx.x % LANES, in_warp = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
     if (LANES == 32 && row >= m)
         return;  // (a whole warp; no barrier follows in this form)
-    const T* src = x + row * ldx;
-    int8_t* dst = q + row * ldq;
-    const int nvec = (k + N - 1) / N;
-    // (rows that start anywhere, and a row's end, come through the 16-byte units that hold them, zeros behind)
+    // elements of the first unit in front of the row
+    const int before = aligned ? 0 : (int)(((uintptr_t)(x + row * ldx) & 15) / sizeof(T));
+    const uint4* src = (const uint4*)(x + row * ldx - before);
+    int8_t* dst = q + row * ldq - before;
+    const unsigned end = (unsigned)before + (unsigned)k;
+    const int nvec = (int)((end - 1) / N) + 1, whole = (int)(end / N), first_whole = before > 0;
     auto load = [&](int v) {
-        return vector_loads && (v + 1) * N <= k ? ((const uint4*)src)[v]
-                                                : ld_any16((const int8_t*)(src + v * N), (k - v * N) * (int)sizeof(T));
+        uint4 w = src[v];
+        if (v < first_whole || v >= whole) {
+            const int from = v == 0 ? before * (int)sizeof(T) : 0;
+            const int to = v < whole ? 16 : (int)(end - (unsigned)v * N) * (int)sizeof(T);
+            uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int lo = min(max(from - 4 * i, 0), 4), hi = min(max(to - 4 * i, 0), 4);
+                u[i] = lo >= hi ? 0u : u[i] >> (8 * lo) << (8 * (lo + 4 - hi)) >> (8 * (4 - hi));
+            }
+            w = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        return w;
     };
     uint4 held[HELD];
     uint32_t vm = 0;
-    if (vector_loads && nvec * N == k) {
+    if (aligned) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const int v = lane + i * LANES;
-            held[i] = v < nvec ? ((const uint4*)src)[v] : make_uint4(0, 0, 0, 0);
+            held[i] = v < whole ? src[v] : make_uint4(0, 0, 0, 0);
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int v = lane + i * LANES;
-            held[i] = v < nvec ? load(v) : make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < HELD; ++i)
+            vm = vec_max<T>(vm, held[i]);
     }
-#pragma unroll
-    for (int i = 0; i < HELD; ++i)
-        vm = vec_max<T>(vm, held[i]);
-    for (int v = lane + HELD * LANES; v < nvec; v += LANES)
+    // (what is not held: the vectors behind, the end of a row, all of a row that starts anywhere)
+    const int rest = aligned ? min(whole, HELD * LANES) : 0;
+#pragma unroll 4
+    for (int v = lane + rest; v < nvec; v += LANES)
         vm = vec_max<T>(vm, load(v));
     uint32_t bits = max_bits<T>(vm);
     bits = __reduce_max_sync(0xffffffffu, bits);
     if (LANES > 32) {
-        if ((threadIdx.x & 31) == 0)
+        if (in_warp == 0)
             part[threadIdx.x >> 5] = bits;
         __syncthreads();
 #pragma unroll
@@ -63,14 +76,17 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(
     const RowScale r = row_scale(bits);
     if (lane == 0)
         scales[row] = r.scale;
-    auto put = [&](int v, const uint4& w) {
+    auto convert = [&](uint32_t(&o)[N / 4], const uint4& w) {
         float f[N];
         Vec<T>::unpack(w, f);
-        uint32_t o[N / 4];
 #pragma unroll
         for (int i = 0; i < N / 4; ++i)
             o[i] = pack_whole(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], r.inv) & r.keep;
-        if (word_stores && (v + 1) * N <= k) {
+    };
+    auto put = [&](int v, const uint4& w) {
+        uint32_t o[N / 4];
+        convert(o, w);
+        if (v < whole) {
             if (N == 8)
                 *(uint2*)(dst + (size_t)v * N) = make_uint2(o[0], o[N / 4 - 1]);
             else
@@ -78,39 +94,80 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                if (v * N + i < k)
+                if (i < k - v * N)
                     dst[(size_t)v * N + i] = (int8_t)(o[i / 4] >> (8 * (i % 4)));
         }
     };
+    // The words that a lane's bytes lie in up to the last one, which the lane behind it stores with its own first bytes
+    // (and lane 0 makes those of the vector in front again). Called by whole warps, for one vector behind the last too.
+    auto put_any = [&](int v) {
+        uint32_t o[N / 4], in_front[N / 4];
+        convert(o, v < nvec ? load(v) : make_uint4(0, 0, 0, 0));
+        if (in_warp == 0)
+            convert(in_front, v > 0 && v <= nvec ? load(v - 1) : make_uint4(0, 0, 0, 0));
+        const uint32_t last = __shfl_up_sync(0xffffffffu, o[N / 4 - 1], 1);
+        if (in_warp > 0)
+            in_front[N / 4 - 1] = last;
+        const int s = (int)((uintptr_t)dst & 3);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
-        if (lane + i * LANES < nvec)
-            put(lane + i * LANES, held[i]);
-    for (int v = lane + HELD * LANES; v < nvec; v += LANES)
-        put(v, load(v));
+        for (int i = 0; i < N / 4; ++i)
+            o[N / 4 - 1 - i] = __funnelshift_l(i < N / 4 - 1 ? o[N / 4 - 2 - i] : in_front[N / 4 - 1], o[N / 4 - 1 - i],
+                                               8 * s);
+        int8_t* to = dst + (long long)v * N - s;
+        if (v > 1 && v < whole) {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i)
+                ((uint32_t*)to)[i] = o[i];
+        } else if (v <= nvec) {
+            const long long at = (long long)v * N - s;
+#pragma unroll 1
+            for (int b = 0; b < N; ++b) {
+                if (at + b >= before && at + b < end)
+                    to[b] = (int8_t)o[0];
+                o[0] = __funnelshift_r(o[0], N == 8 ? o[N / 4 - 1] : 0, 8);
+                if (N == 8)
+                    o[N / 4 - 1] >>= 8;
+            }
+        }
+    };
+    if (aligned) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (lane + i * LANES < whole)
+                put(lane + i * LANES, held[i]);
+#pragma unroll 1
+        for (int v = lane + rest; v < nvec; v += LANES)
+            put(v, load(v));
+    } else {
+#pragma unroll 2
+        for (int v = lane; v - in_warp <= nvec; v += LANES)
+            put_any(v);
+    }
 }
 
 template <class T>
 int quantize_rows(
         const T* x, int m, int k, long long ldx, int8_t* q, long long ldq, float* scales, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
-    const int vector_loads = ((uintptr_t)x & 15) == 0 && (m == 1 || ldx % N == 0);
-    const int word_stores = ((uintptr_t)q & (N - 1)) == 0 && (m == 1 || ldq % N == 0);
+    const int aligned = (((uintptr_t)x & 15) | ((uintptr_t)q & (N - 1))) == 0 &&
+                        (m == 1 || (ldx % N == 0 && ldq % N == 0));
     // (numbers and scales, and what lies between them)
     const uintptr_t q0 = (uintptr_t)q, q1 = q0 + (size_t)(m - 1) * (size_t)ldq + (size_t)k;
     const uintptr_t s0 = (uintptr_t)scales, s1 = s0 + (size_t)m * 4;
     const uintptr_t w0 = q0 < s0 ? q0 : s0, w1 = q1 > s1 ? q1 : s1;
     const Writes writes{(const void*)w0, w1 - w0};
     auto launch = [&](auto kernel, int rows, int threads) {
-        return launch_pdl(writes, kernel, dim3((unsigned)((m - 1) / rows + 1)), dim3((unsigned)threads), 0, st, x, m, k, ldx,
-                          q, ldq, scales, vector_loads, word_stores);
+        return launch_pdl(writes, kernel, dim3((unsigned)((m - 1) / rows + 1)), dim3((unsigned)threads), 0, st, x, m,
+                          k, ldx, q, ldq, scales, aligned);
     };
     // A warp per row where it holds the row and there are rows enough for every SM's warps: 4001 x 4096 fp16 in
-    // 8.6 us, by whole CTAs in 12.3
+    // 7.7 us, by whole CTAs in 12.3. The CTA grows with the row, so that it holds it as long as that goes: 4096 x 14336
+    // fp32 by 512 threads in 43.7 us, by 256 in 54.1.
     const cudaError_t e = m > 1 && k <= 32 * 4 * N            ? launch(quantize_rows_kernel<T, 32, 4, 256>, 8, 256)
                           : m >= 2048 && k <= 32 * 16 * N     ? launch(quantize_rows_kernel<T, 32, 16, 64>, 2, 64)
                           : k <= 256 * 4 * N                  ? launch(quantize_rows_kernel<T, 256, 4, 256>, 1, 256)
-                                                              : launch(quantize_rows_kernel<T, 256, 8, 256>, 1, 256);
+                          : k <= 256 * 8 * N                  ? launch(quantize_rows_kernel<T, 256, 8, 256>, 1, 256)
+                                                              : launch(quantize_rows_kernel<T, 512, 8, 512>, 1, 512);
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "quantize_rows: %s", cudaGetErrorString(e));
     return check_launch("quantize_rows");
@@ -344,7 +401,8 @@ int launch_pad_rows(const PadRows& a, const PadRows& b, cudaStream_t st) {
     const Writes writes{(const void*)lo, hi - lo};
     const cudaError_t e =
             rows < 16 * 148 ? launch_pdl(writes, pad_rows_kernel<256>, dim3((unsigned)rows), dim3(256), 0, st, a, b)
-                            : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, b);
+                            : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
+                                         a, b);
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
     return check_launch("matmul_s8_scaled");

@@ -55,7 +55,7 @@ def check_product(got, q, sa, b, sb, bias):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 7), (3, 64), (1, 4096), (9, 129), (257, 512), (5, 1000),
-                                 (4, 9001), (2, 40000), (1030, 96)])
+                                 (4, 9001), (2, 40000), (1030, 96), (5, 20003), (2100, 4095)])
 def test_quantize_rows(m, k, dtype):
     x = torch.randn((m, k), generator=gen(m + k), device="cuda").to(dtype)
     q, s = ops.quantize_rows_s8(x)
@@ -93,6 +93,24 @@ def test_quantize_rows_that_lie_apart(dtype, offset, pitch):
     q, s = ops.quantize_rows_s8(x)
     want_q, want_s = rows_of(x)
     assert torch.equal(q.double(), want_q) and torch.equal(s, want_s)
+
+
+# Rows of numbers at any byte and any distance, what lies between them untouched
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,pitch,offset", [(3, 5, 7, 1), (7, 300, 303, 2), (1, 1, 1, 3), (2, 4097, 4097, 0),
+                                              (2100, 2047, 2049, 1), (3, 9003, 9006, 3), (40, 256, 256, 5)])
+def test_quantize_to_any_place(m, k, pitch, offset, dtype):
+    from megcc_b200._lib import check, lib
+    x = torch.randn((m, k), generator=gen(m + k), device="cuda").to(dtype)
+    buf = torch.full((offset + m * pitch + 40,), 99, dtype=torch.int8, device="cuda")
+    s = torch.empty(m, device="cuda")
+    check(lib().mb200_quantize_rows_s8(x.data_ptr(), TYPES.index(dtype), m, k, k, buf.data_ptr() + offset, pitch,
+                                       s.data_ptr(), ops._stream()))
+    want_q, want_s = rows_of(x)
+    q = buf.as_strided((m, k), (pitch, 1), offset)
+    assert torch.equal(q.double(), want_q) and torch.equal(s, want_s)
+    q.fill_(99)
+    assert bool((buf == 99).all())
 
 
 SIZES = [(1, 1, 1), (1, 16, 64), (1, 17, 63), (7, 1000, 512), (8, 130, 65), (9, 33, 4096), (16, 48, 48),
@@ -244,6 +262,79 @@ def test_chains_streams_and_graphs(m):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(replayed, chain(x))
+
+
+# A single row of either operand, or of the result, may name any pitch, whichever kernel takes it.
+@pytest.mark.parametrize("m,n,k", [(1, 9600, 4096), (20000, 1, 1001), (20000, 1, 1008), (1, 1, 5), (9000, 1, 64)])
+def test_single_rows(m, n, k):
+    a, b, sa, sb = whole((m, k + 3), 1)[:, :k], whole((n, k), 2), scales(m, 3), scales(n, 4)
+    check_product(ops.matmul_s8_scaled(a, b, sa, sb, None, torch.float16), a, sa, b, sb, None)
+    x = torch.randn((m, k + 1), generator=gen(3), device="cuda").bfloat16()[:, :k]
+    q, sx = rows_of(x)
+    check_product(ops.linear_s8(x, b, sb), q, sx, b, sb, None)
+    y = torch.zeros((m, n), device="cuda", dtype=x.dtype)
+    call_linear(x, b, sb, y, n if m > 1 else 7)
+    check_product(y, q, sx, b, sb, None)
+
+
+# The longest row that an int counts: its last vector ends behind 2^31 elements.
+def test_quantize_the_longest_row():
+    k, part = 2 ** 31 - 1, 1 << 27
+    x = torch.empty((1, k), dtype=torch.float16, device="cuda")
+    for at in range(0, k, part):
+        x[0, at:at + part].normal_(generator=gen(at + 1))
+    x[0, k - 1] = 9.0
+    q, s = ops.quantize_rows_s8(x)
+    for at in range(0, k, part):
+        piece = torch.cat([x[0, at:at + part], x[0, k - 1:]])[None]  # (the largest is the last)
+        want_q, want_s = rows_of(piece)
+        assert torch.equal(q[0, at:at + part].double(), want_q[0, :-1]) and torch.equal(s, want_s)
+
+
+# A result that no GPU holds is torch's own error, and the next call works.
+def test_results_larger_than_memory():
+    b = torch.zeros((2 ** 21, 1), dtype=torch.int8, device="cuda")
+    rows = torch.zeros((2 ** 21, 1), device="cuda")
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.linear_s8(rows, b, torch.ones(2 ** 21, device="cuda"))
+    assert ops.linear_s8(rows[:1], b, torch.ones(2 ** 21, device="cuda")).shape == (1, 2 ** 21)
+
+
+# Two threads with a stream each, at once: results are those of one call alone.
+def test_two_threads_at_once():
+    import threading
+    b, sb = whole((1000, 1040), 2), scales(1000, 4)
+    xs = [torch.randn((m, 1040), generator=gen(m), device="cuda").half() for m in (1, 20, 100, 700)]
+    wants = [ops.linear_s8(x, b, sb) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in order * 25:
+                if not torch.equal(ops.linear_s8(xs[i], b, sb), wants[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(order,)) for order in ([0, 1, 2, 3], [3, 1, 0, 2])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+# Kernels that do not overlap at all give the same bits.
+def test_without_dependent_launches():
+    from megcc_b200._lib import check, lib
+    b, sb = whole((300, 519), 2), scales(300, 4)
+    xs = [torch.randn((m, 519), generator=gen(m), device="cuda") for m in (1, 30, 400)]
+    wants = [ops.linear_s8(x, b, sb) for x in xs]
+    check(lib().mb200_set_option(b"pdl", 0))
+    try:
+        for x, want in zip(xs, wants):
+            assert torch.equal(ops.linear_s8(x, b, sb), want)
+    finally:
+        check(lib().mb200_set_option(b"pdl", 1))
 
 
 def test_addresses_past_32_bits():
