@@ -310,7 +310,7 @@ template <int COLS, int DEPTH, bool ALIGNED>
 struct Up {
     static constexpr int kDepth = DEPTH;
     static constexpr int kHalves = 2;  // warps that share a tile's steps
-    typedef Rows<16, ALIGNED> W;
+    typedef Rows<16, ALIGNED, (DEPTH > 3)> W;
     static constexpr int kRing = kWarps * kDepth * W::kBytes;
     static constexpr int kExchange = kHalves * COLS * kPitch;  // ints; two of them, used in turn
     static int smem(const MoeArgs& a) {
@@ -359,9 +359,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
     const int blocks = (a.f + kUnits - 1) / kUnits;
     // (1024 slots of 4096 blocks at most, in 1024 CTAs: products that 32 bits hold)
     const unsigned tiles = (unsigned)(*route.passes * blocks);
-    const int first = (int)(tiles * blockIdx.x / gridDim.x), last = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
-    if (first == last)
+    // as few CTAs as still take as many tiles each as the busiest would: the last clusters to find room may begin late
+    const unsigned each = (tiles + gridDim.x - 1) / gridDim.x, busy = each ? (tiles + each - 1) / each : 1u;
+    if (blockIdx.x >= busy || tiles == 0)
         return;
+    const int first = (int)(tiles * blockIdx.x / busy), last = (int)(tiles * (blockIdx.x + 1) / busy);
     const int steps = (a.d + kStep - 1) / kStep;
     const int half = warp >> 2;                        // steps half, half + 2, ...
     const int mine = (steps - half + 1) / U::kHalves;  // (none where there is one step only)
@@ -712,20 +714,21 @@ bool few_columns(const MoeArgs& a) {
     return a.t <= 8 || a.t * a.top <= 4 * a.e;
 }
 
-// How many clusters of four the GPU holds at once, asked again where the shared memory is another one
-struct ClustersOfFour {
-    std::atomic<long long> known[64] = {};  // shared memory << 16 | clusters
+// How many clusters the GPU holds at once, asked again where their size or shared memory is another one
+struct ClustersThatFit {
+    std::atomic<long long> known[64] = {};  // shared memory << 20 | size << 16 | clusters
     template <class Kernel>
-    int fit(Kernel kernel, int smem) {
+    int fit(Kernel kernel, int size, int smem) {
         int dev = 0;
         if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
             dev = 0;
         const long long k = known[dev].load(std::memory_order_relaxed);
-        if (k && k >> 16 == smem)
+        const long long key = (long long)smem << 4 | size;
+        if (k && k >> 16 == key)
             return (int)(k & 0xffff);
         umma::ClusterCapacity capacity;
-        const int n = capacity.clusters(kernel, 4, kThreads, smem);
-        known[dev].store((long long)smem << 16 | n, std::memory_order_relaxed);
+        const int n = capacity.clusters(kernel, size, kThreads, smem);
+        known[dev].store(key << 16 | n, std::memory_order_relaxed);
         return n;
     }
 };
@@ -733,19 +736,21 @@ struct ClustersOfFour {
 template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
 cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
+    static MostShared shared;
     static umma::ResidentCtas resident;
-    static ClustersOfFour clusters;
+    static ClustersThatFit clusters;
     auto kernel = moe_up_kernel<T, COLS, DEPTH, CTAS, ALIGNED>;
     const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
+    shared.ask(kernel);
     const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx % Vec<T>::N == 0);
     const long long tiles = (long long)a.t * a.top * ((a.f + kUnits - 1) / kUnits);  // at most
     const Writes writes{a.hq, a.workspace_bytes};
     // clusters of four for the routing of many tokens (whole clusters live inside a GPC: eight would leave SMs idle)
-    const int cluster = a.t <= 8 ? 1 : 4;
+    const int cluster = a.t <= 2 * kWarps ? 1 : a.t <= 4 * kWarps ? 2 : 4;
     const long long fit = cluster == 1 ? (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0)
-                                       : 4LL * clusters.fit(kernel, smem);
+                                       : (long long)cluster * clusters.fit(kernel, cluster, smem);
     const long long some = fit > 0 ? fit : cluster;
     const long long ctas = tiles < some ? (tiles + cluster - 1) / cluster * cluster : some;
     return launch_pdl_cluster(writes, kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, cluster, st, a,
@@ -758,16 +763,18 @@ cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
         return aligned ? launch_up_as<T, 8, 3, 3, true>(a, st) : launch_up_as<T, 8, 3, 3, false>(a, st);
     if (few_columns(a))
         return aligned ? launch_up_as<T, 8, 4, 2, true>(a, st) : launch_up_as<T, 8, 4, 2, false>(a, st);
-    return aligned ? launch_up_as<T, 16, 4, 2, true>(a, st) : launch_up_as<T, 16, 3, 2, false>(a, st);
+    return aligned ? launch_up_as<T, 16, 4, 2, true>(a, st) : launch_up_as<T, 16, 4, 2, false>(a, st);
 }
 
 template <int NT, int DEPTH, int CTAS, bool ALIGNED>
 cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
+    static MostShared shared;
     auto kernel = moe_down_kernel<NT, DEPTH, CTAS, ALIGNED>;
     const int smem = Down<NT, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
+    shared.ask(kernel);
     const Writes writes{a.y, ((size_t)(a.t - 1) * (size_t)a.ldy + (size_t)a.d) * dtype_bytes(a.dtype)};
     // a CTA for every SM where each warp still has two steps (experts with tokens: at most as many as slots)
     const int tiles = (a.d - 1) / kRows + 1, slots = a.t * a.top;

@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "internal.h"
 #include "pdl.h"
 
@@ -204,6 +206,22 @@ __device__ __forceinline__ uint4 pack_piece(const float (&v)[16], const RowScale
 }
 
 #endif  // __CUDACC__
+
+// Kernels that run in turn ask for the same share of an SM's memory as shared memory, all of it: an SM changes the share
+// only when it is empty, so a kernel that asks for more than the one in front cannot begin beside its end.
+struct MostShared {
+    std::atomic<bool> done[64] = {};
+    template <class Kernel>
+    void ask(Kernel kernel) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || done[dev].load(std::memory_order_relaxed))
+            return;
+        // (a preference: the kernel runs without it as well)
+        (void)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                   cudaSharedmemCarveoutMaxShared);
+        done[dev].store(true, std::memory_order_relaxed);
+    }
+};
 
 // c[m][n] = a[m][k] * b[n][k] (whole numbers) * sa[m] * sb[n] [+ bias[n]]
 struct ProductArgs {

@@ -156,18 +156,21 @@ int quantize_rows(
     const uintptr_t s0 = (uintptr_t)scales, s1 = s0 + (size_t)m * 4;
     const uintptr_t w0 = q0 < s0 ? q0 : s0, w1 = q1 > s1 ? q1 : s1;
     const Writes writes{(const void*)w0, w1 - w0};
-    auto launch = [&](auto kernel, int rows, int threads) {
+    auto launch = [&](auto kernel, int rows, int threads, MostShared& shared) {
+        shared.ask(kernel);
         return launch_pdl(writes, kernel, dim3((unsigned)((m - 1) / rows + 1)), dim3((unsigned)threads), 0, st, x, m,
                           k, ldx, q, ldq, scales, aligned);
     };
     // A warp per row where it holds the row and there are rows enough for every SM's warps: 4001 x 4096 fp16 in
     // 7.7 us, by whole CTAs in 12.3. The CTA grows with the row, so that it holds it as long as that goes: 4096 x 14336
     // fp32 by 512 threads in 43.7 us, by 256 in 54.1.
-    const cudaError_t e = m > 1 && k <= 32 * 4 * N            ? launch(quantize_rows_kernel<T, 32, 4, 256>, 8, 256)
-                          : m >= 2048 && k <= 32 * 16 * N     ? launch(quantize_rows_kernel<T, 32, 16, 64>, 2, 64)
-                          : k <= 256 * 4 * N                  ? launch(quantize_rows_kernel<T, 256, 4, 256>, 1, 256)
-                          : k <= 256 * 8 * N                  ? launch(quantize_rows_kernel<T, 256, 8, 256>, 1, 256)
-                                                              : launch(quantize_rows_kernel<T, 512, 8, 512>, 1, 512);
+    static MostShared shared[5];
+    const cudaError_t e =
+            m > 1 && k <= 32 * 4 * N        ? launch(quantize_rows_kernel<T, 32, 4, 256>, 8, 256, shared[0])
+            : m >= 2048 && k <= 32 * 16 * N ? launch(quantize_rows_kernel<T, 32, 16, 64>, 2, 64, shared[1])
+            : k <= 256 * 4 * N              ? launch(quantize_rows_kernel<T, 256, 4, 256>, 1, 256, shared[2])
+            : k <= 256 * 8 * N              ? launch(quantize_rows_kernel<T, 256, 8, 256>, 1, 256, shared[3])
+                                            : launch(quantize_rows_kernel<T, 512, 8, 512>, 1, 512, shared[4]);
     if (e != cudaSuccess)
         return set_error(ST_RUNTIME, "quantize_rows: %s", cudaGetErrorString(e));
     return check_launch("quantize_rows");
@@ -184,21 +187,22 @@ constexpr int kWarps = 8;
 constexpr int kRows = 16;     // weight rows per CTA
 constexpr int kColPitch = 20; // ints per token in the exchange: 2 * 20 = 8 banks apart
 
-template <class XT, int NT, bool ALIGNED, bool SHARED>
+template <class XT, int NT, bool ALIGNED, bool TOKENS, bool SHARED>
 struct Stream {
     static constexpr bool kFloat = sizeof(XT) > 1;
     static constexpr int kCols = 8 * NT;
     static constexpr int kDepth = NT == 1 ? 4 : NT == 2 ? 3 : 2;  // (room for two CTAs per SM)
-    typedef Rows<kRows, ALIGNED> W;
-    typedef Rows<kCols, ALIGNED> A;
+    typedef Rows<kRows, ALIGNED, true> W;
+    typedef Rows<kCols, TOKENS, true> A;
     static constexpr int kStage = W::kBytes + (kFloat ? 0 : A::kBytes);
     static constexpr int kRing = kWarps * kDepth * kStage;
     static constexpr int kCtaRows = SHARED ? kRows : kRows * kWarps;
 };
 
-template <class XT, int NT, bool ALIGNED, bool SHARED>
+// ALIGNED, TOKENS: rows of weights, of int8 tokens are whole 16-byte units
+template <class XT, int NT, bool ALIGNED, bool TOKENS, bool SHARED>
 __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const ProductArgs p, int x_vectors) {
-    typedef Stream<XT, NT, ALIGNED, SHARED> S;
+    typedef Stream<XT, NT, ALIGNED, TOKENS, SHARED> S;
     constexpr bool kFloat = S::kFloat;
     constexpr int kDepth = S::kDepth, kCols = S::kCols;
     extern __shared__ __align__(128) uint8_t dynamic[];  // the rings, then (floats) xs
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
                     t = *(const uint4*)(x_at[nt] + step * kStep + 64 * j);
                 } else {
                     t = S::A::piece16(stage + S::W::kBytes, 8 * nt + g, piece, s_a[nt]);
-                    if (!ALIGNED && step == steps - 1)  // (aligned rows end with a unit, zeros lie behind it)
+                    if (!ALIGNED && step == steps - 1)  // (where rows end with a unit, zeros lie behind it)
                         t = first_bytes(t, k - step * kStep - piece * 16);
                 }
                 mma_64(acc[nt], lo, hi, t);
@@ -344,34 +348,41 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const PadRows a, const Pa
         dst[u] = ld_any16(src + 16 * u, j.k - 16 * u);
 }
 
-template <class XT, int NT, bool ALIGNED, bool SHARED>
+template <class XT, int NT, bool ALIGNED, bool TOKENS, bool SHARED>
 cudaError_t launch_stream_as(const ProductArgs& a, int x_vectors, cudaStream_t st) {
-    typedef Stream<XT, NT, ALIGNED, SHARED> S;
+    typedef Stream<XT, NT, ALIGNED, TOKENS, SHARED> S;
     static umma::KernelReady ready;
+    static MostShared shared;
     static_assert(S::kRing >= kWarps * S::kCols * kColPitch * 4, "the exchange lies where the rings were");
-    auto kernel = product_stream_kernel<XT, NT, ALIGNED, SHARED>;
+    auto kernel = product_stream_kernel<XT, NT, ALIGNED, TOKENS, SHARED>;
     const int smem = S::kRing + (S::kFloat ? (a.m < S::kCols ? a.m : S::kCols) * xs_pitch(a.k) : 0);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
+    shared.ask(kernel);
     const dim3 grid((unsigned)((a.n - 1) / S::kCtaRows + 1), (unsigned)((a.m - 1) / S::kCols + 1));
     const Writes writes{a.c, ((size_t)(a.m - 1) * (size_t)a.ldc + (size_t)a.n) * dtype_bytes(a.c_dtype)};
     return launch_pdl(writes, kernel, grid, dim3(32 * kWarps), (size_t)smem, st, a, x_vectors);
 }
-template <class XT, int NT>
-cudaError_t launch_stream(const ProductArgs& a, bool aligned, int x_vectors, cudaStream_t st) {
+template <class XT, int NT, bool ALIGNED, bool TOKENS>
+cudaError_t launch_stream(const ProductArgs& a, int x_vectors, cudaStream_t st) {
     // warps of their own where shared tiles would take several turns on the SMs for a step or two per warp
     const long long ctas = ((long long)(a.n - 1) / kRows + 1) * ((a.m - 1) / (8 * NT) + 1);
     if (a.k <= 8 * kStep && ctas > 2LL * umma::sm_count())
-        return aligned ? launch_stream_as<XT, NT, true, false>(a, x_vectors, st)
-                       : launch_stream_as<XT, NT, false, false>(a, x_vectors, st);
-    return aligned ? launch_stream_as<XT, NT, true, true>(a, x_vectors, st)
-                   : launch_stream_as<XT, NT, false, true>(a, x_vectors, st);
+        return launch_stream_as<XT, NT, ALIGNED, TOKENS, false>(a, x_vectors, st);
+    return launch_stream_as<XT, NT, ALIGNED, TOKENS, true>(a, x_vectors, st);
+}
+template <int NT>
+cudaError_t launch_stream_whole(const ProductArgs& a, bool aligned, bool tokens, cudaStream_t st) {
+    return !tokens   ? launch_stream<int8_t, NT, false, false>(a, 0, st)
+           : aligned ? launch_stream<int8_t, NT, true, true>(a, 0, st)
+                     : launch_stream<int8_t, NT, false, true>(a, 0, st);
 }
 
 template <class XT>
 cudaError_t launch_stream_float(const ProductArgs& a, bool aligned, cudaStream_t st) {
     const int x_vectors = ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % Vec<XT>::N == 0);
-    return launch_stream<XT, 1>(a, aligned, x_vectors, st);
+    return aligned ? launch_stream<XT, 1, true, true>(a, x_vectors, st)
+                   : launch_stream<XT, 1, false, true>(a, x_vectors, st);
 }
 
 }  // namespace
@@ -399,6 +410,9 @@ int launch_pad_rows(const PadRows& a, const PadRows& b, cudaStream_t st) {
             hi = end > hi ? end : hi;
         }
     const Writes writes{(const void*)lo, hi - lo};
+    static MostShared shared[2];
+    shared[0].ask(pad_rows_kernel<256>);
+    shared[1].ask(pad_rows_kernel<32>);
     const cudaError_t e =
             rows < 16 * 148 ? launch_pdl(writes, pad_rows_kernel<256>, dim3((unsigned)rows), dim3(256), 0, st, a, b)
                             : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
@@ -412,10 +426,10 @@ int launch_product_stream(const ProductArgs& a, cudaStream_t st) {
     const bool b_aligned = ((uintptr_t)a.b & 15) == 0 && (a.n == 1 || a.ldb % 16 == 0) && a.k % 16 == 0;
     cudaError_t e;
     if (a.x_dtype < 0) {
-        const bool aligned = b_aligned && ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % 16 == 0);
-        e = a.m <= 8    ? launch_stream<int8_t, 1>(a, aligned, 0, st)
-            : a.m <= 16 ? launch_stream<int8_t, 2>(a, aligned, 0, st)
-                        : launch_stream<int8_t, 4>(a, aligned, 0, st);
+        const bool tokens = ((uintptr_t)a.a & 15) == 0 && (a.m == 1 || a.lda % 16 == 0);
+        e = a.m <= 8    ? launch_stream_whole<1>(a, b_aligned, tokens, st)
+            : a.m <= 16 ? launch_stream_whole<2>(a, b_aligned, tokens, st)
+                        : launch_stream_whole<4>(a, b_aligned, tokens, st);
     } else if (a.x_dtype == DT_F32) {
         e = launch_stream_float<float>(a, b_aligned, st);
     } else if (a.x_dtype == DT_F16) {

@@ -8,7 +8,9 @@
 // A step is 128 bytes of K of each of 16 rows: whole lines, and few enough instructions per byte (with 64 bytes
 // the expert kernels took 100 to 230 of them per KB and were bound by their issue: 33 us for 100 MB). Rows may
 // start at any byte: ALIGNED rows are eight 16-byte units, others the nine units that hold their 128 bytes,
-// shifted into place when they are read.
+// shifted into place when they are read. WIDE: 16 bytes by two 16-byte loads and selects, where loads of shared memory
+// bound (12 x 4096 x 4104 in 7.4 us, by five 4-byte loads, four lanes of them on each bank, in 11.7); otherwise by those,
+// with half the registers and instructions (two experts of 1928 x 800: 11.4 us, 12.1 with WIDE).
 #pragma once
 #include "scaled_s8.cuh"
 
@@ -56,16 +58,19 @@ __device__ __forceinline__ uint32_t lds4(uint32_t at) {
 }
 
 // ROWS rows of a step in shared memory
-template <int ROWS, bool ALIGNED>
+template <int ROWS, bool ALIGNED, bool WIDE = false>
 struct Rows {
     static constexpr int kUnits = ALIGNED ? 8 : 9;
     static constexpr int kPitch = 16 * kUnits;
     static constexpr int kBytes = ROWS * kPitch;
     static constexpr int kCopies = (ROWS * kUnits + 31) / 32;  // of a lane, per step
 
-    // Where a unit lies in its row: a read of 16 (8) bytes by the lanes of two (four) rows meets every bank once
+    // Where a unit lies: a read of 16 (8) bytes by the lanes of two (four) rows meets every bank once. Eight units are
+    // rearranged within their row; with nine each row begins a unit further round the banks, so the rows are.
     static __device__ __forceinline__ int unit_at(int row, int unit) {
-        return ALIGNED ? unit ^ (((row & 1) << 2) | (row & 2)) : unit;
+        if (ALIGNED)
+            return row * kPitch + (unit ^ (((row & 1) << 2) | (row & 2))) * 16;
+        return (WIDE ? (row & ~7) | (row & 6) >> 1 | (row & 1) << 2 : row) * kPitch + unit * 16;
     }
 
     // what a lane copies next: its units' places in global memory, and how far their rows go from there
@@ -81,7 +86,7 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const int q = lane + 32 * i, r = q / kUnits, u = q % kUnits;
-            to[i] = r * kPitch + unit_at(r, u) * 16;
+            to[i] = unit_at(r, u);
         }
     }
     // row(r): address of row r, or null for one that is not there (row 0 is); k: its bytes; step: the first
@@ -133,13 +138,24 @@ struct Rows {
     }
     // 16 bytes of row r from byte 16 * part on; s: the row's address modulo 16
     static __device__ __forceinline__ uint4 piece16(uint32_t stage, int r, int part, int s) {
+        const uint32_t at = stage + unit_at(r, part);
         if (ALIGNED)
-            return lds16(stage + r * kPitch + unit_at(r, part) * 16);
-        const uint32_t at = stage + r * kPitch + part * 16 + (s & ~3);
-        uint32_t w[5];
+            return lds16(at);
+        uint32_t w[8];
+        if (WIDE) {
+            const uint4 lo = lds16(at), hi = lds16(at + 16);
+            w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
-            w[i] = lds4(at + 4 * i);
+            for (int i = 0; i < 6; ++i)
+                w[i] = s & 8 ? w[i + 2] : w[i];
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+                w[i] = s & 4 ? w[i + 1] : w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+                w[i] = lds4(at + (s & ~3) + 4 * i);
+        }
         const int bits = (s & 3) * 8;
         return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
                           __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
@@ -147,8 +163,9 @@ struct Rows {
     // 8 bytes from byte 8 * part on
     static __device__ __forceinline__ uint2 piece8(uint32_t stage, int r, int part, int s) {
         if (ALIGNED)
-            return lds8(stage + r * kPitch + unit_at(r, part >> 1) * 16 + (part & 1) * 8);
-        const uint32_t at = stage + r * kPitch + part * 8 + (s & ~3);
+            return lds8(stage + unit_at(r, part >> 1) + (part & 1) * 8);
+        // (words: two 8-byte loads and selects took 68 us where these took 63, 40 tokens, 45 experts, 1925 x 803)
+        const uint32_t at = stage + unit_at(r, 0) + part * 8 + (s & ~3);
         const uint32_t a = lds4(at), b = lds4(at + 4), c = lds4(at + 8);
         const int bits = (s & 3) * 8;
         return make_uint2(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits));
