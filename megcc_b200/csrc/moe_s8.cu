@@ -1,5 +1,5 @@
-// A mixture-of-experts layer for a few tokens, experts in int8: two kernels, no exchange between CTAs
-// but what the first one writes and the second one reads.
+// A mixture-of-experts layer for a few tokens, experts in int8: two kernels for up to eight tokens, three for more, no
+// exchange between CTAs but what one kernel writes and the next ones read (and a cluster's sums in the last).
 //
 //   p[t][e] = softmax(logits[t]) over all experts; token t goes to the top_k largest (ties: the lowest
 //             index), with p as it is or divided by the sum of the chosen
@@ -13,7 +13,9 @@
 // HBM: the chosen experts' weights, 3 * d * f bytes each, are read once and everything else is small, so
 // both kernels stream them through rings of asynchronous copies into mma.sync (stream_s8.cuh), over the ends of
 // rows, experts and tiles.
-// Every CTA of either kernel works the routing out for itself: it is a few thousand logits.
+// Up to eight tokens every CTA of either kernel works the routing out for itself, a token per warp. More are routed
+// and made whole numbers by a kernel in front, whose results both of the others read (the last one ahead of the end of
+// the second): 10 tokens, two of 45 experts of 1920 x 800: PLACEHOLDER.
 #include "moe_s8.h"
 #include "stream_s8.cuh"
 #include "umma_ptx.cuh"
@@ -24,6 +26,7 @@ namespace scaled {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kRouteWarps = 32;       // of the kernel in front
 constexpr int kUnits = 32;            // hidden units per tile of the first kernel, and per group of h
 constexpr int kPitch = 2 * kUnits + 4;  // ints per token in its exchange: 2 * 68 = 8 banks apart
 constexpr int kRows = 16;             // rows of w2 per CTA of the second kernel
@@ -180,27 +183,18 @@ __device__ __noinline__ Choices<N> choose_experts(
     return c;
 }
 
-// A value at the same place in another CTA of the cluster
-__device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
-    uint32_t at, v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_address(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
-}
-
-// A warp for a token or two in turn (each a chain of 2 us or more: the CTAs of a cluster share the tokens
-// out); then the slots by expert, cut into passes of at most `cols`. Barriers of the CTA stand before and behind,
-// and with a cluster umma::cluster_wait() has to follow before r.expert's memory is used for something else. With four
-// tokens at most the upper half of the warps has none and calls meanwhile().
-template <class Meanwhile>
-__device__ __forceinline__ void route_tokens(
-        const MoeArgs& a, int cols, const Route& r, int rank, int cluster, Meanwhile meanwhile) {
+// A warp for a token or two in turn (each a chain of 2 us or more); then the slots by expert, cut into passes of
+// at most `cols`. Barriers of the CTA stand before and behind. With four tokens at most the upper half of the warps has
+// none and calls meanwhile().
+template <int WARPS, class Meanwhile>
+__device__ __forceinline__ void route_tokens(const MoeArgs& a, int cols, const Route& r, Meanwhile meanwhile) {
+    constexpr int kThreads = 32 * WARPS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (a.t > 1)
         for (int e = threadIdx.x; e < 2 * a.e; e += kThreads)
             r.tokens[e] = 0;
-    // tokens rank * kWarps + warp, and every cluster * kWarps further, two at a time while there are two
-    const int stride = cluster * kWarps;
+    // every WARPS-th token, two at a time while there are two
+    constexpr int stride = WARPS;
     auto keep = [&](int t, const Choice& c) {
         if (lane < a.top) {
             r.p[t * a.top + lane] = c.p;
@@ -208,7 +202,7 @@ __device__ __forceinline__ void route_tokens(
                 r.expert[t * a.top + lane] = c.expert;
         }
     };
-    int t = rank * kWarps + warp;
+    int t = warp;
 #pragma unroll 1
     for (; t + stride < a.t; t += 2 * stride) {
         const Choices<2> c = choose_experts<2>(a.logits + (size_t)t * a.e, (size_t)stride * a.e, a.e, a.top, a.renormalize);
@@ -236,27 +230,14 @@ __device__ __forceinline__ void route_tokens(
     __syncthreads();
     if (a.t == 1)
         return;
-    if (cluster > 1) {
-        umma::cluster_arrive();
-        umma::cluster_wait();
-    }
     // A bit per expert and token: what an expert's slots are follows from them alone, whatever order they come in, so
     // every CTA cuts them into the same passes.
     const int slots = a.t * a.top;
 #pragma unroll 1
     for (int s = threadIdx.x; s < slots; s += kThreads) {
-        const int token = s / a.top, owner = token / kWarps % cluster;
-        if (owner != rank) {
-            r.p[s] = __uint_as_float(peer_word(r.p + s, owner));
-            r.expert[s] = (int)peer_word(r.expert + s, owner);
-        }
-        const int e = r.expert[s];
+        const int token = s / a.top, e = r.expert[s];
         if (e >= 0)
             atomicOr(r.tokens + 2 * e + (token >> 5), 1u << (token & 31));
-    }
-    if (cluster > 1) {
-        __syncwarp();
-        umma::cluster_arrive();
     }
     __syncthreads();
     if (warp == 0) {
@@ -301,11 +282,38 @@ __device__ __forceinline__ void route_tokens(
     __syncthreads();
 }
 
+// ---- more than eight tokens: the routing, by the first CTA, and a token's whole numbers by each of the others ----
+// What bounds it is the chain of choices, top_k times two reductions over a warp.
+template <class T>
+__global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const MoeArgs a, int cols, int x_vectors) {
+    extern __shared__ __align__(128) uint8_t dynamic[];
+    pdl_start();
+    if (blockIdx.x > 0) {
+        const int t = (int)blockIdx.x - 1, pitch = xs_pitch(a.d);
+        rows_to_whole<T, kRouteWarps>([&](int) { return (const T*)a.x + (long long)t * a.ldx; }, 1, a.d,
+                                      a.xq + (size_t)t * pitch, pitch, a.sx + t, (uint32_t*)dynamic, x_vectors);
+        return;
+    }
+    const int bytes = route_bytes(a.t * a.top, a.e, cols);
+    const Route route = place_route(dynamic, dynamic + bytes, a.t * a.top, a.e, cols);
+    route_tokens<kRouteWarps>(a, cols, route, [] {});
+    for (int i = threadIdx.x; i < bytes / 16; i += 32 * kRouteWarps)
+        a.route[i] = ((const uint4*)dynamic)[i];
+}
+// what the kernel in front has found
+__device__ __forceinline__ void read_route(const MoeArgs& a, int cols, const Route& r) {
+    const int units = route_bytes(a.t * a.top, a.e, cols) / 16;
+    for (int i = threadIdx.x; i < units; i += kThreads)
+        ((uint4*)r.p)[i] = a.route[i];
+    __syncthreads();
+}
+
 // ---- gate, up, activation, and h as whole numbers ----
 // Tiles of 32 hidden units (64 rows of w1), once per pass of their expert; a CTA takes neighbouring ones. Four
 // of its eight warps have 16 rows each (gate, gate, up, up) and every other step of d, the other four the same rows
 // and the remaining steps; each warp's ring runs on over the ends of tiles. COLS tokens at once; with no more
-// tokens than that all of them stay in shared memory for the whole kernel.
+// tokens than that all of them stay in shared memory for the whole kernel. T: of the activations, up to eight tokens;
+// int8_t where they are whole numbers already.
 template <int COLS, int DEPTH, bool ALIGNED>
 struct Up {
     static constexpr int kDepth = DEPTH;
@@ -320,7 +328,7 @@ struct Up {
 };
 
 template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a, int x_vectors, int cluster) {
+__global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a, int x_vectors) {
     typedef Up<COLS, DEPTH, ALIGNED> U;
     constexpr int NT = COLS / 8, kDepth = U::kDepth;
     extern __shared__ __align__(128) uint8_t dynamic[];
@@ -330,36 +338,31 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
     const Route route = place_route((uint8_t*)xs + min(a.t, COLS) * pitch, dynamic, a.t * a.top, a.e, COLS);
     static_assert(U::kRing >= kMostBuild, "the routing is worked out where the rings will be");
     __shared__ float x_scale[COLS];
-    __shared__ uint32_t part[16 * kWarps];
+    constexpr bool kFew = sizeof(T) > 1;
+    __shared__ uint32_t part[kFew ? 16 * kWarps : 1];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
-    const bool resident = a.t <= COLS;
+    const bool resident = kFew || a.t <= COLS;
     pdl_start();
     auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
-    // (the logits, and with few tokens those, are on their way while the routing is worked out)
-    ask_ahead<kThreads>(a.logits, a.t * a.e * 4);
-    if (resident && a.t > 4)
+    if constexpr (kFew) {
+        // (the logits and tokens are on their way while the routing is worked out)
+        ask_ahead<kThreads>(a.logits, a.t * a.e * 4);
+        if (a.t > 4)
 #pragma unroll 1
-        for (int t = 0; t < a.t; ++t)
-            ask_ahead<kThreads>(token_row(t), a.d * (int)sizeof(T));
-    route_tokens(a, COLS, route, cluster > 1 ? (int)umma::cluster_rank() : 0, cluster, [&] {
-        if (resident)
+            for (int t = 0; t < a.t; ++t)
+                ask_ahead<kThreads>(token_row(t), a.d * (int)sizeof(T));
+        route_tokens<kWarps>(a, COLS, route, [&] {
             rows_to_whole<T, 4, 4>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
-    });
-    if (a.t > 8 && blockIdx.x == 0) {
-        const int units = route_bytes(a.t * a.top, a.e, COLS) / 16;
-        for (int i = threadIdx.x; i < units; i += kThreads)
-            a.route[i] = ((const uint4*)route.p)[i];
-    }
-    if (cluster > 1) {
-        __syncwarp();
-        umma::cluster_wait();  // nobody reads this CTA's choices any more
+        });
+    } else {
+        read_route(a, COLS, route);
     }
     const int blocks = (a.f + kUnits - 1) / kUnits;
     // (1024 slots of 4096 blocks at most, in 1024 CTAs: products that 32 bits hold)
     const unsigned tiles = (unsigned)(*route.passes * blocks);
-    // as few CTAs as still take as many tiles each as the busiest would: the last clusters to find room may begin late
+    // as few CTAs as still take as many tiles each as the busiest would
     const unsigned each = (tiles + gridDim.x - 1) / gridDim.x, busy = each ? (tiles + each - 1) / each : 1u;
     if (blockIdx.x >= busy || tiles == 0)
         return;
@@ -408,10 +411,24 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
             e = route.pass_expert[pass];
             cols = route.pass_cols[pass];
             order = route.order + route.pass_start[pass];
-            if (!resident || (tile == first && a.t > 4)) {
-                // (behind the barrier in it all warps are done with the last pass's tokens)
-                rows_to_whole<T, kWarps>([&](int c) { return token_row(resident ? c : order[c] >> 16); },
-                                         resident ? a.t : cols, a.d, xs, pitch, x_scale, part, x_vectors);
+            if constexpr (kFew) {
+                if (tile == first && a.t > 4) {
+                    rows_to_whole<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
+                    __syncthreads();
+                }
+            } else if (!resident || tile == first) {
+                __syncthreads();  // (all warps are done with the last pass's tokens)
+                const int rows = resident ? a.t : cols;
+#pragma unroll 1
+                for (int c = warp; c < rows; c += kWarps) {
+                    const int t = resident ? c : order[c] >> 16;
+                    const uint4* from = (const uint4*)(a.xq + (size_t)t * pitch);
+#pragma unroll 8
+                    for (int i = lane; i < pitch / 16; i += 32)
+                        ((uint4*)(xs + c * pitch))[i] = from[i];
+                    if (lane == 0)
+                        x_scale[c] = a.sx[t];
+                }
                 __syncthreads();
             }
         }
@@ -511,18 +528,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
     const int g = lane >> 2, tig = lane & 3;
     const int rank = cluster > 1 ? (int)umma::cluster_rank() : 0;
     const int d0 = (int)blockIdx.x / cluster * kRows;
-    // Ahead of the first kernel's end: the routing of a few tokens, and with it the first weights. What is read here
-    // was written before the first kernel began, which let this one start behind its own wait for that. The routing
-    // of more takes longer than to fetch the first kernel's.
-    if (a.t <= 8) {
-        route_tokens(a, kCols, route, 0, 1, [] {});
-    } else {
-        pdl_start();
-        const int units = route_bytes(a.t * a.top, a.e, kCols) / 16;
-        for (int i = threadIdx.x; i < units; i += kThreads)
-            ((uint4*)route.p)[i] = a.route[i];
-        __syncthreads();
-    }
+    // Ahead of the end of the kernel in front: the routing, and with it the first weights. What is read here
+    // was written before that kernel began its work, which let this one start behind its own wait for it.
+    if (a.t <= 8)
+        route_tokens<kWarps>(a, kCols, route, [] {});
+    else
+        read_route(a, kCols, route);
     const int groups = (a.f + kUnits - 1) / kUnits, width = groups * kUnits;
     const int steps = (a.f + kStep - 1) / kStep;  // of a pass
     const int total = steps * *route.passes;
@@ -595,8 +606,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
 #pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i)
         copy_weights(ring + (uint32_t)(i * D::kStage));
-    if (a.t <= 8)
-        pdl_start();
+    pdl_start();
 #pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i)
         copy_hidden(ring + (uint32_t)(i * D::kStage));
@@ -714,56 +724,46 @@ bool few_columns(const MoeArgs& a) {
     return a.t <= 8 || a.t * a.top <= 4 * a.e;
 }
 
-// How many clusters the GPU holds at once, asked again where their size or shared memory is another one
-struct ClustersThatFit {
-    std::atomic<long long> known[64] = {};  // shared memory << 20 | size << 16 | clusters
-    template <class Kernel>
-    int fit(Kernel kernel, int size, int smem) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-            dev = 0;
-        const long long k = known[dev].load(std::memory_order_relaxed);
-        const long long key = (long long)smem << 4 | size;
-        if (k && k >> 16 == key)
-            return (int)(k & 0xffff);
-        umma::ClusterCapacity capacity;
-        const int n = capacity.clusters(kernel, size, kThreads, smem);
-        known[dev].store(key << 16 | n, std::memory_order_relaxed);
-        return n;
-    }
-};
+template <class T>
+cudaError_t launch_route(const MoeArgs& a, cudaStream_t st) {
+    static MostShared shared;
+    auto kernel = moe_route_kernel<T>;
+    shared.ask(kernel);
+    const int cols = few_columns(a) ? 8 : 16;
+    const int x_vectors = ((uintptr_t)a.x & 15) == 0 && a.ldx % Vec<T>::N == 0;
+    static_assert(kMostBuild >= 4 * 16 * kRouteWarps, "a row's maxima lie there");
+    return launch_pdl(Writes{a.hq, a.workspace_bytes}, kernel, dim3((unsigned)a.t + 1), dim3(32 * kRouteWarps),
+                      (size_t)(route_bytes(a.t * a.top, a.e, cols) + kMostBuild), st, a, cols, x_vectors);
+}
 
 template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
 cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
     static MostShared shared;
     static umma::ResidentCtas resident;
-    static ClustersThatFit clusters;
     auto kernel = moe_up_kernel<T, COLS, DEPTH, CTAS, ALIGNED>;
     const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     shared.ask(kernel);
-    const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx % Vec<T>::N == 0);
+    const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx * sizeof(T) % 16 == 0);
     const long long tiles = (long long)a.t * a.top * ((a.f + kUnits - 1) / kUnits);  // at most
     const Writes writes{a.hq, a.workspace_bytes};
-    // clusters of four for the routing of many tokens (whole clusters live inside a GPC: eight would leave SMs idle)
-    const int cluster = a.t <= 2 * kWarps ? 1 : a.t <= 4 * kWarps ? 2 : 4;
-    const long long fit = cluster == 1 ? (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0)
-                                       : (long long)cluster * clusters.fit(kernel, cluster, smem);
-    const long long some = fit > 0 ? fit : cluster;
-    const long long ctas = tiles < some ? (tiles + cluster - 1) / cluster * cluster : some;
-    return launch_pdl_cluster(writes, kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, cluster, st, a,
-                              x_vectors, cluster);
+    const long long fit = (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0);
+    const long long ctas = tiles < fit || fit <= 0 ? (tiles < 512 ? tiles : 512) : fit;
+    return launch_pdl(writes, kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, st, a, x_vectors);
 }
 template <class T>
 cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
     const bool aligned = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
     if (a.t <= 8)
         return aligned ? launch_up_as<T, 8, 3, 3, true>(a, st) : launch_up_as<T, 8, 3, 3, false>(a, st);
+    const cudaError_t e = launch_route<T>(a, st);
+    if (e != cudaSuccess)
+        return e;
     if (few_columns(a))
-        return aligned ? launch_up_as<T, 8, 4, 2, true>(a, st) : launch_up_as<T, 8, 4, 2, false>(a, st);
-    return aligned ? launch_up_as<T, 16, 4, 2, true>(a, st) : launch_up_as<T, 16, 4, 2, false>(a, st);
+        return aligned ? launch_up_as<int8_t, 8, 4, 2, true>(a, st) : launch_up_as<int8_t, 8, 4, 2, false>(a, st);
+    return aligned ? launch_up_as<int8_t, 16, 4, 2, true>(a, st) : launch_up_as<int8_t, 16, 4, 2, false>(a, st);
 }
 
 template <int NT, int DEPTH, int CTAS, bool ALIGNED>

@@ -40,7 +40,10 @@ struct MoeArgs {
     // the hidden layer: [slots][f rounded up to 32] whole numbers, [slots][f / 32 rounded up] scales
     int8_t* hq;
     float* sh;
-    uint4* route;  // the first kernel's routing, for the second (more than eight tokens)
+    // more than eight tokens: their routing, and they as whole numbers in rows of xs_pitch(d), with their scales
+    uint4* route;
+    int8_t* xq;
+    float* sx;
     size_t workspace_bytes;
 };
 

@@ -120,9 +120,16 @@ size_t moe_hidden_bytes(const mb200_moe_param* p) {  // whole numbers of the hid
 size_t moe_scale_bytes(const mb200_moe_param* p) {  // and their groups' scales
     return align_up((size_t)p->tokens * p->top_k * (align_up((size_t)p->f, 32) / 32) * sizeof(float), 256);
 }
+size_t moe_route_bytes(const mb200_moe_param* p) {
+    return align_up((size_t)route_bytes(p->tokens * p->top_k, p->experts, 8), 256);
+}
+// the tokens as whole numbers, where a kernel of their own makes them, and their scales behind
+size_t moe_token_bytes(const mb200_moe_param* p) {
+    return p->tokens <= 8 ? 0 : (size_t)p->tokens * (size_t)xs_pitch(p->d);
+}
 size_t moe_bytes(const mb200_moe_param* p) {
-    return moe_hidden_bytes(p) + moe_scale_bytes(p) +
-           align_up((size_t)route_bytes(p->tokens * p->top_k, p->experts, 8), 256);
+    return moe_hidden_bytes(p) + moe_scale_bytes(p) + moe_route_bytes(p) + moe_token_bytes(p) +
+           (p->tokens <= 8 ? 0 : 256);
 }
 
 }  // namespace
@@ -282,6 +289,8 @@ int mb200_moe_s8(
     a.y = y, a.ldy = ldy;
     a.hq = (int8_t*)workspace, a.sh = (float*)((uint8_t*)workspace + moe_hidden_bytes(p));
     a.route = (uint4*)((uint8_t*)a.sh + moe_scale_bytes(p));
+    a.xq = (int8_t*)a.route + moe_route_bytes(p);
+    a.sx = (float*)(a.xq + moe_token_bytes(p));
     a.workspace_bytes = moe_bytes(p);
     return launch_moe(a, (cudaStream_t)stream);
 }

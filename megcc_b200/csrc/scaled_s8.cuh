@@ -196,6 +196,10 @@ __device__ __forceinline__ void mma_64(int (&c)[4], const uint4& lo, const uint4
     mma_16x8x32(c, lo.z, hi.z, lo.w, hi.w, t.z, t.w);
 }
 
+// bytes between rows of whole numbers that are to lie in shared memory: whole steps, and two rows on other banks
+__host__ __device__ constexpr int xs_pitch(int k) {
+    return (k + 127) / 128 * 128 + 64;
+}
 __device__ __forceinline__ uint4 pack_piece(const float (&v)[16], const RowScale& r) {
     uint4 q;
     q.x = pack_whole(v[0], v[1], v[2], v[3], r.inv) & r.keep;

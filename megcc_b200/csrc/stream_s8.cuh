@@ -268,10 +268,6 @@ __device__ __forceinline__ void ask_ahead(const void* p, int bytes) {
     for (int at = threadIdx.x * 128; at < end; at += THREADS * 128)
         asm volatile("prefetch.global.L1 [%0];" ::"l"(first + at));
 }
-// bytes between rows of xs: whole steps, and two rows on other banks
-__host__ __device__ constexpr int xs_pitch(int k) {
-    return (k + 127) / 128 * 128 + 64;
-}
 
 }  // namespace scaled
 }  // namespace mb200
