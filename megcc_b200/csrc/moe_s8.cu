@@ -398,6 +398,27 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
         next_stage<kDepth, U::W::kBytes>(stage_in, ring);
         copy_commit();
     };
+    // tokens of a pass that are whole numbers already (all tokens, where they stay), a warp per row
+    auto each_token = [&](int p, auto copy) {
+        const int rows = resident ? a.t : route.pass_cols[p];
+#pragma unroll 1
+        for (int c = warp; c < rows; c += kWarps) {
+            const int t = resident ? c : route.order[route.pass_start[p] + c] >> 16;
+            copy((uint4*)(xs + c * pitch), (const uint4*)(a.xq + (size_t)t * pitch), x_scale + c, a.sx + t);
+        }
+    };
+    if constexpr (!kFew) {
+        // (the first ones ahead of the weights)
+        each_token(first / blocks, [&](uint4* to, const uint4* from, float* to_scale, const float* scale) {
+            const uint32_t at = shared_address(to);
+#pragma unroll 4
+            for (int i = lane; i < pitch / 16; i += 32)
+                copy_async16(at + 16 * i, from + i);
+            if (lane == 0)
+                copy_async4(shared_address(to_scale), scale);
+        });
+        copy_commit();
+    }
 #pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i)
         copy_next();
@@ -416,19 +437,18 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
                     rows_to_whole<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
                     __syncthreads();
                 }
-            } else if (!resident || tile == first) {
+            } else if (tile == first) {
+                copy_wait<kDepth - 1>();
+                __syncthreads();
+            } else if (!resident) {
                 __syncthreads();  // (all warps are done with the last pass's tokens)
-                const int rows = resident ? a.t : cols;
-#pragma unroll 1
-                for (int c = warp; c < rows; c += kWarps) {
-                    const int t = resident ? c : order[c] >> 16;
-                    const uint4* from = (const uint4*)(a.xq + (size_t)t * pitch);
+                each_token(pass, [&](uint4* to, const uint4* from, float* to_scale, const float* scale) {
 #pragma unroll 8
                     for (int i = lane; i < pitch / 16; i += 32)
-                        ((uint4*)(xs + c * pitch))[i] = from[i];
+                        to[i] = from[i];
                     if (lane == 0)
-                        x_scale[c] = a.sx[t];
-                }
+                        *to_scale = *scale;
+                });
                 __syncthreads();
             }
         }
