@@ -300,7 +300,7 @@ MB200_API int mb200_quantize_rows_s8(
  * fp32, in this order, and rounded to `dtype` once. b_packed: [n][k], the layout mb200_matmul_pack_b makes and
  * most weights have. bias may be NULL.
  * workspace: mb200_matmul_s8_scaled_workspace_bytes of the same operands, 256-byte aligned device memory;
- * 0 bytes (and NULL) where rows of a and b_packed are whole 16-byte units or there are few of a. */
+ * operands whose rows are no whole 16-byte units may be laid out anew there; 0 bytes (and NULL) for others. */
 MB200_API size_t mb200_matmul_s8_scaled_workspace_bytes(
         int m, int n, int k, const int8_t* a, long long lda, const int8_t* b_packed);
 MB200_API int mb200_matmul_s8_scaled(
@@ -316,7 +316,7 @@ MB200_API int mb200_linear_s8(
         const float* b_scales, const float* bias, void* y, long long ldy, void* workspace,
         size_t workspace_bytes, void* stream);
 
-/* A mixture-of-experts layer for a few tokens, in two kernels. For each of `tokens` rows x[t] (d elements) and its
+/* A mixture-of-experts layer for a few tokens, in two or three kernels. For each of `tokens` rows x[t] (d elements) and its
  * logits[t] ([tokens][experts] fp32, contiguous; the router's product is the caller's, mb200_matmul_f32 for
  * instance):
  *   p = softmax over all experts; the top_k largest logits are chosen (ties: the lowest index), their p divided

@@ -1,5 +1,5 @@
-// A mixture-of-experts layer for a few tokens, experts in int8: two kernels for up to eight tokens, three for more, no
-// exchange between CTAs but what one kernel writes and the next ones read (and a cluster's sums in the last).
+// A mixture-of-experts layer for a few tokens, experts in int8: two kernels for up to four tokens, three for more,
+// no exchange between CTAs but what one kernel writes and the next ones read (and a cluster's sums in the last).
 //
 //   p[t][e] = softmax(logits[t]) over all experts; token t goes to the top_k largest (ties: the lowest
 //             index), with p as it is or divided by the sum of the chosen
@@ -13,9 +13,10 @@
 // HBM: the chosen experts' weights, 3 * d * f bytes each, are read once and everything else is small, so
 // both kernels stream them through rings of asynchronous copies into mma.sync (stream_s8.cuh), over the ends of
 // rows, experts and tiles.
-// Up to eight tokens every CTA of either kernel works the routing out for itself, a token per warp. More are routed
-// and made whole numbers by a kernel in front, whose results both of the others read (the last one ahead of the end of
-// the second): 10 tokens, two of 45 experts of 1920 x 800: PLACEHOLDER.
+// Up to four tokens every CTA of either kernel works the routing out for itself, a token per warp, while its other
+// warps make the tokens whole numbers. More are routed and made whole numbers by a kernel in front, whose results both of
+// the others read, the last one ahead of the end of the second. Two of 45 experts of 1920 x 800, by each CTA and by a
+// kernel in front: 10 tokens 26.9 and 23.9 us, five 21.9 and 19.2, four 17.2 and 17.8, two 11.8 and 13.0.
 #include "moe_s8.h"
 #include "stream_s8.cuh"
 #include "umma_ptx.cuh"
@@ -184,8 +185,8 @@ __device__ __noinline__ Choices<N> choose_experts(
 }
 
 // A warp for a token or two in turn (each a chain of 2 us or more); then the slots by expert, cut into passes of
-// at most `cols`. Barriers of the CTA stand before and behind. With four tokens at most the upper half of the warps has
-// none and calls meanwhile().
+// at most `cols`. Barriers of the CTA stand before and behind. Warps that have no token, with kMoeFew at most, call
+// meanwhile().
 template <int WARPS, class Meanwhile>
 __device__ __forceinline__ void route_tokens(const MoeArgs& a, int cols, const Route& r, Meanwhile meanwhile) {
     constexpr int kThreads = 32 * WARPS;
@@ -203,11 +204,14 @@ __device__ __forceinline__ void route_tokens(const MoeArgs& a, int cols, const R
         }
     };
     int t = warp;
+    if constexpr (WARPS > kMoeFew * 2) {
 #pragma unroll 1
-    for (; t + stride < a.t; t += 2 * stride) {
-        const Choices<2> c = choose_experts<2>(a.logits + (size_t)t * a.e, (size_t)stride * a.e, a.e, a.top, a.renormalize);
-        keep(t, c.of[0]);
-        keep(t + stride, c.of[1]);
+        for (; t + stride < a.t; t += 2 * stride) {
+            const Choices<2> c =
+                    choose_experts<2>(a.logits + (size_t)t * a.e, (size_t)stride * a.e, a.e, a.top, a.renormalize);
+            keep(t, c.of[0]);
+            keep(t + stride, c.of[1]);
+        }
     }
     if (t < a.t) {
         const Choice c = choose_experts<1>(a.logits + (size_t)t * a.e, 0, a.e, a.top, a.renormalize).of[0];
@@ -225,7 +229,7 @@ __device__ __forceinline__ void route_tokens(const MoeArgs& a, int cols, const R
                 *r.passes = __popc(some);
         }
     }
-    if (a.t <= 4 && warp >= 4)
+    if (a.t <= kMoeFew && warp >= kMoeFew)
         meanwhile();
     __syncthreads();
     if (a.t == 1)
@@ -245,7 +249,8 @@ __device__ __forceinline__ void route_tokens(const MoeArgs& a, int cols, const R
 #pragma unroll 1
         for (int e0 = 0; e0 < a.e; e0 += 32) {
             const int e = e0 + lane;
-            const int n = e < a.e ? __popc(r.tokens[2 * e]) + __popc(r.tokens[2 * e + 1]) : 0, np = (n + cols - 1) / cols;
+            const int n = e < a.e ? __popc(r.tokens[2 * e]) + __popc(r.tokens[2 * e + 1]) : 0;
+            const int np = (n + cols - 1) / cols;
             int sum = np << 16 | n;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -282,7 +287,7 @@ __device__ __forceinline__ void route_tokens(const MoeArgs& a, int cols, const R
     __syncthreads();
 }
 
-// ---- more than eight tokens: the routing, by the first CTA, and a token's whole numbers by each of the others ----
+// ---- more than four tokens: the routing, by the first CTA, and a token's whole numbers by each of the others ----
 // What bounds it is the chain of choices, top_k times two reductions over a warp.
 template <class T>
 __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const MoeArgs a, int cols, int x_vectors) {
@@ -312,7 +317,7 @@ __device__ __forceinline__ void read_route(const MoeArgs& a, int cols, const Rou
 // Tiles of 32 hidden units (64 rows of w1), once per pass of their expert; a CTA takes neighbouring ones. Four
 // of its eight warps have 16 rows each (gate, gate, up, up) and every other step of d, the other four the same rows
 // and the remaining steps; each warp's ring runs on over the ends of tiles. COLS tokens at once; with no more
-// tokens than that all of them stay in shared memory for the whole kernel. T: of the activations, up to eight tokens;
+// tokens than that all of them stay in shared memory for the whole kernel. T: of the activations, up to four tokens;
 // int8_t where they are whole numbers already.
 template <int COLS, int DEPTH, bool ALIGNED>
 struct Up {
@@ -339,22 +344,18 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
     static_assert(U::kRing >= kMostBuild, "the routing is worked out where the rings will be");
     __shared__ float x_scale[COLS];
     constexpr bool kFew = sizeof(T) > 1;
-    __shared__ uint32_t part[kFew ? 16 * kWarps : 1];
+    __shared__ uint32_t part[kFew ? kMoeFew * (kWarps - kMoeFew) : 1];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;
     const bool resident = kFew || a.t <= COLS;
     pdl_start();
-    auto token_row = [&](int t) { return (const T*)a.x + (long long)t * a.ldx; };
     if constexpr (kFew) {
-        // (the logits and tokens are on their way while the routing is worked out)
+        // (the logits are on their way when the routing begins)
         ask_ahead<kThreads>(a.logits, a.t * a.e * 4);
-        if (a.t > 4)
-#pragma unroll 1
-            for (int t = 0; t < a.t; ++t)
-                ask_ahead<kThreads>(token_row(t), a.d * (int)sizeof(T));
         route_tokens<kWarps>(a, COLS, route, [&] {
-            rows_to_whole<T, 4, 4>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
+            rows_to_whole<T, kWarps - kMoeFew, kMoeFew>([&](int t) { return (const T*)a.x + (long long)t * a.ldx; }, a.t,
+                                                        a.d, xs, pitch, x_scale, part, x_vectors);
         });
     } else {
         read_route(a, COLS, route);
@@ -432,24 +433,21 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
             e = route.pass_expert[pass];
             cols = route.pass_cols[pass];
             order = route.order + route.pass_start[pass];
-            if constexpr (kFew) {
-                if (tile == first && a.t > 4) {
-                    rows_to_whole<T, kWarps>(token_row, a.t, a.d, xs, pitch, x_scale, part, x_vectors);
+            if constexpr (!kFew) {
+                if (tile == first) {
+                    copy_wait<kDepth - 1>();
+                    __syncthreads();
+                } else if (!resident) {
+                    __syncthreads();  // (all warps are done with the last pass's tokens)
+                    each_token(pass, [&](uint4* to, const uint4* from, float* to_scale, const float* scale) {
+#pragma unroll 8
+                        for (int i = lane; i < pitch / 16; i += 32)
+                            to[i] = from[i];
+                        if (lane == 0)
+                            *to_scale = *scale;
+                    });
                     __syncthreads();
                 }
-            } else if (tile == first) {
-                copy_wait<kDepth - 1>();
-                __syncthreads();
-            } else if (!resident) {
-                __syncthreads();  // (all warps are done with the last pass's tokens)
-                each_token(pass, [&](uint4* to, const uint4* from, float* to_scale, const float* scale) {
-#pragma unroll 8
-                    for (int i = lane; i < pitch / 16; i += 32)
-                        to[i] = from[i];
-                    if (lane == 0)
-                        *to_scale = *scale;
-                });
-                __syncthreads();
             }
         }
         // scales of the unit that this lane will finish
@@ -462,7 +460,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
             const int c = min(8 * nt + g, cols - 1);
             frag[nt] = xs + (resident ? order[c] >> 16 : c) * pitch + tig * 16;
         }
-        const int s_lo = (int)((uintptr_t)tile_row(pass, b, g) & 15), s_hi = (int)((uintptr_t)tile_row(pass, b, g + 8) & 15);
+        const int s_lo = (int)((uintptr_t)tile_row(pass, b, g) & 15);
+        const int s_hi = (int)((uintptr_t)tile_row(pass, b, g + 8) & 15);
         int acc[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -476,7 +475,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
             next_stage<kDepth, U::W::kBytes>(stage_out, ring);
 #pragma unroll
             for (int j = 0; j < kStep / 64; ++j) {
-                const uint4 lo = U::W::piece16(stage, g, 4 * j + tig, s_lo), hi = U::W::piece16(stage, g + 8, 4 * j + tig, s_hi);
+                const uint4 lo = U::W::piece16(stage, g, 4 * j + tig, s_lo);
+                const uint4 hi = U::W::piece16(stage, g + 8, 4 * j + tig, s_hi);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     mma_64(acc[nt], lo, hi, *(const uint4*)(frag[nt] + (half + i * U::kHalves) * kStep + 64 * j));
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
     const int d0 = (int)blockIdx.x / cluster * kRows;
     // Ahead of the end of the kernel in front: the routing, and with it the first weights. What is read here
     // was written before that kernel began its work, which let this one start behind its own wait for it.
-    if (a.t <= 8)
+    if (a.t <= kMoeFew)
         route_tokens<kWarps>(a, kCols, route, [] {});
     else
         read_route(a, kCols, route);
@@ -657,7 +657,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
         const uint32_t hidden = stage + D::W::kBytes;
 #pragma unroll
         for (int j = 0; j < D::kGroups; ++j) {
-            const uint2 lo = D::W::piece8(stage, g, 4 * j + tig, sh_lo), hi = D::W::piece8(stage, g + 8, 4 * j + tig, sh_hi);
+            const uint2 lo = D::W::piece8(stage, g, 4 * j + tig, sh_lo);
+            const uint2 hi = D::W::piece8(stage, g + 8, 4 * j + tig, sh_hi);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const uint2 q = D::H::piece8(hidden, 8 * nt + g, 4 * j + tig, 0);
@@ -751,7 +752,7 @@ cudaError_t launch_route(const MoeArgs& a, cudaStream_t st) {
     shared.ask(kernel);
     const int cols = few_columns(a) ? 8 : 16;
     const int x_vectors = ((uintptr_t)a.x & 15) == 0 && a.ldx % Vec<T>::N == 0;
-    static_assert(kMostBuild >= 4 * 16 * kRouteWarps, "a row's maxima lie there");
+    static_assert(kMostBuild >= 4 * kRouteWarps, "a row's maxima lie there");
     return launch_pdl(Writes{a.hq, a.workspace_bytes}, kernel, dim3((unsigned)a.t + 1), dim3(32 * kRouteWarps),
                       (size_t)(route_bytes(a.t * a.top, a.e, cols) + kMostBuild), st, a, cols, x_vectors);
 }
@@ -776,11 +777,13 @@ cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
 template <class T>
 cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
     const bool aligned = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
-    if (a.t <= 8)
+    if (a.t <= kMoeFew)
         return aligned ? launch_up_as<T, 8, 3, 3, true>(a, st) : launch_up_as<T, 8, 3, 3, false>(a, st);
     const cudaError_t e = launch_route<T>(a, st);
     if (e != cudaSuccess)
         return e;
+    if (a.t <= 8)
+        return aligned ? launch_up_as<int8_t, 8, 3, 3, true>(a, st) : launch_up_as<int8_t, 8, 3, 3, false>(a, st);
     if (few_columns(a))
         return aligned ? launch_up_as<int8_t, 8, 4, 2, true>(a, st) : launch_up_as<int8_t, 8, 4, 2, false>(a, st);
     return aligned ? launch_up_as<int8_t, 16, 4, 2, true>(a, st) : launch_up_as<int8_t, 16, 4, 2, false>(a, st);

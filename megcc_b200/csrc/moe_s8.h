@@ -17,6 +17,9 @@ constexpr int kMoeMaxTokens = 64, kMoeMaxTop = 16, kMoeMaxExperts = 512;
 // the tokens' whole numbers lie in shared memory: eight rows (sixteen with more than eight tokens)
 constexpr int kMoeMaxDepthFew = 16384, kMoeMaxDepth = 8192;
 
+// up to here every CTA routes all tokens itself
+constexpr int kMoeFew = 4;
+
 // The routing, as the kernels keep it: bytes for `slots` token-expert pairs in passes of `cols` tokens at most
 MB200_HD constexpr int up16(int v) {
     return (v + 15) / 16 * 16;
@@ -40,7 +43,7 @@ struct MoeArgs {
     // the hidden layer: [slots][f rounded up to 32] whole numbers, [slots][f / 32 rounded up] scales
     int8_t* hq;
     float* sh;
-    // more than eight tokens: their routing, and they as whole numbers in rows of xs_pitch(d), with their scales
+    // more than kMoeFew tokens: their routing, and they as whole numbers in rows of xs_pitch(d), with their scales
     uint4* route;
     int8_t* xq;
     float* sx;

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) product_stream_kernel(const Pr
     constexpr int kDepth = S::kDepth, kCols = S::kCols;
     extern __shared__ __align__(128) uint8_t dynamic[];  // the rings, then (floats) xs
     __shared__ float col_scale[kCols];
-    __shared__ uint32_t part[kFloat ? 16 * kWarps : 1];
+    __shared__ uint32_t part[kFloat ? kCols * kWarps : 1];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tig = lane & 3;

@@ -20,7 +20,8 @@ namespace scaled {
 constexpr int kStep = 128;
 
 __device__ __forceinline__ void copy_async16(uint32_t smem, const void* p, bool there) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem), "l"(p), "r"(there ? 16 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem), "l"(p), "r"(there ? 16 : 0)
+                 : "memory");
 }
 __device__ __forceinline__ void copy_async16(uint32_t smem, const void* p) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem), "l"(p) : "memory");
@@ -186,9 +187,9 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
     return make_uint4(cut(v.x, n), cut(v.y, n - 4), cut(v.z, n - 8), cut(v.w, n - 12));
 }
 
-// Rows of activations (up to 16) as whole numbers in shared memory, by the threads of a CTA; zeros behind each row up
+// Rows of activations as whole numbers (in shared memory, or not), by the threads of a CTA; zeros behind each row up
 // to whole steps. WARPS / rows warps (one at least) share a row, so that a few rows' loads are on their way
-// together. row(r): a row's address; part: [16][WARPS] words of shared memory. With FIRST > 0
+// together. row(r): a row's address; part: [rows][WARPS] words of shared memory. With FIRST > 0
 // the warps from FIRST on do it (WARPS of them; barrier 1 is theirs). A barrier of the CTA has to follow before the
 // rows are read. (Loops stay rolled here and in the kernels where their bodies are long: a launch
 // fetches its instructions anew, and 115 KB of them cost the expert kernels 5 us each.)

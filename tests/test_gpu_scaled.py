@@ -119,7 +119,9 @@ SIZES = [(1, 1, 1), (1, 16, 64), (1, 17, 63), (7, 1000, 512), (8, 130, 65), (9, 
          (1000, 999, 333), (1, 5000, 11008), (2, 24, 131071), (1025, 2048, 256), (1, 100, 8000), (8, 64, 9000),
          # short sums of many columns; tiles of 192 and of 128 columns; K split over two, four and eight CTAs
          (2, 12735, 74), (7, 5000, 1024), (20, 9999, 130), (500, 9700, 1024), (256, 9472, 8192), (130, 4200, 1600),
-         (128, 2000, 4096), (100, 200, 6400)]
+         (128, 2000, 4096), (100, 200, 6400),
+         # rows that no 16-byte copies take, of many weights
+         (9, 4100, 2049), (24, 2100, 4097), (16, 9000, 1001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
