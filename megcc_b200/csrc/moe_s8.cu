@@ -740,9 +740,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
 }
 
 // Passes of eight tokens or of sixteen: eight unless an expert has more than that on average (weights that are read
-// twice come from the L2 the second time, and passes of sixteen leave room for one CTA per SM only)
+// twice come from the L2 the second time, and passes of sixteen leave room for one CTA per SM only). 64 tokens, eight of
+// 64 experts of 2048 x 768: by eight 75 us, by sixteen 90; six of 24 of 1928 x 808: 82 and 68.
 bool few_columns(const MoeArgs& a) {
-    return a.t <= 8 || a.t * a.top <= 4 * a.e;
+    return a.t <= 8 || a.t * a.top <= 8 * a.e;
 }
 
 template <class T>
@@ -792,6 +793,7 @@ cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
 template <int NT, int DEPTH, int CTAS, bool ALIGNED>
 cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
     static umma::KernelReady ready;
+    static umma::ResidentCtas resident;
     static MostShared shared;
     auto kernel = moe_down_kernel<NT, DEPTH, CTAS, ALIGNED>;
     const int smem = Down<NT, DEPTH, ALIGNED>::smem(a);
@@ -799,11 +801,13 @@ cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
         return cudaErrorInvalidValue;
     shared.ask(kernel);
     const Writes writes{a.y, ((size_t)(a.t - 1) * (size_t)a.ldy + (size_t)a.d) * dtype_bytes(a.dtype)};
-    // a CTA for every SM where each warp still has two steps (experts with tokens: at most as many as slots)
+    // a CTA for every SM where each warp still has two steps (experts with tokens: at most as many as slots), and all at
+    // once (64 tokens, two of 8 experts of 2048 x 1024: 31 us, 37 with 256 CTAs for 148 places)
     const int tiles = (a.d - 1) / kRows + 1, slots = a.t * a.top;
     const long long steps = (long long)(slots < a.e ? slots : a.e) * ((a.f + kStep - 1) / kStep);
+    const int fit = umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0);
     int cluster = 1;
-    while (cluster < 8 && tiles * cluster < umma::sm_count() && steps >= 2LL * 2 * cluster * kWarps)
+    while (cluster < 8 && tiles * cluster < umma::sm_count() && 2 * tiles * cluster <= fit && steps >= 2LL * 2 * cluster * kWarps)
         cluster *= 2;
     return launch_pdl_cluster(writes, kernel, dim3((unsigned)(tiles * cluster)), dim3(kThreads), (size_t)smem, cluster,
                               st, a, cluster);
