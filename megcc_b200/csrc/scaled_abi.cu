@@ -63,14 +63,15 @@ bool rows_fit(const void* p, int rows, long long ld) {
 }
 // Few rows of activations, or little of everything: the kernel that streams the weights past them, whatever the
 // operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles): 17 rows 1024 x 1024 1.9 / 5.2,
-// 4096 x 4096 4.4 / 7.0, 4096 x 14336 14.3 / 13.6; 16 rows 4096 x 14336 10.7 / 13.6, 14336 x 4096 13.8 / 12.7,
-// 32768 x 2048 17.8 / 13.3: tiles of whole K win where they are enough for the SMs, or where tokens weigh as much as
-// weights.
+// 4096 x 4096 4.4 / 7.0, 4096 x 14336 14.3 / 13.6; 16 rows 4096 x 14336 10.7 / 13.6, 14336 x 4096 14.4 / 13.7,
+// 32768 x 4096 25.6 / 22.5, 9600 x 4096 10.7 / 11.5, 16384 x 16384 47.3 / 48.8; one row 16384 x 16384 42.2 / 47.2, 65536 x
+// 1024 12.0 / 24.2: tiles of whole K win where they are enough for the SMs and K is neither short (a tile is all start
+// and end then) nor long, or where tokens weigh as much as weights.
 // `fits`: the tiles' operands need no copies (4100 x 4100, 32 rows: 13.7 / 15.4).
 bool streams(int m, int n, int k, bool fits) {
     const long long weights = (long long)n * k, many = 1 << 25;
     if (m <= 16)
-        return !fits || weights <= many || n < 74 * 128;
+        return !fits || weights <= many || k > 4096 || n < 96 * 128 || k <= 1024 || (k <= 2048 && k % 128 == 0);
     if (m <= 32)
         return !fits || weights <= many;
     // a pass over the weights per 32 rows, in no more CTAs than the SMs hold at once

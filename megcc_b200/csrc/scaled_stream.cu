@@ -365,9 +365,13 @@ cudaError_t launch_stream_as(const ProductArgs& a, int x_vectors, cudaStream_t s
 }
 template <class XT, int NT, bool ALIGNED, bool TOKENS>
 cudaError_t launch_stream(const ProductArgs& a, int x_vectors, cudaStream_t st) {
-    // warps of their own where shared tiles would take several turns on the SMs for a step or two per warp
+    // Warps of their own where shared tiles would take several turns on the SMs for a step or two per warp, or up to 2048
+    // bytes where rows are whole lines and there are enough for all SMs (20000 x 2048, one token: 9.0 us, by tiles 19.2;
+    // with lines that two steps share, 8 x 20000 x 1552, 14.4 to 17.3 us for the shared form's 12.2)
     const long long ctas = ((long long)(a.n - 1) / kRows + 1) * ((a.m - 1) / (8 * NT) + 1);
-    if (a.k <= 8 * kStep && ctas > 2LL * umma::sm_count())
+    const long long own = ((long long)(a.n - 1) / (kRows * kWarps) + 1) * ((a.m - 1) / (8 * NT) + 1);
+    if ((a.k <= 8 * kStep && ctas > 2LL * umma::sm_count()) ||
+        (a.k <= 16 * kStep && a.k % kStep == 0 && own >= umma::sm_count()))
         return launch_stream_as<XT, NT, ALIGNED, TOKENS, false>(a, x_vectors, st);
     return launch_stream_as<XT, NT, ALIGNED, TOKENS, true>(a, x_vectors, st);
 }
