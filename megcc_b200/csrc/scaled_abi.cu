@@ -62,18 +62,26 @@ bool rows_fit(const void* p, int rows, long long ld) {
     return !misaligned(p, 16) && (rows == 1 || ld % 16 == 0);
 }
 // Few rows of activations, or little of everything: the kernel that streams the weights past them, whatever the
-// operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles): 17 rows 1024 x 1024 1.9 / 5.2,
-// 4096 x 4096 4.4 / 7.0, 4096 x 14336 14.3 / 13.6; 16 rows 4096 x 14336 10.7 / 13.6, 14336 x 4096 14.4 / 13.7,
-// 32768 x 4096 25.6 / 22.5, 9600 x 4096 10.7 / 11.5, 16384 x 16384 47.3 / 48.8; one row 16384 x 16384 42.2 / 47.2, 65536 x
-// 1024 12.0 / 24.2: tiles of whole K win where they are enough for the SMs and K is neither short (a tile is all start
-// and end then) nor long, or where tokens weigh as much as weights.
-// `fits`: the tiles' operands need no copies (4100 x 4100, 32 rows: 13.7 / 15.4).
+// operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles), n x k:
+//   one row     16384 x 16384 42.2 / 47.2, 65536 x 1024 12.0 / 24.2, 20000 x 2048 9.0 / 11.2
+//   four        16384 x 2048 9.2 / 7.4, 10000 x 1008 5.5 / 4.6, 16384 x 1024 3.4 / 4.3, 6144 x 4096 5.6 / 7.3
+//   sixteen     16384 x 2048 10.1 / 7.4, 10000 x 1536 5.8 / 5.2, 14336 x 4096 14.4 / 13.7, 4096 x 8192 6.8 / 9.9
+//   24          4096 x 4096 6.1 / 9.2, 6144 x 4096 7.3 / 7.6, 8192 x 4096 10.3 / 9.3, 6000 x 1024 5.4 / 4.2
+// Warps of the streaming kernel share K (launch_stream): short K costs them starts and ends, unless each has
+// rows of its own, which wants whole lines. Tiles want many columns, enough for all SMs without cutting K.
+// `fits`: the tiles' operands need no copies (4100 x 4100, 24 rows: 11.5 / 15.5).
 bool streams(int m, int n, int k, bool fits) {
-    const long long weights = (long long)n * k, many = 1 << 25;
-    if (m <= 16)
-        return !fits || weights <= many || k > 4096 || n < 96 * 128 || k <= 1024 || (k <= 2048 && k % 128 == 0);
+    const long long weights = (long long)n * k;
+    if (m <= 32 && !fits)
+        return true;
+    if (m <= 16) {
+        const bool lines = k % 128 == 0;
+        if (k <= 1024)
+            return lines || k <= 512 || n < 8192;
+        return k > 4096 || n < 88 * 128 || (k <= 2048 && lines && n >= 148 * 128);
+    }
     if (m <= 32)
-        return !fits || weights <= many;
+        return weights <= 1 << 22 || (weights <= 1 << 25 && (n < 4800 || (n < 8192 && k > 1024)));
     // a pass over the weights per 32 rows, in no more CTAs than the SMs hold at once
     const long long passes = ((long long)m + 31) / 32;
     return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= 2 * 148;
@@ -85,7 +93,7 @@ bool streams_activations(int m, int k) {
 // int8 tokens that no 16-byte copies take are laid out anew in front of many weights, by which each CTA would shift them
 // into place again: 24 x 11008 x 4097 24.9 us, 38.2 so
 bool lays_out_tokens(int m, int n, int k, const int8_t* a, long long lda) {
-    return m > 8 && (long long)n * k >= 1 << 23 && !rows_fit(a, m, lda);
+    return m > 8 && (long long)n * k >= 1 << 22 && !rows_fit(a, m, lda);
 }
 // (whole lines: 128 bytes of K then come as one line of the L2, not as parts of two)
 long long padded(int k) {

@@ -875,8 +875,11 @@ Choice choose(const UmmaArgs& p, int sms, Fit clusters_that_fit) {
     for (int split = 1; split <= 8; split *= 2) {
         if (split > steps || (split > 1 && tiles > clusters_that_fit(split)))
             break;
-        const long long waves = (tiles * split + sms - 1) / sms;
-        const long long t = waves * ((steps + split - 1) / split * 512 + 2500) + (split > 1 ? 5500 : 1000);
+        // one row of tiles reads its weights once: HBM bounds, not the SM that has a tile more (149 tiles of K = 2048 as
+        // pairs in two turns 16.7 us, 11.2 so)
+        const long long ctas = tiles * split;
+        const long long turns16 = p.m <= kBM && split == 1 && ctas > sms ? 16 * ctas / sms + 1 : (ctas + sms - 1) / sms * 16;
+        const long long t = turns16 * ((steps + split - 1) / split * 512 + 2500) / 16 + (split > 1 ? 5500 : 1000);
         if (t < best) {
             best = t;
             c = {false, kSplitBN, split};
