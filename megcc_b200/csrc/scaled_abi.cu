@@ -82,9 +82,10 @@ bool streams(int m, int n, int k, bool fits) {
     }
     if (m <= 32)
         return weights <= 1 << 22 || (weights <= 1 << 25 && (n < 4800 || (n < 8192 && k > 1024)));
-    // a pass over the weights per 32 rows, in no more CTAs than the SMs hold at once
+    // A pass over the weights per 32 rows, in no more CTAs than the SMs hold at once, or twice as many where the tiles
+    // would need a launch more, for copies (148 x 1614 x 66: 6.0 / 7.8)
     const long long passes = ((long long)m + 31) / 32;
-    return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= 2 * 148;
+    return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= (fits ? 2 : 4) * 148;
 }
 // So few that it makes whole numbers of them itself, every CTA again
 bool streams_activations(int m, int k) {

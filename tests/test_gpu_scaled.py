@@ -121,7 +121,9 @@ SIZES = [(1, 1, 1), (1, 16, 64), (1, 17, 63), (7, 1000, 512), (8, 130, 65), (9, 
          (2, 12735, 74), (7, 5000, 1024), (20, 9999, 130), (500, 9700, 1024), (256, 9472, 8192), (130, 4200, 1600),
          (128, 2000, 4096), (100, 200, 6400),
          # rows that no 16-byte copies take, of many weights
-         (9, 4100, 2049), (24, 2100, 4097), (16, 9000, 1001)]
+         (9, 4100, 2049), (24, 2100, 4097), (16, 9000, 1001), (148, 1614, 66), (300, 900, 201),
+         # one row of tiles on more CTAs than SMs
+         (70, 19072, 640), (3, 20000, 1280), (16, 40000, 1152)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
