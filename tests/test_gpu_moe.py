@@ -82,6 +82,9 @@ def test_moe_of_wide_layers():
     check(layer(1, 4096, 1536, 16, 1), 8, True)
     check(layer(2, 16384, 64, 3, 2), 2, True)
     check(layer(10, 8192, 40, 3, 3), 1, False)
+    check(layer(8, 16384, 40, 4, 6, torch.float32), 2, False)
+    check(layer(5, 16383, 33, 3, 7), 3, True)
+    check(layer(64, 8191, 32, 2, 8), 2, True)
     check(layer(4, 48, 5000, 3, 4), 2, True)
     check(layer(3, 64, 32, 512, 5), 16, True)
 
