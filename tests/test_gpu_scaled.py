@@ -122,6 +122,8 @@ SIZES = [(1, 1, 1), (1, 16, 64), (1, 17, 63), (7, 1000, 512), (8, 130, 65), (9, 
          (128, 2000, 4096), (100, 200, 6400),
          # rows that no 16-byte copies take, of many weights
          (9, 4100, 2049), (24, 2100, 4097), (16, 9000, 1001), (148, 1614, 66), (300, 900, 201),
+         # tiles of several turns, the last one partly filled
+         (4001, 4000, 300), (3900, 3850, 208),
          # one row of tiles on more CTAs than SMs
          (70, 19072, 640), (3, 20000, 1280), (16, 40000, 1152)]
 
