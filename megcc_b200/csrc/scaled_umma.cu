@@ -3,7 +3,7 @@
 // Both operands are K-major, 128 bytes of K per pipeline stage, brought by tiled TMA loads with the
 // 128-byte swizzle; sums stay exact in int32 in tensor memory. The epilogue multiplies by the two scales in
 // fp32, adds the bias, rounds once and turns the tile round in shared memory, 64 bytes of 32 rows at a time, from where
-// the TMA stores it (or, where rows of the result are no whole 16-byte units, the warp).
+// the TMA stores it (or, where rows of the result do not begin and end with 16-byte units, the warp).
 //
 // Two kernels:
 //   pair   256 x 256 tiles (or x 192, x 128, where those come out even) on pairs of SMs (cta_group::2), persistent, two
@@ -38,7 +38,10 @@ struct UmmaArgs {
     const float *sa, *sb, *bias;
     void* c;
     long long ldc;
-    int vector_stores;  // rows of c are whole 16-byte units
+    int vector_stores;  // rows of c begin at 16-byte units
+    // pair: and end with one, so that the TMA may store them: it writes whole units, over what stands behind a row's last
+    // element within its unit
+    int tma_stores;
     int b_early;
     int bn;          // pair: columns of a tile, 256, 192 or 128
     // split:
@@ -481,7 +484,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pro
             Sides sides;
             sides.take(row_scale, col_scale + quarter * 64, col_bias + quarter * 64, p.bias != nullptr);
             store_columns<T>(taddr + (uint32_t)(quarter * 64), sides, p.bias != nullptr, stage, row0, n0 + quarter * 64, p,
-                             p.vector_stores ? &map_c : nullptr, [&] {
+                             p.tma_stores ? &map_c : nullptr, [&] {
                                  // this warp's sums are in registers: one arrival on the leader's barrier
                                  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                                  __syncwarp();
@@ -911,8 +914,9 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
         int rc = encode(&map_a, a.a, a.k, a.m, a.lda, kBM);
         if (!rc)
             rc = encode(&map_b, a.b, a.k, a.n, a.ldb, p.bn / 2);
-        CUtensorMap map_c = map_b;  // (not used where rows of c are no whole 16-byte units)
-        if (!rc && p.vector_stores)
+        CUtensorMap map_c = map_b;  // (not used where the TMA does not store)
+        p.tma_stores = p.vector_stores && (size_t)a.n * sizeof(T) % 16 == 0;
+        if (!rc && p.tma_stores)
             rc = encode_as(&map_c,
                            a.c_dtype == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                            : a.c_dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
