@@ -31,6 +31,8 @@ constexpr int kRouteWarps = 32;       // of the kernel in front
 constexpr int kUnits = 32;            // hidden units per tile of the first kernel, and per group of h
 constexpr int kPitch = 2 * kUnits + 4;  // ints per token in its exchange: 2 * 68 = 8 banks apart
 constexpr int kRows = 16;             // rows of w2 per CTA of the second kernel
+// dynamic shared memory that a CTA may ask for (227 KB less what the kernels declare themselves, 128 bytes)
+constexpr int kMostDynamic = 227 * 1024 - 128;
 
 // Where the tokens go, in shared memory: as large as the call's tokens and experts ask for.
 struct Route {
@@ -326,11 +328,14 @@ struct Up {
     typedef Rows<16, ALIGNED, (DEPTH > 3)> W;
     static constexpr int kRing = kWarps * kDepth * W::kBytes;
     static constexpr int kExchange = kHalves * COLS * kPitch;  // ints; two of them, used in turn
-    static int smem(const MoeArgs& a) {
-        return kRing + 2 * kExchange * 4 + (a.t < COLS ? a.t : COLS) * xs_pitch(a.d) +
-               route_bytes(a.t * a.top, a.e, COLS);
+    static constexpr int smem(int t, int d, int top, int e) {
+        return kRing + 2 * kExchange * 4 + (t < COLS ? t : COLS) * xs_pitch(d) + route_bytes(t * top, e, COLS);
     }
 };
+static_assert(Up<8, 3, false>::smem(8, kMoeMaxDepthFew, kMoeMaxTop, kMoeMaxExperts) <= kMostDynamic &&
+                      Up<8, 4, false>::smem(kMoeMaxTokens, kMoeMaxDepth, kMoeMaxTop, kMoeMaxExperts) <= kMostDynamic &&
+                      Up<16, 4, true>::smem(kMoeMaxTokens, kMoeMaxDepth, kMoeMaxTop, kMoeMaxExperts) <= kMostDynamic,
+              "every layer that is accepted has room (sixteen columns of rows at odd places: few_columns)");
 
 template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a, int x_vectors) {
@@ -530,10 +535,13 @@ struct Down {
     static constexpr int kScales = kGroups * 8 * NT * 4;
     static constexpr int kStage = W::kBytes + H::kBytes + kScales;
     static constexpr int kRing = kWarps * kDepth * kStage;
-    static int smem(const MoeArgs& a) {
-        return kRing + kWarps * a.t * kRows * 4 + route_bytes(a.t * a.top, a.e, 8 * NT);
+    static constexpr int smem(int t, int top, int e) {
+        return kRing + kWarps * t * kRows * 4 + route_bytes(t * top, e, 8 * NT);
     }
 };
+static_assert(Down<1, 3, false>::smem(kMoeMaxTokens, kMoeMaxTop, kMoeMaxExperts) <= kMostDynamic &&
+                      Down<2, 3, false>::smem(kMoeMaxTokens, kMoeMaxTop, kMoeMaxExperts) <= kMostDynamic,
+              "every layer that is accepted has room");
 
 template <int NT, int DEPTH, int CTAS, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs a, int cluster) {
@@ -741,9 +749,15 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_down_kernel(const MoeArgs 
 
 // Passes of eight tokens or of sixteen: eight unless an expert has more than that on average (weights that are read
 // twice come from the L2 the second time, and passes of sixteen leave room for one CTA per SM only). 64 tokens, eight of
-// 64 experts of 2048 x 768: by eight 75 us, by sixteen 90; six of 24 of 1928 x 808: 82 and 68.
+// 64 experts of 2048 x 768: by eight 75 us, by sixteen 90; six of 24 of 1928 x 808: 82 and 68. And eight where sixteen rows
+// of tokens leave no room for the rings of weights at odd places and the routing (62 to 64 tokens, 16 of 81 to 127 experts,
+// d > 8064). All kernels of a call go by this.
+bool first_aligned(const MoeArgs& a) {
+    return ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
+}
 bool few_columns(const MoeArgs& a) {
-    return a.t <= 8 || a.t * a.top <= 8 * a.e;
+    return a.t <= 8 || a.t * a.top <= 8 * a.e ||
+           (!first_aligned(a) && Up<16, 4, false>::smem(a.t, a.d, a.top, a.e) > kMostDynamic);
 }
 
 template <class T>
@@ -764,7 +778,7 @@ cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     static MostShared shared;
     static umma::ResidentCtas resident;
     auto kernel = moe_up_kernel<T, COLS, DEPTH, CTAS, ALIGNED>;
-    const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a);
+    const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a.t, a.d, a.top, a.e);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     shared.ask(kernel);
@@ -777,7 +791,7 @@ cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
 }
 template <class T>
 cudaError_t launch_up(const MoeArgs& a, cudaStream_t st) {
-    const bool aligned = ((uintptr_t)a.w1 & 15) == 0 && a.d % 16 == 0;
+    const bool aligned = first_aligned(a);
     if (a.t <= kMoeFew)
         return aligned ? launch_up_as<T, 8, 3, 3, true>(a, st) : launch_up_as<T, 8, 3, 3, false>(a, st);
     const cudaError_t e = launch_route<T>(a, st);
@@ -796,7 +810,7 @@ cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
     static umma::ResidentCtas resident;
     static MostShared shared;
     auto kernel = moe_down_kernel<NT, DEPTH, CTAS, ALIGNED>;
-    const int smem = Down<NT, DEPTH, ALIGNED>::smem(a);
+    const int smem = Down<NT, DEPTH, ALIGNED>::smem(a.t, a.top, a.e);
     if (!ready.smem(kernel, smem))
         return cudaErrorInvalidValue;
     shared.ask(kernel);
