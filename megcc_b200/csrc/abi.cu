@@ -31,6 +31,11 @@ int check_launch(const char* what) {
     return ST_SUCCESS;
 }
 
+int refused(const char* what, cudaError_t e) {
+    cudaGetLastError();
+    return set_error(ST_RUNTIME, "%s: %s", what, cudaGetErrorString(e));
+}
+
 // One status word per (device, stream): a kernel whose bounded wait runs out records its
 // code in the word of the stream it was launched on, so that a network waiting on its own
 // stream never consumes another network's error. The words are mapped page-locked host memory:
@@ -58,7 +63,7 @@ int* device_status_word(cudaStream_t st) {
     static std::mutex mu;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-        set_error(ST_RUNTIME, "no current CUDA device");
+        refused("no current CUDA device", cudaPeekAtLastError());
         return nullptr;
     }
     std::lock_guard<std::mutex> lock(mu);

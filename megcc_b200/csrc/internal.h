@@ -77,6 +77,9 @@ size_t align_up(size_t v, size_t a);
 int set_error(int code, const char* fmt, ...);
 // cudaGetLastError() after a launch -> status
 int check_launch(const char* what);
+// status of a call that the runtime refused with `e`. The runtime's own record of it is taken with it, or the next call's
+// check_launch, or another library's, would find it there.
+int refused(const char* what, cudaError_t e);
 // the int that kernels launched on `st` set when a bounded wait runs out (one per device
 // and stream, see abi.cu)
 int* device_status_word(cudaStream_t st);

@@ -780,7 +780,7 @@ cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     auto kernel = moe_up_kernel<T, COLS, DEPTH, CTAS, ALIGNED>;
     const int smem = Up<COLS, DEPTH, ALIGNED>::smem(a.t, a.d, a.top, a.e);
     if (!ready.smem(kernel, smem))
-        return cudaErrorInvalidValue;
+        return why_refused();
     shared.ask(kernel);
     const int x_vectors = ((uintptr_t)a.x & 15) == 0 && (a.t == 1 || a.ldx * sizeof(T) % 16 == 0);
     const long long tiles = (long long)a.t * a.top * ((a.f + kUnits - 1) / kUnits);  // at most
@@ -812,7 +812,7 @@ cudaError_t launch_down_as(const MoeArgs& a, cudaStream_t st) {
     auto kernel = moe_down_kernel<NT, DEPTH, CTAS, ALIGNED>;
     const int smem = Down<NT, DEPTH, ALIGNED>::smem(a.t, a.top, a.e);
     if (!ready.smem(kernel, smem))
-        return cudaErrorInvalidValue;
+        return why_refused();
     shared.ask(kernel);
     const Writes writes{a.y, ((size_t)(a.t - 1) * (size_t)a.ldy + (size_t)a.d) * dtype_bytes(a.dtype)};
     // a CTA for every SM where each warp still has two steps (experts with tokens: at most as many as slots), and all at
@@ -849,7 +849,7 @@ int launch_moe(const MoeArgs& a, cudaStream_t st) {
                           : a.dtype == DT_F16 ? launch_both<__half>(a, st)
                                               : launch_both<__nv_bfloat16>(a, st);
     if (e != cudaSuccess)
-        return set_error(ST_RUNTIME, "moe_s8: %s", cudaGetErrorString(e));
+        return refused("moe_s8", e);
     return check_launch("moe_s8");
 }
 

@@ -211,6 +211,12 @@ __device__ __forceinline__ uint4 pack_piece(const float (&v)[16], const RowScale
 
 #endif  // __CUDACC__
 
+// Behind a call of the runtime that has failed
+inline cudaError_t why_refused() {
+    const cudaError_t e = cudaPeekAtLastError();
+    return e != cudaSuccess ? e : cudaErrorUnknown;
+}
+
 // Kernels that run in turn ask for the same share of an SM's memory as shared memory, all of it: an SM changes the share
 // only when it is empty, so a kernel that asks for more than the one in front cannot begin beside its end.
 struct MostShared {
@@ -221,8 +227,9 @@ struct MostShared {
         if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || done[dev].load(std::memory_order_relaxed))
             return;
         // (a preference: the kernel runs without it as well)
-        (void)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                   cudaSharedmemCarveoutMaxShared);
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+            cudaGetLastError();
         done[dev].store(true, std::memory_order_relaxed);
     }
 };

@@ -172,7 +172,7 @@ int quantize_rows(
             : k <= 256 * 8 * N              ? launch(quantize_rows_kernel<T, 256, 8, 256>, 1, 256, shared[3])
                                             : launch(quantize_rows_kernel<T, 512, 8, 512>, 1, 512, shared[4]);
     if (e != cudaSuccess)
-        return set_error(ST_RUNTIME, "quantize_rows: %s", cudaGetErrorString(e));
+        return refused("quantize_rows", e);
     return check_launch("quantize_rows");
 }
 
@@ -357,7 +357,7 @@ cudaError_t launch_stream_as(const ProductArgs& a, int x_vectors, cudaStream_t s
     auto kernel = product_stream_kernel<XT, NT, ALIGNED, TOKENS, SHARED>;
     const int smem = S::kRing + (S::kFloat ? (a.m < S::kCols ? a.m : S::kCols) * xs_pitch(a.k) : 0);
     if (!ready.smem(kernel, smem))
-        return cudaErrorInvalidValue;
+        return why_refused();
     shared.ask(kernel);
     const dim3 grid((unsigned)((a.n - 1) / S::kCtaRows + 1), (unsigned)((a.m - 1) / S::kCols + 1));
     const Writes writes{a.c, ((size_t)(a.m - 1) * (size_t)a.ldc + (size_t)a.n) * dtype_bytes(a.c_dtype)};
@@ -422,7 +422,7 @@ int launch_pad_rows(const PadRows& a, const PadRows& b, cudaStream_t st) {
                             : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
                                          a, b);
     if (e != cudaSuccess)
-        return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
+        return refused("matmul_s8_scaled", e);
     return check_launch("matmul_s8_scaled");
 }
 
@@ -442,7 +442,7 @@ int launch_product_stream(const ProductArgs& a, cudaStream_t st) {
         e = launch_stream_float<__nv_bfloat16>(a, b_aligned, st);
     }
     if (e != cudaSuccess)
-        return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
+        return refused("matmul_s8_scaled", e);
     return check_launch("matmul_s8_scaled");
 }
 

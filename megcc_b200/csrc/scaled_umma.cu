@@ -953,7 +953,7 @@ int launch(const ProductArgs& a, UmmaArgs p, const Writes& writes, cudaStream_t 
                                (size_t)split_dynamic(p.stages, p.a_bytes, p.csplit), p.csplit, st, map_a, map_b, p);
     }
     if (e != cudaSuccess)
-        return set_error(ST_RUNTIME, "matmul_s8_scaled: %s", cudaGetErrorString(e));
+        return refused("matmul_s8_scaled", e);
     return check_launch("matmul_s8_scaled");
 }
 
