@@ -145,13 +145,17 @@ PyObject* guarded(F f) {
     }
     return nullptr;
 }
+// (an exception on its way to guarded() takes the lock again too)
+struct WithoutGil {
+    PyThreadState* state = PyEval_SaveThread();
+    ~WithoutGil() {
+        PyEval_RestoreThread(state);
+    }
+};
 template <class F>
 int without_gil(F f) {
-    int status;
-    Py_BEGIN_ALLOW_THREADS
-    status = f();
-    Py_END_ALLOW_THREADS
-    return status;
+    const WithoutGil released;
+    return f();
 }
 
 PyObject* quantize_rows_s8(PyObject*, PyObject* const* args, Py_ssize_t n) {
