@@ -4,6 +4,7 @@
 
 The shared objects land next to this file so that they travel with the source tree.
 """
+import importlib.metadata
 import os
 import subprocess
 import sys
@@ -74,17 +75,26 @@ def build_fastcall(verbose=False, force=False):
 
 
 def build_torchcall(verbose=False, force=False):
-    """The extension module of operator calls on tensors (C++ against torch's headers)."""
+    """The extension module of operator calls on tensors (C++ against torch's headers). None, with a line to
+    stderr, where torch or its CUDA part is not installed: all else works without it."""
     src = os.path.join(HERE, "fastcall", "torchcall.cpp")
     deps = [src, os.path.join(os.path.dirname(HERE), "include", "megcc_b200.h")]
-    if not force and not _stale(TORCHCALL, deps):
-        return TORCHCALL
-    import torch  # (its headers and libraries; the rest of the build does without)
-    at = os.path.dirname(torch.__file__)
+    try:
+        version = importlib.metadata.version("torch")
+        made_for = f"made for torch {version}"  # (in the module, where a build for another version is known by it)
+        if not force and not _stale(TORCHCALL, deps) and _holds(TORCHCALL, made_for):
+            return TORCHCALL
+        import torch  # (its headers and libraries)
+    except ImportError:
+        torch = None
+    at = os.path.dirname(torch.__file__) if torch else ""
+    if not torch or not os.path.exists(os.path.join(at, "lib", "libc10_cuda.so")):
+        sys.stderr.write("no torch with CUDA: the operator calls on tensors (_torchcall.so) are not built\n")
+        return None
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else os.environ.get("CXX", "g++")
     cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DMADE_FOR="{made_for}"',
            "-isystem", os.path.join(at, "include"),
            "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
            "-isystem", os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"],
@@ -98,6 +108,11 @@ def build_torchcall(verbose=False, force=False):
     return TORCHCALL
 
 
+def _holds(path, text):
+    with open(path, "rb") as f:
+        return text.encode() + b"\0" in f.read()
+
+
 def _stale(target, deps):
     if not os.path.exists(target):
         return True
@@ -108,7 +123,13 @@ def _stale(target, deps):
 def build(verbose=False, force=False):
     build_compiler(verbose, force)
     build_fastcall(verbose, force)
+    build_library(verbose, force)
     build_torchcall(verbose, force)
+    return LIB
+
+
+def build_library(verbose=False, force=False):
+    """The operator library and runtime."""
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     srcs = _sources()
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]

@@ -293,5 +293,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, methods,
 }  // namespace
 
 PyMODINIT_FUNC PyInit__torchcall(void) {
-    return PyModule_Create(&module);
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "made_for", MADE_FOR) < 0)
+        Py_CLEAR(m);
+    return m;
 }
