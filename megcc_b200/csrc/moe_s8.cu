@@ -337,6 +337,13 @@ static_assert(Up<8, 3, false>::smem(8, kMoeMaxDepthFew, kMoeMaxTop, kMoeMaxExper
                       Up<16, 4, true>::smem(kMoeMaxTokens, kMoeMaxDepth, kMoeMaxTop, kMoeMaxExperts) <= kMostDynamic,
               "every layer that is accepted has room (sixteen columns of rows at odd places: few_columns)");
 
+constexpr int kMostUpCtas = 1024;
+constexpr int kMostTiles =
+        most_passes(kMoeMaxTokens * kMoeMaxTop, kMoeMaxExperts, 8) * ((kMaxK + kUnits - 1) / kUnits);
+static_assert((unsigned long long)kMostTiles * kMostUpCtas <= 0xffffffffull, "tiles are shared out in 32 bits");
+// (the second kernel's: a pass's steps, over the warps of a cluster of eight)
+static_assert((unsigned long long)kMostTiles * 8 * kWarps <= 0xffffffffull, "steps are shared out in 32 bits");
+
 template <class T, int COLS, int DEPTH, int CTAS, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a, int x_vectors) {
     typedef Up<COLS, DEPTH, ALIGNED> U;
@@ -366,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) moe_up_kernel(const MoeArgs a,
         read_route(a, COLS, route);
     }
     const int blocks = (a.f + kUnits - 1) / kUnits;
-    // (1024 slots of 4096 blocks at most, in 1024 CTAs: products that 32 bits hold)
+    // (kMostTiles in kMostUpCtas CTAs at most: products that 32 bits hold)
     const unsigned tiles = (unsigned)(*route.passes * blocks);
     // as few CTAs as still take as many tiles each as the busiest would
     const unsigned each = (tiles + gridDim.x - 1) / gridDim.x, busy = each ? (tiles + each - 1) / each : 1u;
@@ -786,7 +793,8 @@ cudaError_t launch_up_as(const MoeArgs& a, cudaStream_t st) {
     const long long tiles = (long long)a.t * a.top * ((a.f + kUnits - 1) / kUnits);  // at most
     const Writes writes{a.hq, a.workspace_bytes};
     const long long fit = (long long)umma::sm_count() * resident.per_sm(kernel, kThreads, smem, 0);
-    const long long ctas = tiles < fit || fit <= 0 ? (tiles < 512 ? tiles : 512) : fit;
+    const long long most = fit <= 0 ? 512 : fit < kMostUpCtas ? fit : kMostUpCtas;
+    const long long ctas = tiles < most ? tiles : most;
     return launch_pdl(writes, kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, st, a, x_vectors);
 }
 template <class T>
