@@ -2,6 +2,7 @@
 #include "../../include/megcc_b200.h"
 #include "moe_s8.h"
 #include "scaled_s8.cuh"
+#include "umma_ptx.cuh"
 
 using namespace mb200;
 using namespace mb200::scaled;
@@ -71,21 +72,21 @@ bool rows_fit(const void* p, int rows, long long ld) {
 // rows of its own, which wants whole lines. Tiles want many columns, enough for all SMs without cutting K.
 // `fits`: the tiles' operands need no copies (4100 x 4100, 24 rows: 11.5 / 15.5).
 bool streams(int m, int n, int k, bool fits) {
-    const long long weights = (long long)n * k;
+    const long long weights = (long long)n * k, sms = umma::sm_count();
     if (m <= 32 && !fits)
         return true;
     if (m <= 16) {
         const bool lines = k % 128 == 0;
         if (k <= 1024)
             return lines || k <= 512 || n < 8192;
-        return k > 4096 || n < 88 * 128 || (k <= 2048 && lines && n >= 148 * 128);
+        return k > 4096 || n < sms * 3 / 5 * 128 || (k <= 2048 && lines && n >= sms * 128);
     }
     if (m <= 32)
         return weights <= 1 << 22 || (weights <= 1 << 25 && (n < 4800 || (n < 8192 && k > 1024)));
     // A pass over the weights per 32 rows, in no more CTAs than the SMs hold at once, or twice as many where the tiles
     // would need a launch more, for copies (148 x 1614 x 66: 6.0 / 7.8)
     const long long passes = ((long long)m + 31) / 32;
-    return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= (fits ? 2 : 4) * 148;
+    return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= (fits ? 2 : 4) * sms;
 }
 // So few that it makes whole numbers of them itself, every CTA again
 bool streams_activations(int m, int k) {

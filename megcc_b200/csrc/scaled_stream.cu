@@ -417,10 +417,10 @@ int launch_pad_rows(const PadRows& a, const PadRows& b, cudaStream_t st) {
     static MostShared shared[2];
     shared[0].ask(pad_rows_kernel<256>);
     shared[1].ask(pad_rows_kernel<32>);
-    const cudaError_t e =
-            rows < 16 * 148 ? launch_pdl(writes, pad_rows_kernel<256>, dim3((unsigned)rows), dim3(256), 0, st, a, b)
-                            : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
-                                         a, b);
+    const cudaError_t e = rows < 16LL * umma::sm_count()
+                                  ? launch_pdl(writes, pad_rows_kernel<256>, dim3((unsigned)rows), dim3(256), 0, st, a, b)
+                                  : launch_pdl(writes, pad_rows_kernel<32>, dim3((unsigned)((rows + 7) / 8)), dim3(256),
+                                               0, st, a, b);
     if (e != cudaSuccess)
         return refused("matmul_s8_scaled", e);
     return check_launch("matmul_s8_scaled");
