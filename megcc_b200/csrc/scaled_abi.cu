@@ -63,14 +63,16 @@ bool rows_fit(const void* p, int rows, long long ld) {
     return !misaligned(p, 16) && (rows == 1 || ld % 16 == 0);
 }
 // Few rows of activations, or little of everything: the kernel that streams the weights past them, whatever the
-// operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles), n x k:
-//   one row     16384 x 16384 42.2 / 47.2, 65536 x 1024 12.0 / 24.2, 20000 x 2048 9.0 / 11.2
-//   four        16384 x 2048 9.2 / 7.4, 10000 x 1008 5.5 / 4.6, 16384 x 1024 3.4 / 4.3, 6144 x 4096 5.6 / 7.3
-//   sixteen     16384 x 2048 10.1 / 7.4, 10000 x 1536 5.8 / 5.2, 14336 x 4096 14.4 / 13.7, 4096 x 8192 6.8 / 9.9
-//   24          4096 x 4096 6.1 / 9.2, 6144 x 4096 7.3 / 7.6, 8192 x 4096 10.3 / 9.3, 6000 x 1024 5.4 / 4.2
+// operands' alignment. Both sides measured (us, streamed and by the TMA-fed tiles, weights from HBM), n x k:
+//   one row     16384 x 16384 42.4 / 47.4, 65536 x 1024 11.8 / 23.9, 20000 x 2048 8.9 / 10.2, 32000 x 4096 24.9 / 21.7
+//   four        16384 x 2048 12.4 / 12.3, 10000 x 1008 8.4 / 6.5, 16384 x 1024 4.6 / 5.0, 6144 x 4096 6.4 / 8.8
+//   sixteen     16384 x 2048 12.8 / 11.8, 14336 x 4096 13.8 / 13.5, 4096 x 8192 6.9 / 10.5, 6144 x 4096 7.8 / 9.1
+//   24          4096 x 4096 5.4 / 7.8, 8192 x 4096 10.4 / 10.0, 6000 x 1024 7.5 / 4.6, 14336 x 4096 18.8 / 12.5
+// Streamed all the same, on the wrong side of a limit that goes by n and k: sixteen rows of 10000 x 1536 (7.3 / 6.4),
+// 24 of 6144 x 4096 (9.9 / 9.2).
 // Warps of the streaming kernel share K (launch_stream): short K costs them starts and ends, unless each has
 // rows of its own, which wants whole lines. Tiles want many columns, enough for all SMs without cutting K.
-// `fits`: the tiles' operands need no copies (4100 x 4100, 24 rows: 11.5 / 15.5).
+// `fits`: the tiles' operands need no copies (4100 x 4100, 24 rows, weights in the L2: 11.5 / 15.5).
 bool streams(int m, int n, int k, bool fits) {
     const long long weights = (long long)n * k, sms = umma::sm_count();
     if (m <= 32 && !fits)
@@ -88,7 +90,10 @@ bool streams(int m, int n, int k, bool fits) {
     const long long passes = ((long long)m + 31) / 32;
     return passes * weights <= 1 << 22 && passes * ((n + 15) / 16) <= (fits ? 2 : 4) * sms;
 }
-// So few that it makes whole numbers of them itself, every CTA again
+// So few that it makes whole numbers of them itself, every CTA again, which saves a launch and a transition. So, and by a
+// kernel in front (us, weights from HBM): 1 x 4096 x 4096 5.1 / 5.8, 1 x 14336 x 4096 13.3 / 15.3, 4 x 4096 x 4096
+// 5.6 / 5.9, 8 x 4096 x 1024 4.2 / 4.3. The rule does not look at n, by which the work is done again: 4 x 14336 x 4096
+// 21.0 / 15.3, 8 x 4096 x 4096 7.2 / 5.9, 8 x 128000 x 4096 183 / 88.
 bool streams_activations(int m, int k) {
     return m <= 8 && (long long)m * k <= 32768;
 }

@@ -12,8 +12,8 @@ namespace {
 // a row fits its registers (no barrier), else a whole CTA. The first HELD * LANES vectors of the row stay
 // in registers between the maximum and the conversion, what lies behind them is read again.
 // Vectors are the 16-byte units that the row lies in, zeros around it: with aligned == 0 rows start anywhere in their
-// first one, and their numbers go anywhere in a word (4001 x 4095 fp16: 21.9 us, 39.3 with its numbers stored one by
-// one).
+// first one, and their numbers go anywhere in a word (4001 x 4095 fp16: 25.8 us; with rows partly in the L2 21.9, and 39.3
+// with its numbers stored one by one).
 template <class T, int LANES, int HELD, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 0) quantize_rows_kernel(
         const T* __restrict__ x, int m, int k, long long ldx, int8_t* __restrict__ q, long long ldq,
@@ -161,9 +161,9 @@ int quantize_rows(
         return launch_pdl(writes, kernel, dim3((unsigned)((m - 1) / rows + 1)), dim3((unsigned)threads), 0, st, x, m,
                           k, ldx, q, ldq, scales, aligned);
     };
-    // A warp per row where it holds the row and there are rows enough for every SM's warps: 4001 x 4096 fp16 in
-    // 7.7 us, by whole CTAs in 12.3. The CTA grows with the row, so that it holds it as long as that goes: 4096 x 14336
-    // fp32 by 512 threads in 43.7 us, by 256 in 54.1.
+    // A warp per row where it holds the row and there are rows enough for every SM's warps: 4001 x 4096 fp16 from HBM in
+    // 9.2 us (5.3 TB/s), by whole CTAs in 10.2. The CTA grows with the row, so that it holds it as long as that goes:
+    // 4096 x 14336 fp32 by 512 threads in 57.3 us (5.1 TB/s), by 256 in 63.9.
     static MostShared shared[5];
     const cudaError_t e =
             m > 1 && k <= 32 * 4 * N        ? launch(quantize_rows_kernel<T, 32, 4, 256>, 8, 256, shared[0])

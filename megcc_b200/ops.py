@@ -139,7 +139,7 @@ def matmul_s8_qs8(a, b_packed, acc_scale, dst_scale):
     return c
 
 
-# ---- int8 products with scales per row (token) and per output channel ----
+# ---- int8 products with scales per row (token) and per output channel: forward only, results carry no gradient ----
 def quantize_rows_s8(x):
     """Rows of an fp32 / fp16 / bf16 matrix as int8 with one fp32 scale each: (q, scales). (A row's
     elements must be neighbours, here and below; rows may lie apart. Arguments that do not fit raise ValueError.)"""
