@@ -344,6 +344,85 @@ MB200_API int mb200_moe_s8(
         const float* w1_scales, const int8_t* w2, const float* w2_scales, void* y, long long ldy, void* workspace,
         size_t workspace_bytes, void* stream);
 
+/* ======================================================================================
+ * Attention with an int8 cache of keys and values, for decoders whose layers are the operators above (the
+ * reference has no attention operator). Activations and results are fp16 or bf16 (MB200_DTYPE_F16, _BF16), forward
+ * only.
+ *
+ * The cache is a pool of pages of page_tokens positions: whole numbers [pages][kv_heads][page_tokens][d], an fp32
+ * scale for each block of MB200_KV_BLOCK positions of a head, [pages][kv_heads][page_tokens / 16], for keys and for
+ * values; the value of an element is number * scale. Row b of block_table [batch], table_stride apart, names the
+ * pages of sequence b: position p is in page block_table[b][p / page_tokens]. Sequences may share a page as long as
+ * nothing is appended to the blocks that they share. What lies behind a sequence's last position is never read as a
+ * value, and entries of the table behind it are not looked at.
+ * d is a multiple of 16 up to 128, page_tokens one of 16; whole numbers are 16-byte aligned (as allocations are).
+ *
+ * Lengths, tables and row numbers are device memory: no call waits for them, and a captured call goes by what they
+ * hold when it is replayed. A position without a page (an entry outside [0, pages), or one beyond the table) is not
+ * stored, reads as 0 and is not seen by queries, and the device status (mb200_device_status) says 0x201.
+ *
+ * Packed rows: sequence b has rows cu[b] <= row < cu[b + 1]; cu holds batch + 1 numbers that do not decrease. Rows in no
+ * sequence are neither read nor written.
+ * ====================================================================================== */
+#define MB200_KV_BLOCK 16
+typedef struct mb200_kv_cache {
+    int8_t *k, *v;
+    float *k_scales, *v_scales;
+    const int32_t* block_table;
+    long long table_stride; /* elements from a sequence's row to the next's */
+    int pages, kv_heads, page_tokens, d;
+    int batch, table_pages; /* sequences, entries of a row */
+} mb200_kv_cache;
+
+/* A tensor [tokens][heads][d] whose heads' own elements are neighbours; it may start at any element. Strides count
+ * elements. Results overlap no operand, and no row or head of a result another one. */
+typedef struct mb200_heads {
+    void* p;
+    long long token_stride, head_stride;
+} mb200_heads;
+
+/* Keys and values of new tokens into the cache, behind the lengths[b] positions that sequence b has there already
+ * (lengths itself is left as it is). cu may be NULL: one token for each sequence, tokens == batch. A sequence with a
+ * negative length has none: its rows are passed over. k, v: [tokens][kv_heads][d].
+ * With tables of cosines and sines ([positions][rot_dims / 2] fp32, both NULL for none) keys are turned before they are
+ * stored, and with q.p, [tokens][heads][d], queries into q_out: of the first rot_dims elements of a head (a multiple of
+ * 16) the pairs (i, i + rot_dims / 2), or the neighbours (2 i, 2 i + 1) if interleaved != 0,
+ *     x' = x cos - y sin,  y' = y cos + x sin   with the position's i-th cosine and sine,
+ * in fp32, products and sums rounded each. q_out and k_out (k_out.p may be NULL) get the results rounded to 16 bits; the
+ * cache is made from the fp32 ones. A position beyond the tables makes its row NaN, and the device status 0x202.
+ * A block's scale is RN(max(amax, 2^-119) * RN(1 / 127)) of the new values in it, or what it was, if the block keeps
+ * older positions and that is larger; whole numbers are x * RN(1 / scale) to the nearest (ties to even). If the scale
+ * grows, older numbers become q * RN(old scale / scale) to the nearest. A block with a NaN or an infinity gets scale
+ * NaN and zeros, and is NaN as long as it keeps them. No block may be appended to by two sequences of a call. */
+typedef struct mb200_kv_append_param {
+    const int32_t *lengths, *cu;
+    int tokens, heads, dtype; /* heads: of q */
+    mb200_heads k, v, q, q_out, k_out;
+    const float *cosines, *sines;
+    int positions, rot_dims, interleaved;
+} mb200_kv_append_param;
+MB200_API int mb200_kv_append_s8(const mb200_kv_cache* cache, const mb200_kv_append_param* p, void* stream);
+
+/* Cached keys and values as 16-bit values, k and v [tokens][kv_heads][d] of packed rows: row cu[b] + i is position
+ * starts[b] + i of sequence b (starts may be NULL: from 0 on). number * scale, rounded to fp32 and then to `dtype`. */
+MB200_API int mb200_kv_read_s8(
+        const mb200_kv_cache* cache, const int32_t* starts, const int32_t* cu, int tokens, int dtype,
+        const mb200_heads* k, const mb200_heads* v, void* stream);
+
+/* Attention of `queries` tokens of each sequence over its cached positions:
+ *     out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)
+ * q and out: [batch * queries][heads][d], heads a multiple of kv_heads: head h goes with key head h / (heads /
+ * kv_heads). lengths[b] positions are in the cache, the queries' own among them: query i of a sequence sees positions
+ * up to lengths[b] - queries + i. A query that sees none gets zeros (a sequence of length <= 0 is not in use).
+ * Keys and values are the cache's exactly; q keeps 11 bits (those of fp16 relative to its row's largest), p_j are rounded to
+ * 11 bits, sums are fp32, in an order that depends on lengths and sizes only.
+ * workspace: mb200_attention_cache_s8_workspace_bytes of device memory, 256-byte aligned, whose content does not
+ * matter; two calls that may run at the same time need one each. */
+MB200_API size_t mb200_attention_cache_s8_workspace_bytes(const mb200_kv_cache* cache, int heads, int queries);
+MB200_API int mb200_attention_cache_s8(
+        const mb200_kv_cache* cache, const int32_t* lengths, int heads, int queries, int dtype, const mb200_heads* q,
+        float scale, const mb200_heads* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Pooling qint8 (kernel_pooling_<MODE>_NCHW_p.._s.._w.._qsi8qsi8,
  * compiler/lib/KernelGen/BareMetal/Pooling.cpp:166-273), NHWC in/out ---- */
 MB200_API int mb200_pooling_qs8_nhwc(

@@ -34,6 +34,26 @@ class MoeParam(C.Structure):
     _fields_ = [(k, C.c_int) for k in ("tokens", "d", "f", "experts", "top_k", "renormalize", "dtype")]
 
 
+class KvCache(C.Structure):
+    """Mirror of ``mb200_kv_cache``."""
+    _fields_ = [(k, C.c_void_p) for k in ("k", "v", "k_scales", "v_scales", "block_table")] + [
+        ("table_stride", C.c_longlong)] + [(k, C.c_int) for k in (
+            "pages", "kv_heads", "page_tokens", "d", "batch", "table_pages")]
+
+
+class Heads(C.Structure):
+    """Mirror of ``mb200_heads``."""
+    _fields_ = [("p", C.c_void_p), ("token_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
+class KvAppendParam(C.Structure):
+    """Mirror of ``mb200_kv_append_param``."""
+    _fields_ = [("lengths", C.c_void_p), ("cu", C.c_void_p), ("tokens", C.c_int), ("heads", C.c_int),
+                ("dtype", C.c_int)] + [(k, Heads) for k in ("k", "v", "q", "q_out", "k_out")] + [
+        ("cosines", C.c_void_p), ("sines", C.c_void_p), ("positions", C.c_int), ("rot_dims", C.c_int),
+        ("interleaved", C.c_int)]
+
+
 _lib = None
 
 # name -> (restype, argtypes); every symbol declared in include/megcc_b200.h
@@ -91,6 +111,12 @@ SIGNATURES = {
     "mb200_moe_s8_workspace_bytes": (C.c_size_t, [C.POINTER(MoeParam)]),
     "mb200_moe_s8": (C.c_int, [C.POINTER(MoeParam), _P, C.c_longlong] + [_P] * 6 + [
         C.c_longlong, _P, C.c_size_t, _P]),
+    "mb200_kv_append_s8": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvAppendParam), _P]),
+    "mb200_kv_read_s8": (C.c_int, [C.POINTER(KvCache), _P, _P, C.c_int, C.c_int, C.POINTER(Heads), C.POINTER(Heads),
+                                   _P]),
+    "mb200_attention_cache_s8_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.c_int, C.c_int]),
+    "mb200_attention_cache_s8": (C.c_int, [C.POINTER(KvCache), _P, C.c_int, C.c_int, C.c_int, C.POINTER(Heads),
+                                           C.c_float, C.POINTER(Heads), _P, C.c_size_t, _P]),
     "mb200_pooling_qs8_nhwc": (C.c_int, [_P, _P] + [C.c_int] * 11 + [_P]),
     "mb200_qelemwise_qs8": (C.c_int, [_P, _P, _P, C.c_int, C.c_size_t, C.c_float, C.c_float,
                                       C.c_float, _P]),
@@ -186,7 +212,8 @@ def tensor_calls():
         _torchcall.bind(check, torch.OutOfMemoryError, *(C.cast(getattr(lib(), name), C.c_void_p).value for name in (
             "mb200_quantize_rows_s8", "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
             "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
-            "mb200_moe_s8")))
+            "mb200_moe_s8", "mb200_kv_append_s8", "mb200_kv_read_s8", "mb200_attention_cache_s8_workspace_bytes",
+            "mb200_attention_cache_s8")))
         _tensor_calls = _torchcall
     return _tensor_calls
 

@@ -4,6 +4,7 @@ Each function mirrors one kernel family of the reference's KernelGen and calls s
 into the C ABI of libmegcc_b200.so on the current torch CUDA stream.
 """
 import ctypes as C
+import typing
 
 import torch
 
@@ -163,6 +164,54 @@ def moe_s8(x, logits, w1, w1_scales, w2, w2_scales, top_k, renormalize=True):
     fp32, int8 weights w1 [experts, 2f, d] (gate rows, then up rows) and w2 [experts, d, f] with fp32 scales
     per row; [t, d] of x's type (see mb200_moe_s8)."""
     return tensor_calls().moe_s8(x, logits, w1, w1_scales, w2, w2_scales, top_k, renormalize)
+
+
+# ---- attention with an int8 cache: 16-bit activations, forward only, results carry no gradient ----
+KV_BLOCK = 16  # positions of a head that share a scale
+
+
+class KvCacheS8(typing.NamedTuple):
+    """Pages of keys and values, [pages, kv_heads, page_tokens, d] int8, with an fp32 scale for each block of KV_BLOCK
+    positions of a head, [pages, kv_heads, page_tokens // KV_BLOCK]. (d is a multiple of 16 up to 128, page_tokens one
+    of 16.) Tables [sequences, pages of a sequence] int32 say which page holds which positions of a sequence."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def kv_cache_s8(pages, kv_heads, page_tokens, d, device="cuda"):
+    """A KvCacheS8 of zeros."""
+    shape, blocks = (pages, kv_heads, page_tokens, d), (pages, kv_heads, page_tokens // KV_BLOCK)
+    return KvCacheS8(torch.zeros(shape, dtype=_S8, device=device), torch.zeros(shape, dtype=_S8, device=device),
+                     torch.zeros(blocks, device=device), torch.zeros(blocks, device=device))
+
+
+def kv_append_s8(cache, block_table, lengths, k, v, q=None, cos=None, sin=None, cu_tokens=None, interleaved=False,
+                 turned_keys=False):
+    """Stores k and v [tokens, kv_heads, d] (fp16 or bf16; heads and tokens may lie apart) behind the lengths[b]
+    positions that each sequence has in the cache: one token for each sequence, or rows cu_tokens[b] .. cu_tokens[b + 1].
+    With cos and sin [positions, turned elements / 2] fp32 keys are turned by their positions first, halves of the turned
+    elements against each other or neighbours (interleaved), and queries q [tokens, heads, d] beside them. Returns (turned
+    queries or None, with turned_keys turned keys or None). lengths stays as it is; a sequence with a negative one is not
+    in use, and its rows of the results are left as they were. (See mb200_kv_append_s8.)"""
+    return tensor_calls().kv_append_s8(*cache, block_table, lengths, k, v, q, cos, sin, cu_tokens, interleaved,
+                                       turned_keys)
+
+
+def kv_read_s8(cache, block_table, starts, cu_tokens, tokens, dtype=torch.bfloat16):
+    """Cached keys and values as `dtype` (fp16 or bf16), two tensors [tokens, kv_heads, d] of packed rows: row
+    cu_tokens[b] + i is position starts[b] + i of sequence b (starts None: from 0 on). For a prompt that continues
+    a cached one: attention_prompt takes them as its keys. Rows behind the last sequence are left as they were."""
+    return tensor_calls().kv_read_s8(*cache, block_table, starts, cu_tokens, tokens, dtype)
+
+
+def attention_cache_s8(q, cache, block_table, lengths, scale=None, out=None):
+    """Attention of one query per sequence, q [sequences, heads, d], or of several, [sequences, queries, heads, d], over
+    its lengths[b] cached positions, the queries' own the last of them: each sees what lies in front of it and itself.
+    fp16 or bf16; heads are a multiple of the cache's. scale: 1 / sqrt(d) unless given. A query that sees nothing gives
+    zeros, a sequence of length 0 (not in use) too. (See mb200_attention_cache_s8.)"""
+    return tensor_calls().attention_cache_s8(q, *cache, block_table, lengths, scale, out)
 
 
 def pooling_qs8_nhwc(src, mode, window, stride, pad):
