@@ -423,6 +423,18 @@ MB200_API int mb200_attention_cache_s8(
         const mb200_kv_cache* cache, const int32_t* lengths, int heads, int queries, int dtype, const mb200_heads* q,
         float scale, const mb200_heads* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention over whole prompts of 16-bit keys and values, packed: q and out [tokens][heads][d] with rows cu_q, k and v
+ * [key_tokens][kv_heads][d] with rows cu_k (NULL: cu_q, and key_tokens == tokens). Head h goes with key head h / (heads
+ * / kv_heads). causal != 0: a sequence's last query sees its last key, and each query one key less than the next; a query
+ * that sees none gets zeros. Without it each sees all of its sequence's. What a query does not see does not reach it,
+ * whatever it holds. (A query whose result is not finite is computed a second time by a far slower way: keys, values or
+ * queries that are no numbers cost time.) p_j as above, but rounded to `dtype`.
+ * q, k, v: 16-byte aligned, strides multiples of 8 elements and not 0. */
+MB200_API int mb200_attention_prompt(
+        int batch, const int32_t* cu_q, const int32_t* cu_k, int tokens, int key_tokens, int heads, int kv_heads, int d,
+        int dtype, const mb200_heads* q, const mb200_heads* k, const mb200_heads* v, int causal, float scale,
+        const mb200_heads* out, void* stream);
+
 /* ---- Pooling qint8 (kernel_pooling_<MODE>_NCHW_p.._s.._w.._qsi8qsi8,
  * compiler/lib/KernelGen/BareMetal/Pooling.cpp:166-273), NHWC in/out ---- */
 MB200_API int mb200_pooling_qs8_nhwc(

@@ -117,6 +117,8 @@ SIGNATURES = {
     "mb200_attention_cache_s8_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.c_int, C.c_int]),
     "mb200_attention_cache_s8": (C.c_int, [C.POINTER(KvCache), _P, C.c_int, C.c_int, C.c_int, C.POINTER(Heads),
                                            C.c_float, C.POINTER(Heads), _P, C.c_size_t, _P]),
+    "mb200_attention_prompt": (C.c_int, [C.c_int, _P, _P] + [C.c_int] * 6 + [C.POINTER(Heads)] * 3 + [
+        C.c_int, C.c_float, C.POINTER(Heads), _P]),
     "mb200_pooling_qs8_nhwc": (C.c_int, [_P, _P] + [C.c_int] * 11 + [_P]),
     "mb200_qelemwise_qs8": (C.c_int, [_P, _P, _P, C.c_int, C.c_size_t, C.c_float, C.c_float,
                                       C.c_float, _P]),
@@ -213,7 +215,7 @@ def tensor_calls():
             "mb200_quantize_rows_s8", "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
             "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
             "mb200_moe_s8", "mb200_kv_append_s8", "mb200_kv_read_s8", "mb200_attention_cache_s8_workspace_bytes",
-            "mb200_attention_cache_s8")))
+            "mb200_attention_cache_s8", "mb200_attention_prompt")))
         _tensor_calls = _torchcall
     return _tensor_calls
 

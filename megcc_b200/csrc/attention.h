@@ -52,5 +52,16 @@ size_t attention_cache_workspace(const mb200_kv_cache& c, int heads, int queries
 int launch_attention_cache(const CacheArgs& a, int dtype, cudaStream_t st);
 
 
+struct PromptArgs {
+    int batch, tokens, key_tokens, heads, kv_heads, d;
+    const int32_t *cu_q, *cu_k;
+    mb200_heads q, k, v, out;
+    int causal;
+    float scale_log2;
+    int* status;
+};
+long long attention_prompt_ctas(int tokens, int batch, int heads);
+int launch_attention_prompt(const PromptArgs& a, int dtype, cudaStream_t st);
+
 }  // namespace attn
 }  // namespace mb200

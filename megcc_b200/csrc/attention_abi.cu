@@ -93,6 +93,16 @@ int check_attention_cache(const mb200_kv_cache* c, int heads, int queries) {
     return ST_SUCCESS;
 }
 
+// what the TMA takes: whole 16-byte units, heads and tokens apart
+int check_units(const mb200_heads& t, int tokens, int heads, const char* name, const char* what) {
+    if (misaligned(t.p, 16) || (tokens > 1 && (t.token_stride % 8 != 0 || t.token_stride == 0)) ||
+        (heads > 1 && (t.head_stride % 8 != 0 || t.head_stride == 0)))
+        return set_error(ST_INVALID_LAYOUT, "%s: %s must be 16-byte aligned, its strides multiples of 8 elements", what, name);
+    if (t.token_stride >= 1LL << 38 || t.head_stride >= 1LL << 38)
+        return set_error(ST_OUT_OF_RANGE, "%s: strides of %s", what, name);
+    return ST_SUCCESS;
+}
+
 }  // namespace
 
 extern "C" {
@@ -230,6 +240,63 @@ int mb200_attention_cache_s8(
     a.workspace = workspace;
     rc = status_word(stream, &a.status);
     return rc ? rc : launch_attention_cache(a, dtype, (cudaStream_t)stream);
+}
+
+int mb200_attention_prompt(
+        int batch, const int32_t* cu_q, const int32_t* cu_k, int tokens, int key_tokens, int heads, int kv_heads, int d,
+        int dtype, const mb200_heads* q, const mb200_heads* k, const mb200_heads* v, int causal, float scale,
+        const mb200_heads* out, void* stream) {
+    const char* what = "attention_prompt";
+    int rc = check_dtype(dtype, what);
+    if (!rc)
+        rc = check_d(d, what);
+    if (rc)
+        return rc;
+    if (batch < 0 || tokens < 0 || key_tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
+        (!cu_k && key_tokens != tokens))
+        return set_error(ST_INVALID_LAYOUT, "%s: %d sequences, %d tokens and %d of keys, %d heads over %d key heads", what,
+                         batch, tokens, key_tokens, heads, kv_heads);
+    if (!isfinite(scale))
+        return set_error(ST_INVALID_LAYOUT, "%s: the scale is not finite", what);
+    if (tokens == 0 || batch == 0)
+        return ST_SUCCESS;
+    if (!cu_q || !q || !k || !v || !out)
+        return set_error(ST_NULL_PTR, "%s: an operand is NULL", what);
+    // (no keys at all: there is nothing to look at, and zeros to write)
+    const int some = key_tokens > 0 ? key_tokens : 1;
+    PromptArgs a{};
+    a.q = *q, a.k = key_tokens > 0 ? *k : *q, a.v = key_tokens > 0 ? *v : *q, a.out = *out;
+    rc = check_heads(a.q, tokens, heads, d, false, "q", what);
+    if (!rc)
+        rc = check_heads(a.k, some, kv_heads, d, false, "k", what);
+    if (!rc)
+        rc = check_heads(a.v, some, kv_heads, d, false, "v", what);
+    if (!rc)
+        rc = check_heads(a.out, tokens, heads, d, true, "out", what);
+    if (!rc)
+        rc = check_units(a.q, tokens, heads, "q", what);
+    if (!rc)
+        rc = check_units(a.k, some, kv_heads, "k", what);
+    if (!rc)
+        rc = check_units(a.v, some, kv_heads, "v", what);
+    if (rc)
+        return rc;
+    if (misaligned(cu_q, 4) || misaligned(cu_k, 4))
+        return set_error(ST_INVALID_LAYOUT, "%s: cu_q and cu_k must be aligned as their types are", what);
+    // (rows of the last tiles are counted in an int)
+    if (tokens > 0x7fffffff - 512 || key_tokens > 0x7fffffff - 512)
+        return set_error(ST_OUT_OF_RANGE, "%s: %d tokens, %d of keys", what, tokens, key_tokens);
+    rc = check_grid(attention_prompt_ctas(tokens, batch, heads), what);
+    if (!rc)
+        rc = status_word(stream, &a.status);
+    if (rc)
+        return rc;
+    a.batch = batch, a.tokens = tokens, a.key_tokens = key_tokens;
+    a.heads = heads, a.kv_heads = kv_heads, a.d = d;
+    a.cu_q = cu_q, a.cu_k = cu_k ? cu_k : cu_q;
+    a.causal = causal != 0;
+    a.scale_log2 = scale * 1.44269504f;
+    return launch_attention_prompt(a, dtype, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -34,6 +34,7 @@ struct Abi {
     decltype(&mb200_kv_read_s8) kv_read;
     decltype(&mb200_attention_cache_s8_workspace_bytes) cache_workspace;
     decltype(&mb200_attention_cache_s8) attention_cache;
+    decltype(&mb200_attention_prompt) attention_prompt;
 } abi;
 PyObject* on_status = nullptr;
 PyObject* out_of_memory = nullptr;  // torch.OutOfMemoryError
@@ -490,8 +491,41 @@ PyObject* attention_cache_s8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+PyObject* attention_prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    double scale;
+    if (!counted(n, 8) || !scale_of(args[6], &scale))
+        return nullptr;
+    const int causal = PyObject_IsTrue(args[5]);
+    if (causal < 0)
+        return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor &q = tensor(args[0], "q"), &k = tensor(args[1], "k"), &cu = tensor(args[3], "cu_q");
+        const mb200_heads hq = heads_of(q, q, "q"), hk = heads_of(k, q, "k");
+        const int64_t d = q.size(2);
+        if (k.size(2) != d)
+            refuse("k: heads of " + std::to_string(d) + " elements, not " + shown(k));
+        const mb200_heads hv = heads_of(tensor(args[2], "v"), k.size(0), k.size(1), d, q, "v");
+        at::Tensor out = result_for(args[7], q);
+        const mb200_heads ho = heads_of(out, q, "out");
+        if (cu.numel() < 1 || cu.numel() > INT32_MAX)
+            refuse("cu_q: sequences + 1 int32 values, not " + shown(cu));
+        const int32_t* cu_q = ints_of(cu, cu.numel(), q, "cu_q");
+        const int32_t* cu_k = args[4] == Py_None ? nullptr : ints_of(tensor(args[4], "cu_k"), cu.numel(), q, "cu_k");
+        if (!cu_k && k.size(0) != q.size(0))
+            refuse("k: of as many tokens as q (or cu_k), not " + shown(k));
+        if (args[6] == Py_None)
+            scale = 1 / std::sqrt((double)d);
+        const int status = without_gil([&] {
+            return abi.attention_prompt((int)cu.numel() - 1, cu_q, cu_k, (int)q.size(0), (int)k.size(0), (int)q.size(1),
+                                        (int)k.size(1), (int)d, dtype_code(q.scalar_type()), &hq, &hk, &hv, causal,
+                                        (float)scale, &ho, stream_of(q));
+        });
+        return done(status) ? THPVariable_Wrap(std::move(out)) : nullptr;
+    });
+}
+
 PyObject* bind(PyObject*, PyObject* args) {
-    constexpr int kFunctions = 11;
+    constexpr int kFunctions = 12;
     unsigned long long at[kFunctions];
     if (PyTuple_GET_SIZE(args) != 2 + kFunctions) {
         PyErr_Format(PyExc_TypeError, "bind takes %d arguments", 2 + kFunctions);
@@ -514,6 +548,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     abi.kv_read = (decltype(abi.kv_read))(uintptr_t)at[8];
     abi.cache_workspace = (decltype(abi.cache_workspace))(uintptr_t)at[9];
     abi.attention_cache = (decltype(abi.attention_cache))(uintptr_t)at[10];
+    abi.attention_prompt = (decltype(abi.attention_prompt))(uintptr_t)at[11];
     Py_INCREF(fail);
     Py_XSETREF(on_status, fail);
     Py_INCREF(memory);
@@ -536,6 +571,8 @@ PyMethodDef methods[] = {
          "(cache.k, .v, .k_scales, .v_scales, block_table, starts, cu_tokens, tokens, dtype) -> (k, v)"},
         {"attention_cache_s8", (PyCFunction)(void*)attention_cache_s8, METH_FASTCALL,
          "(q, cache.k, .v, .k_scales, .v_scales, block_table, lengths, scale, out) -> out"},
+        {"attention_prompt", (PyCFunction)(void*)attention_prompt, METH_FASTCALL,
+         "(q, k, v, cu_q, cu_k, causal, scale, out) -> out"},
         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torchcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -214,6 +214,15 @@ def attention_cache_s8(q, cache, block_table, lengths, scale=None, out=None):
     return tensor_calls().attention_cache_s8(q, *cache, block_table, lengths, scale, out)
 
 
+def attention_prompt(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None):
+    """Attention over whole prompts, packed: q [tokens, heads, d], k and v [key tokens, kv_heads, d], fp16 or bf16, rows
+    cu_q[b] .. cu_q[b + 1] (and cu_k, where a sequence has other keys than its queries', a cached prefix in front of
+    them for instance: kv_read_s8). causal: the last query of a sequence sees its last key. scale: 1 / sqrt(d) unless
+    given. A query that sees nothing gives zeros; rows behind the last sequence are left as they were. (See
+    mb200_attention_prompt.)"""
+    return tensor_calls().attention_prompt(q, k, v, cu_q, cu_k, causal, scale, out)
+
+
 def pooling_qs8_nhwc(src, mode, window, stride, pad):
     n, ih, iw, c = src.shape
     oh, ow = (ih + 2 * pad - window) // stride + 1, (iw + 2 * pad - window) // stride + 1

@@ -122,3 +122,26 @@ def test_tensors_that_do_not_fit():
                  lambda: ops.kv_read_s8(pool(k=None), table, None, lengths, 3)):
         with pytest.raises(ValueError):
             call()
+
+
+def attention_prompt(change):
+    a = dict(batch=3, cu_q=P, cu_k=P, tokens=10, key_tokens=20, heads=4, kv_heads=2, d=64, dtype=1, causal=1, scale=0.1)
+    a.update(rest(change, a))
+    q, k, v, out = heads(change, "q", 4), heads(change, "nk"), heads(change, "nv"), heads(change, "out", 4)
+    return _lib.lib().mb200_attention_prompt(a["batch"], a["cu_q"], a["cu_k"], a["tokens"], a["key_tokens"], a["heads"],
+                                             a["kv_heads"], a["d"], a["dtype"], C.byref(q), C.byref(k), C.byref(v),
+                                             a["causal"], a["scale"], C.byref(out), None)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(batch=-1), LAYOUT), (dict(tokens=-1), LAYOUT), (dict(key_tokens=-1), LAYOUT), (dict(heads=0), LAYOUT),
+    (dict(heads=5), LAYOUT), (dict(kv_heads=0), LAYOUT), (dict(cu_k=None), LAYOUT), (dict(d=24), LAYOUT), (dict(d=-16), LAYOUT),
+    (dict(d=256), OUT_OF_RANGE), (dict(dtype=0), DTYPE), (dict(scale=float("inf")), LAYOUT), (dict(cu_q=None), NULL_PTR),
+    (dict(q=(None, 256, 64)), NULL_PTR), (dict(nk=(None, 128, 64)), NULL_PTR), (dict(nv=(None, 128, 64)), NULL_PTR),
+    (dict(out=(None, 256, 64)), NULL_PTR), (dict(q=(P + 2, 256, 64)), LAYOUT), (dict(nk=(P, 130, 64)), LAYOUT),
+    (dict(nv=(P, 128, 0)), LAYOUT), (dict(nv=(P, 0, 64)), LAYOUT), (dict(q=(P, 256, 68)), LAYOUT),
+    (dict(out=(P, 128, 64)), LAYOUT), (dict(out=(P + 1, 256, 64)), LAYOUT), (dict(cu_q=P + 2), LAYOUT),
+    (dict(nk=(P, 1 << 38, 64)), OUT_OF_RANGE), (dict(key_tokens=(1 << 31) - 1), OUT_OF_RANGE),
+    (dict(batch=1 << 30), OUT_OF_RANGE), (dict(tokens=0, q=(None, 0, 0)), 0), (dict(batch=0), 0)])
+def test_attention_prompt(change, status):
+    assert attention_prompt(change) == status
