@@ -5,22 +5,23 @@
 // over the positions j that a row sees, in one pass: m is a running maximum that is raised only where a score
 // passes it by more than 8 (a vote per block of 16 positions, no reduction), so 2^(t - m) stays below 2^8.
 //
-// Bound by memory: 2 d bytes per position and key head are all there is to read, and eight rows' products take a
-// third of the tensor cores' time at that rate even by mma.sync, whose operands come from registers: whole numbers are
-// exact in fp16, where they are made by a byte permutation into 1024 + (v + 128) and a subtraction. Products are taken
-// transposed, S^T = K Q^T and O^T = V^T P^T, so that positions and dimensions fill the 16 rows of an MMA and 8 query
-// rows its 8 columns: half the instructions and accumulators of the other way round for groups of up to 8. The
-// order of dimensions within S's sum is free: a lane takes 16 neighbouring ones with one load. V^T comes by
-// ldmatrix.trans over pairs of bytes, whose two dimensions the byte permutation separates. P^T is turned by movmatrix.
+// Bound by memory: 2 d bytes per position and key head are all there is to read, and what each byte costs in
+// instructions decides whether that is reached. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that positions
+// and dimensions fill the 16 rows of an mma.sync and 8 query rows its 8 columns: half the instructions and accumulators of
+// the other way round for groups of up to 8.
+//   S: keys are multiplied as they lie, int8 by int8 (m16n8k32, as fast as fp16's k16): queries become whole numbers of 23 bits
+// of their row's power of two, three planes of int8, whose sums are exact. The order of dimensions within a sum is free:
+// a lane takes 16 neighbouring ones with one load.
+//   O: values become fp16, which holds them exactly: a byte permutation makes 1024 + (v + 128) of them, and a subtraction v.
+// V^T comes by ldmatrix.trans over pairs of bytes, whose two dimensions the same permutation separates. P^T is turned by
+// movmatrix. P is rounded to fp16 (2^-12, where results have 2^-9), for fp16 results held as two such numbers, after it
+// took its block's scale of V relative to the largest so far, which keeps it in range.
 //
-// Queries are scaled by a power of two of their row, which makes fp16 of bf16 without loss for all elements within 2^-16
-// of the row's largest; probabilities are rounded to fp16 (a relative 2^-12, under the results' own 2^-9 or
-// 2^-12), after they took their block's scale of V relative to the largest so far, which keeps them in range. Sums and
-// accumulators are fp32.
-//
-// All blocks of all sequences and key heads are one line, cut evenly over the CTAs whatever the lengths, which only
-// the device knows. A CTA's warps take its blocks in turn, each through a ring of asynchronous copies of its own. Where a
-// head's blocks are cut, the parts go to the workspace and a second kernel joins them in order.
+// All blocks of all sequences and key heads are one line of rounds (a step of 32 positions for each of a CTA's warps),
+// cut evenly over the CTAs whatever the lengths, which only the device knows. Each warp has a ring of asynchronous copies of
+// its own. Where a head's rounds are cut, the parts go to the workspace and a second kernel joins them in order.
+#include <type_traits>
+
 #include "kv_cache.cuh"
 #include "umma_ptx.cuh"
 
@@ -28,36 +29,37 @@ namespace mb200 {
 namespace attn {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kLeast = kWarps;       // blocks a CTA takes at least: one for each warp
-constexpr float kAhead = 8.f;        // how far a score may pass the running maximum
-constexpr int kLift = 6;             // probabilities are held 2^6 times: 2^8 * 2 * 2^6 < 65504
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kStep = 2;                   // blocks of a warp's step
+constexpr int kRound = kWarps * kStep;     // blocks of a CTA's round
+constexpr float kAhead = 8.f;              // how far a score may pass the running maximum
+constexpr int kLift = 6;                   // probabilities are held 2^6 times: 2^8 * 2 * 2^6 < 65504
+constexpr int kCtasPerSm = 2;
 
 template <int D>
 struct Ring {
-    static constexpr int kStage = 2 * kBlock * D + 16;  // keys, values, their two scales
-    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kHalf = kStep * kBlock * D;   // keys, then values
+    static constexpr int kStage = 2 * kHalf + 128;     // ... and their four scales (stages begin on whole lines)
+    static constexpr int kStages = D == 128 ? 3 : 5;
     static constexpr int kBytes = kWarps * kStages * kStage;
 };
 // floats from row to row of the warps' sums: a warp's stores reach all banks
 template <int D>
 constexpr int kPitch = D + 4;
 
-// How the line of blocks is cut, found alike by both kernels
-struct Line {
-    long long before, total;  // blocks in front of sequence b (times heads), in all
-    int blocks;               // of sequence b
-};
 struct Shape {
     int rows, tiles, capacity;  // rows of a key head, tiles of them, positions a table has room for
 };
+// How the line is cut, found alike by both kernels
 __device__ __forceinline__ int blocks_of(const CacheArgs& a, int capacity, int b) {
     const int n = a.lengths[b];
     return n <= 0 ? 0 : (min(n, capacity) + kBlock - 1) / kBlock;
 }
+__device__ __forceinline__ int rounds_of(const CacheArgs& a, int capacity, int b) {
+    return b < a.c.batch ? (blocks_of(a, capacity, b) + kRound - 1) / kRound : 0;
+}
 __device__ __forceinline__ long long quota_of(long long total, int ctas) {
-    const long long q = (total + ctas - 1) / ctas;
-    return (q + kLeast - 1) / kLeast * kLeast;
+    return (total + ctas - 1) / ctas;
 }
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) {
@@ -84,11 +86,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
                  : "memory");
     return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t at) {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t at, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -106,6 +103,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
             "{%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -149,85 +153,97 @@ __device__ __forceinline__ long long row_at(const CacheArgs& a, const mb200_head
     return ((long long)b * a.queries + i) * t.token_stride + (long long)(h * group + (r - i * group)) * t.head_stride;
 }
 
-template <class T, int D, int NT, bool VEC>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const CacheArgs a, const Shape shape) {
+// Queries as whole numbers of 23 bits: hi 2^16 + mid 2^8 + lo times 2^(e - 21), e the exponent of the row's largest
+constexpr int kPlanes = 3;
+__device__ __forceinline__ void planes_of(const float (&x)[4], float up, uint32_t (&w)[kPlanes]) {
+    uint32_t b[4][kPlanes];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int q = __float2int_rn(__fmul_rn(x[i], up));
+        const int q1 = (q - (int)(int8_t)q) >> 8;
+        b[i][2] = (uint32_t)q, b[i][1] = (uint32_t)q1, b[i][0] = (uint32_t)((q1 - (int)(int8_t)q1) >> 8);
+    }
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p)
+        w[p] = __byte_perm(__byte_perm(b[0][p], b[1][p], 0x0040), __byte_perm(b[2][p], b[3][p], 0x0040), 0x5410);
+}
+
+// FULL: d == D
+template <class T, int D, int NT, bool VEC, bool FULL>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const CacheArgs a, const Shape shape) {
+    using R = Ring<D>;
     constexpr int kRows = 8 * NT, kChunks = D / 64, kTiles = D / 16;
+    constexpr bool kFine = std::is_same<T, __half>::value;  // P as two fp16 numbers
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_from, s_to, s_blk;
-    __shared__ int s_b, s_at;
+    __shared__ long long s_from, s_to, s_rest;
+    __shared__ int s_b;
     __shared__ float2 s_stats[kWarps][kRows];
     const int tid = threadIdx.x, lane = tid & 31, warp = umma::uniform_warp_index();
     const int g = lane >> 2, c = lane & 3;
-    const int d = a.c.d, group = a.heads / a.c.kv_heads;
+    const int d = FULL ? D : a.c.d, group = a.heads / a.c.kv_heads;
     const int lines = a.c.kv_heads * shape.tiles;  // of a sequence: key heads times tiles of rows
+    const float none = __uint_as_float(0xff800000u);
     pdl_start();
-
-    // sequences without a position: nothing is seen
-    for (int b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
-        if (a.lengths[b] > shape.capacity && tid == 0)
-            *(volatile int*)a.status = ERR_PAGE;
-        if (a.lengths[b] <= 0)
-            for (int i = tid; i < a.queries * a.heads * d; i += kThreads) {
-                const int e = i % d, th = i / d;
-                ((T*)a.out.p)[((long long)b * a.queries + th / a.heads) * a.out.token_stride +
-                              (long long)(th % a.heads) * a.out.head_stride + e] = from_float<T>(0.f);
-            }
-    }
 
     // this CTA's part of the line
     if (warp == 0) {
         long long total = 0;
+        int mine = 0;
         for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-            const int n = b0 + lane < a.c.batch ? blocks_of(a, shape.capacity, b0 + lane) : 0;
-            total += __reduce_add_sync(0xffffffffu, n);
+            mine = rounds_of(a, shape.capacity, b0 + lane);
+            total += __reduce_add_sync(0xffffffffu, mine);
         }
         total *= lines;
         const long long quota = quota_of(total, gridDim.x);
         const long long from = quota * blockIdx.x, to = from + quota < total ? from + quota : total;
         long long before = 0;
-        int at = 0, n = 0;
+        int at = 0;
         if (from < to) {
             for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-                n = b0 + lane < a.c.batch ? blocks_of(a, shape.capacity, b0 + lane) : 0;
+                const int n = a.c.batch <= 32 ? mine : rounds_of(a, shape.capacity, b0 + lane);
                 int sum = n;
 #pragma unroll
                 for (int s = 1; s < 32; s *= 2) {
                     const int v = __shfl_up_sync(0xffffffffu, sum, s);
                     sum += lane >= s ? v : 0;
                 }
-                // (a sequence's blocks are counted lines times, one after the other)
                 const uint32_t beyond = __ballot_sync(0xffffffffu, (before + sum) * lines > from);
                 if (beyond) {
                     const int i = __ffs(beyond) - 1;
                     before += __shfl_sync(0xffffffffu, sum - n, i);
-                    n = __shfl_sync(0xffffffffu, n, i);
                     at = b0 + i;
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
         }
-        if (lane == 0) {
-            s_from = from, s_to = to, s_b = at;
-            const long long rest = from - before * lines;
-            s_at = n ? (int)(rest / n) : 0;
-            s_blk = n ? rest % n : 0;
-        }
+        if (lane == 0)
+            s_from = from, s_to = to, s_b = at, s_rest = from - before * lines;
     }
     __syncthreads();
     long long left = s_to - s_from;
-    int b = s_b, at = s_at, blk = (int)s_blk;
+    int b = s_b, at = 0, blk = 0;
+    if (left > 0) {
+        const int n = rounds_of(a, shape.capacity, b);
+        at = (int)(s_rest / n);
+        blk = (int)(s_rest - (long long)at * n) * kRound;
+    }
     bool first = true;
-    const uint32_t ring = smem_at(smem) + warp * (Ring<D>::kStages * Ring<D>::kStage);
+    const uint32_t ring = smem_at(smem) + warp * (R::kStages * R::kStage);
     // where this lane's 16-byte units of a block go: row r's unit u beside others' so that loads meet all banks
+    constexpr int kUnits = D / 32;  // of a lane
     const int units = d / 16;
-    uint32_t to_k[D / 32], to_v[D / 32];
+    uint32_t to_k[kUnits], to_v[kUnits];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
+    for (int i = 0; i < kUnits; ++i) {
         const int x = lane + 32 * i, r = x / units, u = x - r * units;
         to_k[i] = (uint32_t)(r * D + (u ^ (D == 128 ? (r & 1) << 2 : 0)) * 16);
-        to_v[i] = (uint32_t)(kBlock * D + r * D + (u ^ (D == 128 ? r & 7 : (r >> 1) & 3)) * 16);
+        to_v[i] = (uint32_t)(R::kHalf + r * D + (u ^ (D == 128 ? r & 7 : (r >> 1) & 3)) * 16);
     }
+    const uint32_t at_k = (uint32_t)(g * D + ((c ^ (D == 128 ? (g & 1) << 2 : 0)) << 4));  // (rows g and g + 8 alike)
+    const int vr = lane & 15;
+    // lanes 0-7, 8-15: positions 0-7, 8-15 of an even unit; 16-23, 24-31: of the next one
+    const uint32_t at_v = (uint32_t)(R::kHalf + vr * D), swizzle_v = D == 128 ? vr & 7 : (vr >> 1) & 3;
     const int page_blocks = a.c.page_tokens / kBlock;
 
 #pragma unroll 1
@@ -239,42 +255,105 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
             continue;
         }
         const int h = at / shape.tiles, tile = at - h * shape.tiles;
-        const int count = (int)(left < all - blk ? left : all - blk);
+        const int rounds = (all - blk + kRound - 1) / kRound;
+        const int take = (int)(left < rounds ? left : rounds);
+        const int count = min(all - blk, take * kRound);
         const int row0 = tile * kRows, rows = min(kRows, shape.rows - row0);
 
-        // queries: lane (g, c) holds of row g the dimensions 64 i + 16 c .. + 15 as fp16, and its factor
-        uint32_t qf[NT][kChunks][8];
+        // this warp's steps: blocks blk + 2 warp, + 8, .. and the one behind each
+        const int mine = (count - warp * kStep + kRound - 1) / kRound;
+        const int first_blk = blk + warp * kStep;
+        // a lane knows a block of one turn of 16 steps; -1: no page, or behind the last
+        auto numbers = [&](int turn) {
+            const int p = first_blk + (turn * 16 + (lane >> 1)) * kRound + (lane & 1);
+            if (p >= blk + count)
+                return -1;
+            const int page = page_of(a.c, b, p * kBlock);
+            if (page < 0) {
+                *(volatile int*)a.status = ERR_PAGE;
+                return -1;
+            }
+            return (page * a.c.kv_heads + h) * page_blocks + p % page_blocks;
+        };
+        int now = numbers(0), next = mine > 16 ? numbers(1) : -1;
+        uint32_t there = 0;  // blocks of the stages on their way, two bits each, the newest lowest
+        uint32_t stage_in = ring;
+        auto ask = [&](int i) {
+            if (i < mine) {
+                if (i && (i & 15) == 0) {
+                    now = next;
+                    next = numbers((i >> 4) + 1);
+                }
+                const int n0 = __shfl_sync(0xffffffffu, now, 2 * (i & 15)), n1 = __shfl_sync(0xffffffffu, now, 2 * (i & 15) + 1);
+                there = there << 2 | (n0 >= 0 ? 1u : 0u) | (n1 >= 0 ? 2u : 0u);
+                auto block = [&](int number, int half) {
+                    const long long off = (long long)number * (kBlock * d) + lane * 16;
+                    const int8_t *k = a.c.k + off, *v = a.c.v + off;
+                    const uint32_t to = stage_in + half * (kBlock * D);
+#pragma unroll
+                    for (int j = 0; j < kUnits; ++j)
+                        if (FULL || lane + 32 * j < d) {
+                            copy16(to + to_k[j], k + 512 * j);
+                            copy16(to + to_v[j], v + 512 * j);
+                        }
+                };
+                if (n0 >= 0)
+                    block(n0, 0);
+                if (n1 >= 0)
+                    block(n1, 1);
+                const int n = lane & 1 ? n1 : n0;
+                if (lane < 4 && n >= 0)
+                    copy4(stage_in + 2 * R::kHalf + lane * 4, (lane & 2 ? a.c.v_scales : a.c.k_scales) + n);
+                stage_in = stage_in + R::kStage == ring + R::kStages * R::kStage ? ring : stage_in + R::kStage;
+            }
+            copies_end();
+        };
+#pragma unroll
+        for (int i = 0; i < R::kStages - 1; ++i)
+            ask(i);
+
+        // queries: lane (g, c) holds of row g the dimensions 64 i + 16 c .. + 15, and its factor
+        uint32_t qf[NT][kPlanes][kChunks][4];
         float f0[NT], f1[NT];
         int lim0[NT], lim1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = nt * 8 + g;
-            float x[kChunks][16];
+            float x[kChunks][4][4];
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 const int dim = 64 * i + 16 * c;
                 uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-                if (r < rows && dim < d) {
+                if (r < rows && (FULL || dim < d)) {
                     const long long p = row_at(a, a.q, group, b, h, row0 + r) + dim;
                     lo = load8<VEC>(a.q.p, p);
                     hi = load8<VEC>(a.q.p, p + 8);
                 }
-                Vec<T>::unpack(lo, *reinterpret_cast<float(*)[8]>(&x[i][0]));
-                Vec<T>::unpack(hi, *reinterpret_cast<float(*)[8]>(&x[i][8]));
+                Vec<T>::unpack(lo, &x[i][0][0]);
+                Vec<T>::unpack(hi, &x[i][2][0]);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    most = max(most, magnitude(x[i][e]));
+                    most = max(most, magnitude(x[i][e / 4][e % 4]));
             }
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const int e = exponent_of(most);
-            const float down = power_of_two(-e), factor = __fmul_rn(power_of_two(e), a.scale_log2);
+            const bool finite = most < 0x7f800000u;
+            const int shift = min(126, 21 - e);
+            const float up = finite ? power_of_two(shift) : 0.f;
+            // (a row with a NaN or an infinity has no whole numbers: all of it is NaN)
+            const float factor = finite ? __fmul_rn(power_of_two(-shift), a.scale_log2) : __uint_as_float(0x7fffffffu);
 #pragma unroll
             for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    qf[nt][i][j] = pack_f16(__fmul_rn(x[i][2 * j], down), __fmul_rn(x[i][2 * j + 1], down));
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t w[kPlanes];
+                    planes_of(x[i][j], up, w);
+#pragma unroll
+                    for (int p = 0; p < kPlanes; ++p)
+                        qf[nt][p][i][j] = w[p];
+                }
             f0[nt] = __shfl_sync(0xffffffffu, factor, 8 * c);
             f1[nt] = __shfl_sync(0xffffffffu, factor, 8 * c + 4);
             // positions that rows 2 c and 2 c + 1 of this tile see
@@ -286,119 +365,91 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
         float o[NT][kTiles][4], m0[NT], m1[NT], l0[NT], l1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            m0[nt] = m1[nt] = __uint_as_float(0xff800000u);
+            m0[nt] = m1[nt] = none;
             l0[nt] = l1[nt] = 0.f;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
                 o[nt][t][0] = o[nt][t][1] = o[nt][t][2] = o[nt][t][3] = 0.f;
         }
         int top = -121;  // exponent of the largest scale of V so far
-
-        // this warp's blocks: blk + warp, + 8, ..
-        const int mine = (count - warp + kWarps - 1) / kWarps;
-        // a lane knows the block of the cache of one turn of 32; -1: no page
-        auto numbers = [&](int turn) {
-            const int i = turn * 32 + lane;
-            if (i >= mine)
-                return -1;
-            const int p = blk + warp + i * kWarps;
-            const int page = page_of(a.c, b, p * kBlock);
-            if (page < 0) {
-                *(volatile int*)a.status = ERR_PAGE;
-                return -1;
-            }
-            return (page * a.c.kv_heads + h) * page_blocks + p % page_blocks;
-        };
-        int now = numbers(0), next = numbers(1);
-        uint32_t no_page = 0;  // of the stages on their way, newest in bit 0
-        auto ask = [&](int i) {
-            if (i < mine) {
-                if (i && (i & 31) == 0) {
-                    now = next;
-                    next = numbers((i >> 5) + 1);
-                }
-                const int number = __shfl_sync(0xffffffffu, now, i & 31);
-                no_page = no_page << 1 | (number < 0);
-                if (number >= 0) {
-                    const uint32_t stage = ring + (i % Ring<D>::kStages) * Ring<D>::kStage;
-                    const long long off = (long long)number * kBlock * d + lane * 16;
-#pragma unroll
-                    for (int j = 0; j < D / 32; ++j)
-                        if (lane + 32 * j < d) {
-                            copy16(stage + to_k[j], a.c.k + off + 512 * j);
-                            copy16(stage + to_v[j], a.c.v + off + 512 * j);
-                        }
-                    if (lane < 2)
-                        copy4(stage + 2 * kBlock * D + lane * 4, (lane ? a.c.v_scales : a.c.k_scales) + number);
-                }
-            }
-            copies_end();
-        };
-#pragma unroll
-        for (int i = 0; i < Ring<D>::kStages - 1; ++i)
-            ask(i);
+        uint32_t stage = ring;
 
 #pragma unroll 1
         for (int i = 0; i < mine; ++i) {
-            ask(i + Ring<D>::kStages - 1);
-            copies_wait<Ring<D>::kStages - 1>();
+            ask(i + R::kStages - 1);
+            copies_wait<R::kStages - 1>();
             __syncwarp();
-            const uint32_t stage = ring + (i % Ring<D>::kStages) * Ring<D>::kStage;
             // (stages asked for behind this one: those that there are)
-            const bool nothing = no_page >> (min(mine - 1, i + Ring<D>::kStages - 1) - i) & 1;
-            float2 scales = lds_f2(stage + 2 * kBlock * D);
-            if (nothing)
-                scales = make_float2(0.f, 0.f);
-            float s[NT][4];
+            const uint32_t have = there >> 2 * (min(mine - 1, i + R::kStages - 1) - i) & 3;
+            const uint4 sc = lds128(stage + 2 * R::kHalf);
+            const float ks[2] = {have & 1 ? __uint_as_float(sc.x) : 0.f, have & 2 ? __uint_as_float(sc.y) : 0.f};
+            const float vs[2] = {have & 1 ? __uint_as_float(sc.z) : 0.f, have & 2 ? __uint_as_float(sc.w) : 0.f};
+            // scores of positions g and g + 8 of both blocks, rows 2 c and 2 c + 1
+            float s[kStep][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int x = 0; x < kStep; ++x) {
+                int acc[NT][kPlanes][4];
 #pragma unroll
-            for (int k = 0; k < kChunks; ++k) {
-                const int swizzle = D == 128 ? (g & 1) << 2 : 0;  // (rows g and g + 8 alike)
-                const uint4 w0 = lds128(stage + g * D + (((4 * k + c) ^ swizzle) << 4));
-                const uint4 w1 = lds128(stage + (g + 8) * D + (((4 * k + c) ^ swizzle) << 4));
-                const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t x0 = u0[j] ^ 0x80808080u, x1 = u1[j] ^ 0x80808080u;
-                    const uint32_t frag[4] = {two_f16<0x4140>(x0), two_f16<0x4140>(x1), two_f16<0x4342>(x0),
-                                              two_f16<0x4342>(x1)};
+                    for (int p = 0; p < kPlanes; ++p)
+                        acc[nt][p][0] = acc[nt][p][1] = acc[nt][p][2] = acc[nt][p][3] = 0;
+#pragma unroll
+                for (int k = 0; k < kChunks; ++k) {
+                    // (unit 4 k + c: with the swizzle's 4, k and the other half change places)
+                    const uint32_t key = (stage + x * (kBlock * D) + at_k) ^ (k << 6);
+                    const uint4 w0 = lds128(key), w1 = lds128(key + 8 * D);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        mma_f16(s[nt], frag, qf[nt][k][2 * j], qf[nt][k][2 * j + 1]);
+#pragma unroll
+                        for (int p = 0; p < kPlanes; ++p) {
+                            mma_s8(acc[nt][p], w0.x, w1.x, w0.y, w1.y, qf[nt][p][k][0], qf[nt][p][k][1]);
+                            mma_s8(acc[nt][p], w0.z, w1.z, w0.w, w1.w, qf[nt][p][k][2], qf[nt][p][k][3]);
+                        }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float k0 = __fmul_rn(ks[x], f0[nt]), k1 = __fmul_rn(ks[x], f1[nt]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[x][nt][e] = __fmul_rn(__fmaf_rn((float)acc[nt][0][e], 65536.f, (float)(acc[nt][1][e] * 256 + acc[nt][2][e])),
+                                                e & 1 ? k1 : k0);
                 }
             }
-            // scores of positions g and g + 8, rows 2 c and 2 c + 1
-            const int p0 = (blk + warp + i * kWarps) * kBlock;
+            const int p0 = (first_blk + i * kRound) * kBlock;
+            if (p0 + kStep * kBlock > seen_by_all || have != 3) {
+#pragma unroll
+                for (int x = 0; x < kStep; ++x)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int p = p0 + x * kBlock + g + (e & 2 ? 8 : 0);
+                            const bool seen = (have >> x & 1) && p < (e & 1 ? lim1[nt] : lim0[nt]);
+                            s[x][nt][e] = seen ? s[x][nt][e] : none;
+                        }
+            }
             bool raise = false;
+            float n0[NT], n1[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float k0 = __fmul_rn(scales.x, f0[nt]), k1 = __fmul_rn(scales.x, f1[nt]);
-                s[nt][0] = __fmul_rn(s[nt][0], k0), s[nt][1] = __fmul_rn(s[nt][1], k1);
-                s[nt][2] = __fmul_rn(s[nt][2], k0), s[nt][3] = __fmul_rn(s[nt][3], k1);
-                if (p0 + kBlock > seen_by_all || nothing) {
-                    const float hidden = __uint_as_float(0xff800000u);
-                    const int u0 = nothing ? INT32_MIN : lim0[nt], u1 = nothing ? INT32_MIN : lim1[nt];
-                    s[nt][0] = p0 + g < u0 ? s[nt][0] : hidden, s[nt][1] = p0 + g < u1 ? s[nt][1] : hidden;
-                    s[nt][2] = p0 + g + 8 < u0 ? s[nt][2] : hidden, s[nt][3] = p0 + g + 8 < u1 ? s[nt][3] : hidden;
-                }
-                raise |= fmaxf(s[nt][0], s[nt][2]) > m0[nt] + kAhead || fmaxf(s[nt][1], s[nt][3]) > m1[nt] + kAhead;
+                n0[nt] = fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2]));
+                n1[nt] = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3]));
+                raise |= n0[nt] > m0[nt] + kAhead || n1[nt] > m1[nt] + kAhead;
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float n0 = fmaxf(s[nt][0], s[nt][2]), n1 = fmaxf(s[nt][1], s[nt][3]);
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) {
-                        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-                        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+                        n0[nt] = fmaxf(n0[nt], __shfl_xor_sync(0xffffffffu, n0[nt], x));
+                        n1[nt] = fmaxf(n1[nt], __shfl_xor_sync(0xffffffffu, n1[nt], x));
                     }
-                    n0 = fmaxf(n0, m0[nt]), n1 = fmaxf(n1, m1[nt]);
+                    const float t0 = fmaxf(n0[nt], m0[nt]), t1 = fmaxf(n1[nt], m1[nt]);
                     // (nothing seen so far: there is nothing to scale)
-                    const float r0 = n0 == m0[nt] ? 1.f : exp2_fast(m0[nt] - n0);
-                    const float r1 = n1 == m1[nt] ? 1.f : exp2_fast(m1[nt] - n1);
-                    m0[nt] = n0, m1[nt] = n1;
+                    const float r0 = t0 == m0[nt] ? 1.f : exp2_fast(m0[nt] - t0);
+                    const float r1 = t1 == m1[nt] ? 1.f : exp2_fast(m1[nt] - t1);
+                    m0[nt] = t0, m1[nt] = t1;
                     l0[nt] = __fmul_rn(l0[nt], r0), l1[nt] = __fmul_rn(l1[nt], r1);
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
@@ -408,10 +459,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
                 }
             }
             // (a block without a scale makes its sums NaN whatever they count)
-            const uint32_t size = magnitude(scales.y);
-            const int ev = size >= 0x7f800000u ? top : max(-120, (int)(size >> 23) - 127);
+            int ev = top;
+#pragma unroll
+            for (int x = 0; x < kStep; ++x) {
+                const uint32_t size = magnitude(vs[x]);
+                ev = max(ev, size >= 0x7f800000u ? top : max(-120, (int)(size >> 23) - 127));
+            }
             if (ev > top) {
-                // (first block: the sums are zero)
+                // (first step: the sums are zero)
                 const float r = top == -121 ? 1.f : power_of_two(max(-126, top - ev));
                 top = ev;
 #pragma unroll
@@ -422,41 +477,56 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
                         for (int e = 0; e < 4; ++e)
                             o[nt][t][e] *= r;
             }
-            const float lift = __fmul_rn(scales.y, power_of_two(kLift - top));
-            uint32_t pb[NT][2];
+            const float unit = power_of_two(kLift - top);
+            uint32_t hi[kStep][NT][2], lo[kStep][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float none = __uint_as_float(0xff800000u);
                 const float z0 = m0[nt] == none ? 0.f : m0[nt], z1 = m1[nt] == none ? 0.f : m1[nt];
-                float p[4] = {exp2_fast(s[nt][0] - z0), exp2_fast(s[nt][1] - z1), exp2_fast(s[nt][2] - z0),
-                              exp2_fast(s[nt][3] - z1)};
-                l0[nt] += p[0] + p[2], l1[nt] += p[1] + p[3];
-                // (what is not seen stays 0 whatever the block's scale)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    p[e] = p[e] == 0.f ? 0.f : __fmul_rn(p[e], lift);
-                pb[nt][0] = movmatrix_trans(pack_f16(p[0], p[1]));
-                pb[nt][1] = movmatrix_trans(pack_f16(p[2], p[3]));
+                for (int x = 0; x < kStep; ++x) {
+                    const float lift = __fmul_rn(vs[x], unit);
+                    float p[4] = {exp2_fast(s[x][nt][0] - z0), exp2_fast(s[x][nt][1] - z1), exp2_fast(s[x][nt][2] - z0),
+                                  exp2_fast(s[x][nt][3] - z1)};
+                    l0[nt] += p[0] + p[2], l1[nt] += p[1] + p[3];
+                    // (what is not seen stays 0 whatever the block's scale)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        p[e] = p[e] == 0.f ? 0.f : __fmul_rn(p[e], lift);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t w = pack_f16(p[2 * e], p[2 * e + 1]);
+                        hi[x][nt][e] = movmatrix_trans(w);
+                        if constexpr (kFine) {
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                            lo[x][nt][e] = movmatrix_trans(pack_f16(p[2 * e] - back.x, p[2 * e + 1] - back.y));
+                        }
+                    }
+                }
             }
 #pragma unroll
             for (int t = 0; t < kTiles; t += 2) {
-                // lanes 0-7, 8-15: positions 0-7, 8-15 of unit t; 16-23, 24-31: of unit t + 1
-                const int r = lane & 15, u = t + (lane >> 4);
-                uint32_t v[4];
-                ldmatrix_x4_trans(stage + kBlock * D + r * D + ((u ^ (D == 128 ? r & 7 : (r >> 1) & 3)) << 4), v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] ^= 0x80808080u;
+                for (int x = 0; x < kStep; ++x) {
+                    uint32_t v[4];
+                    ldmatrix_x4_trans(stage + x * (kBlock * D) + at_v + (((t + (lane >> 4)) ^ swizzle_v) << 4), v);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t frag[4] = {two_f16<0x4240>(v[2 * x]), two_f16<0x4341>(v[2 * x]),
-                                              two_f16<0x4240>(v[2 * x + 1]), two_f16<0x4341>(v[2 * x + 1])};
+                    for (int e = 0; e < 4; ++e)
+                        v[e] ^= 0x80808080u;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_f16(o[nt][t + x], frag, pb[nt][0], pb[nt][1]);
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t frag[4] = {two_f16<0x4240>(v[2 * y]), two_f16<0x4341>(v[2 * y]),
+                                                  two_f16<0x4240>(v[2 * y + 1]), two_f16<0x4341>(v[2 * y + 1])};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if constexpr (kFine)
+                                mma_f16(o[nt][t + y], frag, lo[x][nt][0], lo[x][nt][1]);
+                            mma_f16(o[nt][t + y], frag, hi[x][nt][0], hi[x][nt][1]);
+                        }
+                    }
                 }
             }
             __syncwarp();
+            stage = stage + R::kStage == ring + R::kStages * R::kStage ? ring : stage + R::kStage;
         }
         copies_wait<0>();
 
@@ -474,10 +544,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
             }
         }
         __syncthreads();  // (nobody reads the rings any more)
-        const int active = min(kWarps, count);
+        const int active = min(kWarps, (count + kStep - 1) / kStep);
         float* sums = (float*)smem;  // [warp][row][kPitch]
         if (warp < active) {
-            const float up = power_of_two(top - kLift < -126 ? -126 : top - kLift);
+            const float up = power_of_two(max(-126, top - kLift));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -493,10 +563,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
         const long long part = ((long long)blockIdx.x * 2 + !first) * kRows;
         for (int i = tid; i < rows * d; i += kThreads) {
             const int r = i / d, e = i - r * d;
-            float m = __uint_as_float(0xff800000u);
+            float m = none;
             for (int w = 0; w < active; ++w)
                 m = fmaxf(m, s_stats[w][r].x);
-            const float z = m == __uint_as_float(0xff800000u) ? 0.f : m;
+            const float z = m == none ? 0.f : m;
             float sum = 0.f, total = 0.f;
             for (int w = 0; w < active; ++w) {
                 const float2 st = s_stats[w][r];
@@ -515,60 +585,110 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) cache_kernel(const 
         }
         __syncthreads();
         first = false;
-        left -= count;
+        left -= take;
         blk = 0;
         if (++at == lines) {
             at = 0;
             ++b;
         }
     }
+    // sequences without a position: nothing is seen
+    for (b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
+        if (a.lengths[b] > shape.capacity && tid == 0)
+            *(volatile int*)a.status = ERR_PAGE;
+        if (a.lengths[b] <= 0)
+            for (int i = tid; i < a.queries * a.heads * d; i += kThreads) {
+                const int e = i % d, th = i / d;
+                ((T*)a.out.p)[((long long)b * a.queries + th / a.heads) * a.out.token_stride +
+                              (long long)(th % a.heads) * a.out.head_stride + e] = from_float<T>(0.f);
+            }
+    }
 }
 
-// A row of a head whose blocks were cut: the parts in their order
+// A row of a head whose rounds were cut: the parts in their order, shared out over groups of D threads
+constexpr int kJoinThreads = 512, kJoinParts = 512;
 template <class T, int D>
-__global__ void __launch_bounds__(D) join_kernel(const CacheArgs a, const Shape shape, int ctas, int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const CacheArgs a, const Shape shape, int ctas, int tile_rows) {
+    constexpr int kGroups = kJoinThreads / D;
     __shared__ long long s_before, s_total;
+    __shared__ float s_max[kJoinThreads / 32], s_factor[kJoinParts], s_sum[kGroups][D];
     const int lines = a.c.kv_heads * shape.tiles;
     const int b = blockIdx.x / lines, at = blockIdx.x - b * lines;
     const int h = at / shape.tiles, tile = at - h * shape.tiles;
-    const int r = blockIdx.y, row = tile * tile_rows + r, e = threadIdx.x;
-    pdl_start();
-    if (threadIdx.x < 32) {
+    const int r = blockIdx.y, row = tile * tile_rows + r;
+    const int tid = threadIdx.x, e = tid % D, mine = tid / D;
+    const float none = __uint_as_float(0xff800000u);
+    // (lengths are not the kernel's in front, and all others have ended: see pdl.h)
+    if (tid < 32) {
         long long total = 0, before = 0;
         for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-            const int i = b0 + (int)threadIdx.x;
-            const int n = i < a.c.batch ? blocks_of(a, shape.capacity, i) : 0;
+            const int i = b0 + tid, n = rounds_of(a, shape.capacity, i);
             total += __reduce_add_sync(0xffffffffu, n);
             before += __reduce_add_sync(0xffffffffu, i < b ? n : 0);
         }
-        if (threadIdx.x == 0)
+        if (tid == 0)
             s_before = before * lines, s_total = total * lines;
     }
     __syncthreads();
-    const int blocks = blocks_of(a, shape.capacity, b);
-    if (blocks == 0 || row >= shape.rows || e >= a.c.d)
-        return;
-    const long long quota = quota_of(s_total, ctas);
-    const long long from = s_before + (long long)at * blocks, to = from + blocks - 1;
+    const int rounds = rounds_of(a, shape.capacity, b);
+    long long quota = 1, from = 0, to = 0;
+    if (rounds > 0) {
+        quota = quota_of(s_total, ctas);
+        from = s_before + (long long)at * rounds, to = from + rounds - 1;
+    }
     const int c0 = (int)(from / quota), c1 = (int)(to / quota);
-    if (c0 == c1)
+    pdl_start();
+    if (rounds == 0 || row >= shape.rows || c0 == c1)
         return;
     const Parts parts = parts_of(a.workspace, ctas, tile_rows, D);
     const long long first = ((long long)c0 * 2 + (c0 * quota < from)) * tile_rows + r;
     auto part = [&](int c) { return c == c0 ? first : (long long)c * 2 * tile_rows + r; };
-    float m = __uint_as_float(0xff800000u);
-#pragma unroll 8
-    for (int c = c0; c <= c1; ++c)
+    float m = none;
+    for (int c = c0 + tid; c <= c1; c += kJoinThreads)
         m = fmaxf(m, parts.stats[part(c)].x);
-    const float z = m == __uint_as_float(0xff800000u) ? 0.f : m;
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2)
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    if ((tid & 31) == 0)
+        s_max[tid >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kJoinThreads / 32; ++x)
+        m = fmaxf(m, s_max[x]);
+    const float z = m == none ? 0.f : m;
     float sum = 0.f, total = 0.f;
+    for (int base = c0; base <= c1; base += kJoinParts) {
+        const int n = min(kJoinParts, c1 + 1 - base);
+        __syncthreads();
+        float weight = 0.f;
+        if (tid < n) {
+            const float2 st = parts.stats[part(base + tid)];
+            const float f = exp2_fast(st.x - z);
+            s_factor[tid] = f;
+            weight = st.y * f;
+        }
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2)
+            weight += __shfl_xor_sync(0xffffffffu, weight, x);
+        total += weight;
+        __syncthreads();
 #pragma unroll 8
-    for (int c = c0; c <= c1; ++c) {
-        const float2 st = parts.stats[part(c)];
-        const float f = exp2_fast(st.x - z);
-        total += st.y * f;
-        sum += parts.sums[part(c) * D + e] * f;
+        for (int i = mine; i < n; i += kGroups)
+            sum += parts.sums[part(base + i) * D + e] * s_factor[i];
     }
+    s_sum[mine][e] = sum;
+    if ((tid & 31) == 0)
+        s_max[tid >> 5] = total;
+    __syncthreads();
+    if (mine || e >= a.c.d)
+        return;
+    sum = total = 0.f;
+#pragma unroll
+    for (int x = 0; x < kGroups; ++x)
+        sum += s_sum[x][e];
+#pragma unroll
+    for (int x = 0; x < kJoinThreads / 32; ++x)
+        total += s_max[x];
     const int group = a.heads / a.c.kv_heads;
     ((T*)a.out.p)[row_at(a, a.out, group, b, h, row) + e] = from_float<T>(total == 0.f ? 0.f : __fdiv_rn(sum, total));
 }
@@ -576,7 +696,7 @@ __global__ void __launch_bounds__(D) join_kernel(const CacheArgs a, const Shape 
 // How a call is launched: by its sizes alone, so that a captured one serves any lengths
 struct Plan {
     int d, nt, rows, tiles, ctas;
-    long long capacity, most;  // positions of a table, blocks in all that a call may have
+    long long capacity, most;  // positions of a table, rounds that a call may have
     size_t bytes;
 };
 Plan plan_of(const mb200_kv_cache& c, int heads, int queries) {
@@ -588,37 +708,38 @@ Plan plan_of(const mb200_kv_cache& c, int heads, int queries) {
     p.capacity = (long long)c.table_pages * c.page_tokens;
     if (p.capacity > 0x7fffffff - kBlock)
         p.capacity = 0x7fffffff - kBlock;
-    p.most = (p.capacity + kBlock - 1) / kBlock * c.batch * c.kv_heads * p.tiles;
-    const long long useful = (p.most + kLeast - 1) / kLeast, resident = umma::sm_count() * (p.nt == 1 ? 2 : 1);
-    p.ctas = (int)(useful < resident ? useful : resident);
+    p.most = (p.capacity + kRound * kBlock - 1) / (kRound * kBlock) * c.batch * c.kv_heads * p.tiles;
+    const long long resident = umma::sm_count() * kCtasPerSm;
+    p.ctas = (int)(p.most < resident ? p.most : resident);
     if (p.ctas < 1)
         p.ctas = 1;
     p.bytes = p.ctas == 1 ? 0 : align_up((size_t)p.ctas * 2 * 8 * p.nt * (p.d + 2) * sizeof(float), 256);
     return p;
 }
 
-template <class T, int D, int NT, bool VEC>
+template <class T, int D, int NT, bool VEC, bool FULL>
 int launch(const CacheArgs& a, const Plan& p, cudaStream_t st) {
     constexpr int kSums = kWarps * 8 * NT * kPitch<D> * 4;
     constexpr int kSmem = Ring<D>::kBytes > kSums ? Ring<D>::kBytes : kSums;
+    const auto kernel = cache_kernel<T, D, NT, VEC, FULL>;
     const Shape shape{p.rows, p.tiles, (int)p.capacity};
     static umma::KernelReady ready;
-    if (!ready.smem(cache_kernel<T, D, NT, VEC>, kSmem))
+    if (!ready.smem(kernel, kSmem))
         return refused("attention_cache_s8", cudaGetLastError());
     const Writes anything{nullptr, SIZE_MAX};
-    cudaError_t e = launch_pdl(anything, cache_kernel<T, D, NT, VEC>, dim3((unsigned)p.ctas), dim3(kThreads), kSmem, st, a,
-                               shape);
+    cudaError_t e = launch_pdl(anything, kernel, dim3((unsigned)p.ctas), dim3(kThreads), kSmem, st, a, shape);
     if (e == cudaSuccess && p.ctas > 1)
         e = launch_pdl(anything, join_kernel<T, D>,
                        dim3((unsigned)(a.c.batch * a.c.kv_heads * p.tiles), (unsigned)(p.rows < 8 * NT ? p.rows : 8 * NT)),
-                       dim3(D), 0, st, a, shape, p.ctas, 8 * NT);
+                       dim3(kJoinThreads), 0, st, a, shape, p.ctas, 8 * NT);
     return e != cudaSuccess ? refused("attention_cache_s8", e) : check_launch("attention_cache_s8");
 }
 template <class T, int D>
 int launch_rows(const CacheArgs& a, const Plan& p, bool vec, cudaStream_t st) {
+    // (odd heads and queries at odd places by one variant: either costs a few per cent)
     if (p.nt == 1)
-        return vec ? launch<T, D, 1, true>(a, p, st) : launch<T, D, 1, false>(a, p, st);
-    return vec ? launch<T, D, 2, true>(a, p, st) : launch<T, D, 2, false>(a, p, st);
+        return vec && a.c.d == D ? launch<T, D, 1, true, true>(a, p, st) : launch<T, D, 1, false, false>(a, p, st);
+    return vec && a.c.d == D ? launch<T, D, 2, true, true>(a, p, st) : launch<T, D, 2, false, false>(a, p, st);
 }
 
 }  // namespace
