@@ -605,92 +605,141 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
     }
 }
 
-// A row of a head whose rounds were cut: the parts in their order, shared out over groups of D threads
+// Joins the parts of what was cut, in their order: for each item (a sequence's key head and tile of rows), or, where there are more
+// of those than CTAs, for each CTA whose part of the line begins inside an item, the first of that item. With many parts to
+// an item a CTA has one row and its groups of D threads share the parts; else each group has a row of its own.
 constexpr int kJoinThreads = 512, kJoinParts = 512;
 template <class T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const CacheArgs a, const Shape shape, int ctas, int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(
+        const CacheArgs a, const Shape shape, int ctas, int tile_rows, int by_item, int share) {
     constexpr int kGroups = kJoinThreads / D;
     __shared__ long long s_before, s_total;
+    __shared__ int s_b;
     __shared__ float s_max[kJoinThreads / 32], s_factor[kJoinParts], s_sum[kGroups][D];
     const int lines = a.c.kv_heads * shape.tiles;
-    const int b = blockIdx.x / lines, at = blockIdx.x - b * lines;
-    const int h = at / shape.tiles, tile = at - h * shape.tiles;
-    const int r = blockIdx.y, row = tile * tile_rows + r;
     const int tid = threadIdx.x, e = tid % D, mine = tid / D;
+    const int cut = blockIdx.x + 1;
     const float none = __uint_as_float(0xff800000u);
     // (lengths are not the kernel's in front, and all others have ended: see pdl.h)
     if (tid < 32) {
         long long total = 0, before = 0;
-        for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-            const int i = b0 + tid, n = rounds_of(a, shape.capacity, i);
-            total += __reduce_add_sync(0xffffffffu, n);
-            before += __reduce_add_sync(0xffffffffu, i < b ? n : 0);
+        int b = -1;
+        for (int b0 = 0; b0 < a.c.batch; b0 += 32)
+            total += __reduce_add_sync(0xffffffffu, rounds_of(a, shape.capacity, b0 + tid));
+        total *= lines;
+        const long long position = cut * quota_of(total, ctas);
+        if (by_item) {
+            b = blockIdx.x / lines;
+            for (int b0 = 0; b0 < b; b0 += 32)
+                before += __reduce_add_sync(0xffffffffu, b0 + tid < b ? rounds_of(a, shape.capacity, b0 + tid) : 0);
+        }
+        for (int b0 = 0; b0 < a.c.batch && position < total && !by_item; b0 += 32) {
+            const int n = rounds_of(a, shape.capacity, b0 + tid);
+            int sum = n;
+#pragma unroll
+            for (int s = 1; s < 32; s *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, s);
+                sum += tid >= s ? v : 0;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, (before + sum) * lines > position);
+            if (beyond) {
+                const int i = __ffs(beyond) - 1;
+                before += __shfl_sync(0xffffffffu, sum - n, i);
+                b = b0 + i;
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (tid == 0)
-            s_before = before * lines, s_total = total * lines;
+            s_before = before * lines, s_total = total, s_b = b;
     }
     __syncthreads();
-    const int rounds = rounds_of(a, shape.capacity, b);
+    const int b = s_b;
     long long quota = 1, from = 0, to = 0;
+    int at = 0;
+    const int rounds = b < 0 ? 0 : rounds_of(a, shape.capacity, b);
     if (rounds > 0) {
         quota = quota_of(s_total, ctas);
+        at = by_item ? (int)blockIdx.x - b * lines : (int)((cut * quota - s_before) / rounds);
         from = s_before + (long long)at * rounds, to = from + rounds - 1;
     }
     const int c0 = (int)(from / quota), c1 = (int)(to / quota);
     pdl_start();
-    if (rounds == 0 || row >= shape.rows || c0 == c1)
+    if (c0 == c1 || (!by_item && (from == cut * quota || c0 + 1 != cut)))
         return;
+    const int h = at / shape.tiles, tile = at - h * shape.tiles;
+    const int rows = min(tile_rows, shape.rows - tile * tile_rows);
+    const int r = share ? (int)blockIdx.y : (int)blockIdx.y * kGroups + mine;
+    const int groups = share ? kGroups : 1, group_at = share ? mine : 0;
     const Parts parts = parts_of(a.workspace, ctas, tile_rows, D);
-    const long long first = ((long long)c0 * 2 + (c0 * quota < from)) * tile_rows + r;
-    auto part = [&](int c) { return c == c0 ? first : (long long)c * 2 * tile_rows + r; };
-    float m = none;
-    for (int c = c0 + tid; c <= c1; c += kJoinThreads)
-        m = fmaxf(m, parts.stats[part(c)].x);
-#pragma unroll
-    for (int x = 1; x < 32; x *= 2)
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    if ((tid & 31) == 0)
-        s_max[tid >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < kJoinThreads / 32; ++x)
-        m = fmaxf(m, s_max[x]);
-    const float z = m == none ? 0.f : m;
-    float sum = 0.f, total = 0.f;
-    for (int base = c0; base <= c1; base += kJoinParts) {
-        const int n = min(kJoinParts, c1 + 1 - base);
-        __syncthreads();
-        float weight = 0.f;
-        if (tid < n) {
-            const float2 st = parts.stats[part(base + tid)];
-            const float f = exp2_fast(st.x - z);
-            s_factor[tid] = f;
-            weight = st.y * f;
-        }
+    const long long first = ((long long)c0 * 2 + (c0 * quota < from)) * tile_rows;
+    auto part = [&](int c) { return (c == c0 ? first : (long long)c * 2 * tile_rows) + r; };
+    float sum = 0.f, total = 0.f, m = none;
+    if (share) {
+        if (r >= rows)
+            return;
+        for (int c = c0 + tid; c <= c1; c += kJoinThreads)
+            m = fmaxf(m, parts.stats[part(c)].x);
 #pragma unroll
         for (int x = 1; x < 32; x *= 2)
-            weight += __shfl_xor_sync(0xffffffffu, weight, x);
-        total += weight;
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        if ((tid & 31) == 0)
+            s_max[tid >> 5] = m;
         __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kJoinThreads / 32; ++x)
+            m = fmaxf(m, s_max[x]);
+        const float z = m == none ? 0.f : m;
+        for (int base = c0; base <= c1; base += kJoinParts) {
+            const int n = min(kJoinParts, c1 + 1 - base);
+            __syncthreads();
+            float weight = 0.f;
+            if (tid < n) {
+                const float2 st = parts.stats[part(base + tid)];
+                const float f = exp2_fast(st.x - z);
+                s_factor[tid] = f;
+                weight = st.y * f;
+            }
+#pragma unroll
+            for (int x = 1; x < 32; x *= 2)
+                weight += __shfl_xor_sync(0xffffffffu, weight, x);
+            total += weight;
+            __syncthreads();
 #pragma unroll 8
-        for (int i = mine; i < n; i += kGroups)
-            sum += parts.sums[part(base + i) * D + e] * s_factor[i];
+            for (int i = group_at; i < n; i += groups)
+                sum += parts.sums[part(base + i) * D + e] * s_factor[i];
+        }
+        s_sum[mine][e] = sum;
+        if ((tid & 31) == 0)
+            s_max[tid >> 5] = total;
+        __syncthreads();
+        if (mine)
+            return;
+        sum = total = 0.f;
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x)
+            sum += s_sum[x][e];
+#pragma unroll
+        for (int x = 0; x < kJoinThreads / 32; ++x)
+            total += s_max[x];
+    } else {
+        if (r >= rows)
+            return;
+#pragma unroll 8
+        for (int c = c0; c <= c1; ++c)
+            m = fmaxf(m, parts.stats[part(c)].x);
+        const float z = m == none ? 0.f : m;
+#pragma unroll 8
+        for (int c = c0; c <= c1; ++c) {
+            const float2 st = parts.stats[part(c)];
+            const float f = exp2_fast(st.x - z);
+            total += st.y * f;
+            sum += parts.sums[part(c) * D + e] * f;
+        }
     }
-    s_sum[mine][e] = sum;
-    if ((tid & 31) == 0)
-        s_max[tid >> 5] = total;
-    __syncthreads();
-    if (mine || e >= a.c.d)
-        return;
-    sum = total = 0.f;
-#pragma unroll
-    for (int x = 0; x < kGroups; ++x)
-        sum += s_sum[x][e];
-#pragma unroll
-    for (int x = 0; x < kJoinThreads / 32; ++x)
-        total += s_max[x];
-    const int group = a.heads / a.c.kv_heads;
-    ((T*)a.out.p)[row_at(a, a.out, group, b, h, row) + e] = from_float<T>(total == 0.f ? 0.f : __fdiv_rn(sum, total));
+    if (e < a.c.d)
+        ((T*)a.out.p)[row_at(a, a.out, a.heads / a.c.kv_heads, b, h, tile * tile_rows + r) + e] =
+                from_float<T>(total == 0.f ? 0.f : __fdiv_rn(sum, total));
 }
 
 // How a call is launched: by its sizes alone, so that a captured one serves any lengths
@@ -728,10 +777,14 @@ int launch(const CacheArgs& a, const Plan& p, cudaStream_t st) {
         return refused("attention_cache_s8", cudaGetLastError());
     const Writes anything{nullptr, SIZE_MAX};
     cudaError_t e = launch_pdl(anything, kernel, dim3((unsigned)p.ctas), dim3(kThreads), kSmem, st, a, shape);
-    if (e == cudaSuccess && p.ctas > 1)
+    if (e == cudaSuccess && p.ctas > 1) {
+        const int rows = p.rows < 8 * NT ? p.rows : 8 * NT, groups = kJoinThreads / D;
+        const long long items = (long long)a.c.batch * a.c.kv_heads * p.tiles;
+        const bool by_item = items < p.ctas, share = items * 8 <= p.ctas;
         e = launch_pdl(anything, join_kernel<T, D>,
-                       dim3((unsigned)(a.c.batch * a.c.kv_heads * p.tiles), (unsigned)(p.rows < 8 * NT ? p.rows : 8 * NT)),
-                       dim3(kJoinThreads), 0, st, a, shape, p.ctas, 8 * NT);
+                       dim3((unsigned)(by_item ? items : p.ctas - 1), (unsigned)(share ? rows : (rows + groups - 1) / groups)),
+                       dim3(kJoinThreads), 0, st, a, shape, p.ctas, 8 * NT, (int)by_item, (int)share);
+    }
     return e != cudaSuccess ? refused("attention_cache_s8", e) : check_launch("attention_cache_s8");
 }
 template <class T, int D>
