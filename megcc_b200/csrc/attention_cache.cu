@@ -9,7 +9,7 @@
 // instructions decides whether that is reached. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that positions
 // and dimensions fill the 16 rows of an mma.sync and 8 query rows its 8 columns: half the instructions and accumulators of
 // the other way round for groups of up to 8.
-//   S: keys are multiplied as they lie, int8 by int8 (m16n8k32, as fast as fp16's k16): queries become whole numbers of 23 bits
+//   S: keys are multiplied as they lie, int8 by int8 (m16n8k32, as fast as fp16's k16): queries become whole numbers of 22 bits
 // of their row's power of two, three planes of int8, whose sums are exact. The order of dimensions within a sum is free:
 // a lane takes 16 neighbouring ones with one load.
 //   O: values become fp16, which holds them exactly: a byte permutation makes 1024 + (v + 128) of them, and a subtraction v.
@@ -137,14 +137,25 @@ __device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) {
     return e == 0 || e == 255 ? 0 : max(-120, min(120, e - 127));
 }
 
-// rows of the workspace's parts: [cta][first or last][row][D] sums, then [..][row] maxima and totals
+// The workspace: sums [cta][first or last][row][D] of what was cut, then [..][row] maxima and totals, then for each CTA
+// the item (a sequence's key head and tile of rows) inside which its part of the line begins
+struct Cut {
+    int b, at;              // b < 0: it begins with an item, or there is none
+    long long from, quota;  // the item's place in the line; rounds of a CTA
+    int rounds, unused;
+};
 struct Parts {
     float* sums;
     float2* stats;
+    Cut* cuts;
 };
 __host__ __device__ inline Parts parts_of(void* workspace, int ctas, int rows, int d) {
     float* p = (float*)workspace;
-    return Parts{p, (float2*)(p + (size_t)ctas * 2 * rows * d)};
+    const size_t n = (size_t)ctas * 2 * rows;
+    return Parts{p, (float2*)(p + n * d), (Cut*)(p + n * (d + 2))};
+}
+inline size_t parts_bytes(int ctas, int rows, int d) {
+    return (size_t)ctas * 2 * rows * (d + 2) * sizeof(float) + (size_t)ctas * sizeof(Cut);
 }
 
 // Where row r of a tile lies
@@ -153,31 +164,47 @@ __device__ __forceinline__ long long row_at(const CacheArgs& a, const mb200_head
     return ((long long)b * a.queries + i) * t.token_stride + (long long)(h * group + (r - i * group)) * t.head_stride;
 }
 
-// Queries as whole numbers of 23 bits: hi 2^16 + mid 2^8 + lo times 2^(e - 21), e the exponent of the row's largest
+// Queries as whole numbers Q of 22 bits, hi 2^16 + mid 2^8 + lo (lo, mid in -128 .. 127) times 2^(e - 20), e the exponent of the
+// row's largest: 1.5 * 2^23 + 0x8080 added in the multiplication leaves, in the sum's bytes, lo + 128, mid + 128 and
+// hi + 64 (|hi| < 64).
 constexpr int kPlanes = 3;
 __device__ __forceinline__ void planes_of(const float (&x)[4], float up, uint32_t (&w)[kPlanes]) {
-    uint32_t b[4][kPlanes];
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int q = __float2int_rn(__fmul_rn(x[i], up));
-        const int q1 = (q - (int)(int8_t)q) >> 8;
-        b[i][2] = (uint32_t)q, b[i][1] = (uint32_t)q1, b[i][0] = (uint32_t)((q1 - (int)(int8_t)q1) >> 8);
-    }
-#pragma unroll
-    for (int p = 0; p < kPlanes; ++p)
-        w[p] = __byte_perm(__byte_perm(b[0][p], b[1][p], 0x0040), __byte_perm(b[2][p], b[3][p], 0x0040), 0x5410);
+    for (int i = 0; i < 4; ++i)
+        b[i] = __float_as_uint(__fmaf_rn(x[i], up, 12615808.f));
+    const uint32_t l0 = __byte_perm(b[0], b[1], 0x5140), l1 = __byte_perm(b[2], b[3], 0x5140);
+    const uint32_t h0 = __byte_perm(b[0], b[1], 0x0062), h1 = __byte_perm(b[2], b[3], 0x0062);
+    w[2] = __byte_perm(l0, l1, 0x5410) ^ 0x80808080u;
+    w[1] = __byte_perm(l0, l1, 0x7632) ^ 0x80808080u;
+    const uint32_t t = __byte_perm(h0, h1, 0x5410) ^ 0x40404040u;
+    w[0] = t | (t & 0x40404040u) << 1;
 }
 
-// FULL: d == D
+// 4 results; VEC: they start on an 8-byte boundary
+template <class T, bool VEC>
+__device__ __forceinline__ void store4(void* base, long long at, const float4& v) {
+    uint16_t* p = (uint16_t*)base + at;
+    const uint32_t lo = pack2<T>(v.x, v.y), hi = pack2<T>(v.z, v.w);
+    if constexpr (VEC) {
+        *(uint2*)p = make_uint2(lo, hi);
+    } else {
+        p[0] = (uint16_t)lo, p[1] = (uint16_t)(lo >> 16);
+        p[2] = (uint16_t)hi, p[3] = (uint16_t)(hi >> 16);
+    }
+}
+
+// FULL: d == D; VEC: queries and results start on 16-byte boundaries
 template <class T, int D, int NT, bool VEC, bool FULL>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const CacheArgs a, const Shape shape) {
     using R = Ring<D>;
     constexpr int kRows = 8 * NT, kChunks = D / 64, kTiles = D / 16;
     constexpr bool kFine = std::is_same<T, __half>::value;  // P as two fp16 numbers
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_from, s_to, s_rest;
+    __shared__ long long s_from, s_to, s_rest, s_quota;
     __shared__ int s_b;
     __shared__ float2 s_stats[kWarps][kRows];
+    __shared__ float s_weight[kWarps][kRows];
     const int tid = threadIdx.x, lane = tid & 31, warp = umma::uniform_warp_index();
     const int g = lane >> 2, c = lane & 3;
     const int d = FULL ? D : a.c.d, group = a.heads / a.c.kv_heads;
@@ -218,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             }
         }
         if (lane == 0)
-            s_from = from, s_to = to, s_b = at, s_rest = from - before * lines;
+            s_from = from, s_to = to, s_b = at, s_rest = from - before * lines, s_quota = quota;
     }
     __syncthreads();
     long long left = s_to - s_from;
@@ -227,6 +254,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         const int n = rounds_of(a, shape.capacity, b);
         at = (int)(s_rest / n);
         blk = (int)(s_rest - (long long)at * n) * kRound;
+    }
+    const Parts parts = parts_of(a.workspace, gridDim.x, kRows, D);
+    if (tid == 0 && gridDim.x > 1) {
+        Cut cut{};
+        cut.b = left > 0 && blk > 0 ? b : -1;
+        cut.at = at, cut.from = s_from - blk / kRound, cut.quota = s_quota;
+        cut.rounds = left > 0 ? rounds_of(a, shape.capacity, b) : 0;
+        parts.cuts[blockIdx.x] = cut;
     }
     bool first = true;
     const uint32_t ring = smem_at(smem) + warp * (R::kStages * R::kStage);
@@ -260,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         const int count = min(all - blk, take * kRound);
         const int row0 = tile * kRows, rows = min(kRows, shape.rows - row0);
 
+        const int32_t* table = a.c.block_table + (long long)b * a.c.table_stride;
         // this warp's steps: blocks blk + 2 warp, + 8, .. and the one behind each
         const int mine = (count - warp * kStep + kRound - 1) / kRound;
         const int first_blk = blk + warp * kStep;
@@ -268,12 +304,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             const int p = first_blk + (turn * 16 + (lane >> 1)) * kRound + (lane & 1);
             if (p >= blk + count)
                 return -1;
-            const int page = page_of(a.c, b, p * kBlock);
-            if (page < 0) {
+            const int i = p / page_blocks;
+            const int page = table[i];  // (i < table_pages: lengths end with the table)
+            if ((unsigned)page >= (unsigned)a.c.pages) {
                 *(volatile int*)a.status = ERR_PAGE;
                 return -1;
             }
-            return (page * a.c.kv_heads + h) * page_blocks + p % page_blocks;
+            return (page * a.c.kv_heads + h) * page_blocks + p - i * page_blocks;
         };
         int now = numbers(0), next = mine > 16 ? numbers(1) : -1;
         uint32_t there = 0;  // blocks of the stages on their way, two bits each, the newest lowest
@@ -340,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const int e = exponent_of(most);
             const bool finite = most < 0x7f800000u;
-            const int shift = min(126, 21 - e);
+            const int shift = min(126, 20 - e);
             const float up = finite ? power_of_two(shift) : 0.f;
             // (a row with a NaN or an infinity has no whole numbers: all of it is NaN)
             const float factor = finite ? __fmul_rn(power_of_two(-shift), a.scale_log2) : __uint_as_float(0x7fffffffu);
@@ -557,31 +594,45 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
                     *(float2*)(p + kPitch<D>) = make_float2(o[nt][t][1] * up, o[nt][t][3] * up);
                 }
         }
-        __syncthreads();
+        // each warp's weight in a row: what its maximum lies below the largest, over the total where that is all of it
         const bool whole = blk == 0 && count == all;
-        const Parts parts = parts_of(a.workspace, gridDim.x, kRows, D);
-        const long long part = ((long long)blockIdx.x * 2 + !first) * kRows;
-        for (int i = tid; i < rows * d; i += kThreads) {
-            const int r = i / d, e = i - r * d;
+        if (tid < kRows) {
             float m = none;
-            for (int w = 0; w < active; ++w)
-                m = fmaxf(m, s_stats[w][r].x);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                m = fmaxf(m, w < active ? s_stats[w][tid].x : none);
             const float z = m == none ? 0.f : m;
-            float sum = 0.f, total = 0.f;
-            for (int w = 0; w < active; ++w) {
-                const float2 st = s_stats[w][r];
-                const float f = exp2_fast(st.x - z);
-                total += st.y * f;
-                sum += sums[(w * kRows + r) * kPitch<D> + e] * f;
+            float total = 0.f, f[kWarps];
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 st = s_stats[w][tid];
+                f[w] = w < active ? exp2_fast(st.x - z) : 0.f;
+                total += w < active ? st.y * f[w] : 0.f;
             }
-            if (whole) {
-                ((T*)a.out.p)[row_at(a, a.out, group, b, h, row0 + r) + e] =
-                        from_float<T>(total == 0.f ? 0.f : __fdiv_rn(sum, total));
-            } else {
-                parts.sums[(part + r) * D + e] = sum;
-                if (e == 0)
-                    parts.stats[part + r] = make_float2(m, total);
-            }
+            // (nothing seen: zeros)
+            const float over = !whole ? 1.f : total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                s_weight[w][tid] = __fmul_rn(f[w], over);
+            if (!whole)
+                parts.stats[((long long)blockIdx.x * 2 + !first) * kRows + tid] = make_float2(m, total);
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), e = i % (D / 4) * 4;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                if (w < active) {
+                    const float4 v = *(const float4*)(sums + (w * kRows + r) * kPitch<D> + e);
+                    const float f = s_weight[w][r];
+                    sum.x = __fmaf_rn(v.x, f, sum.x), sum.y = __fmaf_rn(v.y, f, sum.y);
+                    sum.z = __fmaf_rn(v.z, f, sum.z), sum.w = __fmaf_rn(v.w, f, sum.w);
+                }
+            if (!whole)
+                *(float4*)(parts.sums + (((long long)blockIdx.x * 2 + !first) * kRows + r) * D + e) = sum;
+            else if (FULL || e < d)
+                store4<T, VEC>(a.out.p, row_at(a, a.out, group, b, h, row0 + r) + e, sum);
         }
         __syncthreads();
         first = false;
@@ -605,141 +656,71 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
     }
 }
 
-// Joins the parts of what was cut, in their order: for each item (a sequence's key head and tile of rows), or, where there are more
-// of those than CTAs, for each CTA whose part of the line begins inside an item, the first of that item. With many parts to
-// an item a CTA has one row and its groups of D threads share the parts; else each group has a row of its own.
-constexpr int kJoinThreads = 512, kJoinParts = 512;
-template <class T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(
-        const CacheArgs a, const Shape shape, int ctas, int tile_rows, int by_item, int share) {
-    constexpr int kGroups = kJoinThreads / D;
-    __shared__ long long s_before, s_total;
-    __shared__ int s_b;
-    __shared__ float s_max[kJoinThreads / 32], s_factor[kJoinParts], s_sum[kGroups][D];
-    const int lines = a.c.kv_heads * shape.tiles;
-    const int tid = threadIdx.x, e = tid % D, mine = tid / D;
-    const int cut = blockIdx.x + 1;
-    const float none = __uint_as_float(0xff800000u);
-    // (lengths are not the kernel's in front, and all others have ended: see pdl.h)
-    if (tid < 32) {
-        long long total = 0, before = 0;
-        int b = -1;
-        for (int b0 = 0; b0 < a.c.batch; b0 += 32)
-            total += __reduce_add_sync(0xffffffffu, rounds_of(a, shape.capacity, b0 + tid));
-        total *= lines;
-        const long long position = cut * quota_of(total, ctas);
-        if (by_item) {
-            b = blockIdx.x / lines;
-            for (int b0 = 0; b0 < b; b0 += 32)
-                before += __reduce_add_sync(0xffffffffu, b0 + tid < b ? rounds_of(a, shape.capacity, b0 + tid) : 0);
-        }
-        for (int b0 = 0; b0 < a.c.batch && position < total && !by_item; b0 += 32) {
-            const int n = rounds_of(a, shape.capacity, b0 + tid);
-            int sum = n;
-#pragma unroll
-            for (int s = 1; s < 32; s *= 2) {
-                const int v = __shfl_up_sync(0xffffffffu, sum, s);
-                sum += tid >= s ? v : 0;
-            }
-            const uint32_t beyond = __ballot_sync(0xffffffffu, (before + sum) * lines > position);
-            if (beyond) {
-                const int i = __ffs(beyond) - 1;
-                before += __shfl_sync(0xffffffffu, sum - n, i);
-                b = b0 + i;
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (tid == 0)
-            s_before = before * lines, s_total = total, s_b = b;
-    }
-    __syncthreads();
-    const int b = s_b;
-    long long quota = 1, from = 0, to = 0;
-    int at = 0;
-    const int rounds = b < 0 ? 0 : rounds_of(a, shape.capacity, b);
-    if (rounds > 0) {
-        quota = quota_of(s_total, ctas);
-        at = by_item ? (int)blockIdx.x - b * lines : (int)((cut * quota - s_before) / rounds);
-        from = s_before + (long long)at * rounds, to = from + rounds - 1;
-    }
-    const int c0 = (int)(from / quota), c1 = (int)(to / quota);
-    pdl_start();
-    if (c0 == c1 || (!by_item && (from == cut * quota || c0 + 1 != cut)))
-        return;
-    const int h = at / shape.tiles, tile = at - h * shape.tiles;
-    const int rows = min(tile_rows, shape.rows - tile * tile_rows);
-    const int r = share ? (int)blockIdx.y : (int)blockIdx.y * kGroups + mine;
-    const int groups = share ? kGroups : 1, group_at = share ? mine : 0;
+// Joins the parts of an item that was cut, in their order: the first CTA whose part of the line begins inside it names it. One
+// row a CTA; its warps share the parts (D / 4 lanes each), all of whose weights every warp finds for itself.
+constexpr int kJoinWarps = 8;
+template <class T, int D, bool VEC>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const CacheArgs a, const Shape shape, int ctas, int tile_rows) {
+    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kStride = kJoinWarps * kAtOnce;
+    __shared__ float4 s_sum[kJoinWarps * kAtOnce][kLanes];
+    const int cta = blockIdx.x + 1, r = blockIdx.y;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Parts parts = parts_of(a.workspace, ctas, tile_rows, D);
-    const long long first = ((long long)c0 * 2 + (c0 * quota < from)) * tile_rows;
-    auto part = [&](int c) { return (c == c0 ? first : (long long)c * 2 * tile_rows) + r; };
-    float sum = 0.f, total = 0.f, m = none;
-    if (share) {
-        if (r >= rows)
-            return;
-        for (int c = c0 + tid; c <= c1; c += kJoinThreads)
-            m = fmaxf(m, parts.stats[part(c)].x);
+    pdl_start();
+    const Cut cut = parts.cuts[cta];
+    if (cut.b < 0)
+        return;
+    const int c0 = (int)(cut.from / cut.quota), c1 = (int)((cut.from + cut.rounds - 1) / cut.quota);
+    const int h = cut.at / shape.tiles, tile = cut.at - h * shape.tiles;
+    if (c0 + 1 != cta || tile * tile_rows + r >= shape.rows)
+        return;
+    const long long first = ((long long)c0 * 2 + (c0 * cut.quota < cut.from)) * tile_rows;
+    auto part = [&](int i) { return (i == 0 ? first : (long long)(c0 + i) * 2 * tile_rows) + r; };
+    const int n = c1 + 1 - c0;
+    const float none = __uint_as_float(0xff800000u);
+    float m = none, total = 0.f;
+    for (int i = lane; i < n; i += 32)
+        m = fmaxf(m, parts.stats[part(i)].x);
 #pragma unroll
-        for (int x = 1; x < 32; x *= 2)
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        if ((tid & 31) == 0)
-            s_max[tid >> 5] = m;
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < kJoinThreads / 32; ++x)
-            m = fmaxf(m, s_max[x]);
-        const float z = m == none ? 0.f : m;
-        for (int base = c0; base <= c1; base += kJoinParts) {
-            const int n = min(kJoinParts, c1 + 1 - base);
-            __syncthreads();
-            float weight = 0.f;
-            if (tid < n) {
-                const float2 st = parts.stats[part(base + tid)];
-                const float f = exp2_fast(st.x - z);
-                s_factor[tid] = f;
-                weight = st.y * f;
-            }
-#pragma unroll
-            for (int x = 1; x < 32; x *= 2)
-                weight += __shfl_xor_sync(0xffffffffu, weight, x);
-            total += weight;
-            __syncthreads();
-#pragma unroll 8
-            for (int i = group_at; i < n; i += groups)
-                sum += parts.sums[part(base + i) * D + e] * s_factor[i];
-        }
-        s_sum[mine][e] = sum;
-        if ((tid & 31) == 0)
-            s_max[tid >> 5] = total;
-        __syncthreads();
-        if (mine)
-            return;
-        sum = total = 0.f;
-#pragma unroll
-        for (int x = 0; x < kGroups; ++x)
-            sum += s_sum[x][e];
-#pragma unroll
-        for (int x = 0; x < kJoinThreads / 32; ++x)
-            total += s_max[x];
-    } else {
-        if (r >= rows)
-            return;
-#pragma unroll 8
-        for (int c = c0; c <= c1; ++c)
-            m = fmaxf(m, parts.stats[part(c)].x);
-        const float z = m == none ? 0.f : m;
-#pragma unroll 8
-        for (int c = c0; c <= c1; ++c) {
-            const float2 st = parts.stats[part(c)];
-            const float f = exp2_fast(st.x - z);
+    for (int x = 1; x < 32; x *= 2)
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    const float z = m == none ? 0.f : m;
+    const int sub = warp * kAtOnce + lane / kLanes, e = lane % kLanes;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = 0; base < n; base += 32) {
+        float f = 0.f;
+        if (base + lane < n) {
+            const float2 st = parts.stats[part(base + lane)];
+            f = exp2_fast(st.x - z);
             total += st.y * f;
-            sum += parts.sums[part(c) * D + e] * f;
+        }
+#pragma unroll 4
+        for (int x = 0; x < 32; x += kStride) {
+            const int i = base + x + sub;
+            const float weight = __shfl_sync(0xffffffffu, f, (x + sub) & 31);
+            if (i < n && x + sub < 32) {
+                const float4 v = *(const float4*)(parts.sums + part(i) * D + 4 * e);
+                sum.x = __fmaf_rn(v.x, weight, sum.x), sum.y = __fmaf_rn(v.y, weight, sum.y);
+                sum.z = __fmaf_rn(v.z, weight, sum.z), sum.w = __fmaf_rn(v.w, weight, sum.w);
+            }
         }
     }
-    if (e < a.c.d)
-        ((T*)a.out.p)[row_at(a, a.out, a.heads / a.c.kv_heads, b, h, tile * tile_rows + r) + e] =
-                from_float<T>(total == 0.f ? 0.f : __fdiv_rn(sum, total));
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2)
+        total += __shfl_xor_sync(0xffffffffu, total, x);
+    s_sum[sub][e] = sum;
+    __syncthreads();
+    if (threadIdx.x >= kLanes || 4 * e >= a.c.d)
+        return;
+    sum = s_sum[0][e];
+#pragma unroll
+    for (int x = 1; x < kJoinWarps * kAtOnce; ++x) {
+        const float4 v = s_sum[x][e];
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const float over = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+    sum.x *= over, sum.y *= over, sum.z *= over, sum.w *= over;
+    store4<T, VEC>(a.out.p, row_at(a, a.out, a.heads / a.c.kv_heads, cut.b, h, tile * tile_rows + r) + 4 * e, sum);
 }
 
 // How a call is launched: by its sizes alone, so that a captured one serves any lengths
@@ -762,7 +743,7 @@ Plan plan_of(const mb200_kv_cache& c, int heads, int queries) {
     p.ctas = (int)(p.most < resident ? p.most : resident);
     if (p.ctas < 1)
         p.ctas = 1;
-    p.bytes = p.ctas == 1 ? 0 : align_up((size_t)p.ctas * 2 * 8 * p.nt * (p.d + 2) * sizeof(float), 256);
+    p.bytes = p.ctas == 1 ? 0 : align_up(parts_bytes(p.ctas, 8 * p.nt, p.d), 256);
     return p;
 }
 
@@ -777,14 +758,10 @@ int launch(const CacheArgs& a, const Plan& p, cudaStream_t st) {
         return refused("attention_cache_s8", cudaGetLastError());
     const Writes anything{nullptr, SIZE_MAX};
     cudaError_t e = launch_pdl(anything, kernel, dim3((unsigned)p.ctas), dim3(kThreads), kSmem, st, a, shape);
-    if (e == cudaSuccess && p.ctas > 1) {
-        const int rows = p.rows < 8 * NT ? p.rows : 8 * NT, groups = kJoinThreads / D;
-        const long long items = (long long)a.c.batch * a.c.kv_heads * p.tiles;
-        const bool by_item = items < p.ctas, share = items * 8 <= p.ctas;
-        e = launch_pdl(anything, join_kernel<T, D>,
-                       dim3((unsigned)(by_item ? items : p.ctas - 1), (unsigned)(share ? rows : (rows + groups - 1) / groups)),
-                       dim3(kJoinThreads), 0, st, a, shape, p.ctas, 8 * NT, (int)by_item, (int)share);
-    }
+    if (e == cudaSuccess && p.ctas > 1)
+        e = launch_pdl(anything, join_kernel<T, D, VEC>,
+                       dim3((unsigned)(p.ctas - 1), (unsigned)(p.rows < 8 * NT ? p.rows : 8 * NT)), dim3(32 * kJoinWarps), 0,
+                       st, a, shape, p.ctas, 8 * NT);
     return e != cudaSuccess ? refused("attention_cache_s8", e) : check_launch("attention_cache_s8");
 }
 template <class T, int D>
@@ -803,7 +780,10 @@ size_t attention_cache_workspace(const mb200_kv_cache& c, int heads, int queries
 
 int launch_attention_cache(const CacheArgs& a, int dtype, cudaStream_t st) {
     const Plan p = plan_of(a.c, a.heads, a.queries);
-    const bool vec = ((uintptr_t)a.q.p & 15) == 0 && a.q.token_stride % 8 == 0 && a.q.head_stride % 8 == 0;
+    auto aligned = [](const mb200_heads& t) {
+        return ((uintptr_t)t.p & 15) == 0 && t.token_stride % 8 == 0 && t.head_stride % 8 == 0;
+    };
+    const bool vec = aligned(a.q) && aligned(a.out);
     if (dtype == MB200_DTYPE_F16)
         return p.d == 64 ? launch_rows<__half, 64>(a, p, vec, st) : launch_rows<__half, 128>(a, p, vec, st);
     return p.d == 64 ? launch_rows<__nv_bfloat16, 64>(a, p, vec, st) : launch_rows<__nv_bfloat16, 128>(a, p, vec, st);
