@@ -56,11 +56,12 @@ struct PromptArgs {
     int batch, tokens, key_tokens, heads, kv_heads, d;
     const int32_t *cu_q, *cu_k;
     mb200_heads q, k, v, out;
-    int causal;
+    int causal, pack;  // pack: log2 of the query heads of a group that share a tile
     float scale_log2;
     int* status;
 };
-long long attention_prompt_ctas(int tokens, int batch, int heads);
+int attention_prompt_pack(const mb200_heads& q, int tokens, int heads, int kv_heads, int d);
+long long attention_prompt_ctas(int tokens, int batch, int heads, int pack);
 int launch_attention_prompt(const PromptArgs& a, int dtype, cudaStream_t st);
 
 }  // namespace attn

@@ -237,7 +237,7 @@ int mb200_attention_cache_s8(
     a.lengths = lengths, a.heads = heads, a.queries = queries;
     a.q = *q, a.out = *out;
     a.scale_log2 = scale * 1.44269504f;
-    a.workspace = workspace;
+    a.workspace = need ? workspace : nullptr;
     rc = status_word(stream, &a.status);
     return rc ? rc : launch_attention_cache(a, dtype, (cudaStream_t)stream);
 }
@@ -286,7 +286,8 @@ int mb200_attention_prompt(
     // (rows of the last tiles are counted in an int)
     if (tokens > 0x7fffffff - 512 || key_tokens > 0x7fffffff - 512)
         return set_error(ST_OUT_OF_RANGE, "%s: %d tokens, %d of keys", what, tokens, key_tokens);
-    rc = check_grid(attention_prompt_ctas(tokens, batch, heads), what);
+    a.pack = attention_prompt_pack(a.q, tokens, heads, kv_heads, d);
+    rc = check_grid(attention_prompt_ctas(tokens, batch, heads, a.pack), what);
     if (!rc)
         rc = status_word(stream, &a.status);
     if (rc)

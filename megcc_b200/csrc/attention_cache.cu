@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         blk = (int)(s_rest - (long long)at * n) * kRound;
     }
     const Parts parts = parts_of(a.workspace, gridDim.x, kRows, D);
-    if (tid == 0 && gridDim.x > 1) {
+    if (tid == 0 && a.workspace) {
         Cut cut{};
         cut.b = left > 0 && blk > 0 ? b : -1;
         cut.at = at, cut.from = s_from - blk / kRound, cut.quota = s_quota;
@@ -743,7 +743,8 @@ Plan plan_of(const mb200_kv_cache& c, int heads, int queries) {
     p.ctas = (int)(p.most < resident ? p.most : resident);
     if (p.ctas < 1)
         p.ctas = 1;
-    p.bytes = p.ctas == 1 ? 0 : align_up(parts_bytes(p.ctas, 8 * p.nt, p.d), 256);
+    // (sequences of one round are never cut)
+    p.bytes = p.ctas == 1 || p.capacity <= kRound * kBlock ? 0 : align_up(parts_bytes(p.ctas, 8 * p.nt, p.d), 256);
     return p;
 }
 
@@ -758,7 +759,7 @@ int launch(const CacheArgs& a, const Plan& p, cudaStream_t st) {
         return refused("attention_cache_s8", cudaGetLastError());
     const Writes anything{nullptr, SIZE_MAX};
     cudaError_t e = launch_pdl(anything, kernel, dim3((unsigned)p.ctas), dim3(kThreads), kSmem, st, a, shape);
-    if (e == cudaSuccess && p.ctas > 1)
+    if (e == cudaSuccess && p.bytes)
         e = launch_pdl(anything, join_kernel<T, D, VEC>,
                        dim3((unsigned)(p.ctas - 1), (unsigned)(p.rows < 8 * NT ? p.rows : 8 * NT)), dim3(32 * kJoinWarps), 0,
                        st, a, shape, p.ctas, 8 * NT);

@@ -2,7 +2,8 @@
 //
 //     o_i = sum_j 2^(t_ij - m_i) v_j / sum_j 2^(t_ij - m_i),   t_ij = scale log2(e) q_i . k_j
 //
-// in one pass over the keys. A CTA has two tiles of 128 queries of a head; keys and values come in tiles of 128 through a
+// in one pass over the keys. A CTA has two tiles of 128 rows, a row for each of a few query heads of a group (the largest power
+// of two that divides it) and token: short prompts fill a tile, and less of one lies beyond the diagonal. Keys and values come in tiles of 128 through a
 // ring of TMA loads. Both products are tcgen05.mma kind::f16: S = Q K^T with both operands in shared memory, O += P V with
 // P in tensor memory, in the columns of the S it was made of (two S and two O of 128 x 128 fill the 512 columns), and
 // V as it lies, the dimension contiguous. Each tile has a warpgroup, a thread per row: it takes its row of S to
@@ -41,6 +42,7 @@ constexpr int kTile = 128;           // rows of a tile of queries, and of a tile
 constexpr int kRows = 2 * kTile;     // queries of a CTA
 constexpr int kThreads = 384;        // two warpgroups with a tile each; the third issues loads and products
 constexpr float kAhead = 8.f;        // how far (a power of two) a score may pass the running maximum
+constexpr int kPolyEvery = 4;        // of so many pairs of powers one is a polynomial
 constexpr float kLift = 6.f;         // P is held 2^6 times: 2^14 at most, and fp16 has room down to 2^-30
 enum : int { ERR_PROMPT_WAIT = 0x203 };
 
@@ -176,18 +178,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ float2 both(float v) {
     return make_float2(v, v);
 }
-__device__ __forceinline__ float max_or_nan(float a, float b) {
+// the largest of three, or a NaN among them
+__device__ __forceinline__ float max_or_nan(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x without the special-function unit, x <= 100; 0 below -126
+// 2^x of numbers up to 100 without the special-function unit; 2^-126 for what is less
 template <class T>
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
     constexpr bool fine = std::is_same<T, __half>::value;
+    x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
     // 1.5 * 2^23 leaves the nearest whole number in the low bits
     const float2 n = add2(x, both(12582912.f));
-    const float2 f = add2(x, make_float2(-(n.x - 12582912.f), -(n.y - 12582912.f)));
+    const float2 f = fma2(add2(n, both(-12582912.f)), both(-1.f), x);
     float2 p;
     if constexpr (fine) {
         p = fma2(both(0.009570102207f), f, both(0.05591785908f));
@@ -199,9 +203,28 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
         p = fma2(p, f, both(0.6932609677f));
         p = fma2(p, f, both(0.9999280572f));
     }
-    const float r0 = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23));
-    const float r1 = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23));
-    return make_float2(x.x >= -126.f ? r0 : max_or_nan(x.x, 0.f), x.y >= -126.f ? r1 : max_or_nan(x.y, 0.f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// A row of scores -> P in tensor memory and its sum. POLY: a part of the powers by the FMA pipe (nothing is hidden: those are
+// not 0)
+template <class T, bool POLY>
+__device__ __forceinline__ void powers(uint32_t (&s)[kTile], float scale, float shift, uint32_t col_s, float2 (&l)[2]) {
+    const float2 z = both(shift), f = both(scale);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        uint32_t p[16];
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+            const int e = 32 * x + 2 * y;
+            float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f, z);
+            v = POLY && y % kPolyEvery == kPolyEvery - 1 ? exp2_poly<T>(v) : make_float2(exp2_fast(v.x), exp2_fast(v.y));
+            l[y & 1] = add2(l[y & 1], v);
+            p[y] = pack2<T>(v.x, v.y);
+        }
+        tmem_st16(col_s + 16 * x, p);
+    }
 }
 
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort, int* status) {
@@ -212,38 +235,36 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
     return false;
 }
 
-// What a CTA works on
+// What a CTA works on: rows are tokens times `1 << pack` heads
 struct Work {
-    int head, kv_head;
-    int q0, rows;     // first row of queries, how many (of 256)
+    int head, kv_head, pack;
+    int q0, tokens;   // first token, how many
     int k0, keys;     // first row of the sequence's keys, how many
-    int seen;         // keys that the first of the rows sees; each next one sees `step` more
+    int seen;         // keys that the first token sees; each next one sees `step` more
     int step;
-    __device__ __forceinline__ int limit(int row) const {  // keys that a row sees
-        return max(0, min(keys, seen + row * step));
+    __device__ __forceinline__ int limit(int token) const {  // keys that a token sees
+        return max(0, min(keys, seen + token * step));
     }
-    __device__ __forceinline__ int tiles(int t) const {  // of keys, for tile t of queries
-        const int n = min(rows - t * kTile, kTile);
-        return n <= 0 ? 0 : (limit(t * kTile + n - 1) + kTile - 1) / kTile;
+    __device__ __forceinline__ int tiles(int t) const {  // of keys, for tile t of rows
+        const int per = kTile >> pack, n = min(tokens - t * per, per);
+        return n <= 0 ? 0 : (limit(t * per + n - 1) + kTile - 1) / kTile;
     }
 };
 
 // A row by plain loops: lanes take keys for the scores, dimensions for the sum. The whole warp calls it.
 template <class T>
-__device__ __noinline__ void row_anew(const PromptArgs& a, const Work& w, int row) {
-    const int lane = threadIdx.x & 31;
-    const long long token = w.q0 + row;
-    const uint16_t* q = (const uint16_t*)a.q.p + token * a.q.token_stride + w.head * a.q.head_stride;
-    const uint16_t* k = (const uint16_t*)a.k.p + w.kv_head * a.k.head_stride;
-    const uint16_t* v = (const uint16_t*)a.v.p + w.kv_head * a.v.head_stride;
+__device__ __noinline__ void row_anew(const PromptArgs& a, long long token, int head, int k0, int n) {
+    const int lane = threadIdx.x & 31, kv_head = head / (a.heads / a.kv_heads);
+    const uint16_t* q = (const uint16_t*)a.q.p + token * a.q.token_stride + head * a.q.head_stride;
+    const uint16_t* k = (const uint16_t*)a.k.p + kv_head * a.k.head_stride;
+    const uint16_t* v = (const uint16_t*)a.v.p + kv_head * a.v.head_stride;
     auto value = [](const uint16_t* p) { return scaled::to_float(*reinterpret_cast<const T*>(p)); };
-    const int n = w.limit(row);
     float m = __uint_as_float(0xff800000u), total = 0.f, sum[kMaxD / 32] = {};
     for (int j0 = 0; j0 < n; j0 += 32) {
         const int j = j0 + lane;
         float t = __uint_as_float(0xff800000u);
         if (j < n) {
-            const uint16_t* key = k + (long long)(w.k0 + j) * a.k.token_stride;
+            const uint16_t* key = k + (long long)(k0 + j) * a.k.token_stride;
             float s = 0.f;
             for (int e = 0; e < a.d; ++e)
                 s = __fmaf_rn(value(q + e), value(key + e), s);
@@ -264,7 +285,7 @@ __device__ __noinline__ void row_anew(const PromptArgs& a, const Work& w, int ro
         const int here = min(32, n - j0);
         for (int x = 0; x < here; ++x) {
             const float f = __shfl_sync(0xffffffffu, p, x);
-            const uint16_t* r = v + (long long)(w.k0 + j0 + x) * a.v.token_stride;
+            const uint16_t* r = v + (long long)(k0 + j0 + x) * a.v.token_stride;
 #pragma unroll
             for (int i = 0; i < kMaxD / 32; ++i)
                 if (lane + 32 * i < a.d)
@@ -274,7 +295,7 @@ __device__ __noinline__ void row_anew(const PromptArgs& a, const Work& w, int ro
 #pragma unroll
     for (int x = 1; x < 32; x *= 2)
         total += __shfl_xor_sync(0xffffffffu, total, x);
-    T* out = (T*)a.out.p + token * a.out.token_stride + w.head * a.out.head_stride;
+    T* out = (T*)a.out.p + token * a.out.token_stride + head * a.out.head_stride;
 #pragma unroll
     for (int i = 0; i < kMaxD / 32; ++i)
         if (lane + 32 * i < a.d)
@@ -323,26 +344,28 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_start();
-    // ---- which queries: sequence b's tiles have the slots from cu[b] / 256 + b on, the last tile first ----
+    // ---- which queries: with n tokens a CTA, sequence b's have the slots from cu[b] / n + b on, the last ones first ----
     Work w;
-    w.head = blockIdx.x % a.heads;
+    w.pack = a.pack;
+    const int packs = a.heads >> a.pack, per_cta = kRows >> a.pack;
+    w.head = (int)(blockIdx.x % packs) << a.pack;
     w.kv_head = w.head / (a.heads / a.kv_heads);
     if (warp == 9) {
-        const int slot = blockIdx.x / a.heads;
-        const int b = first_beyond(a.batch, slot, [&](int i) { return (long long)a.cu_q[i + 1] / kRows + i + 1; });
+        const int slot = blockIdx.x / packs;
+        const int b = first_beyond(a.batch, slot, [&](int i) { return (long long)a.cu_q[i + 1] / per_cta + i + 1; });
         int first = 0, n = 0, k0 = 0, keys = 0, row0 = 0;
         if (b < a.batch) {
             first = a.cu_q[b];
             n = first < 0 ? 0 : min(a.cu_q[b + 1], a.tokens) - first;
             k0 = a.cu_k[b];
             keys = k0 < 0 ? 0 : max(0, min(a.cu_k[b + 1], a.key_tokens) - k0);
-            row0 = ((n + kRows - 1) / kRows - 1 - (slot - (first / kRows + b))) * kRows;
-            if (slot < first / kRows + b || row0 < 0)
+            row0 = ((n + per_cta - 1) / per_cta - 1 - (slot - (first / per_cta + b))) * per_cta;
+            if (slot < first / per_cta + b || row0 < 0)
                 n = row0 = 0;
         }
         if (lane == 0) {
             s_work[0] = first + row0;
-            s_work[1] = max(0, min(n - row0, kRows));
+            s_work[1] = max(0, min(n - row0, per_cta));
             s_work[2] = k0;
             s_work[3] = keys;
             // (a sequence's last query sees its last key)
@@ -352,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
     fence_before();
     __syncthreads();
     fence_after();
-    w.q0 = s_work[0], w.rows = s_work[1], w.k0 = s_work[2], w.keys = s_work[3], w.seen = s_work[4];
+    w.q0 = s_work[0], w.tokens = s_work[1], w.k0 = s_work[2], w.keys = s_work[3], w.seen = s_work[4];
     w.step = a.causal ? 1 : 0;
     const uint32_t tmem = *tmem_slot;
     const int n0 = w.tiles(0), n1 = w.tiles(1), most = max(n0, n1);
@@ -378,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
                 load(i & 1 ? &maps.v : &maps.k, i & 1 ? inside.v : inside.k, ring + s * S::kOperand, full + 8 * s,
                      w.kv_head, w.k0 + (i >> 1) * kTile);
                 if (i == 0)
-                    load(&maps.q, inside.q, smem_u32(smem + S::kOperand), q_full + 8, w.head, w.q0 + kTile);
+                    load(&maps.q, inside.q, smem_u32(smem + S::kOperand), q_full + 8, w.head, w.q0 + (kTile >> w.pack));
             }
             // whoever gave up: the copies on their way land before the CTA ends
             for (int x = max(0, i - kStages); x < i; ++x)
@@ -466,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         const int row = t * kTile + (threadIdx.x & (kTile - 1));
         const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
         const uint32_t col_s = tmem + lanes + kColS + t * kTile, col_o = tmem + lanes + kColO + t * kTile;
-        const int limit = w.limit(row), first_limit = w.limit(row - lane);
+        const int limit = w.limit(row >> w.pack), first_limit = w.limit((row - lane) >> w.pack);
         const float none = __uint_as_float(0xff800000u);
         // (a scale of 0 takes all scores for 0, and what is hidden for -infinity still)
         const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
@@ -492,24 +515,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
                 for (int x = 0; x < kTile; ++x)
                     s[x] ^= 0x80000000u;
             }
-            if ((j + 1) * kTile > first_limit) {
+            const bool hides = (j + 1) * kTile > first_limit;  // (of the warp's rows the first one sees the least)
+            if (hides) {
                 const int here = limit - j * kTile;
 #pragma unroll
                 for (int x = 0; x < kTile; ++x)
                     s[x] = x < here ? s[x] : 0xff800000u;
             }
-            float top[4];
+            float top[4] = {none, none, none, none};
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                top[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 4]));
-#pragma unroll
-            for (int x = 8; x < kTile; ++x)
-                top[x & 3] = fmaxf(top[x & 3], __uint_as_float(s[x]));
-            const float highest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if (__any_sync(0xffffffffu, (highest - m) * scale > kAhead)) {
-                const float to = fmaxf(m, highest);
-                const float down = to == m ? 1.f : exp2_fast((m - to) * scale);
-                m = to;
+            for (int x = 0; x < kTile; x += 2)
+                top[x / 2 & 3] = max_or_nan(top[x / 2 & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+            // (a NaN that a row sees makes all of it NaN)
+            const float highest = max_or_nan(max_or_nan(top[0], top[1], top[2]), top[3], m);
+            // (each row by itself, so that its result depends on no other one)
+            const bool raise = !((highest - m) * scale <= kAhead);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float down = !raise || highest == m ? 1.f : exp2_fast((m - highest) * scale);
+                m = raise ? highest : m;
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
                     l[x].x *= down, l[x].y *= down;
@@ -525,20 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
                     }
                 }
             }
-            const float2 z = both(kLift - (m == none ? 0.f : m * scale)), f = both(scale);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t p[16];
-#pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                    const int e = 32 * x + 2 * y;
-                    float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f, z);
-                    v = y % 4 == 3 ? exp2_poly<T>(v) : make_float2(exp2_fast(v.x), exp2_fast(v.y));
-                    l[y & 1] = add2(l[y & 1], v);
-                    p[y] = pack2<T>(v.x, v.y);
-                }
-                tmem_st16(col_s + 16 * x, p);
-            }
+            const float shift = kLift - (m == none ? 0.f : m * scale);
+            if (hides)
+                powers<T, false>(s, scale, shift, col_s, l);
+            else
+                powers<T, true>(s, scale, shift, col_s, l);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             fence_before();
             __syncwarp();
@@ -574,21 +588,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
                 }
             }
             __syncwarp();
-            T* out = (T*)a.out.p + (long long)(w.q0 + row0) * a.out.token_stride + w.head * a.out.head_stride;
             const bool vec = ((uintptr_t)a.out.p & 15) == 0 && a.out.token_stride % 8 == 0 && a.out.head_stride % 8 == 0;
-            const int here = min(32, w.rows - row0);
+            const int here = min(32, (w.tokens << w.pack) - row0);
             for (int i = lane; i < here * units; i += 32) {
                 const int r = i / units, u = i - r * units;
                 // (with no tile of keys, queries may still be on their way to the stage)
                 const uint4 v = n > 0 ? *(const uint4*)(stage + r * (D * 2) + ((u ^ (r & 7)) << 4)) : make_uint4(0, 0, 0, 0);
+                const long long to = (long long)(w.q0 + ((row0 + r) >> w.pack)) * a.out.token_stride +
+                                     (w.head + ((row0 + r) & ((1 << w.pack) - 1))) * a.out.head_stride + u * 8;
                 if (vec)
-                    store8<true>(out, r * a.out.token_stride + u * 8, v);
+                    store8<true>(a.out.p, to, v);
                 else
-                    store8<false>(out, r * a.out.token_stride + u * 8, v);
+                    store8<false>(a.out.p, to, v);
             }
             __syncwarp();
-            for (uint32_t rows = __ballot_sync(0xffffffffu, bad && row < w.rows); rows; rows &= rows - 1)
-                row_anew<T>(a, w, row0 + __ffs(rows) - 1);
+            for (uint32_t rows = __ballot_sync(0xffffffffu, bad && lane < here); rows; rows &= rows - 1) {
+                const int r = row0 + __ffs(rows) - 1, token = r >> w.pack;
+                row_anew<T>(a, w.q0 + token, w.head + (r & ((1 << w.pack) - 1)), w.k0, w.limit(token));
+            }
         }
     }
     fence_before();
@@ -598,20 +615,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// [tokens][heads][d] in boxes of 64 elements of 128 tokens of a head
-int encode(CUtensorMap* map, bool* tokens_inside, int dtype, const mb200_heads& t, int tokens, int heads, int d) {
+bool tokens_before_heads(const mb200_heads& t, int tokens, int heads, int d) {
+    return heads > 1 && tokens > 1 && t.token_stride < t.head_stride;
+}
+// [tokens][heads][d] in boxes of 64 elements of 128 rows: tokens of 1 << pack heads each
+int encode(CUtensorMap* map, bool* tokens_inside, int dtype, const mb200_heads& t, int tokens, int heads, int d, int pack = 0) {
     const DriverApi& api = driver_api();
     if (!api.ok)
         return set_error(ST_RUNTIME, "cuTensorMapEncode* entry points not found in the driver");
     // (of one head, or token, any distance will do; the map wants whole units)
     const cuuint64_t row = (cuuint64_t)d * 2;
     const cuuint64_t head = heads == 1 ? row : (cuuint64_t)t.head_stride * 2;
-    const cuuint64_t token = tokens == 1 ? (head > row ? head : row) : (cuuint64_t)t.token_stride * 2;
-    const bool in = token < head;
+    const cuuint64_t token = tokens == 1 ? head * heads : (cuuint64_t)t.token_stride * 2;
+    const bool in = tokens_before_heads(t, tokens, heads, d);
     *tokens_inside = in;
     cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)(in ? tokens : heads), (cuuint64_t)(in ? heads : tokens)};
     cuuint64_t strides[2] = {in ? token : head, in ? head : token};
-    cuuint32_t box[3] = {64, in ? (cuuint32_t)kTile : 1u, in ? 1u : (cuuint32_t)kTile}, estr[3] = {1, 1, 1};
+    cuuint32_t box[3] = {64, in ? (cuuint32_t)kTile : 1u << pack, in ? 1u : (cuuint32_t)(kTile >> pack)}, estr[3] = {1, 1, 1};
     const CUresult r = api.tiled(
             map, dtype == MB200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, t.p, dims,
             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -626,7 +646,7 @@ int launch(const PromptMaps& maps, const PromptArgs& a, const TokensInside& insi
         return refused("attention_prompt", cudaGetLastError());
     const Writes writes{a.out.p, ((size_t)(a.tokens - 1) * a.out.token_stride + (size_t)(a.heads - 1) * a.out.head_stride +
                                   a.d) * 2};
-    const unsigned ctas = (unsigned)(((long long)a.tokens / kRows + a.batch) * a.heads);
+    const unsigned ctas = (unsigned)attention_prompt_ctas(a.tokens, a.batch, a.heads, a.pack);
     const cudaError_t e = launch_pdl(writes, prompt_kernel<T, D>, dim3(ctas), dim3(kThreads), Smem<D>::kBytes, st, maps, a,
                                      inside);
     return e != cudaSuccess ? refused("attention_prompt", e) : check_launch("attention_prompt");
@@ -634,14 +654,22 @@ int launch(const PromptMaps& maps, const PromptArgs& a, const TokensInside& insi
 
 }  // namespace
 
-long long attention_prompt_ctas(int tokens, int batch, int heads) {
-    return ((long long)tokens / kRows + batch) * heads;
+// log2 of the heads that share a tile. (Queries whose heads lie further apart than tokens would come in another order.)
+int attention_prompt_pack(const mb200_heads& q, int tokens, int heads, int kv_heads, int d) {
+    int pack = 0;
+    if (!tokens_before_heads(q, tokens, heads, d))
+        while (pack < 6 && heads / kv_heads % (2 << pack) == 0)
+            ++pack;
+    return pack;
+}
+long long attention_prompt_ctas(int tokens, int batch, int heads, int pack) {
+    return ((long long)tokens / (kRows >> pack) + batch) * (heads >> pack);
 }
 
 int launch_attention_prompt(const PromptArgs& a, int dtype, cudaStream_t st) {
     PromptMaps maps;
     TokensInside inside;
-    int rc = encode(&maps.q, &inside.q, dtype, a.q, a.tokens, a.heads, a.d);
+    int rc = encode(&maps.q, &inside.q, dtype, a.q, a.tokens, a.heads, a.d, a.pack);
     const int keys = a.key_tokens > 0 ? a.key_tokens : 1;  // (without keys nothing is loaded)
     if (!rc)
         rc = encode(&maps.k, &inside.k, dtype, a.k, keys, a.kv_heads, a.d);

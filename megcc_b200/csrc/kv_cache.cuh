@@ -57,9 +57,16 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const T x = from_float<T>(a), y = from_float<T>(b);
-    return (uint32_t)*reinterpret_cast<const uint16_t*>(&x) | (uint32_t)*reinterpret_cast<const uint16_t*>(&y) << 16;
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // 8 elements of 16 bits. VEC: they start on a 16-byte boundary

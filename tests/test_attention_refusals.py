@@ -88,12 +88,15 @@ def test_read(change, status):
     assert read(change) == status
 
 
+FIVE = dict(table_pages=5, table_stride=5)  # (pages, which may be cut)
+
+
 @pytest.mark.parametrize("change,status", [
     (dict(lengths=None), NULL_PTR), (dict(heads=3), LAYOUT), (dict(heads=0), LAYOUT), (dict(queries=0), LAYOUT),
     (dict(scale=float("nan")), LAYOUT), (dict(scale=float("inf")), LAYOUT), (dict(q=(None, 256, 64)), NULL_PTR),
     (dict(out=(None, 256, 64)), NULL_PTR), (dict(q=(P + 1, 256, 64)), LAYOUT), (dict(out=(P, 200, 64)), LAYOUT),
-    (dict(out=(P, 256, 0)), LAYOUT), (dict(lengths=P + 1), LAYOUT), (dict(ws=None), NULL_PTR), (dict(ws=P + 128), LAYOUT),
-    (dict(nbytes=100), LAYOUT), (dict(queries=1 << 29), OUT_OF_RANGE), (dict(batch=0, q=(None, 0, 0)), 0)])
+    (dict(out=(P, 256, 0)), LAYOUT), (dict(lengths=P + 1), LAYOUT), (dict(ws=None, **FIVE), NULL_PTR),
+    (dict(ws=P + 128, **FIVE), LAYOUT), (dict(nbytes=100, **FIVE), LAYOUT), (dict(queries=1 << 29), OUT_OF_RANGE), (dict(batch=0, q=(None, 0, 0)), 0)])
 def test_attention_cache(change, status):
     assert attention_cache(change) == status
 
@@ -103,9 +106,10 @@ def test_nothing_to_ask_for():
     assert lib.mb200_kv_append_s8(cache({}), None, None) == NULL_PTR
     assert lib.mb200_attention_cache_s8_workspace_bytes(None, 4, 1) == 0
     assert lib.mb200_attention_cache_s8_workspace_bytes(cache(dict(d=100)), 4, 1) == 0
-    # a table of one page of 32 positions: one CTA has it all
-    assert lib.mb200_attention_cache_s8_workspace_bytes(cache(dict(table_pages=1, batch=1)), 4, 1) == 0
-    assert lib.mb200_attention_cache_s8_workspace_bytes(cache({}), 4, 1) % 256 == 0
+    # tables of up to 128 positions: no sequence is cut
+    assert lib.mb200_attention_cache_s8_workspace_bytes(cache({}), 4, 1) == 0
+    size = lib.mb200_attention_cache_s8_workspace_bytes(cache(dict(table_pages=5, table_stride=5)), 4, 1)
+    assert size > 0 and size % 256 == 0
 
 
 def pool(**change):
