@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kTile = 128;           // rows of a tile of queries, and of a tile of keys
 constexpr int kRows = 2 * kTile;     // queries of a CTA
-constexpr int kThreads = 384;        // two warpgroups with a tile each; the third issues loads and products
+constexpr int kThreads = 320;        // two warpgroups with a tile each; a warp for the products, one for the loads
 constexpr float kAhead = 8.f;        // how far (a power of two) a score may pass the running maximum
 constexpr int kPolyEvery = 4;        // of so many pairs of powers one is a polynomial
 constexpr float kLift = 6.f;         // P is held 2^6 times: 2^14 at most, and fp16 has room down to 2^-30
@@ -443,7 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
             const bool foreign = w.keys % kTile != 0 && most * kTile > w.keys;
             for (int j = 0; j < most && ok; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2;
-                if (!operand(iv))
+                // (both here, where the warp has time: a wait costs it 160 clocks even if there is nothing to wait for)
+                if (!operand(iv) || (j + 1 < most && !operand(ik)))
                     break;
                 if (foreign && j == most - 1) {
                     uint8_t* v = smem + S::kRing + (iv % kStages) * S::kOperand;
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
                     umma_commit_if(leader, o_full + 8 * t);
                     if (j + 1 < n) {
                         // S takes P's columns: the product that reads them has to be complete
-                        if (!operand(ik) || !wait(o_full + 8 * t, j & 1))
+                        if (!wait(o_full + 8 * t, j & 1))
                             break;
                         scores(t, ik);
                     }
