@@ -390,9 +390,9 @@ typedef struct mb200_heads {
  *     x' = x cos - y sin,  y' = y cos + x sin   with the position's i-th cosine and sine,
  * in fp32, products and sums rounded each. q_out and k_out (k_out.p may be NULL) get the results rounded to 16 bits; the
  * cache is made from the fp32 ones. A position beyond the tables makes its row NaN, and the device status 0x202.
- * A block's scale is RN(max(amax, 2^-119) * RN(1 / 127)) of the new values in it, or what it was, if the block keeps
- * older positions and that is larger; whole numbers are x * RN(1 / scale) to the nearest (ties to even). If the scale
- * grows, older numbers become q * RN(old scale / scale) to the nearest. A block with a NaN or an infinity gets scale
+ * A block's scale is max(amax, 2^-119) / 127 of the new values in it, rounded to fp32, or what it was, if the block keeps
+ * older positions and that is larger; whole numbers are x / scale to the nearest (ties to even). If the scale grows, older
+ * numbers become q * (old scale / scale) to the nearest (in 64 bits). A block with a NaN or an infinity gets scale
  * NaN and zeros, and is NaN as long as it keeps them. No block may be appended to by two sequences of a call. */
 typedef struct mb200_kv_append_param {
     const int32_t *lengths, *cu;

@@ -211,11 +211,15 @@ def tensor_calls():
             raise RuntimeError("megcc_b200/_torchcall.so is missing or made for another torch: build it with "
                                "`python -m megcc_b200.build` (there is no fallback)") from e
         import torch
-        _torchcall.bind(check, torch.OutOfMemoryError, *(C.cast(getattr(lib(), name), C.c_void_p).value for name in (
+        def at(*names):
+            return (C.cast(getattr(lib(), name), C.c_void_p).value for name in names)
+
+        _torchcall.bind(check, torch.OutOfMemoryError, *at(
             "mb200_quantize_rows_s8", "mb200_matmul_s8_scaled_workspace_bytes", "mb200_matmul_s8_scaled",
-            "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes",
-            "mb200_moe_s8", "mb200_kv_append_s8", "mb200_kv_read_s8", "mb200_attention_cache_s8_workspace_bytes",
-            "mb200_attention_cache_s8", "mb200_attention_prompt")))
+            "mb200_linear_s8_workspace_bytes", "mb200_linear_s8", "mb200_moe_s8_workspace_bytes", "mb200_moe_s8"))
+        _torchcall.bind_attention(*at(
+            "mb200_kv_append_s8", "mb200_kv_read_s8", "mb200_attention_cache_s8_workspace_bytes",
+            "mb200_attention_cache_s8", "mb200_attention_prompt"))
         _tensor_calls = _torchcall
     return _tensor_calls
 

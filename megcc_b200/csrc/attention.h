@@ -11,6 +11,7 @@ namespace attn {
 
 constexpr int kBlock = MB200_KV_BLOCK;  // positions of a head that share a scale
 constexpr int kMaxD = 128;
+constexpr int kTurnSteps = 8;  // steps of rows of queries that a warp turns
 
 // recorded in the device status word
 enum : int {

@@ -153,7 +153,7 @@ int mb200_kv_append_s8(const mb200_kv_cache* cache, const mb200_kv_append_param*
     const long long slots = p->cu ? p->tokens / kBlock + 2LL * cache->batch : p->tokens;
     a.k = p->k, a.v = p->v, a.q = p->q, a.k_out = p->k_out, a.q_out = p->q_out;
     a.heads = p->heads;
-    const int rows = 4 * (32 / (d / 8));  // that a warp turns
+    const int rows = kTurnSteps * (32 / (d / 8));  // that a warp turns
     a.chunks = p->q.p ? (p->heads + rows - 1) / rows : 1;
     a.cosines = p->cosines, a.sines = p->sines;
     a.positions = p->positions, a.rot = p->cosines ? p->rot_dims : 0, a.interleaved = p->interleaved != 0;

@@ -7,9 +7,12 @@
 // need more than 32 bits.
 //
 // Blocks: the 16 positions of a block and head share a scale, s = max(amax, 2^-119) / 127 of the new values there, or the
-// block's scale of before where that is larger and the block keeps older positions. Where it grows, the older whole
-// numbers are made anew, q' = q * (s_before / s) to the nearest; so the outcome depends on what was appended
-// together, never on the order in which warps run. A block is one warp's: it alone reads and writes it.
+// block's scale of before where that is larger and the block keeps older positions. A value's whole number is the one
+// nearest to the quotient x / s itself: activations of 16 bits have many quotients that lie within a rounding of the
+// middle between two. Where the scale grows, older numbers are made anew, q' = q * (s_before / s) to the nearest; so the
+// outcome depends on what was appended together, never on the order in which warps run. A block is one warp's: it
+// alone reads and writes it. Keys are turned twice, for the largest of them and for their numbers: held in between they
+// took the registers of half of the warps (8191 tokens of 32 + 8 + 8 heads of 128, with reading the blocks back: 94 us, 78 so).
 //
 // What bounds it: for a step of decoding the launch and the four loads that follow from one another (lengths, page, scale,
 // whole numbers); for prompts memory.
@@ -22,7 +25,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kMostSteps = 8;  // steps of a warp over 16 rows: two rows a step at least (d <= 128)
-constexpr int kQuerySteps = 4;
+constexpr int kQuerySteps = kTurnSteps;
 
 // The part of a row that a lane holds: 8 elements from 8 * unit on; `rows` rows at a time, this lane's is `sub`
 struct Lane {
@@ -154,6 +157,20 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, const Lane& l,
     }
 }
 
+__device__ __forceinline__ uint32_t pack4_low(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// The whole number nearest to x / s, ties to even, in the low byte: x * RN(1 / s) comes within one of it, and what is left of
+// x, which one FMA gives exactly, says on which side
+__device__ __forceinline__ uint32_t nearest_quotient(float x, float s, float half, float inv) {
+    const float t = __fmaf_rn(x, inv, 12582912.f);
+    const float left = __fmaf_rn(-__fsub_rn(t, 12582912.f), s, x);
+    const float size = fabsf(left);
+    const uint32_t q = __float_as_uint(t);
+    const bool off = size > half || (size == half && (q & 1));
+    return q + (off ? (left > 0.f ? 1u : 0xffffffffu) : 0u);
+}
+
 // The new keys (or values) of a block of a head
 template <class T, bool VEC>
 __device__ __forceinline__ void append_block(const AppendArgs& a, const Lane& l, int slot, int h, bool keys) {
@@ -205,67 +222,74 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, const Lane& l,
     } else {
         *(volatile int*)a.status = ERR_PAGE;
     }
-    float x[kMostSteps][8];
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kMostSteps; ++i) {
+    // a token's values, turned if they are keys
+    auto values = [&](int i, float (&x)[8]) {
         const int t = i * l.rows + l.sub;
-        if (i * l.rows >= count)  // (the same in all lanes)
-            break;
         if (keys) {
             Angles g;
             const bool turns = take_angles<VEC>(a, l, l.active && t < count, p0 + t, g);
-            turned<T>(a, l, raw[i], turns, g, x[i]);
-            if (a.k_out.p && l.active && t < count)
-                store8<VEC>(a.k_out.p, (token + t) * a.k_out.token_stride + h * a.k_out.head_stride + l.unit * 8,
-                            pack8<T>(x[i]));
+            turned<T>(a, l, raw[i], turns, g, x);
         } else {
-            Vec<T>::unpack(raw[i], x[i]);
+            Vec<T>::unpack(raw[i], x);
         }
-        if (l.active && t < count) {
+        return l.active && t < count;
+    };
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kMostSteps; ++i) {
+        if (i * l.rows >= count)  // (the same in all lanes)
+            break;
+        float x[8];
+        if (values(i, x)) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                most = max(most, magnitude(x[i][e]));
+                most = max(most, magnitude(x[e]));
+            if (keys && a.k_out.p)
+                store8<VEC>(a.k_out.p, (token + i * l.rows + l.sub) * a.k_out.token_stride + h * a.k_out.head_stride + l.unit * 8,
+                            pack8<T>(x));
         }
     }
     if (page < 0)
         return;
     most = __reduce_max_sync(0xffffffffu, most);
     // (bits of non-negative numbers, infinity and the NaNs above: a block that holds one of those has a NaN for its scale)
-    const uint32_t new_bits = __float_as_uint(scaled::row_scale(most).scale);
+    const uint32_t new_bits = most < 0x7f800000u
+                                      ? __float_as_uint(__fdiv_rn(fmaxf(__uint_as_float(most), 0x1p-119f), 127.f))
+                                      : 0x7fffffffu;
     const uint32_t bits = max(new_bits, old_bits);
     const float s = __uint_as_float(bits);
     const bool finite = bits < 0x7f800000u;
-    const float inv = finite ? __frcp_rn(s) : 0.f;
+    const float inv = finite ? __frcp_rn(s) : 0.f, half = __fmul_rn(s, 0.5f);
     const uint32_t mask = finite ? 0xffffffffu : 0u;
 #pragma unroll
     for (int i = 0; i < kMostSteps; ++i) {
-        const int t = i * l.rows + l.sub;
         if (i * l.rows >= count)
             break;
-        if (l.active && t < count) {
-            const uint2 w = make_uint2(scaled::pack_whole(x[i][0], x[i][1], x[i][2], x[i][3], inv) & mask,
-                                       scaled::pack_whole(x[i][4], x[i][5], x[i][6], x[i][7], inv) & mask);
-            *(uint2*)(whole + (long long)(kept + t) * a.c.d) = w;
+        float x[8];
+        if (values(i, x)) {
+            uint32_t q[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                q[e] = nearest_quotient(x[e], s, half, inv);
+            const uint2 w = make_uint2(pack4_low(q[0], q[1], q[2], q[3]) & mask, pack4_low(q[4], q[5], q[6], q[7]) & mask);
+            *(uint2*)(whole + (long long)(kept + i * l.rows + l.sub) * a.c.d) = w;
         }
     }
     if (kept && bits != old_bits) {
-        const float ratio = finite ? __fdiv_rn(__uint_as_float(old_bits), s) : 0.f;
+        const double ratio = finite ? (double)__uint_as_float(old_bits) / (double)s : 0.0;
 #pragma unroll 1
         for (int t = l.sub; t < kept; t += l.rows) {
             if (!l.active)
                 break;
             uint2* p = (uint2*)(whole + (long long)t * a.c.d);
-            uint2 w = *p;
-            float y[8];
+            const uint2 w = *p;
+            uint32_t q[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                y[e] = (float)(int8_t)(w.x >> (8 * e));
-                y[4 + e] = (float)(int8_t)(w.y >> (8 * e));
+                q[e] = (uint32_t)__double2int_rn((double)(int8_t)(w.x >> (8 * e)) * ratio);
+                q[4 + e] = (uint32_t)__double2int_rn((double)(int8_t)(w.y >> (8 * e)) * ratio);
             }
-            w.x = scaled::pack_whole(y[0], y[1], y[2], y[3], ratio);
-            w.y = scaled::pack_whole(y[4], y[5], y[6], y[7], ratio);
-            *p = w;
+            *p = make_uint2(pack4_low(q[0], q[1], q[2], q[3]), pack4_low(q[4], q[5], q[6], q[7]));
         }
     }
     if ((threadIdx.x & 31) == 0 && (!kept || bits != old_bits))
@@ -273,7 +297,7 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, const Lane& l,
 }
 
 template <class T, bool VEC>
-__global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const AppendArgs a) {
     const Lane l(a.c.d);
     pdl_start();
     const unsigned w = blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -310,54 +334,82 @@ __device__ __forceinline__ void values16(const uint4& w, float s, uint4& lo, uin
     hi = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
-// kReadRows packed rows of keys and values a CTA: first where each lies, then 16 whole numbers a thread and turn
+// kReadRows packed rows of keys and values a CTA: a lane each finds where one lies, then a thread takes 16 whole numbers of
+// both tensors at two places at a time, four loads on their way
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
     __shared__ long long where[kReadRows];  // row of head 0, or -1: in no sequence, or -2: in no page
     pdl_start();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row0 = blockIdx.x * kReadRows;
-    for (int r = warp; r < kReadRows; r += kReadThreads / 32) {
-        const int row = row0 + r;
+    if (threadIdx.x < kReadRows) {
+        const int row = row0 + threadIdx.x;
         long long at = -1;
         if (row < a.tokens) {
-            const int b = first_beyond(a.c.batch, row, [&](int i) { return a.cu[i + 1]; });
-            if (b < a.c.batch && a.cu[b] <= row) {
-                const long long p = (long long)(a.starts ? a.starts[b] : 0) + (row - a.cu[b]);
-                const int page = p >= 0 && p <= 0x7fffffff ? page_of(a.c, b, (int)p) : -1;
-                at = page < 0 ? -2 : cache_row(a.c, page, 0, (int)p);
-                if (page < 0 && lane == 0)
-                    *(volatile int*)a.status = ERR_PAGE;
+            int b = 0, end = a.c.batch;  // the first sequence that ends behind the row
+            while (b < end) {
+                const int m = (b + end) / 2;
+                if (a.cu[m + 1] <= row)
+                    b = m + 1;
+                else
+                    end = m;
+            }
+            if (b < a.c.batch) {
+                const int first = a.cu[b], start = a.starts ? a.starts[b] : 0;
+                if (first <= row) {
+                    const long long p = (long long)start + (row - first);
+                    const int page = p >= 0 && p <= 0x7fffffff ? page_of(a.c, b, (int)p) : -1;
+                    at = page < 0 ? -2 : cache_row(a.c, page, 0, (int)p);
+                    if (page < 0)
+                        *(volatile int*)a.status = ERR_PAGE;
+                }
             }
         }
-        if (lane == 0)
-            where[r] = at;
+        where[threadIdx.x] = at;
     }
     __syncthreads();
-    const int units = a.c.d / 16;
-    const int per_row = units * a.c.kv_heads, all = per_row * kReadRows;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < 2 * all; i += kReadThreads) {
-        const bool keys = i < all;
-        const int at = keys ? i : i - all;
-        const int r = at / per_row, rest = at - r * per_row;
-        const int h = rest / units, u = rest - h * units;
-        long long row = where[r];
-        if (row == -1)
-            continue;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        float s = 0.f;
-        if (row >= 0) {
-            row += (long long)h * a.c.page_tokens;
-            w = *(const uint4*)((keys ? a.c.k : a.c.v) + row * a.c.d + u * 16);
-            s = (keys ? a.c.k_scales : a.c.v_scales)[row / kBlock];
+    const uint32_t units = a.c.d / 16, per_row = units * a.c.kv_heads, all = per_row * kReadRows;
+    // (a quotient by n is one product for numbers x with x n < 2^32)
+    const bool small = per_row < 16384;
+    const uint32_t over_row = 0xffffffffu / per_row + 1, over_units = 0xffffffffu / units + 1;
+    auto over = [&](uint32_t x, uint32_t n, uint32_t inverse) { return n == 1 ? x : small ? __umulhi(x, inverse) : x / n; };
+#pragma unroll 1
+    for (uint32_t first = threadIdx.x; first < all; first += 2 * kReadThreads) {
+        uint4 w[4];
+        float s[4];
+        long long from[2];
+        uint32_t r[2], h[2], u[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const uint32_t x = first + y * kReadThreads;
+            r[y] = over(x, per_row, over_row);
+            const uint32_t rest = x - r[y] * per_row;
+            h[y] = over(rest, units, over_units), u[y] = rest - h[y] * units;
+            from[y] = x < all ? where[r[y]] : -1;
+            const long long row = from[y] + (long long)h[y] * a.c.page_tokens;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                w[2 * y + v] = make_uint4(0, 0, 0, 0);
+                s[2 * y + v] = 0.f;
+                if (from[y] >= 0) {
+                    w[2 * y + v] = *(const uint4*)((v ? a.c.v : a.c.k) + row * a.c.d + u[y] * 16);
+                    s[2 * y + v] = (v ? a.c.v_scales : a.c.k_scales)[row / kBlock];
+                }
+            }
         }
-        uint4 lo, hi;
-        values16<T>(w, s, lo, hi);
-        const mb200_heads& dst = keys ? a.k : a.v;
-        const long long to = (row0 + r) * dst.token_stride + h * dst.head_stride + u * 16;
-        store8<VEC>(dst.p, to, lo);
-        store8<VEC>(dst.p, to + 8, hi);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            if (from[y] == -1)
+                continue;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                uint4 lo, hi;
+                values16<T>(w[2 * y + v], s[2 * y + v], lo, hi);
+                const mb200_heads& dst = v ? a.v : a.k;
+                const long long to = (long long)(row0 + (int)r[y]) * dst.token_stride + h[y] * dst.head_stride + u[y] * 16;
+                store8<VEC>(dst.p, to, lo);
+                store8<VEC>(dst.p, to + 8, hi);
+            }
+        }
     }
 }
 

@@ -525,18 +525,10 @@ PyObject* attention_prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyObject* bind(PyObject*, PyObject* args) {
-    constexpr int kFunctions = 12;
-    unsigned long long at[kFunctions];
-    if (PyTuple_GET_SIZE(args) != 2 + kFunctions) {
-        PyErr_Format(PyExc_TypeError, "bind takes %d arguments", 2 + kFunctions);
+    unsigned long long at[7];
+    PyObject *fail, *memory;
+    if (!PyArg_ParseTuple(args, "OOKKKKKKK", &fail, &memory, at, at + 1, at + 2, at + 3, at + 4, at + 5, at + 6))
         return nullptr;
-    }
-    PyObject *fail = PyTuple_GET_ITEM(args, 0), *memory = PyTuple_GET_ITEM(args, 1);
-    for (int i = 0; i < kFunctions; ++i) {
-        at[i] = PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(args, 2 + i));
-        if (PyErr_Occurred())
-            return nullptr;
-    }
     abi.quantize_rows = (decltype(abi.quantize_rows))(uintptr_t)at[0];
     abi.matmul_workspace = (decltype(abi.matmul_workspace))(uintptr_t)at[1];
     abi.matmul = (decltype(abi.matmul))(uintptr_t)at[2];
@@ -544,11 +536,6 @@ PyObject* bind(PyObject*, PyObject* args) {
     abi.linear = (decltype(abi.linear))(uintptr_t)at[4];
     abi.moe_workspace = (decltype(abi.moe_workspace))(uintptr_t)at[5];
     abi.moe = (decltype(abi.moe))(uintptr_t)at[6];
-    abi.kv_append = (decltype(abi.kv_append))(uintptr_t)at[7];
-    abi.kv_read = (decltype(abi.kv_read))(uintptr_t)at[8];
-    abi.cache_workspace = (decltype(abi.cache_workspace))(uintptr_t)at[9];
-    abi.attention_cache = (decltype(abi.attention_cache))(uintptr_t)at[10];
-    abi.attention_prompt = (decltype(abi.attention_prompt))(uintptr_t)at[11];
     Py_INCREF(fail);
     Py_XSETREF(on_status, fail);
     Py_INCREF(memory);
@@ -556,8 +543,21 @@ PyObject* bind(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
+PyObject* bind_attention(PyObject*, PyObject* args) {
+    unsigned long long at[5];
+    if (!PyArg_ParseTuple(args, "KKKKK", at, at + 1, at + 2, at + 3, at + 4))
+        return nullptr;
+    abi.kv_append = (decltype(abi.kv_append))(uintptr_t)at[0];
+    abi.kv_read = (decltype(abi.kv_read))(uintptr_t)at[1];
+    abi.cache_workspace = (decltype(abi.cache_workspace))(uintptr_t)at[2];
+    abi.attention_cache = (decltype(abi.attention_cache))(uintptr_t)at[3];
+    abi.attention_prompt = (decltype(abi.attention_prompt))(uintptr_t)at[4];
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
         {"bind", bind, METH_VARARGS, "bind(raises for a status, torch.OutOfMemoryError, addresses of the library's functions)"},
+        {"bind_attention", bind_attention, METH_VARARGS, "bind_attention(addresses of the library's functions), behind bind"},
         {"quantize_rows_s8", (PyCFunction)(void*)quantize_rows_s8, METH_FASTCALL, "(x) -> (q, scales)"},
         {"matmul_s8_scaled", (PyCFunction)(void*)matmul_s8_scaled, METH_FASTCALL,
          "(a, b_packed, a_scales, b_scales, bias, dtype) -> c"},

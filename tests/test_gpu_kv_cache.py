@@ -1,5 +1,6 @@
 """The int8 cache of keys and values: appending with the position rotation, reading back, against the definition.
-Every step of it is one rounding of numbers that 64 bits hold, so whole numbers, scales and values have to be equal."""
+Every step of it is one rounding (a quotient of 24-bit numbers that is no tie is further from one than 64 bits' rounding), so
+whole numbers, scales and values have to be equal."""
 import pytest
 import torch
 
@@ -61,14 +62,13 @@ def turned(x, cos, sin, position, interleaved):
 
 
 def block_scale(amax):
-    third = torch.tensor(1 / 127, dtype=torch.float32, device="cuda")
-    s = amax.clamp(min=2.0 ** -119) * third
+    s = (amax.double().clamp(min=2.0 ** -119) / 127).float()
     return torch.where(torch.isfinite(amax), s, torch.full_like(s, float("nan")))
 
 
-def whole_of(x, factor):
-    """x and factor of at most 24 bits each: their product is exact in 64"""
-    q = torch.round(x.double() * factor.double())
+def whole_of(x):
+    """64 bits to the nearest whole number; what is none counts 0"""
+    q = torch.round(x)
     return torch.where(torch.isfinite(q), q, torch.zeros_like(q)).to(torch.int8)
 
 
@@ -89,11 +89,10 @@ def append_definition(whole, scales, table, before, counts, x, page):
             if p > first:
                 s = torch.where(torch.isnan(s) | torch.isnan(old), s + old, torch.maximum(s, old))
                 kept = whole[number, :, o:o + p - first]
-                again = whole_of(kept, (old / s)[:, None, None])
+                again = whole_of(kept.double() * (old.double() / s.double())[:, None, None])
                 whole[number, :, o:o + p - first] = torch.where((s == old)[:, None, None], kept, again)
-            inv = torch.ones_like(s) / s
-            inv = torch.where(torch.isnan(s), torch.zeros_like(s), inv)
-            whole[number, :, o + p - first:o + last - first] = whole_of(new.transpose(0, 1), inv[:, None, None])
+            quotient = new.transpose(0, 1).double() / s.double()[:, None, None]
+            whole[number, :, o + p - first:o + last - first] = whole_of(quotient)
             scales[number, :, o // BLOCK] = s
             at, p = at + last - p, last
 
@@ -152,6 +151,24 @@ def test_append(before, counts, heads, kv, d, rot, page, interleaved, dtype):
                 assert torch.equal(x, y), b
     assert torch.equal(cache.k_scales, want.k_scales) and torch.equal(cache.v_scales, want.v_scales)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_quotients_in_the_middle_and_next_to_it(dtype):
+    """Whole multiples of a number: quotients by the scale that are ties, or within a rounding of one."""
+    table, pages = table_of([64], 64, 1)
+    for unit in (1.0, 0.75, 2.0 ** -20, 1.5 * 2.0 ** -90 if dtype == torch.bfloat16 else 3.0):
+        for most in (127, 254, 85, 170, 255, 100):
+            cache = cache_of(pages, 1, 64, 128, 2)
+            want = ops.KvCacheS8(*(t.clone() for t in cache))
+            x = torch.randint(-most, most + 1, (64, 1, 128), generator=gen(most), device="cuda")
+            x[:, 0, 0] = most
+            x = (x.double() * unit).to(dtype)
+            ops.kv_append_s8(cache, table, ints([0]), x, -x, cu_tokens=ints([0, 64]))
+            append_definition(want.k, want.k_scales, table, [0], [64], x.float(), 64)
+            append_definition(want.v, want.v_scales, table, [0], [64], -x.float(), 64)
+            assert torch.equal(cache.k[table[0, 0].long()], want.k[table[0, 0].long()]), (unit, most)
+            assert all(torch.equal(a, b) for a, b in zip(cache, want)), (unit, most)
 
 
 def test_append_without_rotation_and_queries():
