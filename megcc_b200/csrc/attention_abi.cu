@@ -9,6 +9,8 @@ using namespace mb200::attn;
 
 namespace {
 
+constexpr float kLog2E = 1.44269504f;
+
 bool misaligned(const void* p, size_t bytes) {
     return ((uintptr_t)p & (bytes - 1)) != 0;
 }
@@ -216,8 +218,8 @@ int mb200_attention_cache_s8(
         rc = check_dtype(dtype, what);
     if (rc || cache->batch == 0)
         return rc;
-    if (!isfinite(scale))
-        return set_error(ST_INVALID_LAYOUT, "%s: the scale is not finite", what);
+    if (!isfinite(scale * kLog2E))
+        return set_error(ST_INVALID_LAYOUT, "%s: the scale is not finite, or too large", what);
     if (!lengths || !q || !out)
         return set_error(ST_NULL_PTR, "%s: lengths, q or out is NULL", what);
     rc = check_heads(*q, cache->batch * queries, heads, cache->d, false, "q", what);
@@ -236,7 +238,7 @@ int mb200_attention_cache_s8(
     a.c = *cache;
     a.lengths = lengths, a.heads = heads, a.queries = queries;
     a.q = *q, a.out = *out;
-    a.scale_log2 = scale * 1.44269504f;
+    a.scale_log2 = scale * kLog2E;
     a.workspace = need ? workspace : nullptr;
     rc = status_word(stream, &a.status);
     return rc ? rc : launch_attention_cache(a, dtype, (cudaStream_t)stream);
@@ -256,8 +258,8 @@ int mb200_attention_prompt(
         (!cu_k && key_tokens != tokens))
         return set_error(ST_INVALID_LAYOUT, "%s: %d sequences, %d tokens and %d of keys, %d heads over %d key heads", what,
                          batch, tokens, key_tokens, heads, kv_heads);
-    if (!isfinite(scale))
-        return set_error(ST_INVALID_LAYOUT, "%s: the scale is not finite", what);
+    if (!isfinite(scale * kLog2E))
+        return set_error(ST_INVALID_LAYOUT, "%s: the scale is not finite, or too large", what);
     if (tokens == 0 || batch == 0)
         return ST_SUCCESS;
     if (!cu_q || !q || !k || !v || !out)
@@ -296,7 +298,7 @@ int mb200_attention_prompt(
     a.heads = heads, a.kv_heads = kv_heads, a.d = d;
     a.cu_q = cu_q, a.cu_k = cu_k ? cu_k : cu_q;
     a.causal = causal != 0;
-    a.scale_log2 = scale * 1.44269504f;
+    a.scale_log2 = scale * kLog2E;
     return launch_attention_prompt(a, dtype, (cudaStream_t)stream);
 }
 

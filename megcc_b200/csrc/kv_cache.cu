@@ -12,10 +12,12 @@
 // middle between two. Where the scale grows, older numbers are made anew, q' = q * (s_before / s) to the nearest; so the
 // outcome depends on what was appended together, never on the order in which warps run. A block is one warp's: it
 // alone reads and writes it. Keys are turned twice, for the largest of them and for their numbers: held in between they
-// took the registers of half of the warps (8191 tokens of 32 + 8 + 8 heads of 128, with reading the blocks back: 94 us, 78 so).
+// took the registers of half of the warps (8191 tokens of 32 + 8 + 8 heads of 128, with reading the blocks back: 94 us, 74 so).
 //
 // What bounds it: for a step of decoding the launch and the four loads that follow from one another (lengths, page, scale,
-// whole numbers); for prompts memory.
+// whole numbers): 6 to 7 us with reading the blocks back. For prompts the instructions of the blocks' warps (8191 tokens:
+// 2.3 a clock and SM, ALUs half taken, 3.2 TB/s; the floor is 37 us). Reading back is bound by memory (65001 rows of 8
+// heads of 128: 71 us, 5.7 TB/s).
 #include "kv_cache.cuh"
 #include "umma_ptx.cuh"
 
@@ -90,9 +92,8 @@ __device__ __forceinline__ void turned(const AppendArgs& a, const Lane& l, const
         return;
     }
     const int units = a.rot / 16;
-    const bool front = l.unit < units;
     const int lane = threadIdx.x & 31;
-    const int other = turns ? (front ? lane + units : lane - units) : lane;
+    const int other = turns ? (l.unit < units ? lane + units : lane - units) : lane;
     uint4 w;
     w.x = __shfl_sync(0xffffffffu, raw.x, other), w.y = __shfl_sync(0xffffffffu, raw.y, other);
     w.z = __shfl_sync(0xffffffffu, raw.z, other), w.w = __shfl_sync(0xffffffffu, raw.w, other);
@@ -101,8 +102,8 @@ __device__ __forceinline__ void turned(const AppendArgs& a, const Lane& l, const
         Vec<T>::unpack(w, y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float p = __fmul_rn(x[i], g.c[i]), q = __fmul_rn(y[i], g.s[i]);
-            x[i] = front ? __fsub_rn(p, q) : __fadd_rn(p, q);
+            // (the first half's sines are negative here)
+            x[i] = __fadd_rn(__fmul_rn(x[i], g.c[i]), __fmul_rn(y[i], g.s[i]));
         }
     }
 }
@@ -113,6 +114,11 @@ __device__ __forceinline__ bool take_angles(const AppendArgs& a, const Lane& l, 
     if (turns) {
         if (position < a.positions) {
             angles_of<VEC>(a, l, (int)position, g);
+            if (!a.interleaved && l.unit * 16 < a.rot) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    g.s[i] = -g.s[i];
+            }
         } else {
             *(volatile int*)a.status = ERR_POSITION;
 #pragma unroll
@@ -138,12 +144,15 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, const Lane& l,
         return;
     uint4 raw[kQuerySteps];
     const int h0 = chunk * kQuerySteps * l.rows + l.sub;
+    const long long in0 = token * a.q.token_stride + h0 * a.q.head_stride + l.unit * 8, in_step = l.rows * a.q.head_stride;
+    const long long out0 = token * a.q_out.token_stride + h0 * a.q_out.head_stride + l.unit * 8,
+                    out_step = l.rows * a.q_out.head_stride;
 #pragma unroll
     for (int i = 0; i < kQuerySteps; ++i) {
         const int h = h0 + i * l.rows;
         raw[i] = make_uint4(0, 0, 0, 0);
         if (l.active && h < a.heads)
-            raw[i] = load8<VEC>(a.q.p, token * a.q.token_stride + h * a.q.head_stride + l.unit * 8);
+            raw[i] = load8<VEC>(a.q.p, in0 + i * in_step);
     }
     Angles g;
     const bool turns = take_angles<VEC>(a, l, l.active, (long long)before + (token - first), g);
@@ -153,7 +162,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, const Lane& l,
         float x[8];
         turned<T>(a, l, raw[i], turns, g, x);
         if (l.active && h < a.heads)
-            store8<VEC>(a.q_out.p, token * a.q_out.token_stride + h * a.q_out.head_stride + l.unit * 8, pack8<T>(x));
+            store8<VEC>(a.q_out.p, out0 + i * out_step, pack8<T>(x));
     }
 }
 
@@ -268,9 +277,18 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, const Lane& l,
         float x[8];
         if (values(i, x)) {
             uint32_t q[8];
+            bool near = false;  // a quotient that may be on the other side of a middle, or on one
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                q[e] = nearest_quotient(x[e], s, half, inv);
+            for (int e = 0; e < 8; ++e) {
+                const float y = __fmaf_rn(x[e], inv, 12582912.f);
+                near |= fabsf(__fmaf_rn(-__fsub_rn(y, 12582912.f), s, x[e])) >= half;
+                q[e] = __float_as_uint(y);
+            }
+            if (near) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    q[e] = nearest_quotient(x[e], s, half, inv);
+            }
             const uint2 w = make_uint2(pack4_low(q[0], q[1], q[2], q[3]) & mask, pack4_low(q[4], q[5], q[6], q[7]) & mask);
             *(uint2*)(whole + (long long)(kept + i * l.rows + l.sub) * a.c.d) = w;
         }

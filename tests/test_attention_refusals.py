@@ -93,7 +93,8 @@ FIVE = dict(table_pages=5, table_stride=5)  # (pages, which may be cut)
 
 @pytest.mark.parametrize("change,status", [
     (dict(lengths=None), NULL_PTR), (dict(heads=3), LAYOUT), (dict(heads=0), LAYOUT), (dict(queries=0), LAYOUT),
-    (dict(scale=float("nan")), LAYOUT), (dict(scale=float("inf")), LAYOUT), (dict(q=(None, 256, 64)), NULL_PTR),
+    (dict(scale=float("nan")), LAYOUT), (dict(scale=float("inf")), LAYOUT),
+    (dict(scale=3e38), LAYOUT), (dict(q=(None, 256, 64)), NULL_PTR),
     (dict(out=(None, 256, 64)), NULL_PTR), (dict(q=(P + 1, 256, 64)), LAYOUT), (dict(out=(P, 200, 64)), LAYOUT),
     (dict(out=(P, 256, 0)), LAYOUT), (dict(lengths=P + 1), LAYOUT), (dict(ws=None, **FIVE), NULL_PTR),
     (dict(ws=P + 128, **FIVE), LAYOUT), (dict(nbytes=100, **FIVE), LAYOUT), (dict(queries=1 << 29), OUT_OF_RANGE), (dict(batch=0, q=(None, 0, 0)), 0)])
@@ -140,7 +141,8 @@ def attention_prompt(change):
 @pytest.mark.parametrize("change,status", [
     (dict(batch=-1), LAYOUT), (dict(tokens=-1), LAYOUT), (dict(key_tokens=-1), LAYOUT), (dict(heads=0), LAYOUT),
     (dict(heads=5), LAYOUT), (dict(kv_heads=0), LAYOUT), (dict(cu_k=None), LAYOUT), (dict(d=24), LAYOUT), (dict(d=-16), LAYOUT),
-    (dict(d=256), OUT_OF_RANGE), (dict(dtype=0), DTYPE), (dict(scale=float("inf")), LAYOUT), (dict(cu_q=None), NULL_PTR),
+    (dict(d=256), OUT_OF_RANGE), (dict(dtype=0), DTYPE), (dict(scale=float("inf")), LAYOUT), (dict(scale=-3e38), LAYOUT),
+    (dict(cu_q=None), NULL_PTR),
     (dict(q=(None, 256, 64)), NULL_PTR), (dict(nk=(None, 128, 64)), NULL_PTR), (dict(nv=(None, 128, 64)), NULL_PTR),
     (dict(out=(None, 256, 64)), NULL_PTR), (dict(q=(P + 2, 256, 64)), LAYOUT), (dict(nk=(P, 130, 64)), LAYOUT),
     (dict(nv=(P, 128, 0)), LAYOUT), (dict(nv=(P, 0, 64)), LAYOUT), (dict(q=(P, 256, 68)), LAYOUT),
