@@ -332,12 +332,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         *abort = 0;
         s_never = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    } else if (threadIdx.x == 256) {
+    } else if (threadIdx.x == 288) {
         tma_prefetch_map(&maps.q);
         tma_prefetch_map(&maps.k);
         tma_prefetch_map(&maps.v);
     }
     if (warp == 8) {
+        __syncwarp();  // (the whole warp's, .aligned: none of its lanes does anything else in front of this)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(512)
                      : "memory");
@@ -612,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
     fence_before();
     __syncthreads();
     fence_after();
+    __syncwarp();
     if (warp == 8)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
