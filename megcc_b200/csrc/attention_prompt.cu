@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         *abort = 0;
         s_never = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    } else if (threadIdx.x == 288) {
+    } else if (threadIdx.x == 128) {
         tma_prefetch_map(&maps.q);
         tma_prefetch_map(&maps.k);
         tma_prefetch_map(&maps.v);
