@@ -14,8 +14,10 @@
 // a lane takes 16 neighbouring ones with one load.
 //   O: values become fp16, which holds them exactly: a byte permutation makes 1024 + (v + 128) of them, and a subtraction v.
 // V^T comes by ldmatrix.trans over pairs of bytes, whose two dimensions the same permutation separates. P^T is turned by
-// movmatrix. P is rounded to fp16 (2^-12, where results have 2^-9), for fp16 results held as two such numbers, after it
-// took its block's scale of V relative to the largest so far, which keeps it in range.
+// movmatrix. P takes its block's scale of V and is rounded to fp16 (2^-12, where results have 2^-9), for fp16 results held as
+// two such numbers. What keeps it in range there is a power of two of each row's own, of the largest product of a probability
+// and a scale that the row has met: blocks that a row does not see, or that weigh nothing, take no bits from the others
+// whatever their scales.
 //
 // All blocks of all sequences and key heads are one line of rounds (a step of 32 positions for each of a CTA's warps),
 // cut evenly over the CTAs whatever the lengths, which only the device knows. Each warp has a ring of asynchronous copies of
@@ -135,6 +137,38 @@ __device__ __forceinline__ float power_of_two(int e) {
 __device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) {
     const int e = (int)(magnitude_bits >> 23);
     return e == 0 || e == 255 ? 0 : max(-120, min(120, e - 127));
+}
+
+// 1 / x of a power of two whose inverse is a normal number
+__device__ __forceinline__ float inverse_power(float x) {
+    return __uint_as_float((254u << 23) - __float_as_uint(x));
+}
+// The exponent of a block's scale of V, -120 at least. (One that is no number makes its sums NaN whatever they count.)
+__device__ __forceinline__ float exponent_of_scale(float scale) {
+    const uint32_t size = magnitude(scale);
+    return size >= 0x7f800000u ? -120.f : (float)max(-120, (int)(size >> 23) - 127);
+}
+// A row whose scores have passed its maximum m, or whose scores with their scales' exponents have passed w: n and u are this
+// lane's largest of either. Returns what the row's sums are multiplied by. k is at least -110, where 2^-126, the smallest
+// scale, still leaves P 16 bits, and at most 127: w - m is no larger.
+__device__ __forceinline__ float raised(float n, float u, float& m, float& l, float& w, float& up) {
+#pragma unroll
+    for (int x = 4; x < 32; x *= 2) {
+        n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
+        u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, x));
+    }
+    const float t = fmaxf(n, m);
+    w = fmaxf(u, w);
+    if (t == __uint_as_float(0xff800000u))  // (nothing seen so far: there is nothing to scale)
+        return 1.f;
+    const int before = kLift + 127 - (int)(__float_as_uint(up) >> 23);
+    const int k = max(-110, min(127, __float2int_ru(w - t)));
+    const float down = t == m ? 1.f : exp2_fast(m - t);
+    const float r = k == before ? down : exp2_fast((m - t) + (float)(before - k));
+    l = __fmul_rn(l, down);
+    m = t;
+    up = power_of_two(kLift - k);
+    return r;
 }
 
 // The workspace: sums [cta][first or last][row][D] of what was cut, then [..][row] maxima and totals, then for each CTA
@@ -399,16 +433,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         }
         const int seen_by_all = length - a.queries + 1 + row0 / group;
 
-        float o[NT][kTiles][4], m0[NT], m1[NT], l0[NT], l1[NT];
+        // of rows 2 c and 2 c + 1: maximum of the scores, sum of the powers, maximum of scores and their block's exponent
+        // of V, and 2^(kLift - k): the sums hold 2^(kLift - k) times what they are, with m + k >= w
+        float o[NT][kTiles][4], m0[NT], m1[NT], l0[NT], l1[NT], w0[NT], w1[NT], up0[NT], up1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            m0[nt] = m1[nt] = none;
+            m0[nt] = m1[nt] = w0[nt] = w1[nt] = none;
             l0[nt] = l1[nt] = 0.f;
+            up0[nt] = up1[nt] = 1.f;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
                 o[nt][t][0] = o[nt][t][1] = o[nt][t][2] = o[nt][t][3] = 0.f;
         }
-        int top = -121;  // exponent of the largest scale of V so far
         uint32_t stage = ring;
 
 #pragma unroll 1
@@ -467,27 +503,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
                         }
             }
             bool raise = false;
-            float n0[NT], n1[NT];
+            float n0[NT], n1[NT], u0[NT], u1[NT];
+            const float e0 = exponent_of_scale(vs[0]), e1 = exponent_of_scale(vs[1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                n0[nt] = fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2]));
-                n1[nt] = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3]));
+                const float a0 = fmaxf(s[0][nt][0], s[0][nt][2]), b0 = fmaxf(s[1][nt][0], s[1][nt][2]);
+                const float a1 = fmaxf(s[0][nt][1], s[0][nt][3]), b1 = fmaxf(s[1][nt][1], s[1][nt][3]);
+                n0[nt] = fmaxf(a0, b0), n1[nt] = fmaxf(a1, b1);
+                u0[nt] = fmaxf(a0 + e0, b0 + e1), u1[nt] = fmaxf(a1 + e0, b1 + e1);
                 raise |= n0[nt] > m0[nt] + kAhead || n1[nt] > m1[nt] + kAhead;
+                raise |= u0[nt] > w0[nt] + kAhead || u1[nt] > w1[nt] + kAhead;
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int x = 4; x < 32; x *= 2) {
-                        n0[nt] = fmaxf(n0[nt], __shfl_xor_sync(0xffffffffu, n0[nt], x));
-                        n1[nt] = fmaxf(n1[nt], __shfl_xor_sync(0xffffffffu, n1[nt], x));
-                    }
-                    const float t0 = fmaxf(n0[nt], m0[nt]), t1 = fmaxf(n1[nt], m1[nt]);
-                    // (nothing seen so far: there is nothing to scale)
-                    const float r0 = t0 == m0[nt] ? 1.f : exp2_fast(m0[nt] - t0);
-                    const float r1 = t1 == m1[nt] ? 1.f : exp2_fast(m1[nt] - t1);
-                    m0[nt] = t0, m1[nt] = t1;
-                    l0[nt] = __fmul_rn(l0[nt], r0), l1[nt] = __fmul_rn(l1[nt], r1);
+                    const float r0 = raised(n0[nt], u0[nt], m0[nt], l0[nt], w0[nt], up0[nt]);
+                    const float r1 = raised(n1[nt], u1[nt], m1[nt], l1[nt], w1[nt], up1[nt]);
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
                         o[nt][t][0] *= r0, o[nt][t][1] *= r1;
@@ -495,40 +526,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
                     }
                 }
             }
-            // (a block without a scale makes its sums NaN whatever they count)
-            int ev = top;
-#pragma unroll
-            for (int x = 0; x < kStep; ++x) {
-                const uint32_t size = magnitude(vs[x]);
-                ev = max(ev, size >= 0x7f800000u ? top : max(-120, (int)(size >> 23) - 127));
-            }
-            if (ev > top) {
-                // (first step: the sums are zero)
-                const float r = top == -121 ? 1.f : power_of_two(max(-126, top - ev));
-                top = ev;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[nt][t][e] *= r;
-            }
-            const float unit = power_of_two(kLift - top);
             uint32_t hi[kStep][NT][2], lo[kStep][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float z0 = m0[nt] == none ? 0.f : m0[nt], z1 = m1[nt] == none ? 0.f : m1[nt];
 #pragma unroll
                 for (int x = 0; x < kStep; ++x) {
-                    const float lift = __fmul_rn(vs[x], unit);
                     float p[4] = {exp2_fast(s[x][nt][0] - z0), exp2_fast(s[x][nt][1] - z1), exp2_fast(s[x][nt][2] - z0),
                                   exp2_fast(s[x][nt][3] - z1)};
                     l0[nt] += p[0] + p[2], l1[nt] += p[1] + p[3];
                     // (what is not seen stays 0 whatever the block's scale)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        p[e] = p[e] == 0.f ? 0.f : __fmul_rn(p[e], lift);
+                        p[e] = p[e] == 0.f ? 0.f : __fmul_rn(__fmul_rn(p[e], e & 1 ? up1[nt] : up0[nt]), vs[x]);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const uint32_t w = pack_f16(p[2 * e], p[2 * e + 1]);
@@ -584,15 +594,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         const int active = min(kWarps, (count + kStep - 1) / kStep);
         float* sums = (float*)smem;  // [warp][row][kPitch]
         if (warp < active) {
-            const float up = power_of_two(max(-126, top - kLift));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                const float down0 = inverse_power(up0[nt]), down1 = inverse_power(up1[nt]);
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     float* p = sums + (warp * kRows + nt * 8 + 2 * c) * kPitch<D> + 16 * t + 2 * g;
-                    *(float2*)p = make_float2(o[nt][t][0] * up, o[nt][t][2] * up);
-                    *(float2*)(p + kPitch<D>) = make_float2(o[nt][t][1] * up, o[nt][t][3] * up);
+                    *(float2*)p = make_float2(o[nt][t][0] * down0, o[nt][t][2] * down0);
+                    *(float2*)(p + kPitch<D>) = make_float2(o[nt][t][1] * down1, o[nt][t][3] * down1);
                 }
+            }
         }
         // each warp's weight in a row: what its maximum lies below the largest, over the total where that is all of it
         const bool whole = blk == 0 && count == all;
