@@ -535,10 +535,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
                     float p[4] = {exp2_fast(s[x][nt][0] - z0), exp2_fast(s[x][nt][1] - z1), exp2_fast(s[x][nt][2] - z0),
                                   exp2_fast(s[x][nt][3] - z1)};
                     l0[nt] += p[0] + p[2], l1[nt] += p[1] + p[3];
-                    // (what is not seen stays 0 whatever the block's scale)
+                    // (what is not seen stays 0 whatever the block's scale; what is seen is none if that is none, also with p = 0)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        p[e] = p[e] == 0.f ? 0.f : __fmul_rn(__fmul_rn(p[e], e & 1 ? up1[nt] : up0[nt]), vs[x]);
+                        p[e] = s[x][nt][e] == none ? 0.f : __fmul_rn(__fmul_rn(p[e], e & 1 ? up1[nt] : up0[nt]), vs[x]);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const uint32_t w = pack_f16(p[2 * e], p[2 * e + 1]);

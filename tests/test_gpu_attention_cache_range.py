@@ -142,3 +142,14 @@ def test_scales_of_all_sizes(spread):
         check(ops.attention_cache_s8(q, cache, table, ints(lengths)), q, cache, table, lengths, 16)
         cache.v_scales.mul_(2.0 ** (spread - 90))
         check(ops.attention_cache_s8(q, cache, table, ints(lengths)), q, cache, table, lengths, 16)
+
+
+def test_a_position_of_no_probability_whose_values_are_none():
+    """0 times a NaN is one: every query that sees the block has it, however small its probability."""
+    table, pages = table_of([100], 16, 1)
+    for block, score in ((0, -200.0), (3, -200.0), (6, -200.0), (3, 1.0)):
+        cache = cache_of(pages, 1, 16, 64, 2)
+        q = torch.randn((1, 1, 64), generator=gen(3), device="cuda").bfloat16()
+        against(cache, table, 0, block * 16, q[0], score)
+        cache.v_scales[table[0, block].long()] = float("nan")
+        assert bool(torch.isnan(ops.attention_cache_s8(q, cache, table, ints([100]))).all())
