@@ -171,7 +171,7 @@ __device__ __forceinline__ float raised(float n, float u, float& m, float& l, fl
     return r;
 }
 
-// The workspace: sums [cta][first or last][row][D] of what was cut, then [..][row] maxima and totals, then for each CTA
+// The workspace: averages [cta][first or last][row][D] of what was cut, then [..][row] maxima and totals, then for each CTA
 // the item (a sequence's key head and tile of rows) inside which its part of the line begins
 struct Cut {
     int b, at;              // b < 0: it begins with an item, or there is none
@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
     __shared__ long long s_from, s_to, s_rest, s_quota;
     __shared__ int s_b;
     __shared__ float2 s_stats[kWarps][kRows];
-    __shared__ float s_weight[kWarps][kRows];
+    __shared__ float2 s_weight[kWarps][kRows];
+    __shared__ float s_down[kWarps][kRows];
     const int tid = threadIdx.x, lane = tid & 31, warp = umma::uniform_warp_index();
     const int g = lane >> 2, c = lane & 3;
     const int d = FULL ? D : a.c.d, group = a.heads / a.c.kv_heads;
@@ -588,6 +589,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             if (g == 0) {
                 s_stats[warp][nt * 8 + 2 * c] = make_float2(m0[nt], l0[nt]);
                 s_stats[warp][nt * 8 + 2 * c + 1] = make_float2(m1[nt], l1[nt]);
+                s_down[warp][nt * 8 + 2 * c] = inverse_power(up0[nt]);
+                s_down[warp][nt * 8 + 2 * c + 1] = inverse_power(up1[nt]);
             }
         }
         __syncthreads();  // (nobody reads the rings any more)
@@ -595,17 +598,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         float* sums = (float*)smem;  // [warp][row][kPitch]
         if (warp < active) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float down0 = inverse_power(up0[nt]), down1 = inverse_power(up1[nt]);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     float* p = sums + (warp * kRows + nt * 8 + 2 * c) * kPitch<D> + 16 * t + 2 * g;
-                    *(float2*)p = make_float2(o[nt][t][0] * down0, o[nt][t][2] * down0);
-                    *(float2*)(p + kPitch<D>) = make_float2(o[nt][t][1] * down1, o[nt][t][3] * down1);
+                    *(float2*)p = make_float2(o[nt][t][0], o[nt][t][2]);
+                    *(float2*)(p + kPitch<D>) = make_float2(o[nt][t][1], o[nt][t][3]);
                 }
-            }
         }
-        // each warp's weight in a row: what its maximum lies below the largest, over the total where that is all of it
+        // each warp's weight in a row: what its maximum lies below the largest, over the total, and the power of two that its sums
+        // are held away from what they are. In this order nothing on the way to an average is larger than the values are
         const bool whole = blk == 0 && count == all;
         if (tid < kRows) {
             float m = none;
@@ -621,10 +623,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
                 total += w < active ? st.y * f[w] : 0.f;
             }
             // (nothing seen: zeros)
-            const float over = !whole ? 1.f : total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+            const float over = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w)
-                s_weight[w][tid] = __fmul_rn(f[w], over);
+                s_weight[w][tid] = make_float2(__fmul_rn(f[w], over), s_down[w][tid]);
             if (!whole)
                 parts.stats[((long long)blockIdx.x * 2 + !first) * kRows + tid] = make_float2(m, total);
         }
@@ -636,9 +638,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             for (int w = 0; w < kWarps; ++w)
                 if (w < active) {
                     const float4 v = *(const float4*)(sums + (w * kRows + r) * kPitch<D> + e);
-                    const float f = s_weight[w][r];
-                    sum.x = __fmaf_rn(v.x, f, sum.x), sum.y = __fmaf_rn(v.y, f, sum.y);
-                    sum.z = __fmaf_rn(v.z, f, sum.z), sum.w = __fmaf_rn(v.w, f, sum.w);
+                    const float2 f = s_weight[w][r];
+                    sum.x = __fmaf_rn(v.x * f.x, f.y, sum.x), sum.y = __fmaf_rn(v.y * f.x, f.y, sum.y);
+                    sum.z = __fmaf_rn(v.z * f.x, f.y, sum.z), sum.w = __fmaf_rn(v.w * f.x, f.y, sum.w);
                 }
             if (!whole)
                 *(float4*)(parts.sums + (((long long)blockIdx.x * 2 + !first) * kRows + r) * D + e) = sum;
@@ -690,20 +692,29 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const CacheArgs a
     const int n = c1 + 1 - c0;
     const float none = __uint_as_float(0xff800000u);
     float m = none, total = 0.f;
-    for (int i = lane; i < n; i += 32)
-        m = fmaxf(m, parts.stats[part(i)].x);
+    for (int i = lane; i < n; i += 32) {
+        const float2 st = parts.stats[part(i)];
+        const float t = fmaxf(m, st.x), z = t == none ? 0.f : t;
+        total = __fmul_rn(total, exp2_fast(m - z)) + st.y * exp2_fast(st.x - z);
+        m = t;
+    }
+    float most = m;
 #pragma unroll
     for (int x = 1; x < 32; x *= 2)
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    const float z = m == none ? 0.f : m;
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+    const float z = most == none ? 0.f : most;
+    total = __fmul_rn(total, exp2_fast(m - z));
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2)
+        total += __shfl_xor_sync(0xffffffffu, total, x);
+    const float over = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
     const int sub = warp * kAtOnce + lane / kLanes, e = lane % kLanes;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int base = 0; base < n; base += 32) {
         float f = 0.f;
         if (base + lane < n) {
             const float2 st = parts.stats[part(base + lane)];
-            f = exp2_fast(st.x - z);
-            total += st.y * f;
+            f = __fmul_rn(st.y * exp2_fast(st.x - z), over);
         }
 #pragma unroll 4
         for (int x = 0; x < 32; x += kStride) {
@@ -716,9 +727,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const CacheArgs a
             }
         }
     }
-#pragma unroll
-    for (int x = 1; x < 32; x *= 2)
-        total += __shfl_xor_sync(0xffffffffu, total, x);
     s_sum[sub][e] = sum;
     __syncthreads();
     if (threadIdx.x >= kLanes || 4 * e >= a.c.d)
@@ -729,8 +737,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const CacheArgs a
         const float4 v = s_sum[x][e];
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
-    const float over = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
-    sum.x *= over, sum.y *= over, sum.z *= over, sum.w *= over;
     store4<T, VEC>(a.out.p, row_at(a, a.out, a.heads / a.c.kv_heads, cut.b, h, tile * tile_rows + r) + 4 * e, sum);
 }
 

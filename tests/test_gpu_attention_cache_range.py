@@ -153,3 +153,13 @@ def test_a_position_of_no_probability_whose_values_are_none():
         against(cache, table, 0, block * 16, q[0], score)
         cache.v_scales[table[0, block].long()] = float("nan")
         assert bool(torch.isnan(ops.attention_cache_s8(q, cache, table, ints([100]))).all())
+
+
+def test_values_next_to_the_largest():
+    """An average of large values is none larger, whatever their number."""
+    table, pages = table_of([4000], 16, 1)
+    cache = cache_of(pages, 1, 16, 64, 2)
+    cache.v.copy_(cache.v.abs().clamp(min=100))
+    cache.v_scales.fill_(2.0 ** 120 * 0.99)
+    q = torch.randn((1, 1, 4, 64), generator=gen(3), device="cuda").bfloat16()
+    check(ops.attention_cache_s8(q[:, 0].contiguous(), cache, table, ints([4000]))[:, None], q, cache, table, [4000], 16)
