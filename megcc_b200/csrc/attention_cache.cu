@@ -133,11 +133,6 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 __device__ __forceinline__ float power_of_two(int e) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-// the exponent of a finite, normal magnitude; 0 for zero, infinities and NaNs (nothing is scaled then)
-__device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) {
-    const int e = (int)(magnitude_bits >> 23);
-    return e == 0 || e == 255 ? 0 : max(-120, min(120, e - 127));
-}
 
 // 1 / x of a power of two whose inverse is a normal number
 __device__ __forceinline__ float inverse_power(float x) {
@@ -199,8 +194,8 @@ __device__ __forceinline__ long long row_at(const CacheArgs& a, const mb200_head
 }
 
 // Queries as whole numbers Q of 22 bits, hi 2^16 + mid 2^8 + lo (lo, mid in -128 .. 127) times 2^(e - 20), e the exponent of the
-// row's largest: 1.5 * 2^23 + 0x8080 added in the multiplication leaves, in the sum's bytes, lo + 128, mid + 128 and
-// hi + 64 (|hi| < 64).
+// row's largest (from -106 on; below that 2^-126, since the inverse has to be a number as well): 1.5 * 2^23 + 0x8080 added
+// in the multiplication leaves, in the sum's bytes, lo + 128, mid + 128 and hi + 64 (|hi| < 64).
 constexpr int kPlanes = 3;
 __device__ __forceinline__ void planes_of(const float (&x)[4], float up, uint32_t (&w)[kPlanes]) {
     uint32_t b[4];
@@ -410,9 +405,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             }
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int e = exponent_of(most);
             const bool finite = most < 0x7f800000u;
-            const int shift = min(126, 20 - e);
+            const int shift = min(126, 20 + 127 - (int)(most >> 23));
             const float up = finite ? power_of_two(shift) : 0.f;
             // (a row with a NaN or an infinity has no whole numbers: all of it is NaN)
             const float factor = finite ? __fmul_rn(power_of_two(-shift), a.scale_log2) : __uint_as_float(0x7fffffffu);

@@ -163,3 +163,19 @@ def test_values_next_to_the_largest():
     cache.v_scales.fill_(2.0 ** 120 * 0.99)
     q = torch.randn((1, 1, 4, 64), generator=gen(3), device="cuda").bfloat16()
     check(ops.attention_cache_s8(q[:, 0].contiguous(), cache, table, ints([4000]))[:, None], q, cache, table, [4000], 16)
+
+
+@pytest.mark.parametrize("heads,kv,d", [(8, 1, 64), (16, 1, 128), (3, 1, 80)])
+def test_queries_of_all_sizes(heads, kv, d):
+    """Rows from the smallest numbers of bf16 to the largest, with keys that bring their scores to size."""
+    table, pages = table_of([300], 16, 1)
+    for e in (-126, -117, -106, -90, -20, 20, 100, 119, 120, 121, 122, 123, 124, 125, 126, 127):
+        cache = cache_of(pages, kv, 16, d, 2)
+        q = torch.rand((1, 1, heads, d), generator=gen(3), device="cuda") - 0.5
+        q[0, 0, :, 0] = torch.linspace(1, 1.984375, heads, device="cuda")
+        q = (q.double() * 2.0 ** e).bfloat16()
+        assert bool(torch.isfinite(q).all())
+        scale = 2.0 ** (-e / 2) / 3
+        cache.k_scales.mul_(2.0 ** (-e - round(-e / 2)))
+        got = ops.attention_cache_s8(q[:, 0].contiguous(), cache, table, ints([300]), scale=scale)
+        check(got[:, None], q, cache, table, [300], 16, scale)
