@@ -313,8 +313,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
 
 #pragma unroll 1
     while (left > 0) {
-        const int length = min(a.lengths[b], shape.capacity);
-        const int all = (max(length, 0) + kBlock - 1) / kBlock;
+        const int length = a.lengths[b];
+        const int all = blocks_of(a, shape.capacity, b);
         if (all == 0) {
             ++b;
             continue;
@@ -379,6 +379,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
         for (int i = 0; i < R::kStages - 1; ++i)
             ask(i);
 
+        // positions that a row sees, whether the table has them or not
+        auto limit = [&](int row) {
+            const int i = row / group;
+            return min(length - a.queries + 1, 0x7fffffff - i) + i;
+        };
         // queries: lane (g, c) holds of row g the dimensions 64 i + 16 c .. + 15, and its factor
         uint32_t qf[NT][kPlanes][kChunks][4];
         float f0[NT], f1[NT];
@@ -422,11 +427,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
                 }
             f0[nt] = __shfl_sync(0xffffffffu, factor, 8 * c);
             f1[nt] = __shfl_sync(0xffffffffu, factor, 8 * c + 4);
-            // positions that rows 2 c and 2 c + 1 of this tile see
-            lim0[nt] = length - a.queries + 1 + (row0 + nt * 8 + 2 * c) / group;
-            lim1[nt] = length - a.queries + 1 + (row0 + nt * 8 + 2 * c + 1) / group;
+            lim0[nt] = limit(row0 + nt * 8 + 2 * c);
+            lim1[nt] = limit(row0 + nt * 8 + 2 * c + 1);
         }
-        const int seen_by_all = length - a.queries + 1 + row0 / group;
+        const int seen_by_all = limit(row0);
 
         // of rows 2 c and 2 c + 1: maximum of the scores, sum of the powers, maximum of scores and their block's exponent
         // of V, and 2^(kLift - k): the sums hold 2^(kLift - k) times what they are, with m + k >= w

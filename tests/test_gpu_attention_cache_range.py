@@ -179,3 +179,17 @@ def test_queries_of_all_sizes(heads, kv, d):
         cache.k_scales.mul_(2.0 ** (-e - round(-e / 2)))
         got = ops.attention_cache_s8(q[:, 0].contiguous(), cache, table, ints([300]), scale=scale)
         check(got[:, None], q, cache, table, [300], 16, scale)
+
+
+@pytest.mark.parametrize("over", [1, 2, 3, 4, 20, 2 ** 31 - 1 - 64])
+def test_several_queries_of_a_sequence_longer_than_its_table(over):
+    """Positions that the table has no room for are not seen; the others are by every query that comes behind them."""
+    for heads, d in ((4, 64), (1, 128), (24, 64)):
+        table, pages = table_of([64, 30], 16, 1)
+        table = table[:, :4].contiguous()
+        cache = cache_of(pages, 1, 16, d, 2)
+        q = torch.randn((2, 4, heads, d), generator=gen(3), device="cuda").half()
+        got = ops.attention_cache_s8(q, cache, table, ints([64 + over, 30]))
+        torch.cuda.synchronize()
+        assert ops.device_status() == 0x201
+        check(got, q, cache, table, [64 + over, 30], 16)
