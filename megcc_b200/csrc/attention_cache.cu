@@ -37,6 +37,7 @@ constexpr int kRound = kWarps * kStep;     // blocks of a CTA's round
 constexpr float kAhead = 8.f;              // how far a score may pass the running maximum
 constexpr int kLift = 6;                   // probabilities are held 2^6 times: 2^8 * 2 * 2^6 < 65504
 constexpr int kCtasPerSm = 2;
+constexpr int kIdleRows = 1024;
 
 template <int D>
 struct Ring {
@@ -654,15 +655,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) cache_kernel(const Cache
             ++b;
         }
     }
-    // sequences without a position: nothing is seen
-    for (b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
-        if (a.lengths[b] > shape.capacity && tid == 0)
+    // sequences without a position: nothing is seen. kIdleRows rows of one (a query's heads) at a time, a warp each
+    const int all_rows = a.queries * a.heads, pieces = (all_rows - 1) / kIdleRows + 1;
+    for (long long x = blockIdx.x; x < (long long)a.c.batch * pieces; x += gridDim.x) {
+        const int idle = pieces == 1 ? (int)x : (int)(x / pieces), length = a.lengths[idle];
+        const unsigned r0 = (unsigned)(x - (long long)idle * pieces) * kIdleRows, r1 = min(r0 + kIdleRows, (unsigned)all_rows);
+        if (length > shape.capacity && tid == 0 && r0 == 0)
             *(volatile int*)a.status = ERR_PAGE;
-        if (a.lengths[b] <= 0)
-            for (int i = tid; i < a.queries * a.heads * d; i += kThreads) {
-                const int e = i % d, th = i / d;
-                ((T*)a.out.p)[((long long)b * a.queries + th / a.heads) * a.out.token_stride +
-                              (long long)(th % a.heads) * a.out.head_stride + e] = from_float<T>(0.f);
+        if (length <= 0)
+            for (unsigned r = r0 + warp; r < r1; r += kWarps) {
+                const unsigned i = r / a.heads;
+                T* p = (T*)a.out.p + ((long long)idle * a.queries + i) * a.out.token_stride +
+                       (long long)(r - i * a.heads) * a.out.head_stride;
+                for (int e = lane; e < d; e += 32)
+                    p[e] = from_float<T>(0.f);
             }
     }
 }

@@ -193,3 +193,17 @@ def test_several_queries_of_a_sequence_longer_than_its_table(over):
         torch.cuda.synchronize()
         assert ops.device_status() == 0x201
         check(got, q, cache, table, [64 + over, 30], 16)
+
+
+def test_unused_slots_of_more_than_two_to_the_31_elements():
+    """Their results are zeros to the last one."""
+    cache = ops.kv_cache_s8(1, 1, 16, 128)
+    queries, heads = 16385, 1024
+    q = torch.zeros((1, 1, 1, 128), device="cuda").half().expand(1, queries, heads, 128)
+    out = torch.full((1, queries, heads, 128), 7.0, dtype=torch.float16, device="cuda")
+    ops.attention_cache_s8(q, cache, ints([[0]]), ints([0]), out=out)
+    assert not bool(out.view(torch.int32).any())
+    # two slots, one of them in use
+    few = torch.full((2, 40, 64, 128), 7.0, dtype=torch.float16, device="cuda")
+    ops.attention_cache_s8(q[:, :40, :64].expand(2, 40, 64, 128), cache, ints([[0], [0]]), ints([-1, 16]), out=few)
+    assert not bool(few.any())
