@@ -227,8 +227,10 @@ __device__ __forceinline__ void powers(uint32_t (&s)[kTile], float scale, float 
     }
 }
 
+// The whole warp waits, and goes on or gives up as one: what follows (products, loads of tensor memory, __syncwarp) wants
+// all of its lanes
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort, int* status) {
-    if (mbar_wait_u32(bar, parity, abort))
+    if (__all_sync(0xffffffffu, mbar_wait_u32(bar, parity, abort)))
         return true;
     *abort = 1;
     *(volatile int*)status = ERR_PROMPT_WAIT;
@@ -500,8 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         bool ok = true;
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-            // (the vote: loads of tensor memory want the whole warp)
-            ok = __all_sync(0xffffffffu, wait_for(s_full + 8 * t, j & 1, abort, a.status));
+            ok = wait_for(s_full + 8 * t, j & 1, abort, a.status);
             if (!ok)
                 break;
             fence_after();
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         // products are complete ----
         const float total = (l[0].x + l[0].y) + (l[1].x + l[1].y);
         if (ok && n > 0) {
-            ok = __all_sync(0xffffffffu, wait_for(o_full + 8 * t, (n - 1) & 1, abort, a.status));
+            ok = wait_for(o_full + 8 * t, (n - 1) & 1, abort, a.status);
             fence_after();
         }
         if (ok) {
