@@ -204,7 +204,7 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, const Lane& l,
     const long long p0 = from > before ? from : before;
     const long long end = (long long)before + n;
     const long long p1 = from + kBlock < end ? from + kBlock : end;
-    if (j < 0 || p0 >= p1 || p1 > 0x7fffffff)
+    if (j < 0 || p0 >= p1)
         return;
     const int count = (int)(p1 - p0), kept = (int)(p0 - from);
     const int token = first + (int)(p0 - before);
@@ -218,7 +218,7 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, const Lane& l,
         if (l.active && t < count)
             raw[i] = load8<VEC>(src.p, (token + t) * src.token_stride + h * src.head_stride + l.unit * 8);
     }
-    const int page = page_of(a.c, b, (int)from);
+    const int page = from <= 0x7fffffff ? page_of(a.c, b, (int)from) : -1;
     int8_t* whole = nullptr;
     float* scale = nullptr;
     uint32_t old_bits = 0;
