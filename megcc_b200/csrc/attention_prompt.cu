@@ -495,8 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
         const uint32_t col_s = tmem + lanes + kColS + t * kTile, col_o = tmem + lanes + kColO + t * kTile;
         const int limit = w.limit(row >> w.pack), first_limit = w.limit((row - lane) >> w.pack);
         const float none = __uint_as_float(0xff800000u);
-        // (a scale of 0 takes all scores for 0, and what is hidden for -infinity still)
-        const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
+        // (scores get the scale's sign, and with a scale of 0 become 0: what is hidden counts as -infinity still)
+        const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2), sign = a.scale_log2 == 0.f ? 0.f : -1.f;
         float m = none;
         float2 l[2] = {};
         bool ok = true;
@@ -513,10 +513,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(
 #pragma unroll
             for (int x = 0; x < 4; ++x)
                 tmem_ld_wait32(s + 32 * x);
-            if (a.scale_log2 < 0.f) {
+            if (a.scale_log2 <= 0.f) {
 #pragma unroll
                 for (int x = 0; x < kTile; ++x)
-                    s[x] ^= 0x80000000u;
+                    s[x] = __float_as_uint(__uint_as_float(s[x]) * sign);
             }
             const bool hides = (j + 1) * kTile > first_limit;  // (of the warp's rows the first one sees the least)
             if (hides) {
