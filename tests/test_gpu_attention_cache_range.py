@@ -7,6 +7,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from megcc_b200 import ops  # noqa: E402
+from test_gpu_attention_cache import CASES  # noqa: E402
 from test_gpu_kv_cache import IDS, TYPES, cache_of, gen, ints, rows_at, table_of  # noqa: E402
 
 
@@ -207,3 +208,39 @@ def test_unused_slots_of_more_than_two_to_the_31_elements():
     few = torch.full((2, 40, 64, 128), 7.0, dtype=torch.float16, device="cuda")
     ops.attention_cache_s8(q[:, :40, :64].expand(2, 40, 64, 128), cache, ints([[0], [0]]), ints([-1, 16]), out=few)
     assert not bool(few.any())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("length", [1, 3])
+def test_probabilities_have_the_bits_that_results_need(length, dtype):
+    """With a position or three the result is their values themselves, off by what probabilities are rounded to: fp16 results
+    leave room for less than a single fp16 probability."""
+    table, pages = table_of([length], 16, 1)
+    for seed in range(20):
+        cache = cache_of(pages, 2, 16, 64, seed)
+        q = torch.randn((1, 1, 8, 64), generator=gen(seed), device="cuda").to(dtype)
+        got = ops.attention_cache_s8(q[:, 0].contiguous(), cache, table, ints([length]))
+        check(got[:, None], q, cache, table, [length], 16)
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("lengths,queries,heads,kv,d,page", [c for c in CASES if sum(c[0]) * c[2] < 20000])
+def test_attention_within_the_bits_that_it_holds(lengths, queries, heads, kv, d, page, dtype):
+    table, pages = table_of(lengths, page, 1)
+    cache = cache_of(pages, kv, page, d, 2)
+    q = torch.randn((len(lengths), queries, heads, d), generator=gen(3), device="cuda").to(dtype)
+    got = ops.attention_cache_s8(q if queries > 1 else q[:, 0].contiguous(), cache, table, ints(lengths))
+    check(got.view(q.shape), q, cache, table, lengths, page)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_queries_have_more_bits_than_their_type(dtype):
+    """A row with one large element, where the keys have zeros: what the scores come from lies far below it."""
+    table, pages = table_of([50], 16, 1)
+    for down in (2.0 ** -6, 2.0 ** -9, 2.0 ** -11):
+        cache = cache_of(pages, 1, 16, 64, 2)
+        cache.k[..., 0] = 0
+        q = torch.randn((1, 1, 8, 64), generator=gen(3), device="cuda")
+        q[..., 0] = 1.5 / down
+        q = q.to(dtype)
+        got = ops.attention_cache_s8(q[:, 0].contiguous(), cache, table, ints([50]))
+        check(got[:, None], q, cache, table, [50], 16)
