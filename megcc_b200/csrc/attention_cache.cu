@@ -695,8 +695,18 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const CacheArgs a
     auto part = [&](int i) { return (i == 0 ? first : (long long)(c0 + i) * 2 * tile_rows) + r; };
     const int n = c1 + 1 - c0;
     const float none = __uint_as_float(0xff800000u);
-    float m = none, total = 0.f;
-    for (int i = lane; i < n; i += 32) {
+    const int sub = warp * kAtOnce + lane / kLanes, e = lane % kLanes;
+    auto average = [&](int i) {
+        return i < n ? *(const float4*)(parts.sums + part(i) * D + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    // (the first 32 parts are on their way while the weights are found)
+    float4 ahead[32 / kStride];
+#pragma unroll
+    for (int x = 0; x < 32 / kStride; ++x)
+        ahead[x] = average(x * kStride + sub);
+    const float2 nothing = make_float2(none, 0.f), mine = lane < n ? parts.stats[part(lane)] : nothing;
+    float m = mine.x, total = mine.y;
+    for (int i = lane + 32; i < n; i += 32) {
         const float2 st = parts.stats[part(i)];
         const float t = fmaxf(m, st.x), z = t == none ? 0.f : t;
         total = __fmul_rn(total, exp2_fast(m - z)) + st.y * exp2_fast(st.x - z);
@@ -712,24 +722,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const CacheArgs a
     for (int x = 1; x < 32; x *= 2)
         total += __shfl_xor_sync(0xffffffffu, total, x);
     const float over = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
-    const int sub = warp * kAtOnce + lane / kLanes, e = lane % kLanes;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int base = 0; base < n; base += 32) {
-        float f = 0.f;
-        if (base + lane < n) {
-            const float2 st = parts.stats[part(base + lane)];
-            f = __fmul_rn(st.y * exp2_fast(st.x - z), over);
-        }
-#pragma unroll 4
-        for (int x = 0; x < 32; x += kStride) {
-            const int i = base + x + sub;
-            const float weight = __shfl_sync(0xffffffffu, f, (x + sub) & 31);
-            if (i < n && x + sub < 32) {
-                const float4 v = *(const float4*)(parts.sums + part(i) * D + 4 * e);
-                sum.x = __fmaf_rn(v.x, weight, sum.x), sum.y = __fmaf_rn(v.y, weight, sum.y);
-                sum.z = __fmaf_rn(v.z, weight, sum.z), sum.w = __fmaf_rn(v.w, weight, sum.w);
-            }
-        }
+    auto add = [&](const float4& v, float weight) {
+        sum.x = __fmaf_rn(v.x, weight, sum.x), sum.y = __fmaf_rn(v.y, weight, sum.y);
+        sum.z = __fmaf_rn(v.z, weight, sum.z), sum.w = __fmaf_rn(v.w, weight, sum.w);
+    };
+    const float f = __fmul_rn(mine.y * exp2_fast(mine.x - z), over);
+#pragma unroll
+    for (int x = 0; x < 32 / kStride; ++x)
+        add(ahead[x], __shfl_sync(0xffffffffu, f, x * kStride + sub));
+    for (int base = 32; base < n; base += 32) {
+        const float2 st = base + lane < n ? parts.stats[part(base + lane)] : nothing;
+        const float g = __fmul_rn(st.y * exp2_fast(st.x - z), over);
+#pragma unroll
+        for (int x = 0; x < 32 / kStride; ++x)
+            add(average(base + x * kStride + sub), __shfl_sync(0xffffffffu, g, x * kStride + sub));
     }
     s_sum[sub][e] = sum;
     __syncthreads();
