@@ -393,7 +393,9 @@ typedef struct mb200_heads {
  * A block's scale is max(amax, 2^-119) / 127 of the new values in it, rounded to fp32, or what it was, if the block keeps
  * older positions and that is larger; whole numbers are x / scale to the nearest (ties to even). If the scale grows, older
  * numbers become q * (old scale / scale) to the nearest (in 64 bits). A block with a NaN or an infinity gets scale
- * NaN and zeros, and is NaN as long as it keeps them. No block may be appended to by two sequences of a call. */
+ * NaN and zeros, and is NaN as long as it keeps them. No block may be appended to by two sequences of a call.
+ * Positions are dropped by passing a smaller length to the next call; the scale of the block that they lay in stays what they
+ * made it as long as it keeps older positions, and those stay as they were made anew. */
 typedef struct mb200_kv_append_param {
     const int32_t *lengths, *cu;
     int tokens, heads, dtype; /* heads: of q */
@@ -413,9 +415,12 @@ MB200_API int mb200_kv_read_s8(
  *     out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)
  * q and out: [batch * queries][heads][d], heads a multiple of kv_heads: head h goes with key head h / (heads /
  * kv_heads). lengths[b] positions are in the cache, the queries' own among them: query i of a sequence sees positions
- * up to lengths[b] - queries + i. A query that sees none gets zeros (a sequence of length <= 0 is not in use).
- * Keys and values are the cache's exactly; q keeps 11 bits (those of fp16 relative to its row's largest), p_j are rounded to
- * 11 bits, sums are fp32, in an order that depends on lengths and sizes only.
+ * up to lengths[b] - queries + i, of those that the table has room for. A query that sees none gets zeros (a sequence of
+ * length <= 0 is not in use).
+ * Keys and values are the cache's exactly. q keeps 22 bits below its row's largest element, as far as 2^-126. p_j times the
+ * scale of its values is rounded to 11 bits, for fp16 results to 22, and to no less than 2^-30 of the largest such
+ * product of the query (or 2^-140); a p_j below 2^-126 of the query's largest is 0. Sums are fp32, in an order that depends on lengths and
+ * sizes only. Values that are none make every query NaN that sees them.
  * workspace: mb200_attention_cache_s8_workspace_bytes of device memory, 256-byte aligned, whose content does not
  * matter; two calls that may run at the same time need one each. */
 MB200_API size_t mb200_attention_cache_s8_workspace_bytes(const mb200_kv_cache* cache, int heads, int queries);
@@ -428,7 +433,8 @@ MB200_API int mb200_attention_cache_s8(
  * / kv_heads). causal != 0: a sequence's last query sees its last key, and each query one key less than the next; a query
  * that sees none gets zeros. Without it each sees all of its sequence's. What a query does not see does not reach it,
  * whatever it holds. (A query whose result is not finite is computed a second time by a far slower way: keys, values or
- * queries that are no numbers cost time.) p_j as above, but rounded to `dtype`.
+ * queries that are no numbers cost time.) p_j are rounded to `dtype`, sums are fp32. Device status 0x203: a wait inside
+ * the kernel ran out, and rows of the result are not written; nothing that a caller passes leads there.
  * q, k, v: 16-byte aligned, strides multiples of 8 elements and not 0. */
 MB200_API int mb200_attention_prompt(
         int batch, const int32_t* cu_q, const int32_t* cu_k, int tokens, int key_tokens, int heads, int kv_heads, int d,

@@ -17,7 +17,7 @@
 // What bounds it: for a step of decoding the launch and the four loads that follow from one another (lengths, page, scale,
 // whole numbers): 6 to 7 us with reading the blocks back. For prompts the instructions of the blocks' warps (8191 tokens:
 // 2.3 a clock and SM, ALUs half taken, 3.2 TB/s; the floor is 37 us). Reading back is bound by memory (65001 rows of 8
-// heads of 128: 71 us, 5.7 TB/s).
+// heads of 128: 71 to 76 us, 5.3 to 5.6 TB/s).
 #include "kv_cache.cuh"
 #include "umma_ptx.cuh"
 

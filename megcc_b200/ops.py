@@ -194,7 +194,7 @@ def kv_append_s8(cache, block_table, lengths, k, v, q=None, cos=None, sin=None, 
     With cos and sin [positions, turned elements / 2] fp32 keys are turned by their positions first, halves of the turned
     elements against each other or neighbours (interleaved), and queries q [tokens, heads, d] beside them. Returns (turned
     queries or None, with turned_keys turned keys or None). lengths stays as it is; a sequence with a negative one is not
-    in use, and its rows of the results are left as they were. (See mb200_kv_append_s8.)"""
+    in use, and its rows of the results, new tensors, are not written: they hold anything. (See mb200_kv_append_s8.)"""
     return tensor_calls().kv_append_s8(*cache, block_table, lengths, k, v, q, cos, sin, cu_tokens, interleaved,
                                        turned_keys)
 
@@ -202,7 +202,7 @@ def kv_append_s8(cache, block_table, lengths, k, v, q=None, cos=None, sin=None, 
 def kv_read_s8(cache, block_table, starts, cu_tokens, tokens, dtype=torch.bfloat16):
     """Cached keys and values as `dtype` (fp16 or bf16), two tensors [tokens, kv_heads, d] of packed rows: row
     cu_tokens[b] + i is position starts[b] + i of sequence b (starts None: from 0 on). For a prompt that continues
-    a cached one: attention_prompt takes them as its keys. Rows behind the last sequence are left as they were."""
+    a cached one: attention_prompt takes them as its keys. Rows of no sequence are not written: they hold anything."""
     return tensor_calls().kv_read_s8(*cache, block_table, starts, cu_tokens, tokens, dtype)
 
 
@@ -210,7 +210,7 @@ def attention_cache_s8(q, cache, block_table, lengths, scale=None, out=None):
     """Attention of one query per sequence, q [sequences, heads, d], or of several, [sequences, queries, heads, d], over
     its lengths[b] cached positions, the queries' own the last of them: each sees what lies in front of it and itself.
     fp16 or bf16; heads are a multiple of the cache's. scale: 1 / sqrt(d) unless given. A query that sees nothing gives
-    zeros, a sequence of length 0 (not in use) too. (See mb200_attention_cache_s8.)"""
+    zeros, a sequence of length 0 (not in use) too. out, if given, overlaps no operand. (See mb200_attention_cache_s8.)"""
     return tensor_calls().attention_cache_s8(q, *cache, block_table, lengths, scale, out)
 
 
@@ -218,8 +218,8 @@ def attention_prompt(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     """Attention over whole prompts, packed: q [tokens, heads, d], k and v [key tokens, kv_heads, d], fp16 or bf16, rows
     cu_q[b] .. cu_q[b + 1] (and cu_k, where a sequence has other keys than its queries', a cached prefix in front of
     them for instance: kv_read_s8). causal: the last query of a sequence sees its last key. scale: 1 / sqrt(d) unless
-    given. A query that sees nothing gives zeros; rows behind the last sequence are left as they were. (See
-    mb200_attention_prompt.)"""
+    given. A query that sees nothing gives zeros. Rows of no sequence are not written: a new tensor holds anything there, and
+    `out`, which overlaps no operand, what it held. (See mb200_attention_prompt.)"""
     return tensor_calls().attention_prompt(q, k, v, cu_q, cu_k, causal, scale, out)
 
 
